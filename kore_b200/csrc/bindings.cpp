@@ -112,6 +112,27 @@ void nvls_adamw(int64_t mc_grad, int64_t mc_param, const at::Tensor& own_param,
                 double lr, double b1, double b2, double eps, double wd, int64_t step,
                 const c10::optional<at::Tensor>& sumsq, double max_norm, int64_t seed);
 int64_t device_wait_flag(const at::Tensor& flag, int64_t want, double timeout_s);
+void head_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
+              const c10::optional<at::Tensor>& logp, const c10::optional<at::Tensor>& entropy, at::Tensor& lse);
+void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
+              const at::Tensor& lse, const at::Tensor& coef, double inv_temp, at::Tensor& dx, at::Tensor& dw,
+              bool accumulate, int64_t piece);
+void embed_scaled(const at::Tensor& ids, const at::Tensor& table, at::Tensor& out, double scale);
+void embed_grad_sorted(const at::Tensor& ids, const at::Tensor& dy, at::Tensor& dtable, double scale,
+                       bool accumulate);
+void moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx, const c10::optional<at::Tensor>& mask,
+                     double coef, at::Tensor& loss, at::Tensor& counts, at::Tensor& gain);
+void moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
+                     double dloss, at::Tensor& dlogits, bool accumulate);
+void act8_save(const at::Tensor& x, at::Tensor& q, at::Tensor& s);
+void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out);
+void act8_rmsnorm_save(const at::Tensor& x, const at::Tensor& w, at::Tensor& hn, at::Tensor& rstd, at::Tensor& q,
+                       at::Tensor& s, double eps);
+void act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s, const at::Tensor& w, at::Tensor& x, at::Tensor& hn,
+                       at::Tensor& rstd, double eps);
+void act8_swiglu_save(const at::Tensor& gu, at::Tensor& a, at::Tensor& q, at::Tensor& s);
+void act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s, at::Tensor& dgu,
+                     at::Tensor& a);
 int read_and_clear_device_error();
 }  // namespace kore
 
@@ -175,5 +196,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("symm_gather_ce", &kore::symm_gather_ce, "all-gather of heap shards on the copy engines");
   m.def("nvls_sumsq", &kore::nvls_sumsq, "sum of squares of the switch-reduced gradient shard (multimem)");
   m.def("nvls_adamw", &kore::nvls_adamw, "AdamW on the switch-reduced gradient shard, multicast parameter store");
+  m.def("head_fwd", &kore::head_fwd, "log-probs, entropy and logsumexp of the LM head without logits");
+  m.def("head_bwd", &kore::head_bwd, "gradient of the LM head loss in pieces of the vocabulary");
+  m.def("embed_scaled", &kore::embed_scaled);
+  m.def("embed_grad_sorted", &kore::embed_grad_sorted, "embedding gradient by sorted tokens");
+  m.def("moe_balance_fwd", &kore::moe_balance_fwd, "load-balancing loss and per-expert counts");
+  m.def("moe_balance_bwd", &kore::moe_balance_bwd);
+  m.def("act8_save", &kore::act8_save, "8-bit copy of an activation");
+  m.def("act8_load", &kore::act8_load);
+  m.def("act8_rmsnorm_save", &kore::act8_rmsnorm_save);
+  m.def("act8_rmsnorm_load", &kore::act8_rmsnorm_load);
+  m.def("act8_swiglu_save", &kore::act8_swiglu_save);
+  m.def("act8_swiglu_bwd", &kore::act8_swiglu_bwd);
   m.def("read_and_clear_device_error", &kore::read_and_clear_device_error);
 }

@@ -5,6 +5,8 @@
 //   * moe_combine:   y[t] = sum_j w[t,j] * src[pos[t,j]] (+ residual); with
 //                    w == nullptr it is the un-permute sum used by the backward
 //   * moe_combine_bwd: dsrc[pos[t,j]] = w[t,j] * dy[t];  dw[t,j] = <dy[t], src[pos[t,j]]>
+//   * moe_balance_fwd / _bwd: load-balancing loss with per-expert counts, and its
+//                    gradient to the router logits
 // The expert GEMMs run on the grouped tcgen05 GEMM; the row permutation is a
 // gather with the embedding kernel. Reference parity: HF Qwen3MoeSparseMoeBlock
 // (router softmax -> top-k -> norm_topk_prob -> experts -> weighted sum); the
@@ -393,6 +395,121 @@ inline int warps_grid(long n, int warps_per_block = 8) {
   return (int)((n + warps_per_block - 1) / warps_per_block);
 }
 
+// ---------------------------------------------------------------- balance loss
+//   n = sum_t m_t,  c_e = #{(t, j): m_t, idx_tj = e},  P_e = sum_t m_t p_te
+//   L = coef E / n^2 sum_e c_e P_e        g_e = dL/dp_te = coef E c_e / n^2  (c_e is constant)
+//   dlogits_te = m_t dL p_te (g_e - sum_j g_j p_tj)      through the router's softmax
+// Counts are integers; P sums in fp32 in an order that only T and E fix: a
+// warp's tokens, a block's warps, then the blocks. Masked tokens are not read.
+constexpr int kBalThreads = 256;
+
+// one warp per token at a time; part: [blocks][E] sums, cnt: [blocks][E + 1] counts and tokens
+__global__ void __launch_bounds__(kBalThreads) balance_part_kernel(
+    const float* __restrict__ probs, const int* __restrict__ idx, const bool* __restrict__ mask, int T, int E, int k,
+    float* __restrict__ part, int* __restrict__ cnt) {
+  __shared__ float s_sum[kBalThreads / 32][kMaxE];
+  __shared__ int s_cnt[kMaxE + 1];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e <= E; e += kBalThreads) s_cnt[e] = 0;
+  __syncthreads();
+  float acc[kMaxE / 32];
+#pragma unroll
+  for (int i = 0; i < kMaxE / 32; ++i) acc[i] = 0.f;
+  int tokens = 0;
+  for (long t = (long)blockIdx.x * (kBalThreads / 32) + warp; t < T; t += (long)gridDim.x * (kBalThreads / 32)) {
+    if (mask != nullptr && !mask[t]) continue;
+    ++tokens;
+#pragma unroll
+    for (int i = 0; i < kMaxE / 32; ++i) {
+      const int e = lane + 32 * i;
+      if (e < E) acc[i] += probs[t * E + e];
+    }
+    if (lane < k) {
+      const int e = idx[t * k + lane];
+      if (e >= 0 && e < E) atomicAdd(&s_cnt[e], 1);
+    }
+  }
+  if (lane == 0) atomicAdd(&s_cnt[E], tokens);
+#pragma unroll
+  for (int i = 0; i < kMaxE / 32; ++i) s_sum[warp][lane + 32 * i] = acc[i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kBalThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kBalThreads / 32; ++w) v += s_sum[w][e];
+    part[(size_t)blockIdx.x * E + e] = v;
+  }
+  for (int e = threadIdx.x; e <= E; e += kBalThreads) cnt[(size_t)blockIdx.x * (E + 1) + e] = s_cnt[e];
+}
+
+__global__ void __launch_bounds__(kMaxE) balance_join_kernel(const float* __restrict__ part,
+                                                             const int* __restrict__ cnt, int blocks, int E,
+                                                             float coef, float* __restrict__ loss,
+                                                             int* __restrict__ counts, float* __restrict__ gain) {
+  __shared__ float s_red[kMaxE / 32];
+  __shared__ int s_n;
+  const int e = threadIdx.x;
+  if (e == 0) {
+    int n = 0;
+    for (int b = 0; b < blocks; ++b) n += cnt[(size_t)b * (E + 1) + E];
+    s_n = n;
+  }
+  float sum = 0.f;
+  int c = 0;
+  if (e < E)
+    for (int b = 0; b < blocks; ++b) {
+      sum += part[(size_t)b * E + e];
+      c += cnt[(size_t)b * (E + 1) + e];
+    }
+  __syncthreads();
+  const float n = (float)max(s_n, 1);
+  const float g = coef * (float)E * (float)c / (n * n);
+  if (e < E) {
+    counts[e] = c;
+    gain[e] = g;
+  }
+  float v = e < E && c > 0 ? g * sum : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
+  if ((e & 31) == 0) s_red[e / 32] = v;
+  __syncthreads();
+  if (e == 0) {
+    for (int w = 1; w < kMaxE / 32; ++w) v += s_red[w];
+    *loss = v;
+  }
+}
+
+__global__ void __launch_bounds__(kBalThreads) balance_bwd_kernel(const float* __restrict__ probs,
+                                                                  const float* __restrict__ gain,
+                                                                  const bool* __restrict__ mask, int T, int E,
+                                                                  float dloss, int add, float* __restrict__ dlogits) {
+  const int lane = threadIdx.x & 31;
+  float g[kMaxE / 32];
+#pragma unroll
+  for (int i = 0; i < kMaxE / 32; ++i) g[i] = lane + 32 * i < E ? gain[lane + 32 * i] * dloss : 0.f;
+  for (long t = (long)blockIdx.x * (kBalThreads / 32) + threadIdx.x / 32; t < T;
+       t += (long)gridDim.x * (kBalThreads / 32)) {
+    const bool live = mask == nullptr || mask[t];
+    if (!live && add) continue;
+    float p[kMaxE / 32], dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxE / 32; ++i) {
+      p[i] = live && lane + 32 * i < E ? probs[t * E + lane + 32 * i] : 0.f;
+      dot += p[i] * g[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffff, dot, o);
+#pragma unroll
+    for (int i = 0; i < kMaxE / 32; ++i) {
+      const int e = lane + 32 * i;
+      if (e < E) {
+        const float d = p[i] * (g[i] - dot);
+        dlogits[t * E + e] = add ? dlogits[t * E + e] + d : d;
+      }
+    }
+  }
+}
+
 }  // namespace moe
 
 // Device routing plan (no host synchronisation): idx int32 [T, k] expert ids;
@@ -515,6 +632,70 @@ void moe_combine_bwd(const at::Tensor& dy, const at::Tensor& src, const at::Tens
       (const __nv_bfloat16*)dy.data_ptr(), (const __nv_bfloat16*)src.data_ptr(), pos.data_ptr<int>(),
       w.data_ptr<float>(), (__nv_bfloat16*)dsrc.data_ptr(), dw.data_ptr<float>(), T, H, k);
   check_cuda(cudaGetLastError(), "moe_combine_bwd");
+}
+
+
+namespace {
+void check_balance(const at::Tensor& probs, const c10::optional<at::Tensor>& mask) {
+  TORCH_CHECK(probs.is_cuda() && probs.scalar_type() == at::kFloat && probs.dim() == 2 && probs.is_contiguous(),
+              "balance: probs must be contiguous fp32 [T, E]");
+  TORCH_CHECK(probs.size(1) >= 1 && probs.size(1) <= moe::kMaxE, "balance: 1 to 256 experts");
+  TORCH_CHECK(probs.size(0) < (int64_t(1) << 30), "balance: at most 2^30 tokens");
+  if (mask)
+    TORCH_CHECK(mask->device() == probs.device() && mask->scalar_type() == at::kBool && mask->dim() == 1 &&
+                    mask->size(0) == probs.size(0) && mask->is_contiguous(),
+                "balance: mask must be bool [T]");
+}
+void check_balance_vec(const at::Tensor& t, const at::Tensor& probs, at::ScalarType dt, const char* name) {
+  TORCH_CHECK(t.device() == probs.device() && t.scalar_type() == dt && t.dim() == 1 && t.is_contiguous() &&
+                  t.size(0) == probs.size(1),
+              "balance: ", name, " must have one entry per expert");
+}
+}  // namespace
+
+void moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx, const c10::optional<at::Tensor>& mask,
+                     double coef, at::Tensor& loss, at::Tensor& counts, at::Tensor& gain) {
+  check_balance(probs, mask);
+  TORCH_CHECK(idx.device() == probs.device() && idx.scalar_type() == at::kInt && idx.dim() == 2 &&
+                  idx.is_contiguous() && idx.size(0) == probs.size(0) && idx.size(1) >= 1 &&
+                  idx.size(1) <= moe::kMaxK,
+              "balance: idx must be contiguous int32 [T, k], 1 <= k <= 16");
+  check_balance_vec(counts, probs, at::kInt, "counts");
+  check_balance_vec(gain, probs, at::kFloat, "gain");
+  TORCH_CHECK(loss.device() == probs.device() && loss.scalar_type() == at::kFloat && loss.numel() == 1,
+              "balance: loss must be one fp32 value");
+  c10::cuda::CUDAGuard g(probs.device());
+  const int T = probs.size(0), E = probs.size(1), k = idx.size(1);
+  const int rows = moe::kBalThreads / 32;
+  const int blocks = std::max(1, std::min((T + 4 * rows - 1) / (4 * rows), num_sms(probs.get_device()) * 2));
+  at::Tensor part = at::empty({(int64_t)blocks * (2 * E + 1)}, probs.options());
+  float* sums = part.data_ptr<float>();
+  int* cnt = reinterpret_cast<int*>(sums + (size_t)blocks * E);
+  auto st = at::cuda::getCurrentCUDAStream();
+  moe::balance_part_kernel<<<blocks, moe::kBalThreads, 0, st>>>(
+      probs.data_ptr<float>(), idx.data_ptr<int>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, k, sums, cnt);
+  check_cuda(cudaGetLastError(), "balance sums");
+  moe::balance_join_kernel<<<1, moe::kMaxE, 0, st>>>(sums, cnt, blocks, E, (float)coef, loss.data_ptr<float>(),
+                                                     counts.data_ptr<int>(), gain.data_ptr<float>());
+  check_cuda(cudaGetLastError(), "balance join");
+}
+
+void moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
+                     double dloss, at::Tensor& dlogits, bool accumulate) {
+  check_balance(probs, mask);
+  check_balance_vec(gain, probs, at::kFloat, "gain");
+  TORCH_CHECK(dlogits.device() == probs.device() && dlogits.scalar_type() == at::kFloat &&
+                  dlogits.sizes() == probs.sizes() && dlogits.is_contiguous(),
+              "balance: dlogits must be contiguous fp32 [T, E]");
+  const int T = probs.size(0), E = probs.size(1);
+  if (T == 0) return;
+  c10::cuda::CUDAGuard g(probs.device());
+  const int rows = moe::kBalThreads / 32;
+  const int blocks = std::min((T + rows - 1) / rows, num_sms(probs.get_device()) * 8);
+  moe::balance_bwd_kernel<<<blocks, moe::kBalThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
+      probs.data_ptr<float>(), gain.data_ptr<float>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, (float)dloss,
+      accumulate ? 1 : 0, dlogits.data_ptr<float>());
+  check_cuda(cudaGetLastError(), "balance_bwd");
 }
 
 }  // namespace kore

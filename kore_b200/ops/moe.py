@@ -44,6 +44,49 @@ def route_bwd(probs, idx, w, dw, norm: bool = True):
     return probs * (gp - (gp * probs).sum(-1, keepdim=True))
 
 
+def balance_loss(probs: torch.Tensor, idx: torch.Tensor, mask: Optional[torch.Tensor] = None, coef: float = 1.0):
+    """Load-balancing loss of a router and the experts' token counts.
+
+    L = coef E / n^2 sum_e c_e P_e with n the number of tokens, c_e how often
+    expert e is among their choices ``idx`` [T, k] and P_e the sum of its
+    probabilities ``probs`` [T, E] (fp32); perfectly even routing gives
+    coef k. ``mask`` (bool [T]) leaves padding tokens out of all three, whatever
+    their probabilities hold; entries of ``idx`` outside [0, E) are not counted.
+    Returns (loss [] fp32, counts [E] int32, gain [E] fp32); gain_e = dL/dp_te
+    is what ``balance_bwd`` takes. The counts are constants of the gradient."""
+    T, E = probs.shape
+    loss = torch.empty((), dtype=torch.float32, device=probs.device)
+    counts = torch.empty(E, dtype=torch.int32, device=probs.device)
+    gain = torch.empty(E, dtype=torch.float32, device=probs.device)
+    if probs.is_cuda:
+        native().moe_balance_fwd(probs, idx, mask, float(coef), loss, counts, gain)
+        return loss, counts, gain
+    keep = torch.ones(T, dtype=torch.bool) if mask is None else mask
+    sel = idx[keep].long().reshape(-1)
+    counts.copy_(torch.bincount(sel[(sel >= 0) & (sel < E)], minlength=E))
+    n = max(1, int(keep.sum()))
+    gain.copy_(coef * E * counts.float() / (float(n) * n))
+    used = counts > 0
+    loss.copy_((gain * probs[keep].float().sum(0))[used].sum())
+    return loss, counts, gain
+
+
+def balance_bwd(probs: torch.Tensor, gain: torch.Tensor, mask: Optional[torch.Tensor] = None, dloss: float = 1.0,
+                dlogits: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``dloss * balance_loss`` with respect to the router logits
+    (fp32 [T, E]), added to ``dlogits`` when it is given. Masked tokens get 0
+    (with ``dlogits``: are left as they are)."""
+    if probs.is_cuda:
+        out = torch.empty_like(probs) if dlogits is None else dlogits
+        native().moe_balance_bwd(probs, gain, mask, float(dloss), out, dlogits is not None)
+        return out
+    g = gain * dloss
+    d = probs * (g - (probs * g).sum(-1, keepdim=True))
+    if mask is not None:
+        d = torch.where(mask.unsqueeze(-1), d, torch.zeros_like(d))
+    return d if dlogits is None else dlogits.add_(d)
+
+
 def permutation(idx: torch.Tensor, num_experts: int, expert_range: Optional[Tuple[int, int]] = None):
     """Expert-major ordering of the (token, slot) pairs.
 

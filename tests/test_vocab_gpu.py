@@ -1,0 +1,303 @@
+"""Head loss in vocabulary pieces and embedding with sorted gradient: the native
+kernels against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from kore_b200 import ops
+from kore_b200.ops import vocab
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float64
+
+
+def _inputs(T, V, H, seed=0, lean=8.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn(V, H, generator=g, device="cuda") * 0.5 / math.sqrt(H)).bfloat16()
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    wy = w[y].float()
+    x = torch.randn(T, H, generator=g, device="cuda") + lean * torch.rand(T, 1, generator=g, device="cuda") * wy / \
+        wy.square().sum(-1, keepdim=True)
+    coef = torch.randn(T, generator=g, device="cuda") / T
+    return x.bfloat16(), w, y, coef
+
+
+def _oracle(x, w, y, coef, tau):
+    """64-bit values, and the sums of magnitudes that rounding errors scale with."""
+    x, w, coef = x.to(F8), w.to(F8), coef.to(F8)
+    lp = torch.log_softmax(x @ w.t() / tau, -1)
+    ok = (y >= 0) & (y < w.shape[0])
+    yy = torch.where(ok, y, torch.zeros_like(y))
+    logp = torch.where(ok, lp.gather(1, yy[:, None])[:, 0], torch.zeros((), dtype=F8, device=x.device))
+    lse = torch.logsumexp(x @ w.t() / tau, -1)
+    p = lp.exp()
+    ent = -(p * lp).sum(-1)
+    one = torch.zeros_like(p)
+    one[torch.arange(len(y), device=x.device), yy] = ok.to(F8)
+    live = (coef != 0)[:, None]
+    dz = torch.where(live, (coef / tau)[:, None] * (one - p), torch.zeros_like(p))
+    xm = torch.where(live, x, torch.zeros_like(x))
+    # a logit is off by delta: the tensor cores add 16 products at a time and truncate the fp32
+    # partial sum, by at most 2^-23 of it; dz is off by 2^-8 of itself (bf16) and p delta
+    mag = (x.abs() @ w.abs().t()).amax(-1)
+    delta = (x.shape[1] / 16 + 2) * 2.0 ** -23 * mag / tau + 2e-6 * (1 + lse.abs())
+    slack = 2.0 ** -8 * dz.abs() + torch.where(live, 2 * delta[:, None] * p * (coef.abs() / tau)[:, None], torch.zeros_like(p))
+    dx, dw = dz @ w, dz.t() @ xm
+    # plus the fp32 sums (2^-18 of the magnitudes is 32 roundings of the partial sums) and the output's own rounding
+    tdx = (slack + 2.0 ** -18 * dz.abs()) @ w.abs() + 2.0 ** -8 * dx.abs() + 1e-30
+    tdw = (slack + 2.0 ** -18 * dz.abs()).t() @ xm.abs() + 2.0 ** -8 * dw.abs() + 1e-30
+    return dict(logp=logp, lse=lse, ent=ent, dx=dx, dw=dw, delta=delta, tdx=tdx, tdw=tdw)
+
+
+def _check_fwd(o, logp, ent, lse):
+    assert ops.check_device_error() == 0
+    assert ((lse.to(F8) - o["lse"]).abs() <= o["delta"]).all()
+    assert ((logp.to(F8) - o["logp"]).abs() <= 2 * o["delta"]).all()
+    if ent is not None:
+        # d ent = -sum p (log p + ent) dz: delta times the spread of log p
+        spread = 2 + o["lse"].abs() + o["ent"].abs()
+        assert ((ent.to(F8) - o["ent"]).abs() <= 4 * o["delta"] * spread).all()
+
+
+SHAPES = [(1, 8, 8), (1, 1, 64), (3, 17, 72), (129, 1000, 256), (127, 32000, 256), (257, 4097, 264), (300, 513, 1032),
+          (1000, 9999, 640), (64, 151936, 128), (513, 20011, 5120)]
+
+
+@pytest.mark.parametrize("T,V,H", SHAPES)
+@pytest.mark.parametrize("tau", [1.0, 0.6])
+def test_head_forward(T, V, H, tau):
+    x, w, y, coef = _inputs(T, V, H)
+    if T > 2:
+        y[1], y[2] = -1, V
+    o = _oracle(x, w, y, coef, tau)
+    logp, ent, lse = vocab.head_fwd(x, w, y, tau, want_entropy=True)
+    _check_fwd(o, logp, ent, lse)
+    logp2, none, lse2 = vocab.head_fwd(x, w, y, tau)
+    assert none is None
+    _check_fwd(o, logp2, None, lse2)
+    nolp, _, lse3 = vocab.head_fwd(x, w, None, tau)
+    assert nolp is None and torch.equal(lse2, lse3)
+
+
+@pytest.mark.parametrize("T,V,H", SHAPES)
+@pytest.mark.parametrize("piece", [0, 264])
+def test_head_backward(T, V, H, piece):
+    if piece and V > 30000:
+        piece = 50008
+    tau = 0.8
+    x, w, y, coef = _inputs(T, V, H, seed=1)
+    coef[::4] = 0
+    if T > 3:
+        y[1] = -1
+        coef[1] = 0.3
+    o = _oracle(x, w, y, coef, tau)
+    _, _, lse = vocab.head_fwd(x, w, y, tau)
+    dx, dw = vocab.head_bwd(x, w, y, lse, coef, tau, piece=piece)
+    assert ops.check_device_error() == 0
+    extra = 2 if piece else 1               # dx of several pieces: fp32 sums of the pieces
+    assert ((dx.to(F8) - o["dx"]).abs() <= extra * o["tdx"]).all()
+    assert ((dw.to(F8) - o["dw"]).abs() <= o["tdw"]).all()
+    assert (dx[coef == 0] == 0).all()
+    # fp32 gradient buffer, added to
+    base = torch.randn(V, H, device="cuda") * 0.01
+    acc = base.clone()
+    vocab.head_bwd(x, w, y, lse, coef, tau, dw=acc, accumulate=True, piece=piece)
+    assert ((acc.to(F8) - base.to(F8) - o["dw"]).abs() <= o["tdw"] + 2.0 ** -22 * base.abs()).all()
+
+
+def test_head_backward_is_the_gradient():
+    """Directional differences of the loss in 64 bits."""
+    T, V, H, tau = 37, 523, 64, 1.3
+    x, w, y, coef = _inputs(T, V, H, seed=2, lean=4.0)
+    _, _, lse = vocab.head_fwd(x, w, y, tau)
+    dx, dw = vocab.head_bwd(x, w, y, lse, coef, tau)
+
+    def loss(x, w):
+        return (coef.to(F8) * torch.log_softmax(x @ w.t() / tau, -1).gather(1, y[:, None])[:, 0]).sum()
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = 1e-4
+    for a, d in ((x, dx), (w, dw)):
+        for _ in range(4):
+            v = torch.randn(a.shape, generator=g, device="cuda", dtype=F8)
+            args = ((x.to(F8) + h * v, w.to(F8)), (x.to(F8) - h * v, w.to(F8))) if a is x else \
+                ((x.to(F8), w.to(F8) + h * v), (x.to(F8), w.to(F8) - h * v))
+            num = (loss(*args[0]) - loss(*args[1])) / (2 * h)
+            # independent roundings of 2^-8 per entry along a random direction: 6 sigma
+            assert abs(num - (d.to(F8) * v).sum()) <= 6 * 2.0 ** -8 * (d.to(F8) * v).norm() + 1e-6
+
+
+def test_head_strides_streams_and_repeats():
+    T, V, H = 200, 3001, 136
+    x, w, y, coef = _inputs(T, V, H, seed=4)
+    wide = torch.full((T, H + 24), float("nan"), device="cuda", dtype=torch.bfloat16)
+    wide[:, 8:8 + H] = x
+    ww = torch.full((V, H + 8), float("nan"), device="cuda", dtype=torch.bfloat16)
+    ww[:, :H] = w
+    logp, _, lse = vocab.head_fwd(x, w, y)
+    dx, dw = vocab.head_bwd(x, w, y, lse, coef)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        l2, _, e2 = vocab.head_fwd(wide[:, 8:8 + H], ww[:, :H], y)
+        dx2, dw2 = vocab.head_bwd(wide[:, 8:8 + H], ww[:, :H], y, e2, coef)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in ((logp, l2), (lse, e2), (dx, dx2), (dw, dw2)):
+        assert torch.equal(a, b)
+
+
+def test_head_masked_rows_may_hold_anything():
+    T, V, H = 70, 777, 64
+    x, w, y, coef = _inputs(T, V, H, seed=5)
+    coef[5], coef[6], y[6] = 0, 0, -1
+    clean = vocab.head_fwd(x, w, y)
+    dx, dw = vocab.head_bwd(x, w, y, clean[2], coef)
+    bad = x.clone()
+    bad[5], bad[6] = float("inf"), float("nan")
+    logp, ent, lse = vocab.head_fwd(bad, w, y, want_entropy=True)
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[5] = rest[6] = False
+    assert torch.equal(lse[rest], clean[2][rest]) and torch.equal(logp[rest], clean[0][rest])
+    assert torch.isnan(lse[5:7]).all() and torch.isnan(ent[5:7]).all()
+    dx2, dw2 = vocab.head_bwd(bad, w, y, lse, coef)
+    assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
+
+
+def test_head_logits_of_minus_inf():
+    """Vocabulary entries with logit -inf have probability 0; the rest is as without them."""
+    T, V, H = 40, 600, 64
+    x, w, y, _ = _inputs(T, V, H, seed=6)
+    x[:, 0] = 1.0
+    w[:, 0] = 0.0
+    keep = torch.ones(V, dtype=torch.bool, device="cuda")
+    keep[100:420] = False
+    y = y % 100
+    want = vocab.head_fwd(x, w[keep].contiguous(), y, want_entropy=True)
+    w[100:420, 0] = float("-inf")
+    w[100:420, 1:] = 0.0
+    got = vocab.head_fwd(x, w, y, want_entropy=True)
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b, rtol=2e-5, atol=2e-5)
+
+
+def test_head_no_rows_and_refusals():
+    x, w, y, coef = _inputs(4, 32, 16)
+    e = torch.empty(0, 16, device="cuda", dtype=torch.bfloat16)
+    n = torch.empty(0, dtype=torch.long, device="cuda")
+    logp, ent, lse = vocab.head_fwd(e, w, n, want_entropy=True)
+    assert logp.numel() == ent.numel() == lse.numel() == 0
+    dx, dw = vocab.head_bwd(e, w, n, lse, torch.empty(0, device="cuda"))
+    assert dx.shape == (0, 16) and (dw == 0).all()
+    kept = torch.ones_like(w)
+    vocab.head_bwd(e, w, n, lse, torch.empty(0, device="cuda"), dw=kept, accumulate=True)
+    assert (kept == 1).all()
+    lse4 = torch.zeros(4, device="cuda")
+    bad = [lambda: vocab.head_fwd(x.float(), w, y), lambda: vocab.head_fwd(x, w[:, :8], y),
+           lambda: vocab.head_fwd(x, w, y[:3]), lambda: vocab.head_fwd(x, w, y.int()),
+           lambda: vocab.head_fwd(x, w, y, 0.0), lambda: vocab.head_fwd(x, w, y, float("nan")),
+           lambda: vocab.head_fwd(x[:, :12], w[:, :12], y), lambda: vocab.head_fwd(x.t(), w[:, :4], None),
+           lambda: vocab.head_fwd(x[:, 4:12], w[:, 4:12], y), lambda: vocab.head_fwd(x, w.cpu(), y),
+           lambda: vocab.head_fwd(x, w[:0], y),
+           lambda: vocab.head_bwd(x, w, y, lse4[:2], coef), lambda: vocab.head_bwd(x, w, y, lse4, coef.half()),
+           lambda: vocab.head_bwd(x, w, y, lse4, coef, accumulate=True),
+           lambda: vocab.head_bwd(x, w, y, lse4, coef, piece=-1),
+           lambda: vocab.head_bwd(x, w, y, lse4, coef, dw=torch.empty(31, 16, device="cuda")),
+           lambda: vocab.head_bwd(x, w, y, lse4, coef, dx=torch.empty(4, 16, device="cuda"))]
+    for f in bad:
+        with pytest.raises((RuntimeError, ValueError)):
+            f()
+
+
+@pytest.mark.parametrize("M,N,K,pad", [(77, 128, 200, 3), (300, 256, 131, 5), (1001, 512, 64, 7), (8, 64, 9, 7)])
+def test_gemm_ragged_contiguous_extents(M, N, K, pad):
+    """K (or M of a transposed A) need not be a multiple of 8 when the rows are padded."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    A = torch.full((M, K + pad + (-(K + pad)) % 8), float("nan"), device="cuda", dtype=torch.bfloat16)
+    A[:, :K] = torch.randn(M, K, generator=g, device="cuda")
+    B = torch.randn(K, N, generator=g, device="cuda").bfloat16()
+    want = A[:, :K].to(F8) @ B.to(F8)
+    tol = 2.0 ** -8 * (A[:, :K].to(F8).abs() @ B.to(F8).abs())
+    assert ((ops.mm(A[:, :K], B, b_t=False).to(F8) - want).abs() <= tol).all()
+    At = torch.full((K, M + pad + (-(M + pad)) % 8), float("nan"), device="cuda", dtype=torch.bfloat16)
+    At[:, :M] = A[:, :K].t()
+    assert ((ops.mm(At[:, :M], B, a_t=True, b_t=False).to(F8) - want).abs() <= tol).all()
+    assert ops.check_device_error() == 0
+
+
+# ------------------------------------------------------------------ embedding
+def _ids(T, V, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = torch.exp(torch.rand(T, generator=g, device="cuda") * math.log(V)).long().clamp_(1, V) - 1
+    return r
+
+
+EMBED = [(0, 8, 8), (1, 1, 8), (5, 3, 16), (33, 4, 264), (64, 1000, 256), (4096, 50, 128), (4097, 32000, 256),
+         (10001, 100, 1032), (20000, 151936, 64)]
+
+
+@pytest.mark.parametrize("T,V,H", EMBED)
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_embed_grad(T, V, H, dt):
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    ids = _ids(T, V)
+    if T > 4:
+        ids[2], ids[4] = -1, V
+    dy = torch.randn(T, H + 8, generator=g, device="cuda").bfloat16()[:, :H]
+    ok = (ids >= 0) & (ids < V)
+    want, mag = torch.zeros(V, H, dtype=F8, device="cuda"), torch.zeros(V, H, dtype=F8, device="cuda")
+    want.index_put_((ids[ok],), dy[ok].to(F8), accumulate=True)
+    mag.index_put_((ids[ok],), dy[ok].to(F8).abs(), accumulate=True)
+    count = torch.zeros(V, dtype=F8, device="cuda").index_put_((ids[ok],), torch.ones((), dtype=F8, device="cuda"), accumulate=True)
+    unit = 2.0 ** -24 if dt == torch.float32 else 2.0 ** -8
+    # an fp32 sum of n terms is off by at most n roundings of its magnitudes
+    tol = (count[:, None] + 2) * 2.0 ** -24 * mag
+    for scale in (1.0, 3.7):
+        got = vocab.embed_grad(ids, dy, torch.full((V, H), float("nan"), device="cuda", dtype=dt), scale, accumulate=False)
+        assert ((got.to(F8) - scale * want).abs() <= 1.001 * scale * (tol + unit * want.abs()) + 1e-30).all()
+        base = torch.randn(V, H, generator=g, device="cuda").to(dt)
+        acc = vocab.embed_grad(ids, dy, base.clone(), scale)
+        assert ((acc.to(F8) - base.to(F8) - scale * want).abs()
+                <= 1.001 * (scale * tol + 2 * unit * (base.to(F8).abs() + scale * mag)) + 1e-30).all()
+        assert torch.equal(acc[count == 0], base[count == 0])
+    again = vocab.embed_grad(ids, dy.clone(), torch.empty(V, H, device="cuda", dtype=dt), 3.7, accumulate=False)
+    assert torch.equal(again, got)                                   # equal calls, equal bits
+
+
+@pytest.mark.parametrize("T,V,H", EMBED)
+def test_embed_lookup(T, V, H):
+    g = torch.Generator(device="cuda").manual_seed(T)
+    table = torch.randn(V, H + 16, generator=g, device="cuda").bfloat16()[:, 8:8 + H]
+    ids = _ids(T, V)
+    if T > 4:
+        ids[2], ids[4] = -5, V + 3
+    ok = (ids >= 0) & (ids < V)
+    for scale in (1.0, 0.3):
+        got = vocab.embed(ids, table, scale)
+        want = torch.where(ok[:, None], table[torch.where(ok, ids, 0)].float() * scale, torch.zeros((), device="cuda")).bfloat16()
+        assert torch.equal(got, want)
+
+
+def test_embed_grad_keeps_rows_apart():
+    """inf and NaN stay in the rows of their own tokens."""
+    T, V, H = 300, 40, 64
+    ids = torch.arange(T, device="cuda") % V
+    dy = torch.ones(T, H, device="cuda").bfloat16()
+    dy[7] = float("nan")
+    dy[9] = float("inf")
+    out = vocab.embed_grad(ids, dy, torch.empty(V, H, device="cuda"), accumulate=False)
+    assert torch.isnan(out[7]).all() and torch.isinf(out[9]).all()
+    assert torch.isfinite(out[10:]).all() and torch.isfinite(out[:7]).all()
+
+
+def test_embed_refusals():
+    ids = torch.zeros(4, dtype=torch.long, device="cuda")
+    dy = torch.zeros(4, 16, device="cuda", dtype=torch.bfloat16)
+    tab = torch.zeros(8, 16, device="cuda", dtype=torch.bfloat16)
+    for f in (lambda: vocab.embed(ids.int(), tab), lambda: vocab.embed(ids, tab.float()),
+              lambda: vocab.embed(ids, tab[:, :12]), lambda: vocab.embed(ids.cpu(), tab),
+              lambda: vocab.embed_grad(ids[:3], dy, tab), lambda: vocab.embed_grad(ids, dy.float(), tab),
+              lambda: vocab.embed_grad(ids, dy, tab[:, :8]), lambda: vocab.embed_grad(ids, dy, tab.half()),
+              lambda: vocab.embed_grad(ids, dy, tab.cpu()), lambda: vocab.embed_grad(ids, dy.t(), tab)):
+        with pytest.raises(RuntimeError):
+            f()
