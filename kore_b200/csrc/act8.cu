@@ -23,19 +23,29 @@ namespace kore {
 namespace act8 {
 
 constexpr int kBlock = 128;
-constexpr int kNormVecs = 1024;  // RMSNorm rows: H <= 8192
+constexpr int kMaxNorm = 8192;  // columns of an RMSNorm row
 
-KORE_DEV void unpack8(const uint4& u, float (&f)[8]) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+// 8 values of a 16-byte vector as 4 pairs (packed fp32 instructions: the kernels
+// are near the issue limit with single ones)
+KORE_DEV void unpack8(const uint4& u, uint64_t (&f)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+KORE_DEV uint4 pack8(const uint64_t (&f)[4]) {
+  uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 t = __bfloat1622float2(h[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
+    float lo, hi;
+    f2_unpack(f[i], lo, hi);
+    w[i] = pack_bf16(lo, hi);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-KORE_DEV uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+KORE_DEV float sum_pair(uint64_t v) {
+  float lo, hi;
+  f2_unpack(v, lo, hi);
+  return lo + hi;
 }
 
 // Quantises the 8 values of this lane; the 16 lanes of a half warp share a
@@ -59,14 +69,20 @@ KORE_DEV uint2 quantise(const uint4& raw, float& scale) {
     inv = __fmul_rn(__frcp_rn(a * p), 127.f) * p;
     scale = __fmul_rn(a, 1.f / 127.f);
   }
-  float f[8];
+  uint64_t f[4];
   unpack8(raw, f);
+  const uint64_t magic = f2_pack(12582912.f, 12582912.f);
   uint32_t b[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int i = 0; i < 4; ++i) {
     // adding 1.5 * 2^23 rounds to the nearest integer and leaves its low byte
-    // in the low byte of the sum
-    b[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[e], inv), 12582912.f));
+    // in the low byte of the sum; the product is rounded first (a packed product
+    // would be fused with the addition)
+    float lo, hi;
+    f2_unpack(f[i], lo, hi);
+    f2_unpack(f2_add(f2_pack(__fmul_rn(lo, inv), __fmul_rn(hi, inv)), magic), lo, hi);
+    b[2 * i] = __float_as_uint(lo);
+    b[2 * i + 1] = __float_as_uint(hi);
   }
   if (top >= 0x7f80u) return make_uint2(0, 0);
   const uint32_t lo0 = __byte_perm(b[0], b[1], 0x0040), lo1 = __byte_perm(b[2], b[3], 0x0040);
@@ -76,12 +92,15 @@ KORE_DEV uint2 quantise(const uint4& raw, float& scale) {
 
 // The 8 values that the bytes stand for. 0x4B000000 | (q + 128) is the float
 // 2^23 + 128 + q.
-KORE_DEV void restore(const uint2& q, float scale, float (&f)[8]) {
+KORE_DEV void restore(const uint2& q, float scale, uint64_t (&f)[4]) {
   const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+  const uint64_t off = f2_pack(-8388736.f, -8388736.f), s2 = f2_pack(scale, scale);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t bits = __byte_perm(w[e / 4], 0x4B000000u, 0x7440 | (e & 3));
-    f[e] = __fmul_rn(__fadd_rn(__uint_as_float(bits), -8388736.f), scale);
+  for (int i = 0; i < 4; ++i) {
+    const int e = 2 * i;
+    const uint32_t lo = __byte_perm(w[e / 4], 0x4B000000u, 0x7440 | (e & 3));
+    const uint32_t hi = __byte_perm(w[e / 4], 0x4B000000u, 0x7440 | ((e + 1) & 3));
+    f[i] = f2_mul(f2_add(f2_pack(__uint_as_float(lo), __uint_as_float(hi)), off), s2);
   }
 }
 
@@ -91,209 +110,263 @@ struct Held {
   int H, nb;
 };
 
+// Element-wise kernels: a thread owns one 8-column vector j and walks rows with
+// the grid's y; the loads of a few rows are issued before the first is used.
+// More rows cost registers and so resident warps (5003 x 5120 and 8192 x 17408, us,
+// with 1, 2, 4 rows: save -, 41, 49; load -, 49, 45; SwiGLU save 208, 185, -;
+// backward 229, 246, -).
+constexpr int kSaveRows = 2;
+constexpr int kLoadRows = 4;
+
 // ---------------------------------------------------------------- save / load
-__global__ void save_kernel(const __nv_bfloat16* __restrict__ x, long ldx, Held h, long T) {
-  const long total = T * h.nb;
-  const int sub = threadIdx.x & 15;
-  // whole half warps step together; the warp's two halves may be in different rows
-  for (long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) / 16; i - ((threadIdx.x >> 4) & 1) < total;
-       i += (long)gridDim.x * blockDim.x / 16) {
-    const long t = i / h.nb;
-    const int b = (int)(i - t * h.nb);
-    const int col = b * kBlock + sub * 8;
-    const bool live = i < total && col < h.H;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live) raw = *reinterpret_cast<const uint4*>(x + t * ldx + col);
-    float scale;
-    const uint2 q = quantise(raw, scale);
-    if (live) *reinterpret_cast<uint2*>(h.q + t * h.H + col) = q;
-    if (live && sub == 0) h.s[i] = scale;
+__global__ void __launch_bounds__(256) save_kernel(const __nv_bfloat16* __restrict__ x, long ldx, Held h, long T) {
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  const bool live = j * 8 < h.H;
+  pdl_wait();
+  pdl_trigger();
+  for (long t0 = (long)blockIdx.y * kSaveRows; t0 < T; t0 += (long)gridDim.y * kSaveRows) {
+    uint4 raw[kSaveRows];
+#pragma unroll
+    for (int r = 0; r < kSaveRows; ++r) {
+      raw[r] = make_uint4(0, 0, 0, 0);
+      if (live && t0 + r < T) raw[r] = __ldg(reinterpret_cast<const uint4*>(x + (t0 + r) * ldx) + j);
+    }
+#pragma unroll
+    for (int r = 0; r < kSaveRows; ++r) {
+      float scale;
+      const uint2 q = quantise(raw[r], scale);
+      if (live && t0 + r < T) {
+        reinterpret_cast<uint2*>(h.q + (t0 + r) * h.H)[j] = q;
+        if ((j & 15) == 0) h.s[(t0 + r) * h.nb + j / 16] = scale;
+      }
+    }
   }
 }
 
-__global__ void load_kernel(Held h, __nv_bfloat16* __restrict__ out, long ldo, long T) {
-  const int nvec = h.H / 8;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < T * nvec; i += (long)gridDim.x * blockDim.x) {
-    const long t = i / nvec;
-    const int j = (int)(i - t * nvec);
-    float f[8];
-    restore(*reinterpret_cast<const uint2*>(h.q + i * 8), h.s[t * h.nb + j / 16], f);
-    *reinterpret_cast<uint4*>(out + t * ldo + j * 8) = pack8(f);
+__global__ void __launch_bounds__(256) load_kernel(Held h, __nv_bfloat16* __restrict__ out, long ldo, long T) {
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  if (j * 8 >= h.H) return;
+  for (long t0 = (long)blockIdx.y * kLoadRows; t0 < T; t0 += (long)gridDim.y * kLoadRows) {
+    uint2 q[kLoadRows];
+    float s[kLoadRows];
+#pragma unroll
+    for (int r = 0; r < kLoadRows; ++r)
+      if (t0 + r < T) {
+        q[r] = __ldg(reinterpret_cast<const uint2*>(h.q + (t0 + r) * h.H) + j);
+        s[r] = __ldg(h.s + (t0 + r) * h.nb + j / 16);
+      }
+#pragma unroll
+    for (int r = 0; r < kLoadRows; ++r)
+      if (t0 + r < T) {
+        uint64_t f[4];
+        restore(q[r], s[r], f);
+        reinterpret_cast<uint4*>(out + (t0 + r) * ldo)[j] = pack8(f);
+      }
   }
 }
 
 // ------------------------------------------------------------------- RMSNorm
-template <int THREADS>
+// One block per row, blockDim.x * VPT vectors (H <= 8192); the row stays in registers.
 KORE_DEV float block_sum(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
-  __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
   float t = 0.f;
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) t += red[i];
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) t += red[i];
   return t;
 }
 
 // hn = x rstd w and the 8-bit copy of x, one read of x
-template <int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS) norm_save_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
-                                                            const __nv_bfloat16* __restrict__ w,
-                                                            __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
-                                                            Held h, long T, float eps) {
-  __shared__ float red[THREADS / 32];
+// (5 blocks of 256 threads: 48 registers; 16384 x 5120: 69 us, 74 with 62 registers)
+template <int VPT>
+__global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
+                                                        const __nv_bfloat16* __restrict__ w,
+                                                        __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
+                                                        Held h, float eps) {
+  __shared__ float red[8];
   const int nvec = h.H / 8;
-  for (long t = blockIdx.x; t < T; t += gridDim.x) {
-    uint4 raw[VPT];
-    float ss = 0.f;
+  const long t = blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  uint4 raw[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = threadIdx.x + i * THREADS;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (j < nvec) raw[i] = *reinterpret_cast<const uint4*>(x + t * ldx + j * 8);
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (j < nvec) raw[i] = __ldg(reinterpret_cast<const uint4*>(x + t * ldx) + j);
+  }
+  uint64_t ss = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    uint64_t f[4];
+    unpack8(raw[i], f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss = f2_fma(f[e], f[e], ss);
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    float scale;
+    const uint2 q = quantise(raw[i], scale);
+    if (j < nvec) {
+      reinterpret_cast<uint2*>(h.q + t * h.H)[j] = q;
+      if ((j & 15) == 0) h.s[t * h.nb + j / 16] = scale;
     }
+  }
+  const float rs = rsqrtf(block_sum(sum_pair(ss), red) / h.H + eps);
+  const uint64_t rs2 = f2_pack(rs, rs);
+  if (threadIdx.x == 0) rstd[t] = rs;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = threadIdx.x + i * THREADS;
-      float f[8], scale;
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    if (j < nvec) {
+      uint64_t f[4], g[4];
       unpack8(raw[i], f);
+      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
-      const uint2 q = quantise(raw[i], scale);
-      if (j < nvec) *reinterpret_cast<uint2*>(h.q + t * h.H + j * 8) = q;
-      if (j < nvec && (j & 15) == 0) h.s[t * h.nb + j / 16] = scale;
-    }
-    const float rs = rsqrtf(block_sum<THREADS>(ss, red) / h.H + eps);
-    if (threadIdx.x == 0) rstd[t] = rs;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = threadIdx.x + i * THREADS;
-      if (j < nvec) {
-        float f[8], g[8];
-        unpack8(raw[i], f);
-        unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f[e] * rs * g[e];
-        *reinterpret_cast<uint4*>(hn + t * h.H + j * 8) = pack8(f);
-      }
+      for (int e = 0; e < 4; ++e) f[e] = f2_mul(f2_mul(f[e], rs2), g[e]);
+      reinterpret_cast<uint4*>(hn + t * h.H)[j] = pack8(f);
     }
   }
 }
 
 // x back from 8 bits (bf16), and its RMSNorm from the unrounded values
-template <int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS) norm_load_kernel(Held h, const __nv_bfloat16* __restrict__ w,
-                                                            __nv_bfloat16* __restrict__ x,
-                                                            __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
-                                                            long T, float eps) {
-  __shared__ float red[THREADS / 32];
+template <int VPT>
+__global__ void __launch_bounds__(256) norm_load_kernel(Held h, const __nv_bfloat16* __restrict__ w,
+                                                        __nv_bfloat16* __restrict__ x,
+                                                        __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
+                                                        float eps) {
+  __shared__ float red[8];
   const int nvec = h.H / 8;
-  for (long t = blockIdx.x; t < T; t += gridDim.x) {
-    float f[VPT][8];
-    float ss = 0.f;
+  const long t = blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  uint2 q[VPT];
+  float s[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = threadIdx.x + i * THREADS;
-      if (j < nvec) {
-        restore(*reinterpret_cast<const uint2*>(h.q + t * h.H + j * 8), h.s[t * h.nb + j / 16], f[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
-        *reinterpret_cast<uint4*>(x + t * h.H + j * 8) = pack8(f[i]);
-      }
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    q[i] = make_uint2(0, 0);
+    s[i] = 0.f;
+    if (j < nvec) {
+      q[i] = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H) + j);
+      s[i] = __ldg(h.s + t * h.nb + j / 16);
     }
-    const float rs = rsqrtf(block_sum<THREADS>(ss, red) / h.H + eps);
-    if (threadIdx.x == 0) rstd[t] = rs;
+  }
+  uint64_t ss = 0;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = threadIdx.x + i * THREADS;
-      if (j < nvec) {
-        float g[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    uint64_t f[4];
+    restore(q[i], s[i], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = f[i][e] * rs * g[e];
-        *reinterpret_cast<uint4*>(hn + t * h.H + j * 8) = pack8(g);
-      }
+    for (int e = 0; e < 4; ++e) ss = f2_fma(f[e], f[e], ss);
+    if (j < nvec) reinterpret_cast<uint4*>(x + t * h.H)[j] = pack8(f);
+  }
+  const float rs = rsqrtf(block_sum(sum_pair(ss), red) / h.H + eps);
+  const uint64_t rs2 = f2_pack(rs, rs);
+  if (threadIdx.x == 0) rstd[t] = rs;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    if (j < nvec) {
+      uint64_t f[4], g[4];
+      restore(q[i], s[i], f);
+      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = f2_mul(f2_mul(f[e], rs2), g[e]);
+      reinterpret_cast<uint4*>(hn + t * h.H)[j] = pack8(f);
     }
   }
 }
 
 // -------------------------------------------------------------------- SwiGLU
 //   a = silu(gate) up;  dgate = d up sg (1 + gate (1 - sg)),  dup = d gate sg,  sg = sigmoid(gate)
-KORE_DEV float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+constexpr int kGluRows = 2;   // forward; the backward takes one row at a time
 
-// F % 128 == 0: a block lies wholly in gate or in up, and one half warp takes
-// the block of gate and the block of up of the same columns
-__global__ void swiglu_save_kernel(const __nv_bfloat16* __restrict__ gu, long ldg, __nv_bfloat16* __restrict__ a,
-                                   Held h, long T) {
-  const int F = h.H / 2, fb = F / kBlock;
-  const long total = T * fb;
-  const int sub = threadIdx.x & 15;
-  for (long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) / 16; i - ((threadIdx.x >> 4) & 1) < total;
-       i += (long)gridDim.x * blockDim.x / 16) {
-    const long t = i / fb;
-    const int b = (int)(i - t * fb);
-    const int col = b * kBlock + sub * 8;
-    const bool live = i < total;
-    uint4 g = make_uint4(0, 0, 0, 0), u = g;
-    if (live) {
-      g = *reinterpret_cast<const uint4*>(gu + t * ldg + col);
-      u = *reinterpret_cast<const uint4*>(gu + t * ldg + F + col);
-    }
-    float sg, su;
-    const uint2 qg = quantise(g, sg), qu = quantise(u, su);
-    float gf[8], uf[8];
-    unpack8(g, gf);
-    unpack8(u, uf);
+KORE_DEV uint64_t sigmoid(uint64_t x) {
+  float lo, hi;
+  f2_unpack(x, lo, hi);
+  return f2_pack(1.f / (1.f + __expf(-lo)), 1.f / (1.f + __expf(-hi)));
+}
+
+// HOLD (F % 128 == 0, so that a block lies wholly in gate or in up): also
+// writes the 8-bit copy
+template <bool HOLD>
+__global__ void __launch_bounds__(256) swiglu_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
+                                                     __nv_bfloat16* __restrict__ a, Held h, long T) {
+  const int F = h.H / 2;
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  const bool live = j * 8 < F;
+  pdl_wait();
+  pdl_trigger();
+  for (long t0 = (long)blockIdx.y * kGluRows; t0 < T; t0 += (long)gridDim.y * kGluRows) {
+    uint4 g[kGluRows], u[kGluRows];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gf[e] = gf[e] * sigmoid(gf[e]) * uf[e];
-    if (live) {
-      *reinterpret_cast<uint4*>(a + t * F + col) = pack8(gf);
-      *reinterpret_cast<uint2*>(h.q + t * h.H + col) = qg;
-      *reinterpret_cast<uint2*>(h.q + t * h.H + F + col) = qu;
-      if (sub == 0) {
-        h.s[t * h.nb + b] = sg;
-        h.s[t * h.nb + fb + b] = su;
+    for (int r = 0; r < kGluRows; ++r) {
+      g[r] = u[r] = make_uint4(0, 0, 0, 0);
+      if (live && t0 + r < T) {
+        g[r] = __ldg(reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg) + j);
+        u[r] = __ldg(reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg + F) + j);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kGluRows; ++r) {
+      const long t = t0 + r;
+      const bool ok = live && t < T;
+      uint64_t gf[4], uf[4];
+      unpack8(g[r], gf);
+      unpack8(u[r], uf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) gf[e] = f2_mul(f2_mul(gf[e], sigmoid(gf[e])), uf[e]);
+      if (ok) reinterpret_cast<uint4*>(a + t * F)[j] = pack8(gf);
+      if (HOLD) {
+        float sg, su;
+        const uint2 qg = quantise(g[r], sg), qu = quantise(u[r], su);
+        if (ok) {
+          reinterpret_cast<uint2*>(h.q + t * h.H)[j] = qg;
+          reinterpret_cast<uint2*>(h.q + t * h.H + F)[j] = qu;
+          if ((j & 15) == 0) {
+            h.s[t * h.nb + j / 16] = sg;
+            h.s[t * h.nb + (F / 8 + j) / 16] = su;
+          }
+        }
       }
     }
   }
 }
 
-__global__ void swiglu_kernel(const __nv_bfloat16* __restrict__ gu, long ldg, __nv_bfloat16* __restrict__ a, int F,
-                              long T) {
-  const int nvec = F / 8;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < T * nvec; i += (long)gridDim.x * blockDim.x) {
-    const long t = i / nvec;
-    const int j = (int)(i - t * nvec) * 8;
-    float gf[8], uf[8];
-    unpack8(*reinterpret_cast<const uint4*>(gu + t * ldg + j), gf);
-    unpack8(*reinterpret_cast<const uint4*>(gu + t * ldg + F + j), uf);
+__global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bfloat16* __restrict__ dout, long ldd,
+                                                         __nv_bfloat16* __restrict__ dgu,
+                                                         __nv_bfloat16* __restrict__ a, long T) {
+  const int F = h.H / 2;
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  if (j * 8 >= F) return;
+  for (long t = blockIdx.y; t < T; t += gridDim.y) {
+    const uint2 qg = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H) + j);
+    const uint2 qu = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H + F) + j);
+    const uint4 dv = __ldg(reinterpret_cast<const uint4*>(dout + t * ldd) + j);
+    const float sg = __ldg(h.s + t * h.nb + j / 16), su = __ldg(h.s + t * h.nb + (F / 8 + j) / 16);
+    uint64_t g[4], u[4], d[4], dg[4];
+    restore(qg, sg, g);
+    restore(qu, su, u);
+    unpack8(dv, d);
+    const uint64_t one = f2_pack(1.f, 1.f), neg = f2_pack(-1.f, -1.f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gf[e] = gf[e] * sigmoid(gf[e]) * uf[e];
-    *reinterpret_cast<uint4*>(a + t * F + j) = pack8(gf);
-  }
-}
-
-__global__ void swiglu_bwd_kernel(Held h, const __nv_bfloat16* __restrict__ dout, long ldd,
-                                  __nv_bfloat16* __restrict__ dgu, __nv_bfloat16* __restrict__ a, long T) {
-  const int F = h.H / 2, nvec = F / 8;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < T * nvec; i += (long)gridDim.x * blockDim.x) {
-    const long t = i / nvec;
-    const int j = (int)(i - t * nvec) * 8;
-    float g[8], u[8], d[8], dg[8];
-    restore(*reinterpret_cast<const uint2*>(h.q + t * h.H + j), h.s[t * h.nb + j / kBlock], g);
-    restore(*reinterpret_cast<const uint2*>(h.q + t * h.H + F + j), h.s[t * h.nb + (F + j) / kBlock], u);
-    unpack8(*reinterpret_cast<const uint4*>(dout + t * ldd + j), d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float sg = sigmoid(g[e]), act = g[e] * sg;
-      dg[e] = d[e] * u[e] * (sg + act * (1.f - sg));
-      u[e] = act * u[e];   // the activation again
-      d[e] = d[e] * act;   // dup
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t s = sigmoid(g[e]), act = f2_mul(g[e], s);
+      dg[e] = f2_mul(f2_mul(d[e], u[e]), f2_fma(act, f2_fma(s, neg, one), s));
+      u[e] = f2_mul(act, u[e]);   // the activation again
+      d[e] = f2_mul(d[e], act);   // dup
     }
-    *reinterpret_cast<uint4*>(dgu + t * h.H + j) = pack8(dg);
-    *reinterpret_cast<uint4*>(dgu + t * h.H + F + j) = pack8(d);
-    *reinterpret_cast<uint4*>(a + t * F + j) = pack8(u);
+    reinterpret_cast<uint4*>(dgu + t * h.H)[j] = pack8(dg);
+    reinterpret_cast<uint4*>(dgu + t * h.H + F)[j] = pack8(d);
+    reinterpret_cast<uint4*>(a + t * F)[j] = pack8(u);
   }
 }
 
@@ -302,41 +375,64 @@ void check_bf16(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1 &&
                   (t.size(0) <= 1 || t.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               "act8: ", name, " must be a 2-D bf16 CUDA tensor with contiguous 16-byte aligned rows");
+  TORCH_CHECK(t.size(1) >= 8 && t.size(1) % 8 == 0, "act8: the width of ", name, " must be a positive multiple of 8");
 }
 
-void check_out(const at::Tensor& t, const at::Tensor& like, int64_t T, int64_t H, const char* name) {
-  check_bf16(t, name);
-  TORCH_CHECK(t.device() == like.device() && t.size(0) == T && t.size(1) == H && t.is_contiguous(), "act8: ", name,
-              " must be contiguous [T, H]");
+Held held_of(const at::Tensor& q, const at::Tensor& s) {
+  Held h;
+  h.q = q.data_ptr<int8_t>();
+  h.s = s.data_ptr<float>();
+  h.H = (int)q.size(1);
+  h.nb = (int)s.size(1);
+  return h;
 }
 
 Held check_held(const at::Tensor& q, const at::Tensor& s) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kChar && q.dim() == 2 && q.is_contiguous() &&
                   q.size(1) >= 8 && q.size(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               "act8: q must be contiguous int8 [T, H], H a multiple of 8");
-  const int64_t nb = (q.size(1) + kBlock - 1) / kBlock;
   TORCH_CHECK(s.device() == q.device() && s.scalar_type() == at::kFloat && s.dim() == 2 && s.is_contiguous() &&
-                  s.size(0) == q.size(0) && s.size(1) == nb,
+                  s.size(0) == q.size(0) && s.size(1) == (q.size(1) + kBlock - 1) / kBlock,
               "act8: scales must be contiguous fp32 [T, ceil(H / 128)]");
-  Held h;
-  h.q = q.data_ptr<int8_t>();
-  h.s = s.data_ptr<float>();
-  h.H = (int)q.size(1);
-  h.nb = (int)nb;
-  return h;
+  return held_of(q, s);
 }
 
-void check_vec(const at::Tensor& t, const at::Tensor& like, int64_t n, at::ScalarType dt, const char* name) {
-  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == dt && t.dim() == 1 && t.is_contiguous() &&
-                  t.size(0) == n && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              "act8: ", name, " has the wrong type or length");
+void check_weight(const at::Tensor& w, const at::Tensor& like, int64_t H) {
+  TORCH_CHECK(H <= kMaxNorm, "act8: RMSNorm rows hold at most 8192 columns");
+  TORCH_CHECK(w.device() == like.device() && w.scalar_type() == at::kBFloat16 && w.dim() == 1 && w.is_contiguous() &&
+                  w.size(0) == H && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
+              "act8: w must be contiguous bf16 [H] on 16 bytes");
+}
+
+std::pair<at::Tensor, at::Tensor> new_held(int64_t T, int64_t H, const at::Tensor& like) {
+  return {at::empty({T, H}, like.options().dtype(at::kChar)),
+          at::empty({T, (H + kBlock - 1) / kBlock}, like.options().dtype(at::kFloat))};
 }
 
 long stride_of(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-int grid_for(long threads, int dev) {
-  return (int)std::max<long>(1, std::min<long>((threads + 255) / 256, (long)num_sms(dev) * 8));
+// Element-wise launch over nvec vectors by T rows, `rows` rows per thread and
+// step: the block width that leaves the fewest idle lanes at the row's end, and
+// about 8 blocks of 256 threads per SM in all.
+struct Shape {
+  dim3 grid;
+  int threads;
+};
+Shape shape_for(int nvec, long T, int rows, int dev) {
+  int best = 32, idle = -1;
+  for (int th = 256; th >= 64; th -= 32) {
+    const int waste = (nvec + th - 1) / th * th - nvec;
+    if (idle < 0 || waste < idle) { idle = waste; best = th; }
+  }
+  if (nvec <= 32) best = 32;
+  const int gx = (nvec + best - 1) / best;
+  const long resident = (long)num_sms(dev) * (2048 / best);
+  const long gy = std::min<long>((T + rows - 1) / rows, std::max<long>(1, resident / gx));
+  return {dim3(gx, (unsigned)std::min<long>(gy, 65535)), best};
 }
+
+// vectors per thread: 4 for wide rows (a row in 64 to 256 threads), else 1
+int norm_vpt(int nvec) { return nvec > 128 ? 4 : 1; }
 
 }  // namespace act8
 
@@ -348,9 +444,9 @@ void act8_save(const at::Tensor& x, at::Tensor& q, at::Tensor& s) {
   const long T = x.size(0);
   if (T == 0) return;
   c10::cuda::CUDAGuard g(x.device());
-  save_kernel<<<grid_for(T * h.nb * 16, x.get_device()), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      (const __nv_bfloat16*)x.data_ptr(), stride_of(x), h, T);
-  check_cuda(cudaGetLastError(), "act8_save");
+  const Shape sh = shape_for(h.H / 8, T, kSaveRows, x.get_device());
+  launch_after("act8_save", save_kernel, sh.grid, dim3(sh.threads), 0, at::cuda::getCurrentCUDAStream(),
+               (const __nv_bfloat16*)x.data_ptr(), stride_of(x), h, T);
 }
 
 void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out) {
@@ -362,109 +458,99 @@ void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out) {
   const long T = q.size(0);
   if (T == 0) return;
   c10::cuda::CUDAGuard g(q.device());
-  load_kernel<<<grid_for(T * h.H / 8, q.get_device()), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      h, (__nv_bfloat16*)out.data_ptr(), stride_of(out), T);
-  check_cuda(cudaGetLastError(), "act8_load");
+  const Shape sh = shape_for(h.H / 8, T, kLoadRows, q.get_device());
+  launch_after("act8_load", load_kernel, sh.grid, dim3(sh.threads), 0, at::cuda::getCurrentCUDAStream(), h,
+               (__nv_bfloat16*)out.data_ptr(), stride_of(out), T);
 }
 
-#define KORE_ACT8_NORM(LAUNCH)                \
-  if (nvec <= 128) { LAUNCH(128, 1); }        \
-  else if (nvec <= 256) { LAUNCH(256, 1); }   \
-  else if (nvec <= 512) { LAUNCH(256, 2); }   \
-  else if (nvec <= 768) { LAUNCH(256, 3); }   \
-  else { LAUNCH(256, 4); }
-
-void act8_rmsnorm_save(const at::Tensor& x, const at::Tensor& w, at::Tensor& hn, at::Tensor& rstd, at::Tensor& q,
-                       at::Tensor& s, double eps) {
+// Returns (hn, rstd, q, scales).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_save(const at::Tensor& x,
+                                                                             const at::Tensor& w, double eps) {
   using namespace act8;
   check_bf16(x, "x");
-  Held h = check_held(q, s);
   const long T = x.size(0);
-  TORCH_CHECK(q.device() == x.device() && q.size(0) == T && q.size(1) == x.size(1), "act8: q must match x");
-  TORCH_CHECK(h.H <= kNormVecs * 8, "act8: RMSNorm rows hold at most 8192 columns");
-  check_out(hn, x, T, h.H, "hn");
-  check_vec(w, x, h.H, at::kBFloat16, "w");
-  check_vec(rstd, x, T, at::kFloat, "rstd");
-  if (T == 0) return;
+  const int64_t H = x.size(1);
+  check_weight(w, x, H);
   c10::cuda::CUDAGuard g(x.device());
-  const int nvec = h.H / 8;
+  at::Tensor hn = at::empty({T, H}, x.options()), rstd = at::empty({T}, x.options().dtype(at::kFloat));
+  auto [q, s] = new_held(T, H, x);
+  if (T == 0) return {hn, rstd, q, s};
+  const int nvec = H / 8;
   auto st = at::cuda::getCurrentCUDAStream();
-  const int sms = num_sms(x.get_device());
-#define KORE_LAUNCH(TH, VP)                                                                                  \
-  norm_save_kernel<TH, VP><<<(int)std::min<long>(T, (long)sms * (2048 / TH)), TH, 0, st>>>(                  \
-      (const __nv_bfloat16*)x.data_ptr(), stride_of(x), (const __nv_bfloat16*)w.data_ptr(),                  \
-      (__nv_bfloat16*)hn.data_ptr(), rstd.data_ptr<float>(), h, T, (float)eps)
-  KORE_ACT8_NORM(KORE_LAUNCH)
-#undef KORE_LAUNCH
-  check_cuda(cudaGetLastError(), "act8_rmsnorm_save");
+  const int vpt = norm_vpt(nvec);
+  launch_after("act8_rmsnorm_save", vpt == 4 ? norm_save_kernel<4> : norm_save_kernel<1>, dim3((unsigned)T),
+               dim3(((nvec + vpt - 1) / vpt + 31) / 32 * 32), 0, st, (const __nv_bfloat16*)x.data_ptr(), stride_of(x),
+               (const __nv_bfloat16*)w.data_ptr(), (__nv_bfloat16*)hn.data_ptr(), rstd.data_ptr<float>(),
+               held_of(q, s), (float)eps);
+  return {hn, rstd, q, s};
 }
 
-void act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s, const at::Tensor& w, at::Tensor& x, at::Tensor& hn,
-                       at::Tensor& rstd, double eps) {
+// Returns (x, hn, rstd).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s,
+                                                                 const at::Tensor& w, double eps) {
   using namespace act8;
   Held h = check_held(q, s);
   const long T = q.size(0);
-  TORCH_CHECK(h.H <= kNormVecs * 8, "act8: RMSNorm rows hold at most 8192 columns");
-  check_out(x, q, T, h.H, "x");
-  check_out(hn, q, T, h.H, "hn");
-  check_vec(w, q, h.H, at::kBFloat16, "w");
-  check_vec(rstd, q, T, at::kFloat, "rstd");
-  if (T == 0) return;
+  check_weight(w, q, h.H);
   c10::cuda::CUDAGuard g(q.device());
+  at::Tensor x = at::empty({T, h.H}, w.options()), hn = at::empty({T, h.H}, w.options());
+  at::Tensor rstd = at::empty({T}, s.options());
+  if (T == 0) return {x, hn, rstd};
   const int nvec = h.H / 8;
   auto st = at::cuda::getCurrentCUDAStream();
-  const int sms = num_sms(q.get_device());
-#define KORE_LAUNCH(TH, VP)                                                                                  \
-  norm_load_kernel<TH, VP><<<(int)std::min<long>(T, (long)sms * (2048 / TH)), TH, 0, st>>>(                  \
-      h, (const __nv_bfloat16*)w.data_ptr(), (__nv_bfloat16*)x.data_ptr(), (__nv_bfloat16*)hn.data_ptr(),    \
-      rstd.data_ptr<float>(), T, (float)eps)
-  KORE_ACT8_NORM(KORE_LAUNCH)
-#undef KORE_LAUNCH
-  check_cuda(cudaGetLastError(), "act8_rmsnorm_load");
+  const int vpt = norm_vpt(nvec);
+  launch_after("act8_rmsnorm_load", vpt == 4 ? norm_load_kernel<4> : norm_load_kernel<1>, dim3((unsigned)T),
+               dim3(((nvec + vpt - 1) / vpt + 31) / 32 * 32), 0, st, h, (const __nv_bfloat16*)w.data_ptr(),
+               (__nv_bfloat16*)x.data_ptr(), (__nv_bfloat16*)hn.data_ptr(), rstd.data_ptr<float>(), (float)eps);
+  return {x, hn, rstd};
 }
 
-void act8_swiglu_save(const at::Tensor& gu, at::Tensor& a, at::Tensor& q, at::Tensor& s) {
+// Returns (a, q, scales).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_swiglu_save(const at::Tensor& gu) {
   using namespace act8;
   check_bf16(gu, "gate|up");
-  Held h = check_held(q, s);
   const long T = gu.size(0);
-  TORCH_CHECK(q.device() == gu.device() && q.size(0) == T && q.size(1) == gu.size(1), "act8: q must match gate|up");
-  TORCH_CHECK(h.H % 16 == 0, "act8: SwiGLU's width must be a multiple of 8");
-  const int F = h.H / 2;
-  check_out(a, gu, T, F, "a");
-  if (T == 0) return;
+  const int64_t H = gu.size(1);
+  TORCH_CHECK(H % 16 == 0, "act8: the width of gate|up must be a multiple of 16");
+  const int F = H / 2;
   c10::cuda::CUDAGuard g(gu.device());
+  at::Tensor a = at::empty({T, F}, gu.options());
+  auto [q, s] = new_held(T, H, gu);
+  if (T == 0) return {a, q, s};
   auto st = at::cuda::getCurrentCUDAStream();
   const int dev = gu.get_device();
+  const Held h = held_of(q, s);
   const __nv_bfloat16* gp = (const __nv_bfloat16*)gu.data_ptr();
   __nv_bfloat16* ap = (__nv_bfloat16*)a.data_ptr();
+  const Shape sh = shape_for(F / 8, T, kGluRows, dev);
   if (F % kBlock == 0) {
-    swiglu_save_kernel<<<grid_for(T * (F / 8), dev), 256, 0, st>>>(gp, stride_of(gu), ap, h, T);
+    launch_after("act8_swiglu_save", swiglu_kernel<true>, sh.grid, dim3(sh.threads), 0, st, gp, stride_of(gu), ap, h, T);
   } else {
     // the block at the border holds columns of gate and of up: two passes
-    save_kernel<<<grid_for(T * h.nb * 16, dev), 256, 0, st>>>(gp, stride_of(gu), h, T);
-    swiglu_kernel<<<grid_for(T * (F / 8), dev), 256, 0, st>>>(gp, stride_of(gu), ap, F, T);
+    const Shape ss = shape_for(h.H / 8, T, kSaveRows, dev);
+    launch_after("act8_swiglu_save", save_kernel, ss.grid, dim3(ss.threads), 0, st, gp, stride_of(gu), h, T);
+    launch_after("act8_swiglu_save", swiglu_kernel<false>, sh.grid, dim3(sh.threads), 0, st, gp, stride_of(gu), ap, h, T);
   }
-  check_cuda(cudaGetLastError(), "act8_swiglu_save");
+  return {a, q, s};
 }
 
-void act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s, at::Tensor& dgu,
-                     at::Tensor& a) {
+// Returns (dgate|dup, a).
+std::tuple<at::Tensor, at::Tensor> act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s) {
   using namespace act8;
   check_bf16(dout, "dout");
   Held h = check_held(q, s);
   const long T = q.size(0);
-  TORCH_CHECK(h.H % 16 == 0, "act8: SwiGLU's width must be a multiple of 8");
+  TORCH_CHECK(h.H % 16 == 0, "act8: the width of gate|up must be a multiple of 16");
   const int F = h.H / 2;
   TORCH_CHECK(dout.device() == q.device() && dout.size(0) == T && dout.size(1) == F, "act8: dout must be [T, F]");
-  check_out(dgu, q, T, h.H, "dgu");
-  check_out(a, q, T, F, "a");
-  if (T == 0) return;
   c10::cuda::CUDAGuard g(q.device());
-  swiglu_bwd_kernel<<<grid_for(T * (F / 8), q.get_device()), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      h, (const __nv_bfloat16*)dout.data_ptr(), stride_of(dout), (__nv_bfloat16*)dgu.data_ptr(),
-      (__nv_bfloat16*)a.data_ptr(), T);
-  check_cuda(cudaGetLastError(), "act8_swiglu_bwd");
+  at::Tensor dgu = at::empty({T, h.H}, dout.options()), a = at::empty({T, F}, dout.options());
+  if (T == 0) return {dgu, a};
+  const Shape sh = shape_for(F / 8, T, 1, q.get_device());
+  launch_after("act8_swiglu_bwd", swiglu_bwd_kernel, sh.grid, dim3(sh.threads), 0, at::cuda::getCurrentCUDAStream(), h,
+               (const __nv_bfloat16*)dout.data_ptr(), stride_of(dout), (__nv_bfloat16*)dgu.data_ptr(),
+               (__nv_bfloat16*)a.data_ptr(), T);
+  return {dgu, a};
 }
 
 }  // namespace kore

@@ -112,27 +112,28 @@ void nvls_adamw(int64_t mc_grad, int64_t mc_param, const at::Tensor& own_param,
                 double lr, double b1, double b2, double eps, double wd, int64_t step,
                 const c10::optional<at::Tensor>& sumsq, double max_norm, int64_t seed);
 int64_t device_wait_flag(const at::Tensor& flag, int64_t want, double timeout_s);
-void head_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
-              const c10::optional<at::Tensor>& logp, const c10::optional<at::Tensor>& entropy, at::Tensor& lse);
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, at::Tensor> head_fwd(
+    const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
+    bool want_entropy);
 void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
               const at::Tensor& lse, const at::Tensor& coef, double inv_temp, at::Tensor& dx, at::Tensor& dw,
               bool accumulate, int64_t piece);
-void embed_scaled(const at::Tensor& ids, const at::Tensor& table, at::Tensor& out, double scale);
+at::Tensor embed_scaled(const at::Tensor& ids, const at::Tensor& table, const c10::optional<at::Tensor>& into,
+                        double scale);
 void embed_grad_sorted(const at::Tensor& ids, const at::Tensor& dy, at::Tensor& dtable, double scale,
                        bool accumulate);
-void moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx, const c10::optional<at::Tensor>& mask,
-                     double coef, at::Tensor& loss, at::Tensor& counts, at::Tensor& gain);
-void moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
-                     double dloss, at::Tensor& dlogits, bool accumulate);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx,
+                                                               const c10::optional<at::Tensor>& mask, double coef);
+at::Tensor moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
+                           double dloss, const c10::optional<at::Tensor>& dlogits);
 void act8_save(const at::Tensor& x, at::Tensor& q, at::Tensor& s);
 void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out);
-void act8_rmsnorm_save(const at::Tensor& x, const at::Tensor& w, at::Tensor& hn, at::Tensor& rstd, at::Tensor& q,
-                       at::Tensor& s, double eps);
-void act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s, const at::Tensor& w, at::Tensor& x, at::Tensor& hn,
-                       at::Tensor& rstd, double eps);
-void act8_swiglu_save(const at::Tensor& gu, at::Tensor& a, at::Tensor& q, at::Tensor& s);
-void act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s, at::Tensor& dgu,
-                     at::Tensor& a);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_save(const at::Tensor& x,
+                                                                             const at::Tensor& w, double eps);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s,
+                                                                 const at::Tensor& w, double eps);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_swiglu_save(const at::Tensor& gu);
+std::tuple<at::Tensor, at::Tensor> act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s);
 int read_and_clear_device_error();
 }  // namespace kore
 

@@ -66,6 +66,14 @@ KORE_DEV bool elect_one() {
   return pred != 0;
 }
 
+// ---------------------------------------------------------------- dependent launches
+// A kernel launched with launch_after() may start while the kernel before it in
+// the stream still runs: pdl_wait() returns when that one has finished and its
+// writes are visible, so nothing that it wrote or still reads may be touched
+// earlier. pdl_trigger() lets the next such kernel start once all blocks are here.
+KORE_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+KORE_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier
 KORE_DEV void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));

@@ -15,8 +15,7 @@
 // the accumulator on.
 // Backward: per piece of the vocabulary the same GEMM runs again and its
 // epilogue turns z into dz (bf16, the operand type of the two products that
-// follow: its rounding, at most 2^-8 of a value, is of the size of the rounding
-// of dx and dW themselves); then dW[piece] = dz^T x and dx += dz W[piece] run on the
+// follow; few rows: two bf16 terms); then dW[piece] = dz^T x and dx += dz W[piece] run on the
 // plain GEMM. dW rows are final after their piece (one rounding); dx sums its
 // pieces in fp32 and is rounded once.
 // Rows with coefficient 0 have dz = 0 whatever x or the statistics hold there,
@@ -42,35 +41,69 @@ namespace head {
 
 constexpr int BM = 128;        // rows per CTA (256 per pair)
 constexpr int BK = 64;
-constexpr int kMaxBN = 256;    // vocabulary columns of a pair's tile
-constexpr int kThreads = 192;  // TMA producer, MMA issuer, 4 epilogue warps
-constexpr int kEpiWarps = 4;
-constexpr int kStages = 6;
+constexpr int kMaxBN = 256;    // columns of a pair's tile
+constexpr int kEpiWarps = 8;   // two per TMEM lane quadrant, each takes half of the columns
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // TMA producer, MMA issuer, epilogue
 constexpr int kABytes = BM * BK * 2;
 constexpr int kBBytes = (kMaxBN / 2) * BK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStoreBytes = 32 * 128;  // one store box: 32 rows x 64 bf16
-constexpr int kEpiOff = kStages * kStageBytes;
-constexpr int kBarOff = kEpiOff + kEpiWarps * 2 * kStoreBytes;
-constexpr int kSmem = kBarOff + 256 + 1024;
-constexpr int kRowBlock = 32768;       // rows per forward launch: bounds the statistics workspace
+constexpr int kStoreBytes = 32 * 128;  // one store box: 32 rows x 128 bytes
+// The tensor cores truncate the fp32 accumulator at every 16 products, which
+// biases a long sum towards zero: log-probs were off by 2.6e-6 of themselves at
+// H = 5120, against 0.7e-6 for an fp32 matrix product. The forward therefore
+// reads the accumulator out after each part of K and adds the parts in registers
+// with rounding. A read-out stalls the MMAs by about 1100 clocks (a k-block takes
+// 720). With parts of 8, 12, 16 k-blocks the error was 2.2e-7, 3.3e-7, 4.7e-7 and
+// the time 11.8, 11.0, 10.3 ms (T = 8192, V = 151936); unsplit 10.3 ms. Short
+// sums take a few parts too: 8.6e-7 with one at H = 1024.
+__host__ __device__ constexpr int k_parts(int kblocks) {
+  return kblocks <= 8 ? 1 : kblocks <= 16 ? 2 : kblocks <= 48 ? 3 : (kblocks + 15) / 16;
+}
+// dz is rounded to bf16 for the products that follow: at most 2^-8 of a value,
+// which the sums over many rows and entries average out. With few rows a single
+// rounding shows in a whole row of dW (2.9e-3 of it, against 1.6e-3 from the
+// rounding of the output), and the products are bound by W and dW: up to this
+// many rows dz is kept as the sum of two bf16 terms, which fill otherwise idle
+// rows and k-blocks of the same tiles.
+constexpr int kTwoTerms = 128;
+constexpr int kRowBlock = 32768;  // rows per forward launch: bounds the statistics workspace
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// What a launch does with its tiles of A B^T:
+//   STATS  A = x, B = W piece: row statistics          (columns: vocabulary, K = H)
+//   GRAD   A = x, B = W piece: dz, bf16                (columns: vocabulary, K = H)
+//   DX     A = dz, B = W piece^T: fp32 partials of dx  (columns: H, K = vocabulary, split)
+enum Mode { STATS, GRAD, DX };
+
+template <Mode M>
+struct Layout {
+  static constexpr int kStages = M == STATS ? 7 : 6;
+  static constexpr int kEpiOff = kStages * kStageBytes;
+  static constexpr int kBarOff = kEpiOff + (M == STATS ? 0 : kEpiWarps * kStoreBytes);
+  static constexpr int kSmem = kBarOff + 256 + 1024;
+};
+
 struct Params {
-  int T, V, H;          // rows, columns of this launch's W, contraction
+  int rows, cols, K;    // A rows, B rows (columns of the product), contraction
   int bn;               // columns per tile (multiple of 16, <= 256)
+  const long* targets;  // STATS, GRAD; may be null
   int v0;               // vocabulary id of column 0
-  float scale;          // log2(e) / tau: epilogue works in powers of two
+  float scale;          // log2(e) / tau: the epilogue works in powers of two
   float inv_temp;
-  const long* targets;  // may be null
-  // statistics
-  float* stats;         // [planes][num_n][T]: m, s, (u)
-  float* zt;            // [T] label logit in units of log2
+  // STATS
+  float* stats;         // [planes][2 num_n][rows]: m, s, (u)
+  float* zt;            // [rows] label logit in units of log2
   int entropy;
-  // gradient
+  // GRAD
   const float* lse;
   const float* coef;
+  __nv_bfloat16* low;   // not null: what bf16 leaves of dz goes here, row stride low_ld
+  long low_ld;
+  // DX
+  int splits;           // parts of K; part i is stored at row i * split_rows
+  int split_rows;
+  int add;              // add to the partials of earlier pieces
 };
 
 KORE_DEV float ex2(float x) {
@@ -79,8 +112,16 @@ KORE_DEV float ex2(float x) {
   return y;
 }
 
-// groups of 8 row blocks walk the vocabulary together, so a W tile is read
-// from HBM once per 2048 rows and the group's x rows stay in L2
+KORE_DEV void tma_reduce_add_2d(const CUtensorMap* d, const void* smem_src, int x, int y) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(d)),
+      "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// groups of 8 row blocks walk the columns together, so a B tile is read
+// from HBM once per 2048 rows and the group's A rows stay in L2
 KORE_DEV void tile_coords(int t, int num_m, int num_n, int& tm, int& tn) {
   constexpr int G = 8;
   const int per_group = G * num_n;
@@ -92,13 +133,15 @@ KORE_DEV void tile_coords(int t, int num_m, int num_n, int& tm, int& tn) {
   tn = r / gsize;
 }
 
-template <bool GRAD>
+template <Mode M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    head_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+    head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmD, const Params p) {
+  using L = Layout<M>;
+  constexpr int kStages = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* tfull_bar = empty_bar + kStages;  // [2]
   uint64_t* tempty_bar = tfull_bar + 2;       // [2] (leader: both CTAs' epilogue warps arrive)
@@ -109,10 +152,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
   const int bn = p.bn;
-  const int num_m = (p.T + 2 * BM - 1) / (2 * BM);
-  const int num_n = (p.V + bn - 1) / bn;
-  const int num_tiles = num_m * num_n;
-  const int kblocks = (p.H + BK - 1) / BK;
+  const int num_m = (p.rows + 2 * BM - 1) / (2 * BM);
+  const int num_n = (p.cols + bn - 1) / bn;
+  const int num_mn = num_m * num_n;
+  const int num_tiles = M == DX ? num_mn * p.splits : num_mn;
+  const int kblocks = (p.K + BK - 1) / BK;
+  const int part = (kblocks + k_parts(kblocks) - 1) / k_parts(kblocks);  // STATS: k-blocks per part
+  // k-blocks [k0, k1) of work item t
+  auto k_range = [&](int t, int& k0, int& k1) {
+    k0 = 0;
+    k1 = kblocks;
+    if (M == DX) {
+      const long s = t / num_mn;
+      k0 = (int)(s * kblocks / p.splits);
+      k1 = (int)((s + 1) * kblocks / p.splits);
+    }
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -125,38 +180,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     *abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tmX);
-    tma_prefetch_desc(&tmW);
-    if (GRAD) tma_prefetch_desc(&tmD);
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (M != STATS) tma_prefetch_desc(&tmD);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 2 * kMaxBN);
   tc_fence_before();
   cluster_sync();  // both CTAs' barriers initialised and TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
     if (elect_one()) {
-      const uint32_t b_box = (uint32_t)(bn / 2) * BK * 2;
       int stage = 0;
       uint32_t phase = 0;
       for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
-        int tm, tn;
-        tile_coords(t, num_m, num_n, tm, tn);
+        int tm, tn, k0, k1;
+        tile_coords(t % num_mn, num_m, num_n, tm, tn);
+        k_range(t, k0, k1);
         const int m0 = tm * 2 * BM, n0 = tn * bn;
-        // a box that lies wholly past the rows or the vocabulary is not loaded
+        // a box that lies wholly past the rows or the columns is not loaded
         // (its part of the accumulator is never used)
-        const bool a1 = m0 + BM < p.T, b1 = n0 + bn / 2 < p.V;
-        const uint32_t bytes = kABytes * (a1 ? 2 : 1) + b_box * (b1 ? 2 : 1);
-        const bool load_a = rank == 0 || a1, load_b = rank == 0 || b1;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        auto a_live = [&](int r) { return m0 + r * BM < p.rows; };
+        auto b_bytes = [&](int r) -> uint32_t {
+          const int n = n0 + r * (bn / 2);
+          if (M != DX) return n < p.cols ? (uint32_t)(bn / 2) * BK * 2 : 0u;
+          return (n < p.cols ? 8192u : 0u) + (n + 64 < p.cols ? 8192u : 0u);
+        };
+        const uint32_t bytes = (a_live(0) ? kABytes : 0) + (a_live(1) ? kABytes : 0) + b_bytes(0) + b_bytes(1);
+        const int my_n = n0 + (int)rank * (bn / 2);
+        for (int kb = k0; kb < k1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1)) { *abort_flag = 1; break; }
           uint8_t* sA = smem + stage * kStageBytes;
+          uint8_t* sB = sA + kABytes;
           const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), 0);
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], bytes);
-          if (load_a) tma_load_2d_pair(sA, &tmX, fb, kb * BK, m0 + (int)rank * BM);
-          if (load_b) tma_load_2d_pair(sA + kABytes, &tmW, fb, kb * BK, n0 + (int)rank * (bn / 2));
+          if (a_live((int)rank)) tma_load_2d_pair(sA, &tmA, fb, kb * BK, m0 + (int)rank * BM);
+          if (M != DX) {
+            if (my_n < p.cols) tma_load_2d_pair(sB, &tmB, fb, kb * BK, my_n);
+          } else {  // W piece is [K, columns]: two 64-column boxes
+            if (my_n < p.cols) tma_load_2d_pair(sB, &tmB, fb, my_n, kb * BK);
+            if (my_n + 64 < p.cols) tma_load_2d_pair(sB + 8192, &tmB, fb, my_n + 64, kb * BK);
+          }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
       }
@@ -165,154 +233,221 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader)
     if (rank == 0 && elect_one()) {
-      const uint32_t idesc = make_idesc_bf16(2 * BM, bn, false, false);
+      const uint32_t idesc = make_idesc_bf16(2 * BM, bn, false, M == DX);
       int stage = 0, it = 0;
       uint32_t phase = 0;
-      for (int t = pair; t < num_tiles && !*abort_flag; t += npairs, ++it) {
-        const int acc = it & 1;
-        if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1)) { *abort_flag = 1; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * kMaxBN;
-        bool ok = true;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase)) { ok = false; break; }
+      for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
+        int k0, k1;
+        k_range(t, k0, k1);
+        for (int c0 = k0; c0 < k1; ++it) {
+          const int c1 = M == STATS ? min(c0 + part, k1) : k1;
+          const int acc = it & 1;
+          if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1)) { *abort_flag = 1; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + stage * kStageBytes);
+          const uint32_t d_tmem = tmem_base + acc * kMaxBN;
+          bool ok = true;
+          for (int kb = c0; kb < c1; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + stage * kStageBytes);
+            const uint32_t b_addr = a_addr + kABytes;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            umma_f16_ss_pair(d_tmem, make_sw128_desc(a_addr + k * 32, 16, 1024),
-                             make_sw128_desc(a_addr + kABytes + k * 32, 16, 1024), idesc, (kb | k) != 0);
-          umma_commit_pair(&empty_bar[stage], 0x3);
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+            for (int k = 0; k < BK / 16; ++k)
+              umma_f16_ss_pair(d_tmem, make_sw128_desc(a_addr + k * 32, 16, 1024),
+                               M == DX ? make_sw128_desc(b_addr + k * 2048, 8192, 1024)
+                                       : make_sw128_desc(b_addr + k * 32, 16, 1024),
+                               idesc, kb != c0 || k != 0);
+            umma_commit_pair(&empty_bar[stage], 0x3);
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+          }
+          if (!ok) { *abort_flag = 1; break; }
+          umma_commit_pair(&tfull_bar[acc], 0x3);
+          c0 = c1;
         }
-        if (!ok) { *abort_flag = 1; break; }
-        umma_commit_pair(&tfull_bar[acc], 0x3);
       }
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int q = warp & 3;  // TMEM lane quadrant this warp may access
-    uint8_t* stage_buf = smem + kEpiOff + (warp - 2) * 2 * kStoreBytes;
+    const int q = warp & 3;            // TMEM lane quadrant this warp may access
+    const int half = (warp - 2) / 4;   // and its half of the columns
+    const int width = (bn + 63) / 64 * 32, h0 = half * width;
+    uint8_t* stage_buf = smem + L::kEpiOff + (warp - 2) * kStoreBytes;
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty_bar[0]), 0),
                                        mapa_shared(smem_u32(&tempty_bar[1]), 0)};
-    int buf = 0, it = 0;
-    for (int t = pair; t < num_tiles && !*abort_flag; t += npairs, ++it) {
-      int tm, tn;
-      tile_coords(t, num_m, num_n, tm, tn);
-      const int n0 = tn * bn;
+    int it = 0;
+    for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
+      int tm, tn, k0, k1;
+      tile_coords(t % num_mn, num_m, num_n, tm, tn);
+      k_range(t, k0, k1);
+      if (k0 >= k1) continue;  // a narrow last piece leaves some parts of K empty: nothing was issued
+      const int n0 = tn * bn + h0;
       const int row0 = tm * 2 * BM + (int)rank * BM + q * 32;
       const int row = row0 + lane;
-      const int cols = min(bn, p.V - n0);
-      const int acc = it & 1;
-      const bool live = row < p.T;
-      // column of the label in this tile (outside [0, cols): not here)
+      const int cols = row0 < p.rows ? min(min(width, bn - h0), p.cols - n0) : 0;  // this warp's columns
+      const bool live = row < p.rows;
+      // column of the label among them (negative: not here)
       int tc = -1;
       float lse2 = 0.f, c = 0.f;
-      if (live && p.targets != nullptr) {
+      if (M != DX && live && p.targets != nullptr) {
         const long y = p.targets[row] - p.v0 - n0;
         if (y >= 0 && y < cols) tc = (int)y;
       }
-      if (GRAD && live) {
+      if (M == GRAD && live) {
         lse2 = p.lse[row] * kLog2e;
         c = p.coef[row] * p.inv_temp;
       }
-      if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { *abort_flag = 1; break; }
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kMaxBN;
-      if (!GRAD) {
-        float m = -INFINITY, s = 0.f, u = 0.f;
-        if (row0 < p.T)
-        for (int c0 = 0; c0 < cols; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld32(t_row + c0, r);
-          tmem_wait_ld();
-          if (c0 + 32 > cols) {
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + h0;
+      // hands the accumulator back to the MMA warp
+      auto release = [&](int acc) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty_leader[acc]);
+      };
+      if (M == STATS) {
+        float v[kMaxBN / 2];
+        bool ok = true;
+        for (int c0 = k0; c0 < k1; c0 += part, ++it) {
+          const int acc = it & 1;
+          if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { ok = false; break; }
+          tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i >= cols) r[i] = 0xff800000u;  // -inf: not a column of the vocabulary
-          }
-          const int ti = tc - c0;
-          if (ti >= 0 && ti < 32) {
-            float z = 0.f;
+          for (int j = 0; j < kMaxBN / 64; ++j)
+            if (32 * j < cols) {
+              uint32_t r[32];
+              tmem_ld32(t_row + acc * kMaxBN + 32 * j, r);
+              tmem_wait_ld();
+              if (c0 == k0) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i == ti) z = __uint_as_float(r[i]);
-            p.zt[row] = z * p.scale;
-          }
-          float cm = __uint_as_float(r[0]);
+                for (int i = 0; i < 32; ++i) v[32 * j + i] = __uint_as_float(r[i]);
+              } else {
 #pragma unroll
-          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, __uint_as_float(r[i]));
-          const float nm = fmaxf(m, cm * p.scale);
-          const float base = nm == -INFINITY ? 0.f : nm;  // all columns so far -inf: keep their terms 0
-          const float d = m == -INFINITY ? 0.f : m - base;
-          const float corr = ex2(d);
-          u = corr * (u + d * s);
-          s *= corr;
-          m = nm;
-          if (p.entropy) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float zr = fmaf(__uint_as_float(r[i]), p.scale, -base);
-              const float e = ex2(zr);
-              s += e;
-              u += e == 0.f ? 0.f : e * zr;
+                for (int i = 0; i < 32; ++i) v[32 * j + i] += __uint_as_float(r[i]);
+              }
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s += ex2(fmaf(__uint_as_float(r[i]), p.scale, -base));
-          }
+          release(acc);
         }
+        if (!ok) { *abort_flag = 1; break; }
+        float m = -INFINITY, s = 0.f, u = 0.f;
+#pragma unroll
+        for (int j = 0; j < kMaxBN / 64; ++j)
+          if (32 * j < cols) {
+            float* r = v + 32 * j;
+            if (32 * j + 32 > cols) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * j + i >= cols) r[i] = -INFINITY;  // not a column of the vocabulary
+            }
+            const int ti = tc - 32 * j;
+            if (ti >= 0 && ti < 32) {
+              float z = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i == ti) z = r[i];
+              p.zt[row] = z * p.scale;
+            }
+            float cm = r[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) cm = fmaxf(cm, r[i]);
+            const float nm = fmaxf(m, cm * p.scale);
+            const float base = nm == -INFINITY ? 0.f : nm;  // all columns so far -inf: keep their terms 0
+            const float d = m == -INFINITY ? 0.f : m - base;
+            const float corr = ex2(d);
+            u = corr * (u + d * s);
+            s *= corr;
+            m = nm;
+            if (p.entropy) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float zr = fmaf(r[i], p.scale, -base);
+                const float e = ex2(zr);
+                s += e;
+                u += e == 0.f ? 0.f : e * zr;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s += ex2(fmaf(r[i], p.scale, -base));
+            }
+          }
         if (live) {
-          const size_t o = (size_t)tn * p.T + row, plane = (size_t)num_n * p.T;
+          const size_t o = (size_t)(2 * tn + half) * p.rows + row, plane = (size_t)2 * num_n * p.rows;
           p.stats[o] = m;
           p.stats[o + plane] = s;
           if (p.entropy) p.stats[o + 2 * plane] = u;
         }
       } else {
-        if (row0 < p.T)
-        for (int c0 = 0; c0 < cols; c0 += 64) {
-          float v[64];
+        const int acc = it & 1;
+        if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { *abort_flag = 1; break; }
+        ++it;
+        tc_fence_after();
+        constexpr int kBox = M == GRAD ? 64 : 32;  // columns of 128 bytes
+        for (int c0 = 0; c0 < cols; c0 += kBox) {
+          auto store = [&](const uint4 (&out)[8], int y) {
+            if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
+            __syncwarp();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(stage_buf + lane * 128 + ((j ^ (lane & 7)) * 16)) = out[j];
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (M == DX && p.add) tma_reduce_add_2d(&tmD, stage_buf, n0 + c0, y);
+              else tma_store_2d(&tmD, stage_buf, n0 + c0, y);
+              tma_store_commit();
+            }
+          };
+          uint4 out[8];
+          if (M == GRAD) {
+            float f[64];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[32];
+              tmem_ld32(t_row + acc * kMaxBN + c0 + 32 * h, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float e = ex2(fmaf(__uint_as_float(r[i]), p.scale, -lse2));
+                // coefficient 0, or past the piece's last column: 0
+                f[32 * h + i] = c == 0.f || c0 + 32 * h + i >= cols ? 0.f : -c * e;
+              }
+            }
+            const int ti = tc - c0;
+            if (ti >= 0 && ti < 64) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (i == ti) f[i] += c;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              out[j] = make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
+                                  pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7]));
+            store(out, row0);
+            if (p.low != nullptr && live) {
+              __nv_bfloat16* low = p.low + row * p.low_ld + n0 + c0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t w[4] = {out[j].x, out[j].y, out[j].z, out[j].w};
+                uint32_t l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  l[e] = pack_bf16(f[8 * j + 2 * e] - __uint_as_float(w[e] << 16),
+                                   f[8 * j + 2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+                if (c0 + 8 * j < cols) *reinterpret_cast<uint4*>(low + 8 * j) = make_uint4(l[0], l[1], l[2], l[3]);
+              }
+            }
+          } else {
             uint32_t r[32];
-            tmem_ld32(t_row + c0 + 32 * h, r);
+            tmem_ld32(t_row + acc * kMaxBN + c0, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float e = ex2(fmaf(__uint_as_float(r[i]), p.scale, -lse2));
-              // coefficient 0, or past the piece's last column: 0
-              v[32 * h + i] = c == 0.f || c0 + 32 * h + i >= cols ? 0.f : -c * e;
-            }
+            for (int j = 0; j < 8; ++j) out[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            store(out, (t / num_mn) * p.split_rows + row0);
           }
-          const int ti = tc - c0;
-          if (ti >= 0 && ti < 64) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i == ti) v[i] += c;
-          }
-          if (lane == 0) tma_store_wait_read<1>();
-          __syncwarp();
-          uint8_t* sb = stage_buf + buf * kStoreBytes + lane * 128;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(sb + ((j ^ (lane & 7)) * 16)) =
-                make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
-                           pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmD, stage_buf + buf * kStoreBytes, n0 + c0, row0);
-            tma_store_commit();
-          }
-          buf ^= 1;
         }
+        release(acc);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader[acc]);
     }
-    if (GRAD && lane == 0) tma_store_wait_all<0>();
+    if (M != STATS && lane == 0) tma_store_wait_all<0>();
     __syncwarp();
   }
 
@@ -324,29 +459,159 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the tiles' triples of each row: 32 rows per block, 32 threads per row.
+// ---------------------------------------------------------------- few rows
+// One or two rows are bound by reading W once. Fused multiply-adds keep up with
+// that, and start and finish sooner than the tensor-core pipeline (measured, us,
+// this kernel / the 256-row tiles: T = 1, V = 151936, H = 5120: 267 / 300; T = 2:
+// 310 / 300; T = 4: 338 / 300; T = 1, V = 32000, H = 256: 16.5 / 23; T = 4: 19 / 23).
+// A warp takes 4 vocabulary entries at a time, lanes stride H, x stays in
+// shared memory; products and sums are fp32 (two per instruction).
+constexpr int kFew = 2;
+constexpr int kFewThreads = 512;
+constexpr int kFewMaxH = 8192;
+
+KORE_DEV void fold(float& m, float& s, float& u, float m2, float s2, float u2) {
+  // parts (m, s, u); one whose logits are all -inf has m = -inf and s = u = 0 (or NaN)
+  const float nm = fmaxf(m, m2);
+  const float base = nm == -INFINITY ? 0.f : nm;
+  const float d1 = m == -INFINITY ? 0.f : m - base, d2 = m2 == -INFINITY ? 0.f : m2 - base;
+  const float c1 = ex2(d1), c2 = ex2(d2);
+  u = c1 * (u + d1 * s) + c2 * (u2 + d2 * s2);
+  s = c1 * s + c2 * s2;
+  m = nm;
+}
+
+KORE_DEV uint64_t bf2_to_f2(uint32_t v) {
+  return f2_pack(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
+                                                               const __nv_bfloat16* __restrict__ w, long ldw,
+                                                               const Params p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint4* sx = reinterpret_cast<uint4*>(smem_raw);  // [NT][H / 8]
+  __shared__ float s_part[kFewThreads / 32][4][NT][3];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int T = p.rows, V = p.cols, nvec = p.K / 8;
+  pdl_wait();
+  pdl_trigger();
+  for (int i = threadIdx.x; i < NT * nvec; i += kFewThreads) {
+    const int t = i / nvec, j = i - t * nvec;
+    sx[i] = t < T ? reinterpret_cast<const uint4*>(x + t * ldx)[j] : make_uint4(0, 0, 0, 0);
+  }
+  int tgt[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const long y = p.targets != nullptr && t < T ? p.targets[t] : -1;
+    tgt[t] = y >= 0 && y < V ? (int)y : -1;
+  }
+  float m[NT], s[NT], u[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    s[t] = u[t] = 0.f;
+  }
+  __syncthreads();
+  const int warps = kFewThreads / 32;
+  const int mine = (lane >> 4) + 2 * ((lane >> 3) & 1);  // the entry whose sum this lane ends up with
+  for (int r0 = ((int)blockIdx.x * warps + warp) * 4; r0 < V; r0 += (int)gridDim.x * warps * 4) {
+    uint64_t acc[4][NT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[r][t] = 0;
+#pragma unroll 2
+    for (int j = lane; j < nvec; j += 32) {
+      uint4 wv[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        wv[r] = r0 + r < V ? __ldg(reinterpret_cast<const uint4*>(w + (r0 + r) * ldw) + j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint4 xv = sx[t * nvec + j];
+        const uint64_t x0 = bf2_to_f2(xv.x), x1 = bf2_to_f2(xv.y), x2 = bf2_to_f2(xv.z), x3 = bf2_to_f2(xv.w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[r][t] = f2_fma(bf2_to_f2(wv[r].x), x0, acc[r][t]);
+          acc[r][t] = f2_fma(bf2_to_f2(wv[r].y), x1, acc[r][t]);
+          acc[r][t] = f2_fma(bf2_to_f2(wv[r].z), x2, acc[r][t]);
+          acc[r][t] = f2_fma(bf2_to_f2(wv[r].w), x3, acc[r][t]);
+        }
+      }
+    }
+    const int v = r0 + mine;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float z[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float hi;
+        f2_unpack(acc[r][t], z[r], hi);
+        z[r] += hi;
+      }
+      // four sums over 32 lanes: halve the number of sums, then of lanes
+      float a = (lane & 16) ? z[1] : z[0], b = (lane & 16) ? z[3] : z[2];
+      a += __shfl_xor_sync(0xffffffff, (lane & 16) ? z[0] : z[1], 16);
+      b += __shfl_xor_sync(0xffffffff, (lane & 16) ? z[2] : z[3], 16);
+      float c = (lane & 8) ? b : a;
+      c += __shfl_xor_sync(0xffffffff, (lane & 8) ? a : b, 8);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffff, c, o);
+      if (v < V) {
+        c *= p.scale;
+        if (v == tgt[t] && (lane & 7) == 0) p.zt[t] = c;
+        // one more logit: m is its own maximum, s = 1, u = 0 (of a NaN: s = NaN)
+        if (c == -INFINITY) continue;
+        fold(m[t], s[t], u[t], c, c == c ? 1.f : c, 0.f);
+      }
+    }
+  }
+  // the 4 streams of each warp, then the warps
+  if ((lane & 7) == 0)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s_part[warp][mine][t][0] = m[t];
+      s_part[warp][mine][t][1] = s[t];
+      s_part[warp][mine][t][2] = u[t];
+    }
+  __syncthreads();
+  if (warp < NT && warp < T) {  // warp t joins row t: lanes over the 4 * warps streams
+    float fm = -INFINITY, fs = 0.f, fu = 0.f;
+    for (int i = lane; i < 4 * warps; i += 32) {
+      const float* q = s_part[i >> 2][i & 3][warp];
+      fold(fm, fs, fu, q[0], q[1], q[2]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffff, fm, o);
+      const float s2 = __shfl_xor_sync(0xffffffff, fs, o);
+      const float u2 = __shfl_xor_sync(0xffffffff, fu, o);
+      fold(fm, fs, fu, m2, s2, u2);
+    }
+    if (lane == 0) {
+      const size_t o = (size_t)blockIdx.x * T + warp, plane = (size_t)gridDim.x * T;
+      p.stats[o] = fm;
+      p.stats[o + plane] = fs;
+      if (p.entropy) p.stats[o + 2 * plane] = fu;
+    }
+  }
+}
+
+// Joins the parts (half tiles, or blocks of few_rows_kernel) of each row: 32 rows per block, 32 threads per row.
 __global__ void __launch_bounds__(1024) head_join_kernel(
-    const float* __restrict__ stats, const float* __restrict__ zt, const long* __restrict__ targets, int num_n,
+    const float* __restrict__ stats, const float* __restrict__ zt, const long* __restrict__ targets, int parts,
     int T, int V, float* __restrict__ logp, float* __restrict__ ent, float* __restrict__ lse) {
   __shared__ float sm[32][33], ss[32][33], su[32][33];
+  pdl_wait();
   const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + r;
-  const size_t plane = (size_t)num_n * T;
+  const size_t plane = (size_t)parts * T;
   float m = -INFINITY, s = 0.f, u = 0.f;
-  // a part whose logits are all -inf has m = -inf and s = u = 0 (or NaN)
-  auto fold = [&](float m2, float s2, float u2) {
-    const float nm = fmaxf(m, m2);
-    const float base = nm == -INFINITY ? 0.f : nm;
-    const float d1 = m == -INFINITY ? 0.f : m - base, d2 = m2 == -INFINITY ? 0.f : m2 - base;
-    const float c1 = ex2(d1), c2 = ex2(d2);
-    u = c1 * (u + d1 * s) + c2 * (u2 + d2 * s2);
-    s = c1 * s + c2 * s2;
-    m = nm;
-  };
   if (row < T)
-    for (int i = g; i < num_n; i += 32) {
+    for (int i = g; i < parts; i += 32) {
       const size_t o = (size_t)i * T + row;
-      fold(stats[o], stats[o + plane], ent != nullptr ? stats[o + 2 * plane] : 0.f);
+      fold(m, s, u, stats[o], stats[o + plane], ent != nullptr ? stats[o + 2 * plane] : 0.f);
     }
   sm[g][r] = m;
   ss[g][r] = s;
@@ -361,7 +626,7 @@ __global__ void __launch_bounds__(1024) head_join_kernel(
     const float m2 = __shfl_xor_sync(0xffffffff, m, o);
     const float s2 = __shfl_xor_sync(0xffffffff, s, o);
     const float u2 = __shfl_xor_sync(0xffffffff, u, o);
-    fold(m2, s2, u2);
+    fold(m, s, u, m2, s2, u2);
   }
   const int out = blockIdx.x * 32 + g;
   if (r == 0 && out < T) {
@@ -375,9 +640,11 @@ __global__ void __launch_bounds__(1024) head_join_kernel(
   }
 }
 
-// out = x with the rows of coefficient 0 set to zero (8 elements per thread)
+// out = x with the rows of coefficient 0 set to zero, once or twice (8 elements per thread)
 __global__ void mask_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const float* __restrict__ coef,
-                                 __nv_bfloat16* __restrict__ out, int T, int H) {
+                                 __nv_bfloat16* __restrict__ out, int T, int H, int copies) {
+  pdl_wait();
+  pdl_trigger();
   const int nvec = H / 8;
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < (long)T * nvec; i += (long)gridDim.x * blockDim.x) {
     const long t = i / nvec;
@@ -385,47 +652,86 @@ __global__ void mask_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, 
     uint4 v = make_uint4(0, 0, 0, 0);
     if (coef[t] != 0.f) v = *reinterpret_cast<const uint4*>(x + t * ldx + j);
     *reinterpret_cast<uint4*>(out + t * H + j) = v;
+    if (copies == 2) *reinterpret_cast<uint4*>(out + (T + t) * H + j) = v;
   }
 }
 
-__global__ void round_kernel(const float* __restrict__ src, __nv_bfloat16* __restrict__ dst, long ld, int T, int H) {
+// dx = the sum of the K parts (and of dz's two terms, T rows apart), rounded once
+__global__ void sum_parts_kernel(const float* __restrict__ src, int parts, int copies, long part_stride,
+                                 __nv_bfloat16* __restrict__ dst, long ld, int T, int H) {
+  pdl_wait();
+  pdl_trigger();
   const int nvec = H / 8;
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < (long)T * nvec; i += (long)gridDim.x * blockDim.x) {
     const long t = i / nvec;
     const int j = (int)(i - t * nvec) * 8;
-    const float4 a = *reinterpret_cast<const float4*>(src + t * H + j);
-    const float4 b = *reinterpret_cast<const float4*>(src + t * H + j + 4);
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < parts * copies; ++s) {
+      const float* r = src + (s / copies) * part_stride + (s % copies) * (long)T * H + i * 8;
+      const float4 a = *reinterpret_cast<const float4*>(r), b = *reinterpret_cast<const float4*>(r + 4);
+      f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+      f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+    }
     *reinterpret_cast<uint4*>(dst + t * ld + j) =
-        make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
+        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
   }
 }
 
-template <bool GRAD>
-void launch(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& td, const Params& p, int dev,
+template <Mode M>
+void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Params& p, int dev,
             cudaStream_t st) {
   static bool attr_set[64] = {};
   TORCH_CHECK(dev >= 0 && dev < 64, "head: device index");
-  auto k = head_kernel<GRAD>;
+  auto k = head_kernel<M>;
+  constexpr int smem = Layout<M>::kSmem;
   if (!attr_set[dev]) {
-    check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+    check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                "cudaFuncSetAttribute(head smem)");
     attr_set[dev] = true;
   }
-  const long tiles = (long)((p.T + 2 * BM - 1) / (2 * BM)) * ((p.V + p.bn - 1) / p.bn);
+  const long tiles = (long)((p.rows + 2 * BM - 1) / (2 * BM)) * ((p.cols + p.bn - 1) / p.bn) * p.splits;
   const int grid = (int)std::min<long>(2 * tiles, num_sms(dev) & ~1);
-  k<<<grid, kThreads, kSmem, st>>>(tx, tw, td, p);
-  check_cuda(cudaGetLastError(), "head launch");
+  launch_after("head launch", k, dim3(grid), dim3(kThreads), (size_t)smem, st, ta, tb, td, p);
 }
 
-// Tile width of the forward: the pairs of a wave stop together, so the width is
-// the multiple of 16 that leaves the least work in the last wave (ties: wider,
-// which reads x from shared memory less often).
+template <int NT>
+void launch_few(const __nv_bfloat16* x, long ldx, const __nv_bfloat16* w, long ldw, const Params& p, int blocks,
+                int dev, cudaStream_t st) {
+  static bool attr_set[64] = {};
+  TORCH_CHECK(dev >= 0 && dev < 64, "head: device index");
+  auto k = few_rows_kernel<NT>;
+  if (!attr_set[dev]) {
+    check_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, NT * kFewMaxH * 2),
+               "cudaFuncSetAttribute(head few rows smem)");
+    attr_set[dev] = true;
+  }
+  launch_after("head few rows", k, dim3(blocks), dim3(kFewThreads), (size_t)NT * p.K * 2, st, x, ldx, w, ldw, p);
+}
+
+// Parts of dx's contraction (the piece's vocabulary): as many as fill the pairs
+// when T x H has few tiles; each part costs a pass over [T, H] in fp32. In units
+// of one k-block of a tile (0.27 us): 1.5 MB of HBM traffic.
+int pick_splits(long tiles, long kblocks, long dx_elems, int pairs) {
+  int best = 1;
+  double best_cost = -1;
+  for (int s = 1; s <= 32 && s <= (kblocks + 3) / 4; ++s) {
+    const double cost = (double)((tiles * s + pairs - 1) / pairs) * ((kblocks + s - 1) / s) + dx_elems * 8e-6 / 1.5 * s;
+    if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = s; }
+  }
+  return best;
+}
+
+// Tile width of the forward. The pairs of a wave stop together, so a narrower
+// tile can leave less idle in the last wave, but reads x from shared memory and
+// the accumulator out more often: about 68 columns' time per tile (T = 1003,
+// V = 151936, H = 5120: 33 waves of 256 columns 1.33 ms, 40 of 208 1.37 ms; T = 8192:
+// 257 of 256 10.6 ms, 411 of 160 12.0 ms).
 int pick_bn(long num_m, long V, int pairs) {
   int best = 256;
   long best_cost = -1;
   for (int bn = 256; bn >= 128; bn -= 16) {
     const long tiles = num_m * ((V + bn - 1) / bn);
-    const long cost = ((tiles + pairs - 1) / pairs) * bn;
+    const long cost = ((tiles + pairs - 1) / pairs) * (bn + 68);
     if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = bn; }
   }
   return best;
@@ -461,45 +767,54 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 
 }  // namespace head
 
-void head_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
-              const c10::optional<at::Tensor>& logp, const c10::optional<at::Tensor>& entropy, at::Tensor& lse) {
+// Returns (logp if there are targets, entropy if wanted, lse).
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, at::Tensor> head_fwd(
+    const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
+    bool want_entropy) {
   using namespace head;
   check_operands(x, w, targets, inv_temp);
-  check_rows(lse, x, "lse");
-  if (logp) {
-    check_rows(*logp, x, "logp");
-    TORCH_CHECK(targets.has_value(), "head: logp needs targets");
-  }
-  if (entropy) check_rows(*entropy, x, "entropy");
   const int T = x.size(0), V = w.size(0), H = x.size(1);
-  if (T == 0) return;
   c10::cuda::CUDAGuard g(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  at::Tensor lse = at::empty({T}, f32);
+  c10::optional<at::Tensor> logp, entropy;
+  if (targets) logp = at::empty({T}, f32);
+  if (want_entropy) entropy = at::empty({T}, f32);
+  if (T == 0) return {logp, entropy, lse};
   const int dev = x.get_device();
   auto st = at::cuda::getCurrentCUDAStream();
   Params p = {};
-  p.V = V; p.H = H;
-  p.bn = pick_bn((std::min(T, kRowBlock) + 2 * BM - 1) / (2 * BM), V, num_sms(dev) / 2);
+  p.cols = V; p.K = H; p.splits = 1;
   p.scale = (float)(inv_temp * 1.4426950408889634);
   p.inv_temp = (float)inv_temp;
   p.entropy = entropy.has_value();
-  const int num_n = (V + p.bn - 1) / p.bn;
+  const int block = std::min(T, kRowBlock), sms = num_sms(dev);
+  const bool few = T <= kFew && H <= kFewMaxH;
+  p.bn = pick_bn((block + 2 * BM - 1) / (2 * BM), V, sms / 2);
+  const int few_blocks = std::min((V + kFewThreads / 8 - 1) / (kFewThreads / 8), 2 * sms);
+  const int parts = few ? few_blocks : 2 * ((V + p.bn - 1) / p.bn);
+  at::Tensor ws = at::empty({((int64_t)parts * (p.entropy ? 3 : 2) + 1) * block}, f32);
   auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap tw = make_tmap_2d(w.data_ptr(), bf, 2, H, V, row_stride(w), BK, p.bn / 2);
-  at::Tensor ws = at::empty({((int64_t)num_n * (p.entropy ? 3 : 2) + 1) * std::min(T, kRowBlock)},
-                            x.options().dtype(at::kFloat));
   for (int t0 = 0; t0 < T; t0 += kRowBlock) {
-    p.T = std::min(T - t0, kRowBlock);
+    p.rows = std::min(T - t0, kRowBlock);
     p.zt = ws.data_ptr<float>();
-    p.stats = p.zt + p.T;
+    p.stats = p.zt + p.rows;
     p.targets = logp ? targets->data_ptr<long>() + t0 : nullptr;
-    CUtensorMap tx = make_tmap_2d((const __nv_bfloat16*)x.data_ptr() + t0 * row_stride(x), bf, 2, H, p.T,
-                                  row_stride(x), BK, BM);
-    launch<false>(tx, tw, tx, p, dev, st);
-    head_join_kernel<<<(p.T + 31) / 32, 1024, 0, st>>>(
-        p.stats, p.zt, p.targets, num_n, p.T, V, logp ? logp->data_ptr<float>() + t0 : nullptr,
-        entropy ? entropy->data_ptr<float>() + t0 : nullptr, lse.data_ptr<float>() + t0);
-    check_cuda(cudaGetLastError(), "head join");
+    const __nv_bfloat16* xp = (const __nv_bfloat16*)x.data_ptr() + t0 * row_stride(x);
+    if (few) {
+      const __nv_bfloat16* wp = (const __nv_bfloat16*)w.data_ptr();
+      if (T == 1) launch_few<1>(xp, row_stride(x), wp, row_stride(w), p, few_blocks, dev, st);
+      else launch_few<2>(xp, row_stride(x), wp, row_stride(w), p, few_blocks, dev, st);
+    } else {
+      CUtensorMap tw = make_tmap_2d(w.data_ptr(), bf, 2, H, V, row_stride(w), BK, p.bn / 2);
+      CUtensorMap tx = make_tmap_2d(xp, bf, 2, H, p.rows, row_stride(x), BK, BM);
+      launch<STATS>(tx, tw, tx, p, dev, st);
+    }
+    launch_after("head join", head_join_kernel, dim3((p.rows + 31) / 32), dim3(1024), 0, st, p.stats, p.zt, p.targets,
+                 parts, p.rows, V, logp ? logp->data_ptr<float>() + t0 : nullptr,
+                 entropy ? entropy->data_ptr<float>() + t0 : nullptr, lse.data_ptr<float>() + t0);
   }
+  return {logp, entropy, lse};
 }
 
 void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
@@ -533,42 +848,56 @@ void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::
   const int64_t n_pieces = (V + width - 1) / width;
   if (piece == 0) width = ((V + n_pieces - 1) / n_pieces + kMaxBN - 1) / kMaxBN * kMaxBN;
   width = std::min<int64_t>((width + 7) / 8 * 8, ((int64_t)V + 7) / 8 * 8);
-  const bool one = width >= V;
-  at::Tensor dz = at::empty({T, width}, x.options());
-  at::Tensor xm = at::empty({T, H}, x.options());
-  at::Tensor acc = one ? dx : at::empty({T, H}, x.options().dtype(at::kFloat));
+  const int sms = num_sms(dev);
+  // up to kTwoTerms rows dz is held as two bf16 terms, 2 T rows in all
+  const int copies = T <= kTwoTerms ? 2 : 1, R = T * copies, r32 = (R + 31) / 32 * 32;
+  const int splits = pick_splits((long)((R + 2 * BM - 1) / (2 * BM)) * ((H + kMaxBN - 1) / kMaxBN),
+                                 (std::min<int64_t>(width, V) + BK - 1) / BK, (long)R * H, sms / 2);
+  at::Tensor dz = at::empty({R, width}, x.options());
+  at::Tensor xm = at::empty({R, H}, x.options());
+  at::Tensor acc = at::empty({(int64_t)splits * r32, H}, x.options().dtype(at::kFloat));
   const long nvec = (long)T * H / 8;
-  const int grid = (int)std::min<long>((nvec + 255) / 256, (long)num_sms(dev) * 8);
-  mask_rows_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x.data_ptr(), row_stride(x), coef.data_ptr<float>(),
-                                         (__nv_bfloat16*)xm.data_ptr(), T, H);
-  check_cuda(cudaGetLastError(), "head mask rows");
+  const int grid = (int)std::min<long>((nvec + 255) / 256, (long)sms * 8);
+  launch_after("head mask rows", mask_rows_kernel, dim3(grid), dim3(256), 0, st, (const __nv_bfloat16*)x.data_ptr(),
+               row_stride(x), coef.data_ptr<float>(), (__nv_bfloat16*)xm.data_ptr(), T, H, copies);
   auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tx = make_tmap_2d(x.data_ptr(), bf, 2, H, T, row_stride(x), BK, BM);
+  CUtensorMap tacc = make_tmap_2d(acc.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, H, (uint64_t)splits * r32, H, 32,
+                                  32);
   Params p = {};
-  p.T = T; p.H = H;
+  p.rows = T; p.K = H;
   p.bn = kMaxBN;
+  p.splits = 1;
   p.scale = (float)(inv_temp * 1.4426950408889634);
   p.inv_temp = (float)inv_temp;
   p.targets = targets ? targets->data_ptr<long>() : nullptr;
   p.lse = lse.data_ptr<float>();
   p.coef = coef.data_ptr<float>();
+  p.low = copies == 2 ? (__nv_bfloat16*)dz.data_ptr() + (long)T * width : nullptr;
+  p.low_ld = width;
+  Params d = {};
+  d.rows = R; d.cols = H;
+  d.bn = kMaxBN;
+  d.splits = splits;
+  d.split_rows = r32;
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int n = (int)std::min<int64_t>(width, V - v0);
     at::Tensor wp = w.narrow(0, v0, n);
     at::Tensor dwp = dw.narrow(0, v0, n);
-    at::Tensor dzp = dz.narrow(1, 0, n);
-    p.V = n;
+    p.cols = n;
     p.v0 = (int)v0;
     CUtensorMap tw = make_tmap_2d(wp.data_ptr(), bf, 2, H, n, row_stride(w), BK, kMaxBN / 2);
     CUtensorMap td = make_tmap_2d(dz.data_ptr(), bf, 2, (n + 7) / 8 * 8, T, width, 64, 32);
-    launch<true>(tx, tw, td, p, dev, st);
-    gemm_bf16(dzp, xm, dwp, true, true, 1.0, accumulate, c10::nullopt, 0);
-    gemm_bf16(dzp, wp, acc, false, true, 1.0, !one && v0 > 0, c10::nullopt, 0);
+    launch<GRAD>(tx, tw, td, p, dev, st);
+    gemm_bf16(dz.narrow(1, 0, n), xm, dwp, true, true, 1.0, accumulate, c10::nullopt, 0);
+    CUtensorMap tz = make_tmap_2d(dz.data_ptr(), bf, 2, n, R, width, BK, BM);
+    CUtensorMap tk = make_tmap_2d(wp.data_ptr(), bf, 2, H, n, row_stride(w), 64, BK);
+    d.K = n;
+    d.add = v0 > 0;
+    launch<DX>(tz, tk, tacc, d, dev, st);
   }
-  if (!one) {
-    round_kernel<<<grid, 256, 0, st>>>(acc.data_ptr<float>(), (__nv_bfloat16*)dx.data_ptr(), row_stride(dx), T, H);
-    check_cuda(cudaGetLastError(), "head round");
-  }
+  launch_after("head sum parts", sum_parts_kernel, dim3(grid), dim3(256), 0, st, acc.data_ptr<float>(), splits, copies,
+               (long)r32 * H, (__nv_bfloat16*)dx.data_ptr(), row_stride(dx), T, H);
 }
 
 }  // namespace kore

@@ -401,111 +401,173 @@ inline int warps_grid(long n, int warps_per_block = 8) {
 //   dlogits_te = m_t dL p_te (g_e - sum_j g_j p_tj)      through the router's softmax
 // Counts are integers; P sums in fp32 in an order that only T and E fix: a
 // warp's tokens, a block's warps, then the blocks. Masked tokens are not read.
-constexpr int kBalThreads = 256;
+constexpr int kBalUnroll = 4;   // tokens that a warp has in flight
 
-// one warp per token at a time; part: [blocks][E] sums, cnt: [blocks][E + 1] counts and tokens
-__global__ void __launch_bounds__(kBalThreads) balance_part_kernel(
-    const float* __restrict__ probs, const int* __restrict__ idx, const bool* __restrict__ mask, int T, int E, int k,
-    float* __restrict__ part, int* __restrict__ cnt) {
-  __shared__ float s_sum[kBalThreads / 32][kMaxE];
-  __shared__ int s_cnt[kMaxE + 1];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e <= E; e += kBalThreads) s_cnt[e] = 0;
+// Sums of this block's tokens (warps take kBalUnroll consecutive tokens at a
+// time): s_sum [warps][32 NI], s_cnt [E + 1] (counts, then tokens).
+template <int NI>
+KORE_DEV void balance_sums(const float* __restrict__ probs, const int* __restrict__ idx,
+                           const bool* __restrict__ mask, int T, int E, int k, float* s_sum, int* s_cnt) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  pdl_wait();
+  pdl_trigger();
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) s_cnt[e] = 0;
   __syncthreads();
-  float acc[kMaxE / 32];
+  float acc[NI];
 #pragma unroll
-  for (int i = 0; i < kMaxE / 32; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NI; ++i) acc[i] = 0.f;
   int tokens = 0;
-  for (long t = (long)blockIdx.x * (kBalThreads / 32) + warp; t < T; t += (long)gridDim.x * (kBalThreads / 32)) {
-    if (mask != nullptr && !mask[t]) continue;
-    ++tokens;
+  for (long t0 = ((long)blockIdx.x * warps + warp) * kBalUnroll; t0 < T; t0 += (long)gridDim.x * warps * kBalUnroll) {
+    bool live[kBalUnroll];
+    float v[kBalUnroll][NI];
 #pragma unroll
-    for (int i = 0; i < kMaxE / 32; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E) acc[i] += probs[t * E + e];
+    for (int r = 0; r < kBalUnroll; ++r) {
+      live[r] = t0 + r < T && (mask == nullptr || mask[t0 + r]);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        v[r][i] = live[r] && lane + 32 * i < E ? __ldg(probs + (t0 + r) * E + lane + 32 * i) : 0.f;
     }
-    if (lane < k) {
-      const int e = idx[t * k + lane];
-      if (e >= 0 && e < E) atomicAdd(&s_cnt[e], 1);
+    for (int j = lane; j < kBalUnroll * k; j += 32) {
+      const int r = j / k;
+      if (t0 + r < T && (mask == nullptr || mask[t0 + r])) {
+        const int e = idx[t0 * k + j];
+        if (e >= 0 && e < E) atomicAdd(&s_cnt[e], 1);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kBalUnroll; ++r) {
+      tokens += live[r];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i] += v[r][i];
     }
   }
   if (lane == 0) atomicAdd(&s_cnt[E], tokens);
 #pragma unroll
-  for (int i = 0; i < kMaxE / 32; ++i) s_sum[warp][lane + 32 * i] = acc[i];
+  for (int i = 0; i < NI; ++i) s_sum[warp * 32 * NI + lane + 32 * i] = acc[i];
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kBalThreads) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kBalThreads / 32; ++w) v += s_sum[w][e];
-    part[(size_t)blockIdx.x * E + e] = v;
-  }
-  for (int e = threadIdx.x; e <= E; e += kBalThreads) cnt[(size_t)blockIdx.x * (E + 1) + e] = s_cnt[e];
 }
 
-__global__ void __launch_bounds__(kMaxE) balance_join_kernel(const float* __restrict__ part,
-                                                             const int* __restrict__ cnt, int blocks, int E,
-                                                             float coef, float* __restrict__ loss,
-                                                             int* __restrict__ counts, float* __restrict__ gain) {
-  __shared__ float s_red[kMaxE / 32];
-  __shared__ int s_n;
-  const int e = threadIdx.x;
-  if (e == 0) {
-    int n = 0;
-    for (int b = 0; b < blocks; ++b) n += cnt[(size_t)b * (E + 1) + E];
-    s_n = n;
-  }
-  float sum = 0.f;
-  int c = 0;
-  if (e < E)
-    for (int b = 0; b < blocks; ++b) {
-      sum += part[(size_t)b * E + e];
-      c += cnt[(size_t)b * (E + 1) + e];
-    }
-  __syncthreads();
-  const float n = (float)max(s_n, 1);
-  const float g = coef * (float)E * (float)c / (n * n);
+// Loss and gains from expert e's count and sum (thread e < E; all threads take part).
+KORE_DEV void balance_finish(int e, int E, int c, float sum, int n, float coef, float* loss, int* counts, float* gain) {
+  __shared__ float s_red[32];
+  const float nf = (float)max(n, 1);
+  const float g = coef * (float)E * (float)c / (nf * nf);
+  float v = 0.f;
   if (e < E) {
     counts[e] = c;
     gain[e] = g;
+    if (c > 0) v = g * sum;
   }
-  float v = e < E && c > 0 ? g * sum : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
-  if ((e & 31) == 0) s_red[e / 32] = v;
+  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x / 32] = v;
   __syncthreads();
-  if (e == 0) {
-    for (int w = 1; w < kMaxE / 32; ++w) v += s_red[w];
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < (int)blockDim.x / 32; ++w) v += s_red[w];
     *loss = v;
   }
 }
 
-__global__ void __launch_bounds__(kBalThreads) balance_bwd_kernel(const float* __restrict__ probs,
-                                                                  const float* __restrict__ gain,
-                                                                  const bool* __restrict__ mask, int T, int E,
-                                                                  float dloss, int add, float* __restrict__ dlogits) {
+// part: [blocks][E] sums, cnt: [blocks][E + 1] counts and tokens; a launch of
+// one block finishes by itself (part == nullptr).
+template <int NI>
+__global__ void __launch_bounds__(1024) balance_part_kernel(
+    const float* __restrict__ probs, const int* __restrict__ idx, const bool* __restrict__ mask, int T, int E, int k,
+    float* __restrict__ part, int* __restrict__ cnt, float coef, float* __restrict__ loss, int* __restrict__ counts,
+    float* __restrict__ gain) {
+  __shared__ float s_sum[32 * 32 * NI];
+  __shared__ int s_cnt[kMaxE + 1];
+  balance_sums<NI>(probs, idx, mask, T, E, k, s_sum, s_cnt);
+  const int e = threadIdx.x;   // blocks have at least E threads
+  float v = 0.f;
+  if (e < E)
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) v += s_sum[w * 32 * NI + e];
+  if (part == nullptr) {
+    balance_finish(e, E, e < E ? s_cnt[e] : 0, v, s_cnt[E], coef, loss, counts, gain);
+    return;
+  }
+  if (e < E) part[(size_t)blockIdx.x * E + e] = v;
+  if (e <= E) cnt[(size_t)blockIdx.x * (E + 1) + e] = s_cnt[e];
+  if (e == 0 && E >= (int)blockDim.x) cnt[(size_t)blockIdx.x * (E + 1) + E] = s_cnt[E];
+}
+
+// One block: lane groups of E' = E rounded up to a warp each sum every
+// (1024 / E')-th block; the groups are added in order.
+__global__ void __launch_bounds__(1024) balance_join_kernel(const float* __restrict__ part,
+                                                            const int* __restrict__ cnt, int blocks, int E,
+                                                            float coef, float* __restrict__ loss,
+                                                            int* __restrict__ counts, float* __restrict__ gain) {
+  __shared__ float s_sum[1024];
+  __shared__ int s_cnt[1024];
+  __shared__ int s_n;
+  pdl_wait();
+  pdl_trigger();
+  const int wide = (E + 31) / 32 * 32, groups = 1024 / wide;
+  const int g = threadIdx.x / wide, e = threadIdx.x % wide;
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  float sum = 0.f;
+  int c = 0, n = 0;
+  if (g < groups && e < E) {
+#pragma unroll 4
+    for (int b = g; b < blocks; b += groups) {
+      sum += part[(size_t)b * E + e];
+      c += cnt[(size_t)b * (E + 1) + e];
+    }
+  }
+  for (int b = threadIdx.x; b < blocks; b += 1024) n += cnt[(size_t)b * (E + 1) + E];
+  if (n != 0) atomicAdd(&s_n, n);
+  s_sum[threadIdx.x] = sum;
+  s_cnt[threadIdx.x] = c;
+  __syncthreads();
+  sum = 0.f;
+  c = 0;
+  if (threadIdx.x < E)
+    for (int i = 0; i < groups; ++i) {
+      sum += s_sum[i * wide + threadIdx.x];
+      c += s_cnt[i * wide + threadIdx.x];
+    }
+  balance_finish(threadIdx.x, E, c, sum, s_n, coef, loss, counts, gain);
+}
+
+template <int NI>
+__global__ void __launch_bounds__(256) balance_bwd_kernel(const float* __restrict__ probs,
+                                                          const float* __restrict__ gain,
+                                                          const bool* __restrict__ mask, int T, int E, float dloss,
+                                                          int add, float* __restrict__ dlogits) {
   const int lane = threadIdx.x & 31;
-  float g[kMaxE / 32];
+  pdl_wait();
+  pdl_trigger();
+  float g[NI];
 #pragma unroll
-  for (int i = 0; i < kMaxE / 32; ++i) g[i] = lane + 32 * i < E ? gain[lane + 32 * i] * dloss : 0.f;
-  for (long t = (long)blockIdx.x * (kBalThreads / 32) + threadIdx.x / 32; t < T;
-       t += (long)gridDim.x * (kBalThreads / 32)) {
-    const bool live = mask == nullptr || mask[t];
-    if (!live && add) continue;
-    float p[kMaxE / 32], dot = 0.f;
+  for (int i = 0; i < NI; ++i) g[i] = lane + 32 * i < E ? gain[lane + 32 * i] * dloss : 0.f;
+  for (long t0 = ((long)blockIdx.x * 8 + threadIdx.x / 32) * kBalUnroll; t0 < T; t0 += (long)gridDim.x * 8 * kBalUnroll) {
+    bool live[kBalUnroll];
+    float p[kBalUnroll][NI], dot[kBalUnroll];
 #pragma unroll
-    for (int i = 0; i < kMaxE / 32; ++i) {
-      p[i] = live && lane + 32 * i < E ? probs[t * E + lane + 32 * i] : 0.f;
-      dot += p[i] * g[i];
+    for (int r = 0; r < kBalUnroll; ++r) {
+      live[r] = t0 + r < T && (mask == nullptr || mask[t0 + r]);
+      dot[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        p[r][i] = live[r] && lane + 32 * i < E ? __ldg(probs + (t0 + r) * E + lane + 32 * i) : 0.f;
+        dot[r] += p[r][i] * g[i];
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffff, dot, o);
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < kMaxE / 32; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E) {
-        const float d = p[i] * (g[i] - dot);
-        dlogits[t * E + e] = add ? dlogits[t * E + e] + d : d;
-      }
+      for (int r = 0; r < kBalUnroll; ++r) dot[r] += __shfl_xor_sync(0xffffffff, dot[r], o);
+#pragma unroll
+    for (int r = 0; r < kBalUnroll; ++r) {
+      if (t0 + r >= T || (!live[r] && add)) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (lane + 32 * i < E) {
+          float* o = dlogits + (t0 + r) * E + lane + 32 * i;
+          const float d = p[r][i] * (g[i] - dot[r]);
+          *o = add ? *o + d : d;
+        }
     }
   }
 }
@@ -646,56 +708,80 @@ void check_balance(const at::Tensor& probs, const c10::optional<at::Tensor>& mas
                     mask->size(0) == probs.size(0) && mask->is_contiguous(),
                 "balance: mask must be bool [T]");
 }
-void check_balance_vec(const at::Tensor& t, const at::Tensor& probs, at::ScalarType dt, const char* name) {
-  TORCH_CHECK(t.device() == probs.device() && t.scalar_type() == dt && t.dim() == 1 && t.is_contiguous() &&
-                  t.size(0) == probs.size(1),
-              "balance: ", name, " must have one entry per expert");
-}
 }  // namespace
 
-void moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx, const c10::optional<at::Tensor>& mask,
-                     double coef, at::Tensor& loss, at::Tensor& counts, at::Tensor& gain) {
+// E rounded up to 1, 2, 4 or 8 values per lane
+#define KORE_BALANCE_NI(E, LAUNCH) \
+  if (E <= 32) { LAUNCH(1); }      \
+  else if (E <= 64) { LAUNCH(2); } \
+  else if (E <= 128) { LAUNCH(4); } \
+  else { LAUNCH(8); }
+
+// Returns (loss [], counts [E] int32, gain [E]).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_balance_fwd(const at::Tensor& probs, const at::Tensor& idx,
+                                                               const c10::optional<at::Tensor>& mask, double coef) {
   check_balance(probs, mask);
   TORCH_CHECK(idx.device() == probs.device() && idx.scalar_type() == at::kInt && idx.dim() == 2 &&
                   idx.is_contiguous() && idx.size(0) == probs.size(0) && idx.size(1) >= 1 &&
                   idx.size(1) <= moe::kMaxK,
               "balance: idx must be contiguous int32 [T, k], 1 <= k <= 16");
-  check_balance_vec(counts, probs, at::kInt, "counts");
-  check_balance_vec(gain, probs, at::kFloat, "gain");
-  TORCH_CHECK(loss.device() == probs.device() && loss.scalar_type() == at::kFloat && loss.numel() == 1,
-              "balance: loss must be one fp32 value");
   c10::cuda::CUDAGuard g(probs.device());
   const int T = probs.size(0), E = probs.size(1), k = idx.size(1);
-  const int rows = moe::kBalThreads / 32;
-  const int blocks = std::max(1, std::min((T + 4 * rows - 1) / (4 * rows), num_sms(probs.get_device()) * 2));
-  at::Tensor part = at::empty({(int64_t)blocks * (2 * E + 1)}, probs.options());
-  float* sums = part.data_ptr<float>();
-  int* cnt = reinterpret_cast<int*>(sums + (size_t)blocks * E);
+  at::Tensor loss = at::empty({}, probs.options());
+  at::Tensor counts = at::empty({E}, probs.options().dtype(at::kInt));
+  at::Tensor gain = at::empty({E}, probs.options());
   auto st = at::cuda::getCurrentCUDAStream();
-  moe::balance_part_kernel<<<blocks, moe::kBalThreads, 0, st>>>(
-      probs.data_ptr<float>(), idx.data_ptr<int>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, k, sums, cnt);
-  check_cuda(cudaGetLastError(), "balance sums");
-  moe::balance_join_kernel<<<1, moe::kMaxE, 0, st>>>(sums, cnt, blocks, E, (float)coef, loss.data_ptr<float>(),
-                                                     counts.data_ptr<int>(), gain.data_ptr<float>());
-  check_cuda(cudaGetLastError(), "balance join");
+  // one block reads 128 KB in about the time that a second launch takes
+  const bool one = (long)T * E <= 32768;
+  const int threads = one ? 1024 : 256;
+  const int per_block = threads / 32 * moe::kBalUnroll;
+  const int blocks = one ? 1 : std::min((T + per_block - 1) / per_block, num_sms(probs.get_device()));
+  at::Tensor part;
+  float* sums = nullptr;
+  int* cnt = nullptr;
+  if (!one) {
+    part = at::empty({(int64_t)blocks * (2 * E + 1)}, probs.options());
+    sums = part.data_ptr<float>();
+    cnt = reinterpret_cast<int*>(sums + (size_t)blocks * E);
+  }
+#define KORE_LAUNCH(NI)                                                                                            \
+  launch_after("balance sums", moe::balance_part_kernel<NI>, dim3(blocks), dim3(threads), 0, st,                   \
+               probs.data_ptr<float>(), idx.data_ptr<int>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, k, sums, \
+               cnt, (float)coef, loss.data_ptr<float>(), counts.data_ptr<int>(), gain.data_ptr<float>())
+  KORE_BALANCE_NI(E, KORE_LAUNCH)
+#undef KORE_LAUNCH
+  if (!one)
+    launch_after("balance join", moe::balance_join_kernel, dim3(1), dim3(1024), 0, st, sums, cnt, blocks, E, (float)coef,
+                 loss.data_ptr<float>(), counts.data_ptr<int>(), gain.data_ptr<float>());
+  return {loss, counts, gain};
 }
 
-void moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
-                     double dloss, at::Tensor& dlogits, bool accumulate) {
+// Gradient of the logits, added to dlogits when it is given.
+at::Tensor moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
+                           double dloss, const c10::optional<at::Tensor>& dlogits) {
   check_balance(probs, mask);
-  check_balance_vec(gain, probs, at::kFloat, "gain");
-  TORCH_CHECK(dlogits.device() == probs.device() && dlogits.scalar_type() == at::kFloat &&
-                  dlogits.sizes() == probs.sizes() && dlogits.is_contiguous(),
-              "balance: dlogits must be contiguous fp32 [T, E]");
+  TORCH_CHECK(gain.device() == probs.device() && gain.scalar_type() == at::kFloat && gain.dim() == 1 &&
+                  gain.is_contiguous() && gain.size(0) == probs.size(1),
+              "balance: gain must have one entry per expert");
+  if (dlogits)
+    TORCH_CHECK(dlogits->device() == probs.device() && dlogits->scalar_type() == at::kFloat &&
+                    dlogits->sizes() == probs.sizes() && dlogits->is_contiguous(),
+                "balance: dlogits must be contiguous fp32 [T, E]");
   const int T = probs.size(0), E = probs.size(1);
-  if (T == 0) return;
   c10::cuda::CUDAGuard g(probs.device());
-  const int rows = moe::kBalThreads / 32;
+  at::Tensor out = dlogits ? *dlogits : at::empty_like(probs);
+  if (T == 0) return out;
+  const int rows = 8 * moe::kBalUnroll;
   const int blocks = std::min((T + rows - 1) / rows, num_sms(probs.get_device()) * 8);
-  moe::balance_bwd_kernel<<<blocks, moe::kBalThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
-      probs.data_ptr<float>(), gain.data_ptr<float>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, (float)dloss,
-      accumulate ? 1 : 0, dlogits.data_ptr<float>());
-  check_cuda(cudaGetLastError(), "balance_bwd");
+  auto st = at::cuda::getCurrentCUDAStream();
+#define KORE_LAUNCH(NI)                                                                                          \
+  launch_after("balance_bwd", moe::balance_bwd_kernel<NI>, dim3(blocks), dim3(256), 0, st, probs.data_ptr<float>(), \
+               gain.data_ptr<float>(), mask ? mask->data_ptr<bool>() : nullptr, T, E, (float)dloss, dlogits ? 1 : 0, \
+               out.data_ptr<float>())
+  KORE_BALANCE_NI(E, KORE_LAUNCH)
+#undef KORE_LAUNCH
+  return out;
 }
+#undef KORE_BALANCE_NI
 
 }  // namespace kore

@@ -35,6 +35,24 @@ inline void check_cuda(cudaError_t e, const char* what) {
     throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// Launches a kernel that calls pdl_wait() before it touches memory: its launch
+// overlaps the end of the kernel before it in the stream.
+template <typename... P, typename... A>
+void launch_after(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                  A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), what);
+}
+
 // Reads and clears the device-side error word (1 = barrier wait timeout,
 // 2 = peer flag timeout). Synchronizes the current device.
 int read_and_clear_device_error();

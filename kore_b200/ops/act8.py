@@ -92,13 +92,11 @@ def load(a: Act8, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch
 
 def rmsnorm_save(x: torch.Tensor, w: torch.Tensor, eps: float):
     """Forward: (hn = rmsnorm(x) * w, rstd [T] fp32, x in 8 bits), one read of x."""
-    T, H = x.shape
-    hn = torch.empty(T, H, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(T, dtype=torch.float32, device=x.device)
-    a = empty(T, H, x.device)
     if x.is_cuda:
-        native().act8_rmsnorm_save(x, w, hn, rstd, a.q, a.s, float(eps))
-        return hn, rstd, a
+        hn, rstd, q, s = native().act8_rmsnorm_save(x, w, float(eps))
+        return hn, rstd, Act8(q, s)
+    T, H = x.shape
+    hn, rstd, a = torch.empty_like(x), torch.empty(T), empty(T, H, x.device)
     xf = x.float()
     r = torch.rsqrt(xf.pow(2).mean(-1) + eps)
     rstd.copy_(r)
@@ -110,13 +108,10 @@ def rmsnorm_save(x: torch.Tensor, w: torch.Tensor, eps: float):
 def rmsnorm_load(a: Act8, w: torch.Tensor, eps: float):
     """Backward: (x, hn, rstd) again from the 8-bit copy. hn and rstd are those
     of the held values before x's rounding to the weight's type."""
-    T, H = a.shape
-    x = torch.empty(T, H, dtype=w.dtype, device=w.device)
-    hn = torch.empty_like(x)
-    rstd = torch.empty(T, dtype=torch.float32, device=w.device)
     if a.q.is_cuda:
-        native().act8_rmsnorm_load(a.q, a.s, w, x, hn, rstd, float(eps))
-        return x, hn, rstd
+        return native().act8_rmsnorm_load(a.q, a.s, w, float(eps))
+    x = torch.empty(a.shape, dtype=w.dtype)
+    hn, rstd = torch.empty_like(x), torch.empty(x.shape[0])
     v = _values(a)
     r = torch.rsqrt(v.pow(2).mean(-1) + eps)
     rstd.copy_(r)
@@ -130,11 +125,10 @@ def swiglu_save(gu: torch.Tensor):
     T, f2 = gu.shape
     if f2 % 16:
         raise ValueError(f"act8: [gate | up] needs a width that is a multiple of 16, got {f2}")
-    a = torch.empty(T, f2 // 2, dtype=gu.dtype, device=gu.device)
-    held = empty(T, f2, gu.device)
     if gu.is_cuda:
-        native().act8_swiglu_save(gu, a, held.q, held.s)
-        return a, held
+        a, q, s = native().act8_swiglu_save(gu)
+        return a, Act8(q, s)
+    a, held = torch.empty(T, f2 // 2, dtype=gu.dtype), empty(T, f2, gu.device)
     g, u = gu.float().chunk(2, -1)
     a.copy_(F.silu(g) * u)
     _quantise(gu, held)
@@ -145,12 +139,10 @@ def swiglu_bwd(dout: torch.Tensor, held: Act8):
     """Backward from the 8-bit [gate | up]: (d[gate | up] [T, 2 F], the
     activation silu(gate) * up again [T, F], for the down projection's weight
     gradient)."""
-    T, f2 = held.shape
-    dgu = torch.empty(T, f2, dtype=dout.dtype, device=dout.device)
-    a = torch.empty(T, f2 // 2, dtype=dout.dtype, device=dout.device)
     if dout.is_cuda:
-        native().act8_swiglu_bwd(dout, held.q, held.s, dgu, a)
-        return dgu, a
+        return native().act8_swiglu_bwd(dout, held.q, held.s)
+    T, f2 = held.shape
+    dgu, a = torch.empty(T, f2, dtype=dout.dtype), torch.empty(T, f2 // 2, dtype=dout.dtype)
     g, u = _values(held).chunk(2, -1)
     d = dout.float()
     sg = torch.sigmoid(g)

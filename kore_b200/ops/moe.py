@@ -54,13 +54,10 @@ def balance_loss(probs: torch.Tensor, idx: torch.Tensor, mask: Optional[torch.Te
     their probabilities hold; entries of ``idx`` outside [0, E) are not counted.
     Returns (loss [] fp32, counts [E] int32, gain [E] fp32); gain_e = dL/dp_te
     is what ``balance_bwd`` takes. The counts are constants of the gradient."""
-    T, E = probs.shape
-    loss = torch.empty((), dtype=torch.float32, device=probs.device)
-    counts = torch.empty(E, dtype=torch.int32, device=probs.device)
-    gain = torch.empty(E, dtype=torch.float32, device=probs.device)
     if probs.is_cuda:
-        native().moe_balance_fwd(probs, idx, mask, float(coef), loss, counts, gain)
-        return loss, counts, gain
+        return native().moe_balance_fwd(probs, idx, mask, float(coef))
+    T, E = probs.shape
+    loss, counts, gain = torch.empty(()), torch.empty(E, dtype=torch.int32), torch.empty(E)
     keep = torch.ones(T, dtype=torch.bool) if mask is None else mask
     sel = idx[keep].long().reshape(-1)
     counts.copy_(torch.bincount(sel[(sel >= 0) & (sel < E)], minlength=E))
@@ -77,9 +74,7 @@ def balance_bwd(probs: torch.Tensor, gain: torch.Tensor, mask: Optional[torch.Te
     (fp32 [T, E]), added to ``dlogits`` when it is given. Masked tokens get 0
     (with ``dlogits``: are left as they are)."""
     if probs.is_cuda:
-        out = torch.empty_like(probs) if dlogits is None else dlogits
-        native().moe_balance_bwd(probs, gain, mask, float(dloss), out, dlogits is not None)
-        return out
+        return native().moe_balance_bwd(probs, gain, mask, float(dloss), dlogits)
     g = gain * dloss
     d = probs * (g - (probs * g).sum(-1, keepdim=True))
     if mask is not None:

@@ -27,14 +27,13 @@ def head_fwd(x: torch.Tensor, w: torch.Tensor, targets: Optional[torch.Tensor] =
     fp32. The logits are never stored: they go from the fp32 accumulator into
     the rows' running maxima and sums. ``logp`` is 0 where the target is
     outside [0, V) (no label). ``lse`` is what :func:`head_bwd` needs."""
-    T, dev = x.shape[0], x.device
     inv = _inv_temp(temperature)
+    if x.is_cuda:
+        return native().head_fwd(x, w, targets, inv, want_entropy)
+    T, dev = x.shape[0], x.device
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     logp = torch.empty(T, dtype=torch.float32, device=dev) if targets is not None else None
     ent = torch.empty(T, dtype=torch.float32, device=dev) if want_entropy else None
-    if x.is_cuda:
-        native().head_fwd(x, w, targets, inv, logp, ent, lse)
-        return logp, ent, lse
     z = (x.float() @ w.float().t()) * inv
     l = torch.logsumexp(z, -1)
     lse.copy_(l)
@@ -93,11 +92,10 @@ def head_bwd(x: torch.Tensor, w: torch.Tensor, targets: Optional[torch.Tensor], 
 def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None):
     """out[t] = scale * table[ids[t]] (rounded once); ids outside the table give zero rows."""
     flat = ids.reshape(-1)
+    if table.is_cuda:
+        return native().embed_scaled(flat, table, out, float(scale))
     if out is None:
         out = torch.empty(flat.numel(), table.shape[1], dtype=table.dtype, device=table.device)
-    if table.is_cuda:
-        native().embed_scaled(flat, table, out, float(scale))
-        return out
     ok = (flat >= 0) & (flat < table.shape[0])
     rows = table[torch.where(ok, flat, torch.zeros_like(flat))].float() * scale
     out.copy_(torch.where(ok.unsqueeze(1), rows, torch.zeros_like(rows)))
