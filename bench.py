@@ -306,6 +306,18 @@ def dpo_main(args) -> None:
             "impl": "kore"}), flush=True)
 
 
+def step_ops(names: str) -> dict:
+    """CausalLMTrainer arguments of ``--step-ops``."""
+    table = {"pieces": {"head": "pieces"}, "sorted": {"embed_grad": "sorted"}, "act8": {"act8": True},
+             "aux": {"router_aux": True}}
+    out = {}
+    for n in [n for n in names.split(",") if n]:
+        if n not in table:
+            raise SystemExit(f"--step-ops: unknown {n!r} (pieces, sorted, act8, aux)")
+        out.update(table[n])
+    return out
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -335,6 +347,8 @@ def main(argv=None):
                     help="data plane of the sharded optimizer (N > 1)")
     ap.add_argument("--recompute", default="auto", choices=["auto", "full", "none"],
                     help="activation recompute: auto keeps whole layers' contexts while HBM allows")
+    ap.add_argument("--step-ops", default="", help="sft: comma list of pieces (head loss in vocabulary pieces), "
+                    "sorted (embedding gradient), act8 (8-bit activation checkpoints), aux (router balance loss)")
     ap.add_argument("--zero", type=int, default=2, choices=[2, 3],
                     help="2: resident params, sharded grads/optimizer; 3: decoder layers fully sharded")
     args = ap.parse_args(argv)
@@ -367,7 +381,7 @@ def main(argv=None):
     trainer = CausalLMTrainer(cfg, ctx, lr=1e-5, max_grad_norm=1.0, seed=0,
                               micro_batch_size=args.micro_batch,
                               comm=args.comm, zero_stage=args.zero,
-                              recompute=args.recompute)
+                              recompute=args.recompute, **step_ops(args.step_ops))
     B, S = args.seqs_per_gpu, args.seq
     g = torch.Generator().manual_seed(1234 + ctx.rank)
     # a fresh token block every step (cycled over NB distinct blocks)
@@ -451,6 +465,7 @@ def main(argv=None):
                        "loss": "last 50% of each sequence", "micro_batch": args.micro_batch,
                        "optimizer": f"AdamW fp32 moments, master={trainer.master_mode}",
                        "activation_recompute": _recompute_note(trainer, cfg),
+                       **({"step_ops": args.step_ops} if args.step_ops else {}),
                        "l2": "inputs larger than L2 (29.5 GB of weights streamed per step)"},
             "loss": loss_v, "clocks": clocks, "gpu_launches": launches, "e2e": e2e, "memory": memory,
             "impl": "kore",

@@ -294,9 +294,9 @@ KORE_DEV uint64_t sigmoid(uint64_t x) {
 }
 
 // HOLD (F % 128 == 0, so that a block lies wholly in gate or in up): also
-// writes the 8-bit copy
+// writes the 8-bit copy (4 blocks of 256 threads per SM: 193 us at 8192 x 17408, 211 without)
 template <bool HOLD>
-__global__ void __launch_bounds__(256) swiglu_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
+__global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
                                                      __nv_bfloat16* __restrict__ a, Held h, long T) {
   const int F = h.H / 2;
   const int j = blockIdx.x * blockDim.x + threadIdx.x;

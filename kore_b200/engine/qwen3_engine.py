@@ -17,6 +17,18 @@ Losses are expressed through per-token coefficients c_t = dL/dlogp_t:
 SFT/midtrain pass them up front (one pass); GRPO/DPO pass a callable that
 maps the micro-batch's token log-probs to coefficients (two-phase head).
 
+Options of the step (defaults leave it as described above):
+
+  head="pieces"       the head runs in pieces of the vocabulary without logits
+                      (ops.vocab): fp32 log-probs, dW written once
+  embed_grad="sorted" the embedding gradient sums each token's rows in fp32 in
+                      a fixed order instead of with bf16 atomics
+  act8=True           layer inputs, and the contexts of layers that skip the
+                      recompute, are kept in 8 bits (ops.act8): about a third of
+                      a bf16 context, so three times the layers keep theirs
+  router_aux_coef     load-balancing loss of the MoE routers (mean over the MoE
+                      layers and the step's micro-batches), with expert counts
+
 Reference parity: the step the reference runs inside HF Trainer / TRL
 (kore/policy/sft.py:346-399, kore/policy/dpo.py:237-364) and its per-sample
 GRPO backward (kore/policy/grpo.py:613-701).
@@ -31,8 +43,10 @@ import torch
 
 from .. import ops
 from ..models.qwen3 import Qwen3Weights
+from ..ops import act8 as a8
 from ..ops import attention as attn
 from ..ops import reference as ref
+from ..ops import vocab
 
 
 @dataclass
@@ -102,7 +116,16 @@ class Qwen3Engine:
 
     def __init__(self, weights: Qwen3Weights, *, grad_dtype: Optional[torch.dtype] = None,
                  logits_chunk: int = 4096, temperature: float = 1.0, allocate_grads: bool = True,
-                 save_attention: bool = True, grad_alloc=None):
+                 save_attention: bool = True, grad_alloc=None, head: str = "chunks",
+                 embed_grad: str = "atomic", act8: bool = False, router_aux_coef: float = 0.0):
+        if head not in ("chunks", "pieces"):
+            raise ValueError("head must be chunks|pieces")
+        if embed_grad not in ("atomic", "sorted"):
+            raise ValueError("embed_grad must be atomic|sorted")
+        if router_aux_coef < 0:
+            raise ValueError("router_aux_coef must not be negative")
+        self.head, self.embed_grad, self.act8 = head, embed_grad, bool(act8)
+        self.router_aux_coef = float(router_aux_coef)
         self.w = weights
         self.cfg = weights.cfg
         self.dev = weights.device
@@ -122,6 +145,12 @@ class Qwen3Engine:
         c = self.cfg
         self.hq, self.hkv, self.D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
         self.eps = c.rms_norm_eps
+        self.moe_layers = sum(c.layer_is_moe(i) for i in range(c.num_hidden_layers))
+        # balance loss since zero_grad, and how often each expert of a layer was
+        # chosen; aux_scale: this micro-batch's share of the step
+        self.aux_scale = 1.0
+        self.aux_loss = torch.zeros((), dtype=torch.float32, device=self.dev)
+        self.expert_counts = {}
         self.cos, self.sin = ref.rope_tables(c.max_position_embeddings, c.head_dim, c.rope_theta,
                                              self.dev)
         self.grads: List[Optional[torch.Tensor]] = [None] * weights.num_units
@@ -149,6 +178,8 @@ class Qwen3Engine:
                 g.zero_()
         for g in self.expert_grads.values():
             g.zero_()
+        self.aux_loss.zero_()
+        self.expert_counts = {}
 
     def grad_views(self, u: int):
         v = self.w.layouts[u].views(self.grads[u])
@@ -164,14 +195,23 @@ class Qwen3Engine:
         return ops.mm(a, b, **kw)
 
     # ------------------------------------------------------------------ layer
-    def _layer_fwd(self, u: int, x: torch.Tensor, b: Batch, keep: bool, attn_saved=None,
-                   save_attn: Optional[list] = None):
+    def _layer_fwd(self, u: int, x, b: Batch, keep: bool, attn_saved=None,
+                   save_attn: Optional[list] = None, hold: Optional[dict] = None, hold_all: bool = False):
+        """``x``: the layer's input, or its 8-bit copy (backward recompute).
+        ``hold`` receives 8-bit copies: of the input ("x"), and with
+        ``hold_all`` of everything that ``_held_ctx`` rebuilds the layer's
+        context from without a GEMM."""
         W = self.w.views(u)
         T = x.shape[0]
         qd, kd = self.hq * self.D, self.hkv * self.D
-        f32 = dict(dtype=torch.float32, device=x.device)
-        rstd1 = torch.empty(T, **f32)
-        hn = ops.rmsnorm_fwd(x, W["ln1"], self.eps, rstd=rstd1)
+        f32 = dict(dtype=torch.float32, device=self.dev)
+        if isinstance(x, a8.Act8):
+            x, hn, rstd1 = a8.rmsnorm_load(x, W["ln1"], self.eps)
+        elif hold is not None:
+            hn, rstd1, hold["x"] = a8.rmsnorm_save(x, W["ln1"], self.eps)
+        else:
+            rstd1 = torch.empty(T, **f32)
+            hn = ops.rmsnorm_fwd(x, W["ln1"], self.eps, rstd=rstd1)
         qkv = self._mm(hn, W["qkv"])
         qk = ops.qk_norm_rope_fwd(qkv, W["q_norm"], W["k_norm"], b.pos, self.cos, self.sin,
                                   self.hq, self.hkv, self.eps)
@@ -186,25 +226,43 @@ class Qwen3Engine:
             save_attn.append((o, lse))
         o2 = o.reshape(T, qd)
         x2 = self._mm(o2, W["o"], residual=x)
+        if hold_all:
+            hold.update(qkv=a8.save(qkv), o=o, lse=lse)
+            hn2, rstd2, hold["x2"] = a8.rmsnorm_save(x2, W["ln2"], self.eps)
+            gu = self._mm(hn2, W["gate_up"])
+            a, hold["gu"] = a8.swiglu_save(gu)
+            return self._mm(a, W["down"], residual=x2), None
         rstd2 = torch.empty(T, **f32)
         hn2 = ops.rmsnorm_fwd(x2, W["ln2"], self.eps, rstd=rstd2)
         ctx = None
         if self.w.layouts[u].kind == "moe_layer":
-            x3, mctx = self._moe_fwd(W, hn2, x2)
+            x3, mctx = self._moe_fwd(W, hn2, x2, u if keep else None)
             if keep:
-                ctx = dict(rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=o, lse=lse, x2=x2, rstd2=rstd2, hn2=hn2)
+                ctx = dict(x=x, rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=o, lse=lse, x2=x2, rstd2=rstd2, hn2=hn2)
                 ctx.update(mctx)             # the expert-parallel context may carry its own hn2
             return x3, ctx
         gu = self._mm(hn2, W["gate_up"])
         a = ops.swiglu_fwd(gu)
         x3 = self._mm(a, W["down"], residual=x2)
         if keep:
-            ctx = dict(rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=o, lse=lse, x2=x2, rstd2=rstd2,
+            ctx = dict(x=x, rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=o, lse=lse, x2=x2, rstd2=rstd2,
                        hn2=hn2, gu=gu, a=a)
         return x3, ctx
 
+    def _held_ctx(self, u: int, held: dict, b: Batch) -> dict:
+        """A dense layer's context from its 8-bit copies (no GEMM, no attention);
+        gate|up stays in 8 bits: its backward reads it there."""
+        W = self.w.views(u)
+        x, hn, rstd1 = a8.rmsnorm_load(held["x"], W["ln1"], self.eps)
+        qkv = a8.load(held["qkv"], dtype=self.dtype)
+        qk = ops.qk_norm_rope_fwd(qkv, W["q_norm"], W["k_norm"], b.pos, self.cos, self.sin,
+                                  self.hq, self.hkv, self.eps)
+        x2, hn2, rstd2 = a8.rmsnorm_load(held["x2"], W["ln2"], self.eps)
+        return dict(x=x, rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=held["o"], lse=held["lse"], x2=x2, rstd2=rstd2,
+                    hn2=hn2, gu8=held["gu"])
+
     # ------------------------------------------------------------------ MoE
-    def _moe_fwd(self, W, hn2, x2):
+    def _moe_fwd(self, W, hn2, x2, u=None):
         """Router -> top-k -> expert-major permutation -> grouped SwiGLU experts
         -> weighted combine (+ residual). Experts outside this rank's range (EP)
         are handled by the expert-parallel dispatcher when one is attached."""
@@ -212,8 +270,15 @@ class Qwen3Engine:
         c = self.cfg
         logits = ops.mm(hn2, W["router"], out_dtype=torch.float32)
         probs, idx, wts = moe.route(logits, c.num_experts_per_tok, c.norm_topk_prob)
+        balance = {}
+        if u is not None and self.router_aux_coef > 0:     # (the backward's pass over the layer)
+            aux, counts, gain = moe.balance_loss(probs, idx, None, self.router_aux_coef / self.moe_layers)
+            self.aux_loss.add_(aux, alpha=self.aux_scale)
+            self.expert_counts[u] = counts if u not in self.expert_counts else self.expert_counts[u] + counts
+            balance = dict(gain=gain)
         if self.ep is not None:
-            return self.ep.forward(self, W, hn2, x2, probs, idx, wts)
+            x3, mctx = self.ep.forward(self, W, hn2, x2, probs, idx, wts)
+            return x3, dict(mctx, **balance)
         # device routing plan (padded expert-major rows): no host synchronisation
         pl = moe.plan(idx, c.num_experts)
         xp = moe.plan_gather(hn2, pl)
@@ -221,7 +286,7 @@ class Qwen3Engine:
         a = ops.swiglu_fwd(gu)
         yp = moe.plan_mm(a, W["experts_down"], pl)
         x3 = moe.combine(yp, pl.pos, wts, resid=x2)
-        return x3, dict(probs=probs, idx=idx, wts=wts, plan=pl, pos=pl.pos, xp=xp, gu=gu, a=a, yp=yp)
+        return x3, dict(probs=probs, idx=idx, wts=wts, plan=pl, pos=pl.pos, xp=xp, gu=gu, a=a, yp=yp, **balance)
 
     def _moe_bwd(self, W, G, ctx, dx3, acc):
         """Returns d(hn2) of the MoE block; accumulates expert and router grads."""
@@ -240,6 +305,8 @@ class Qwen3Engine:
             self._plan_wgrad(G["experts_gate_up"], dgu, ctx["xp"], pl)
             dhn2 = moe.combine(dxp, pl.pos, None)
         dlogits = moe.route_bwd(ctx["probs"], ctx["idx"], ctx["wts"], dw, c.norm_topk_prob)
+        if "gain" in ctx:
+            moe.balance_bwd(ctx["probs"], ctx["gain"], None, self.aux_scale, dlogits)
         dl = dlogits.to(self.dtype)
         self._mm(dl, W["router"], b_t=False, out=dhn2, accumulate=True)
         self._mm(dl, ctx["hn2"], a_t=True, b_t=False, out=G["router"], accumulate=acc)
@@ -273,8 +340,13 @@ class Qwen3Engine:
             dhn2 = self._moe_bwd(W, G, ctx, dx3, acc)
         else:
             da = self._mm(dx3, W["down"], b_t=False)                       # [T, F]
-            self._mm(dx3, ctx["a"], a_t=True, b_t=False, out=G["down"], accumulate=acc)
-            dgu = ops.swiglu_bwd(da, ctx["gu"], ctx["gu"])                  # in place
+            if "gu8" in ctx:                                               # from 8 bits; a again
+                dgu, a = a8.swiglu_bwd(da, ctx["gu8"])
+                self._mm(dx3, a, a_t=True, b_t=False, out=G["down"], accumulate=acc)
+                del a
+            else:
+                self._mm(dx3, ctx["a"], a_t=True, b_t=False, out=G["down"], accumulate=acc)
+                dgu = ops.swiglu_bwd(da, ctx["gu"], ctx["gu"])              # in place
             del da
             dhn2 = self._mm(dgu, W["gate_up"], b_t=False)                  # [T, H]
             self._mm(dgu, ctx["hn2"], a_t=True, b_t=False, out=G["gate_up"], accumulate=acc)
@@ -364,6 +436,23 @@ class Qwen3Engine:
             del logits, dh, hrows
         return dhn
 
+    def _head_pieces(self, hn: torch.Tensor, targets: torch.Tensor, rows: torch.Tensor, want_entropy: bool):
+        """(rows of hn, their targets, logp, entropy, lse) without logits."""
+        hrows, tg = hn.index_select(0, rows), targets.index_select(0, rows)
+        lp, ent, lse = vocab.head_fwd(hrows, self.w.lm_head_weight(), tg, self.temperature,
+                                      want_entropy=want_entropy)
+        return hrows, tg, lp, ent, lse
+
+    def _head_pieces_bwd(self, hn: torch.Tensor, rows: torch.Tensor, hrows, tg, lse, coef) -> torch.Tensor:
+        u_head = self.w.num_units - 1
+        tied = self.cfg.tie_word_embeddings
+        u_lm = 0 if tied else u_head
+        Glm = self.grad_views(0)["embed"] if tied else self.grad_views(u_head)["lm_head"]
+        dh, _ = vocab.head_bwd(hrows, self.w.lm_head_weight(), tg, lse, coef.contiguous(), self.temperature, dw=Glm,
+                               accumulate=not self._fresh[u_lm])
+        self._fresh[u_lm] = False
+        return torch.zeros_like(hn).index_copy_(0, rows, dh)
+
     # ------------------------------------------------------------------ public
     def activation_bytes_per_layer(self, tokens: int) -> int:
         """HBM a dense layer's kept forward context takes for ``tokens`` tokens
@@ -372,6 +461,8 @@ class Qwen3Engine:
         c = self.cfg
         qd, kd = self.hq * self.D, self.hkv * self.D
         H, F = c.hidden_size, c.intermediate_size
+        if self.act8:                                                # qkv x2 gu in 8 bits, a scale per 128
+            return int(tokens * (qd + 2 * kd + H + 2 * F) * (1 + 4 / a8.BLOCK))
         elems = H + (qd + 2 * kd) + (qd + kd) + H + H + 2 * F + F   # hn qkv qk x2 hn2 gu a
         return tokens * (elems * self.w.dtype.itemsize + 8)           # + two fp32 rstd
 
@@ -390,11 +481,21 @@ class Qwen3Engine:
         hook = self.param_hook
         last = self.w.num_units - 2
         for u in range(1, self.w.num_units - 1):
-            if checkpoints is not None:
+            if checkpoints is not None and not self.act8:
                 checkpoints.append(x)
             if hook is not None:
                 hook.acquire(u, u + 1 if u < last else None)
-            if contexts is not None and self._kept(u) and self.w.layouts[u].kind != "moe_layer":
+            kept = contexts is not None and self._kept(u) and self.w.layouts[u].kind != "moe_layer"
+            if checkpoints is not None and self.act8:
+                hold: dict = {}
+                x, _ = self._layer_fwd(u, x, b, keep=False, save_attn=None if kept else attn_saves, hold=hold,
+                                       hold_all=kept)
+                checkpoints.append(hold["x"])
+                if kept:
+                    contexts[u] = hold
+                    if attn_saves is not None:
+                        attn_saves.append(None)
+            elif kept:
                 xin = x
                 x, contexts[u] = self._layer_fwd(u, x, b, keep=True)
                 if attn_saves is not None:
@@ -433,7 +534,10 @@ class Qwen3Engine:
         Wn = self.w.views(self.w.num_units - 1)["norm"]
         hn = ops.rmsnorm_fwd(x, Wn, self.eps)
         rows = torch.nonzero(b.targets >= 0).reshape(-1)
-        lp_rows, ent_rows = self._head_stats(hn, b.targets, rows, want_entropy)
+        if self.head == "pieces":
+            _, _, lp_rows, ent_rows, _ = self._head_pieces(hn, b.targets, rows, want_entropy)
+        else:
+            lp_rows, ent_rows = self._head_stats(hn, b.targets, rows, want_entropy)
         lp = torch.zeros(b.num_tokens, dtype=torch.float32, device=x.device)
         lp[rows] = lp_rows
         ent = None
@@ -467,15 +571,24 @@ class Qwen3Engine:
             valid = valid & (coef != 0)
         rows = torch.nonzero(valid).reshape(-1)
         lp_full = torch.zeros(T, dtype=torch.float32, device=x.device)
+        pieces = self.head == "pieces"
+        if pieces:
+            hrows, tg_rows, lp_rows, _, lse_rows = self._head_pieces(hn, b.targets, rows, False)
         if coef_fn is not None:
-            lp_rows, _ = self._head_stats(hn, b.targets, rows, False)
+            if not pieces:
+                lp_rows, _ = self._head_stats(hn, b.targets, rows, False)
             lp_full[rows] = lp_rows
             coef_full, loss = coef_fn(lp_full)
             coef_rows = coef_full.float()[rows]
         else:
             coef_rows = coef.float()[rows]
             loss = None
-        dhn = self._head_bwd(hn, b.targets, rows, coef_rows)
+        if pieces:
+            dhn = self._head_pieces_bwd(hn, rows, hrows, tg_rows, lse_rows, coef_rows)
+            self._last_rows_logp = lp_rows
+            del hrows
+        else:
+            dhn = self._head_bwd(hn, b.targets, rows, coef_rows)
         if coef_fn is None:
             # the gradient pass also produced log p(target) for the loss rows
             lp_full[rows] = self._last_rows_logp
@@ -494,7 +607,9 @@ class Qwen3Engine:
             ctx = kept.pop(u, None)
             if ctx is None:
                 _, ctx = self._layer_fwd(u, xin, b, keep=True, attn_saved=saved)
-            dx = self._layer_bwd(u, xin, dx, ctx, b)
+            elif self.act8:
+                ctx = self._held_ctx(u, ctx, b)
+            dx = self._layer_bwd(u, ctx["x"], dx, ctx, b)
             if self.param_hook is not None:
                 self.param_hook.end_bwd(u)
             del ctx, saved
@@ -503,9 +618,13 @@ class Qwen3Engine:
                 asaves[u - 1] = None
         # embedding
         Ge = self.grad_views(0)["embed"]
-        if self._fresh[0] and not self.cfg.tie_word_embeddings:
-            Ge.zero_()
-        ops.embed_bwd(b.ids, dx, Ge)
+        fresh = self._fresh[0] and not self.cfg.tie_word_embeddings
+        if self.embed_grad == "sorted":
+            vocab.embed_grad(b.ids, dx, Ge, accumulate=not fresh)
+        else:
+            if fresh:
+                Ge.zero_()
+            ops.embed_bwd(b.ids, dx, Ge)
         self._fresh[0] = False
         return {"loss": loss, "logp": lp_full}
 

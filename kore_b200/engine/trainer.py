@@ -43,7 +43,12 @@ class CausalLMTrainer:
                  warmup_steps: int = 0, total_steps: int = 1, comm: str = "nccl",
                  weights: Optional[Qwen3Weights] = None, micro_tokens_hint: int = 8192,
                  ep_capacity: float = 2.0, zero_stage: int = 2, recompute: str = "auto",
-                 activation_reserve_gb: float = 12.0, moment_offload: str = "auto", ep_dispatch: str = "push"):
+                 activation_reserve_gb: float = 12.0, moment_offload: str = "auto", ep_dispatch: str = "push",
+                 head: str = "chunks", embed_grad: str = "atomic", act8: bool = False, router_aux: bool = False):
+        """``head``, ``embed_grad`` and ``act8``: see :class:`Qwen3Engine`.
+        ``router_aux`` adds the routers' load-balancing loss with the model's
+        ``router_aux_loss_coef``; it is not part of the returned loss but in
+        ``eng.aux_loss``, the experts' counts in ``eng.expert_counts``."""
         self.ctx = ctx or get_context()
         self.cfg = cfg
         dev = self.ctx.device
@@ -95,7 +100,9 @@ class CausalLMTrainer:
                 weights = nw
         self.w = weights or Qwen3Weights(cfg, device=dev, dtype=dtype, seed=seed,
                                          pad_multiple=128 * max(1, self.ctx.world), ep=ep)
-        self.eng = Qwen3Engine(self.w, logits_chunk=logits_chunk, grad_alloc=grad_alloc)
+        self.eng = Qwen3Engine(self.w, logits_chunk=logits_chunk, grad_alloc=grad_alloc, head=head,
+                               embed_grad=embed_grad, act8=act8,
+                               router_aux_coef=cfg.router_aux_loss_coef if router_aux and cfg.is_moe else 0.0)
         if self.w.ep is not None:
             from ..parallel.ep import ExpertParallel, FusedExpertParallel
             if fused:
@@ -214,6 +221,7 @@ class CausalLMTrainer:
         self.eng.zero_grad()
         loss = torch.zeros((), dtype=torch.float32, device=ids.device)
         starts = list(range(0, B, self.mbs))
+        self.eng.aux_scale = 1.0 / (max(1, len(starts)) * self.ctx.world)
         shuttle = self._moment_shuttle(len(starts), min(self.mbs, B) * S)
         for i, s in enumerate(starts):
             if shuttle is not None:
@@ -242,14 +250,15 @@ class CausalLMTrainer:
         self.ctx.all_reduce(tot)
         self.eng.zero_grad()
         loss = torch.zeros((), dtype=torch.float32, device=dev)
-        order = list(range(len(seqs)))
-        i = 0
-        while i < len(order):
-            chunk, ntok = [], 0
-            while i < len(order) and (not chunk or ntok + len(seqs[order[i]]) <= micro_tokens):
-                chunk.append(order[i])
-                ntok += len(seqs[order[i]])
-                i += 1
+        chunks, ntok = [], 0
+        for j in range(len(seqs)):
+            if not chunks or ntok + len(seqs[j]) > micro_tokens:
+                chunks.append([])
+                ntok = 0
+            chunks[-1].append(j)
+            ntok += len(seqs[j])
+        self.eng.aux_scale = 1.0 / (max(1, len(chunks)) * self.ctx.world)
+        for chunk in chunks:
             b = Batch.from_sequences([torch.as_tensor(seqs[j]) for j in chunk],
                                      [torch.as_tensor(label_masks[j]) for j in chunk], device=dev)
             coef = torch.zeros(b.num_tokens, dtype=torch.float32)

@@ -55,6 +55,10 @@ class DistributedMixin:
     comm: str = "nccl"                 # "nccl" | "fused": data plane of the sharded optimizer
     micro_batch_tokens: int = 0        # pack micro-batches up to this many tokens (0 = per sample)
     save_attention: bool = True        # selective activation checkpointing
+    head: str = "chunks"               # "chunks" | "pieces": head loss over logits chunks, or in vocabulary pieces
+    embed_grad: str = "atomic"         # "atomic" | "sorted": embedding gradient
+    act8: bool = False                 # activation checkpoints and kept layer contexts in 8 bits
+    router_aux: bool = False           # MoE: balance loss with the model's router_aux_loss_coef
 
 
 @dataclass
@@ -319,6 +323,12 @@ def parallel_kwargs(config, world: int) -> dict:
     if z == 3:
         return {"zero_stage": 3, "comm": "nccl"}
     return {"zero_stage": 2, "comm": getattr(config, "comm", "nccl")}
+
+
+def step_kwargs(config) -> dict:
+    """CausalLMTrainer arguments that choose the training step's operators."""
+    return {"head": getattr(config, "head", "chunks"), "embed_grad": getattr(config, "embed_grad", "atomic"),
+            "act8": bool(getattr(config, "act8", False)), "router_aux": bool(getattr(config, "router_aux", False))}
 
 
 def build_fsdp_kwargs(config) -> dict:

@@ -32,7 +32,7 @@ from ..models.hf_io import load_pretrained_or_init
 from ..obs import configure, get_logger
 from ..parallel.dist import init_distributed
 from ._loop import plan_steps, run_loop
-from .configs import DPOConfig, dpo_config_from_dict
+from .configs import DPOConfig, dpo_config_from_dict, step_kwargs
 
 log = get_logger("policy.dpo")
 
@@ -96,7 +96,7 @@ class DPOTrainer:
                                   max_grad_norm=float(getattr(config, "max_grad_norm", 1.0)),
                                   seed=config.seed, schedule=config.lr_scheduler_type,
                                   warmup_steps=int(config.warmup_ratio * total_steps), total_steps=total_steps,
-                                  weights=weights, comm=config.comm)
+                                  weights=weights, comm=config.comm, **step_kwargs(config))
         self.ref_placement = self._choose_placement(getattr(config, "ref_placement", "auto"))
         self.ref = Qwen3Engine(self._build_ref(ref_weights), allocate_grads=False)
         if self.ref_placement != "resident":

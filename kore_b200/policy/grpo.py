@@ -41,7 +41,7 @@ from ..env.base import RolloutEnv, SyntheticRewardEnv, TurnResult
 from ..obs import configure, get_logger
 from ..parallel.dist import DistContext, get_context, init_distributed
 from . import rl_math as M
-from .configs import GRPOConfig, grpo_config_from_dict
+from .configs import GRPOConfig, grpo_config_from_dict, step_kwargs
 
 log = get_logger("policy.grpo")
 
@@ -97,7 +97,7 @@ class GRPOTrainer:
                                        schedule=config.lr_scheduler_type,
                                        warmup_steps=int(config.warmup_ratio * config.total_steps),
                                        total_steps=config.total_steps, weights=weights,
-                                       comm=getattr(config, "comm", "nccl"))
+                                       comm=getattr(config, "comm", "nccl"), **step_kwargs(config))
         self.trainer.eng.temperature = config.temperature
         # the trainer may have moved the weights (e.g. into the symmetric heap of
         # the fused optimizer): rollout and reference read the trainer's copy

@@ -19,6 +19,7 @@ from ..obs import configure, get_logger
 from ..parallel.dist import init_distributed
 from ._loop import plan_steps, run_loop
 from .configs import parallel_kwargs as _parallel_kwargs
+from .configs import step_kwargs
 from .configs import MidTrainConfig, midtrain_config_from_dict
 
 log = get_logger("policy.midtrain")
@@ -56,7 +57,8 @@ def train_midtrain(config: MidTrainConfig, corpus_path=None, *, model_cfg=None, 
     tr = CausalLMTrainer(w.cfg, ctx, lr=config.learning_rate, weight_decay=config.weight_decay,
                          max_grad_norm=config.max_grad_norm, seed=config.seed,
                          schedule=config.lr_scheduler_type, warmup_steps=int(config.warmup_ratio * total),
-                         total_steps=total, weights=w, **_parallel_kwargs(config, ctx.world))
+                         total_steps=total, weights=w, **_parallel_kwargs(config, ctx.world),
+                         **step_kwargs(config))
 
     def step_fn(wins):
         seqs = [d for win in wins for d in win]

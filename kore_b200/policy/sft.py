@@ -25,6 +25,7 @@ from ..obs import configure, get_logger
 from ..parallel.dist import init_distributed
 from ._loop import plan_steps, run_loop
 from .configs import parallel_kwargs as _parallel_kwargs
+from .configs import step_kwargs
 from .configs import SFTConfig, sft_config_from_dict
 
 log = get_logger("policy.sft")
@@ -61,7 +62,8 @@ def train_sft(config: SFTConfig, dataset_path: Optional[str] = None, *, model_cf
     tr = CausalLMTrainer(w.cfg, ctx, lr=config.learning_rate, weight_decay=config.weight_decay,
                          max_grad_norm=config.max_grad_norm, seed=config.seed,
                          schedule=config.lr_scheduler_type, warmup_steps=int(config.warmup_ratio * total),
-                         total_steps=total, weights=w, **_parallel_kwargs(config, ctx.world))
+                         total_steps=total, weights=w, **_parallel_kwargs(config, ctx.world),
+                         **step_kwargs(config))
     tr.eng.save_attention = config.save_attention
     budget = config.micro_batch_tokens or max(config.max_seq_length, 8192)
     step_fn = lambda exs: tr.train_step_sequences([e[0] for e in exs], [e[1] for e in exs],

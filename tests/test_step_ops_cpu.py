@@ -1,0 +1,127 @@
+"""The training step with the vocabulary, balance and 8-bit checkpoint operators
+switched on, against the step without them (fp32 on the CPU)."""
+import pytest
+import torch
+
+from kore_b200.engine.qwen3_engine import Batch, Qwen3Engine
+from kore_b200.engine.trainer import CausalLMTrainer
+from kore_b200.models import Qwen3Config, Qwen3Weights
+from kore_b200.parallel.dist import get_context
+from kore_b200.policy.configs import SFTConfig, step_kwargs
+
+
+def _cfg(moe=False, tied=False):
+    kw = dict(vocab_size=211, hidden_size=64, intermediate_size=128, num_hidden_layers=3, num_attention_heads=4,
+              num_key_value_heads=2, head_dim=16, max_position_embeddings=128, tie_word_embeddings=tied)
+    if moe:
+        kw.update(model_type="qwen3_moe", num_experts=4, num_experts_per_tok=2, moe_intermediate_size=32)
+    return Qwen3Config(**kw)
+
+
+def _engine(cfg, **kw):
+    w = Qwen3Weights(cfg, device=torch.device("cpu"), dtype=torch.float32, seed=3)
+    return Qwen3Engine(w, **kw)
+
+
+def _batch(cfg):
+    g = torch.Generator().manual_seed(0)
+    seqs = [torch.randint(0, cfg.vocab_size, (n,), generator=g) for n in (21, 9)]
+    masks = [torch.arange(len(s)) > 4 for s in seqs]
+    return Batch.from_sequences(seqs, masks)
+
+
+def _step(eng, b, coef_fn=None):
+    eng.zero_grad()
+    out = eng.forward_backward(b, coef_fn=coef_fn) if coef_fn else eng.forward_backward(b, coef=eng.sft_coef(b))
+    return out, [g.clone() for g in eng.grads]
+
+
+@pytest.mark.parametrize("moe", [False, True])
+@pytest.mark.parametrize("tied", [False, True])
+def test_pieces_and_sorted_give_the_same_step(moe, tied):
+    cfg = _cfg(moe, tied)
+    b = _batch(cfg)
+    plain, other = _engine(cfg), _engine(cfg, head="pieces", embed_grad="sorted")
+    for fn in (None, lambda lp: (-0.1 * (1 + lp.exp()), lp.sum())):
+        a, ga = _step(plain, b, fn)
+        c, gc = _step(other, b, fn)
+        assert torch.allclose(a["logp"], c["logp"], atol=1e-5) and torch.allclose(a["loss"], c["loss"], rtol=1e-5)
+        for x, y in zip(ga, gc):
+            assert torch.allclose(x, y, rtol=1e-4, atol=1e-6)
+    # a second micro-batch adds
+    other.forward_backward(b, coef=other.sft_coef(b))
+    plain.forward_backward(b, coef=plain.sft_coef(b))
+    for x, y in zip(plain.grads, other.grads):
+        assert torch.allclose(x, y, rtol=1e-4, atol=1e-6)
+    lp, ent = plain.token_logprobs(b, want_entropy=True)
+    lp2, ent2 = other.token_logprobs(b, want_entropy=True)
+    assert torch.allclose(lp, lp2, atol=1e-5) and torch.allclose(ent, ent2, atol=1e-4)
+
+
+@pytest.mark.parametrize("moe", [False, True])
+@pytest.mark.parametrize("keep", [0, 2])
+def test_act8_gradients_stay_near(moe, keep):
+    cfg = _cfg(moe)
+    b = _batch(cfg)
+    plain, held = _engine(cfg), _engine(cfg, act8=True)
+    held.keep_layers = keep
+    a, ga = _step(plain, b)
+    c, gc = _step(held, b)
+    assert torch.equal(a["logp"], c["logp"])                 # the forward pass is not touched
+    for u, (x, y) in enumerate(zip(ga, gc)):
+        # values are off by amax / 254 of their block (rms about 0.5% here)
+        assert (x - y).norm() <= 0.03 * x.norm(), u
+    assert held.activation_bytes_per_layer(1024) < plain.activation_bytes_per_layer(1024) / 4
+
+
+def test_router_balance_gradient_by_differences():
+    cfg = _cfg(moe=True)
+    b = _batch(cfg)
+    zero = torch.zeros(b.num_tokens)
+    eng = _engine(cfg, router_aux_coef=0.5)
+    eng.aux_scale = 0.25
+    eng.zero_grad()
+    eng.forward_backward(b, coef=zero)                        # only the balance loss has a gradient
+    total = eng.aux_loss.clone()
+    assert sorted(eng.expert_counts) == [1, 2, 3]
+    assert all(int(c.sum()) == 2 * b.num_tokens for c in eng.expert_counts.values())
+    last = 3                                                  # the last layer's router feeds nothing but its own loss
+    grad = eng.grad_views(last)["router"].clone()
+    g = torch.Generator().manual_seed(1)
+    d = torch.randn(grad.shape, generator=g)
+    d *= 1e-3 / d.norm()
+    W = eng.w.views(last)["router"]
+    vals = []
+    for sign in (1, -1):
+        W.add_(d, alpha=sign)
+        eng.zero_grad()
+        eng.forward_backward(b, coef=zero)
+        vals.append(float(eng.aux_loss))
+        W.add_(d, alpha=-sign)
+    num, want = (vals[0] - vals[1]) / 2, float((grad * d).sum())
+    assert float(total) > 0 and abs(num - want) <= 0.02 * abs(want) + 1e-7
+    off = _engine(cfg)
+    off.forward_backward(b, coef=zero)
+    assert float(off.aux_loss) == 0 and off.expert_counts == {}
+
+
+def test_trainer_runs_all_of_them_together():
+    cfg = _cfg(moe=True)
+    conf = SFTConfig(head="pieces", embed_grad="sorted", act8=True, router_aux=True)
+    assert step_kwargs(SFTConfig()) == dict(head="chunks", embed_grad="atomic", act8=False, router_aux=False)
+    tr = CausalLMTrainer(cfg, get_context(), lr=1e-2, dtype=torch.float32, seed=1, **step_kwargs(conf))
+    assert tr.eng.router_aux_coef == cfg.router_aux_loss_coef
+    g = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, cfg.vocab_size, (4, 16), generator=g)
+    losses = [tr.train_step(ids) for _ in range(8)]
+    assert losses[-1] < losses[0] and float(tr.eng.aux_loss) > 0
+    seqs = [torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist() for n in (9, 14, 5)]
+    assert tr.train_step_sequences(seqs, [[1] * len(s) for s in seqs], micro_tokens=16) > 0
+    assert tr.eng.aux_scale == 1 / 3                          # 9 + 14 and 14 + 5 are over 16: three micro-batches
+
+
+def test_options_are_checked():
+    cfg = _cfg()
+    for kw in (dict(head="rows"), dict(embed_grad="hash"), dict(router_aux_coef=-1.0)):
+        with pytest.raises(ValueError):
+            _engine(cfg, **kw)
