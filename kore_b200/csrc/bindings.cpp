@@ -115,9 +115,9 @@ int64_t device_wait_flag(const at::Tensor& flag, int64_t want, double timeout_s)
 std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, at::Tensor> head_fwd(
     const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets, double inv_temp,
     bool want_entropy);
-void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
-              const at::Tensor& lse, const at::Tensor& coef, double inv_temp, at::Tensor& dx, at::Tensor& dw,
-              bool accumulate, int64_t piece);
+at::Tensor head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
+                    const at::Tensor& lse, const at::Tensor& coef, double inv_temp,
+                    const c10::optional<at::Tensor>& into, at::Tensor& dw, bool accumulate, int64_t piece);
 at::Tensor embed_scaled(const at::Tensor& ids, const at::Tensor& table, const c10::optional<at::Tensor>& into,
                         double scale);
 void embed_grad_sorted(const at::Tensor& ids, const at::Tensor& dy, at::Tensor& dtable, double scale,

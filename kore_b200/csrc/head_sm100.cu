@@ -15,9 +15,10 @@
 // the accumulator on.
 // Backward: per piece of the vocabulary the same GEMM runs again and its
 // epilogue turns z into dz (bf16, the operand type of the two products that
-// follow; few rows: two bf16 terms); then dW[piece] = dz^T x and dx += dz W[piece] run on the
-// plain GEMM. dW rows are final after their piece (one rounding); dx sums its
-// pieces in fp32 and is rounded once.
+// follow; few rows: two bf16 terms); then one launch computes
+// dW[piece] = dz^T x and dx += dz W[piece]: the tiles of both products fill the
+// last waves of one another. dW rows are final after their piece (one rounding);
+// dx sums its pieces in fp32 and is rounded once.
 // Rows with coefficient 0 have dz = 0 whatever x or the statistics hold there,
 // and dW reads such rows of x as zeros, so an inf or NaN in them stays out.
 //
@@ -32,10 +33,6 @@
 #include "tma_host.h"
 
 namespace kore {
-
-void gemm_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn,
-               double alpha, bool accumulate, const c10::optional<at::Tensor>& residual,
-               int64_t max_ctas);
 
 namespace head {
 
@@ -71,10 +68,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // What a launch does with its tiles of A B^T:
-//   STATS  A = x, B = W piece: row statistics          (columns: vocabulary, K = H)
-//   GRAD   A = x, B = W piece: dz, bf16                (columns: vocabulary, K = H)
-//   DX     A = dz, B = W piece^T: fp32 partials of dx  (columns: H, K = vocabulary, split)
-enum Mode { STATS, GRAD, DX };
+//   STATS  A = x, B = W piece: row statistics      (columns: vocabulary, K = H)
+//   GRAD   A = x, B = W piece: dz, bf16            (columns: vocabulary, K = H)
+//   PRODS  first A = dz, B = W piece^T: fp32 parts of dx   (columns: H, K = vocabulary, split)
+//          then  A = dz^T, B = x^T: dW of the piece        (rows: vocabulary, columns: H, K = dz's rows)
+enum Mode { STATS, GRAD, PRODS };
 
 template <Mode M>
 struct Layout {
@@ -100,10 +98,17 @@ struct Params {
   const float* coef;
   __nv_bfloat16* low;   // not null: what bf16 leaves of dz goes here, row stride low_ld
   long low_ld;
-  // DX
-  int splits;           // parts of K; part i is stored at row i * split_rows
+  // PRODS
+  int splits;           // parts of dx's K; part i is stored at row i * split_rows
   int split_rows;
-  int add;              // add to the partials of earlier pieces
+  int add;              // add to the dx parts of earlier pieces
+  void* dw;             // the piece's rows of dW, contiguous
+  int dw_f32, dw_add;   // fp32 (else bf16); add to what is there
+};
+
+// The tensor maps of a launch: A, B and the output; PRODS: those of dx, then of dW.
+struct Maps {
+  CUtensorMap a, b, d, a2, b2, d2;
 };
 
 KORE_DEV float ex2(float x) {
@@ -135,8 +140,7 @@ KORE_DEV void tile_coords(int t, int num_m, int num_n, int& tm, int& tn) {
 
 template <Mode M>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ CUtensorMap tmD, const Params p) {
+    head_kernel(const __grid_constant__ Maps maps, const Params p) {
   using L = Layout<M>;
   constexpr int kStages = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -155,18 +159,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int num_m = (p.rows + 2 * BM - 1) / (2 * BM);
   const int num_n = (p.cols + bn - 1) / bn;
   const int num_mn = num_m * num_n;
-  const int num_tiles = M == DX ? num_mn * p.splits : num_mn;
   const int kblocks = (p.K + BK - 1) / BK;
   const int part = (kblocks + k_parts(kblocks) - 1) / k_parts(kblocks);  // STATS: k-blocks per part
-  // k-blocks [k0, k1) of work item t
-  auto k_range = [&](int t, int& k0, int& k1) {
-    k0 = 0;
-    k1 = kblocks;
-    if (M == DX) {
-      const long s = t / num_mn;
-      k0 = (int)(s * kblocks / p.splits);
-      k1 = (int)((s + 1) * kblocks / p.splits);
+  const int dw_m = M == PRODS ? (p.K + 2 * BM - 1) / (2 * BM) : 0;
+  const int first_dw = M == PRODS ? num_mn * p.splits : num_mn;          // work items before dW's
+  const int num_items = first_dw + dw_m * num_n;
+  // work item t: is it a tile of dW, its first row and column, its k-blocks [k0, k1)
+  struct Item {
+    bool dw;
+    int m0, n0, tn, k0, k1, rows, split;
+  };
+  auto item = [&](int t) {
+    Item w;
+    int tm;
+    w.dw = M == PRODS && t >= first_dw;
+    w.k0 = 0;
+    w.k1 = kblocks;
+    w.split = 0;
+    w.rows = p.rows;
+    if (w.dw) {
+      tile_coords(t - first_dw, dw_m, num_n, tm, w.tn);
+      w.k1 = (p.rows + BK - 1) / BK;
+      w.rows = p.K;
+    } else {
+      tile_coords(M == PRODS ? t % num_mn : t, num_m, num_n, tm, w.tn);
+      if (M == PRODS) {
+        w.split = t / num_mn;
+        w.k0 = (int)((long)w.split * kblocks / p.splits);
+        w.k1 = (int)((long)(w.split + 1) * kblocks / p.splits);
+      }
     }
+    w.m0 = tm * 2 * BM;
+    w.n0 = w.tn * bn;
+    return w;
   };
 
   if (threadIdx.x == 0) {
@@ -180,9 +205,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     *abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
-    if (M != STATS) tma_prefetch_desc(&tmD);
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b);
+    if (M != STATS) tma_prefetch_desc(&maps.d);
+    if (M == PRODS) {
+      tma_prefetch_desc(&maps.a2);
+      tma_prefetch_desc(&maps.b2);
+      tma_prefetch_desc(&maps.d2);
+    }
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 2 * kMaxBN);
   tc_fence_before();
@@ -197,33 +227,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
-        int tm, tn, k0, k1;
-        tile_coords(t % num_mn, num_m, num_n, tm, tn);
-        k_range(t, k0, k1);
-        const int m0 = tm * 2 * BM, n0 = tn * bn;
+      for (int t = pair; t < num_items && !*abort_flag; t += npairs) {
+        const Item w = item(t);
         // a box that lies wholly past the rows or the columns is not loaded
         // (its part of the accumulator is never used)
-        auto a_live = [&](int r) { return m0 + r * BM < p.rows; };
+        auto a_bytes = [&](int r) -> uint32_t {
+          const int m = w.m0 + r * BM;
+          if (!w.dw) return m < w.rows ? kABytes : 0u;
+          return (m < w.rows ? 8192u : 0u) + (m + 64 < w.rows ? 8192u : 0u);
+        };
         auto b_bytes = [&](int r) -> uint32_t {
-          const int n = n0 + r * (bn / 2);
-          if (M != DX) return n < p.cols ? (uint32_t)(bn / 2) * BK * 2 : 0u;
+          const int n = w.n0 + r * (bn / 2);
+          if (M != PRODS) return n < p.cols ? (uint32_t)(bn / 2) * BK * 2 : 0u;
           return (n < p.cols ? 8192u : 0u) + (n + 64 < p.cols ? 8192u : 0u);
         };
-        const uint32_t bytes = (a_live(0) ? kABytes : 0) + (a_live(1) ? kABytes : 0) + b_bytes(0) + b_bytes(1);
-        const int my_n = n0 + (int)rank * (bn / 2);
-        for (int kb = k0; kb < k1; ++kb) {
+        const uint32_t bytes = a_bytes(0) + a_bytes(1) + b_bytes(0) + b_bytes(1);
+        const int m = w.m0 + (int)rank * BM, n = w.n0 + (int)rank * (bn / 2);
+        for (int kb = w.k0; kb < w.k1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1)) { *abort_flag = 1; break; }
           uint8_t* sA = smem + stage * kStageBytes;
           uint8_t* sB = sA + kABytes;
           const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          const int k = kb * BK;
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], bytes);
-          if (a_live((int)rank)) tma_load_2d_pair(sA, &tmA, fb, kb * BK, m0 + (int)rank * BM);
-          if (M != DX) {
-            if (my_n < p.cols) tma_load_2d_pair(sB, &tmB, fb, kb * BK, my_n);
-          } else {  // W piece is [K, columns]: two 64-column boxes
-            if (my_n < p.cols) tma_load_2d_pair(sB, &tmB, fb, my_n, kb * BK);
-            if (my_n + 64 < p.cols) tma_load_2d_pair(sB + 8192, &tmB, fb, my_n + 64, kb * BK);
+          if (!w.dw) {
+            if (m < w.rows) tma_load_2d_pair(sA, &maps.a, fb, k, m);
+          } else {  // dz is [K, rows]: two 64-column boxes
+            if (m < w.rows) tma_load_2d_pair(sA, &maps.a2, fb, m, k);
+            if (m + 64 < w.rows) tma_load_2d_pair(sA + 8192, &maps.a2, fb, m + 64, k);
+          }
+          if (M != PRODS) {
+            if (n < p.cols) tma_load_2d_pair(sB, &maps.b, fb, k, n);
+          } else {  // W piece and x are [K, columns]
+            const CUtensorMap* mb = w.dw ? &maps.b2 : &maps.b;
+            if (n < p.cols) tma_load_2d_pair(sB, mb, fb, n, k);
+            if (n + 64 < p.cols) tma_load_2d_pair(sB + 8192, mb, fb, n + 64, k);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
@@ -233,14 +271,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader)
     if (rank == 0 && elect_one()) {
-      const uint32_t idesc = make_idesc_bf16(2 * BM, bn, false, M == DX);
+      const uint32_t idesc_x = make_idesc_bf16(2 * BM, bn, false, M == PRODS);
+      const uint32_t idesc_w = make_idesc_bf16(2 * BM, bn, true, true);
       int stage = 0, it = 0;
       uint32_t phase = 0;
-      for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
-        int k0, k1;
-        k_range(t, k0, k1);
-        for (int c0 = k0; c0 < k1; ++it) {
-          const int c1 = M == STATS ? min(c0 + part, k1) : k1;
+      for (int t = pair; t < num_items && !*abort_flag; t += npairs) {
+        const Item w = item(t);
+        const uint32_t idesc = w.dw ? idesc_w : idesc_x;
+        for (int c0 = w.k0; c0 < w.k1; ++it) {
+          const int c1 = M == STATS ? min(c0 + part, w.k1) : w.k1;
           const int acc = it & 1;
           if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1)) { *abort_flag = 1; break; }
           tc_fence_after();
@@ -253,9 +292,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t b_addr = a_addr + kABytes;
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              umma_f16_ss_pair(d_tmem, make_sw128_desc(a_addr + k * 32, 16, 1024),
-                               M == DX ? make_sw128_desc(b_addr + k * 2048, 8192, 1024)
-                                       : make_sw128_desc(b_addr + k * 32, 16, 1024),
+              umma_f16_ss_pair(d_tmem,
+                               w.dw ? make_sw128_desc(a_addr + k * 2048, 8192, 1024)
+                                    : make_sw128_desc(a_addr + k * 32, 16, 1024),
+                               M == PRODS ? make_sw128_desc(b_addr + k * 2048, 8192, 1024)
+                                          : make_sw128_desc(b_addr + k * 32, 16, 1024),
                                idesc, kb != c0 || k != 0);
             umma_commit_pair(&empty_bar[stage], 0x3);
             if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -276,20 +317,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty_bar[0]), 0),
                                        mapa_shared(smem_u32(&tempty_bar[1]), 0)};
     int it = 0;
-    for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
-      int tm, tn, k0, k1;
-      tile_coords(t % num_mn, num_m, num_n, tm, tn);
-      k_range(t, k0, k1);
-      if (k0 >= k1) continue;  // a narrow last piece leaves some parts of K empty: nothing was issued
-      const int n0 = tn * bn + h0;
-      const int row0 = tm * 2 * BM + (int)rank * BM + q * 32;
+    for (int t = pair; t < num_items && !*abort_flag; t += npairs) {
+      const Item w = item(t);
+      if (w.k0 >= w.k1) continue;  // a narrow last piece leaves some parts of K empty: nothing was issued
+      const int n0 = w.n0 + h0;
+      const int row0 = w.m0 + (int)rank * BM + q * 32;
       const int row = row0 + lane;
-      const int cols = row0 < p.rows ? min(min(width, bn - h0), p.cols - n0) : 0;  // this warp's columns
-      const bool live = row < p.rows;
+      const int cols = row0 < w.rows ? min(min(width, bn - h0), p.cols - n0) : 0;  // this warp's columns
+      const bool live = row < w.rows;
       // column of the label among them (negative: not here)
       int tc = -1;
       float lse2 = 0.f, c = 0.f;
-      if (M != DX && live && p.targets != nullptr) {
+      if (M != PRODS && live && p.targets != nullptr) {
         const long y = p.targets[row] - p.v0 - n0;
         if (y >= 0 && y < cols) tc = (int)y;
       }
@@ -307,7 +346,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (M == STATS) {
         float v[kMaxBN / 2];
         bool ok = true;
-        for (int c0 = k0; c0 < k1; c0 += part, ++it) {
+        for (int c0 = w.k0; c0 < w.k1; c0 += part, ++it) {
           const int acc = it & 1;
           if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { ok = false; break; }
           tc_fence_after();
@@ -317,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               uint32_t r[32];
               tmem_ld32(t_row + acc * kMaxBN + 32 * j, r);
               tmem_wait_ld();
-              if (c0 == k0) {
+              if (c0 == w.k0) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[32 * j + i] = __uint_as_float(r[i]);
               } else {
@@ -370,7 +409,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
           }
         if (live) {
-          const size_t o = (size_t)(2 * tn + half) * p.rows + row, plane = (size_t)2 * num_n * p.rows;
+          const size_t o = (size_t)(2 * w.tn + half) * p.rows + row, plane = (size_t)2 * num_n * p.rows;
           p.stats[o] = m;
           p.stats[o + plane] = s;
           if (p.entropy) p.stats[o + 2 * plane] = u;
@@ -380,9 +419,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { *abort_flag = 1; break; }
         ++it;
         tc_fence_after();
-        constexpr int kBox = M == GRAD ? 64 : 32;  // columns of 128 bytes
-        for (int c0 = 0; c0 < cols; c0 += kBox) {
-          auto store = [&](const uint4 (&out)[8], int y) {
+        const int box = M == GRAD || (w.dw && !p.dw_f32) ? 64 : 32;  // columns of 128 bytes
+        for (int c0 = 0; c0 < cols; c0 += box) {
+          // sends the warp's 32 rows x 128 bytes; add: into what is there
+          auto store = [&](const CUtensorMap* map, const uint4 (&out)[8], int y, bool add) {
             if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
             __syncwarp();
 #pragma unroll
@@ -391,8 +431,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (M == DX && p.add) tma_reduce_add_2d(&tmD, stage_buf, n0 + c0, y);
-              else tma_store_2d(&tmD, stage_buf, n0 + c0, y);
+              if (add) tma_reduce_add_2d(map, stage_buf, n0 + c0, y);
+              else tma_store_2d(map, stage_buf, n0 + c0, y);
               tma_store_commit();
             }
           };
@@ -421,27 +461,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 8; ++j)
               out[j] = make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
                                   pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7]));
-            store(out, row0);
+            store(&maps.d, out, row0, false);
             if (p.low != nullptr && live) {
               __nv_bfloat16* low = p.low + row * p.low_ld + n0 + c0;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const uint32_t w[4] = {out[j].x, out[j].y, out[j].z, out[j].w};
+                const uint32_t hi[4] = {out[j].x, out[j].y, out[j].z, out[j].w};
                 uint32_t l[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  l[e] = pack_bf16(f[8 * j + 2 * e] - __uint_as_float(w[e] << 16),
-                                   f[8 * j + 2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+                  l[e] = pack_bf16(f[8 * j + 2 * e] - __uint_as_float(hi[e] << 16),
+                                   f[8 * j + 2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
                 if (c0 + 8 * j < cols) *reinterpret_cast<uint4*>(low + 8 * j) = make_uint4(l[0], l[1], l[2], l[3]);
               }
             }
+          } else if (w.dw && !p.dw_f32) {
+            float f[64];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[32];
+              tmem_ld32(t_row + acc * kMaxBN + c0 + 32 * h, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) f[32 * h + i] = __uint_as_float(r[i]);
+            }
+            if (p.dw_add && live) {  // one rounding of the sum: no bf16 reduction of a rounded tile
+              const __nv_bfloat16* old = (const __nv_bfloat16*)p.dw + (size_t)row * p.cols + n0 + c0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c0 + 8 * j < cols) {
+                  const uint4 u = *reinterpret_cast<const uint4*>(old + 8 * j);
+                  const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float2 o = __bfloat1622float2(o2[e]);
+                    f[8 * j + 2 * e] += o.x;
+                    f[8 * j + 2 * e + 1] += o.y;
+                  }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              out[j] = make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
+                                  pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7]));
+            store(&maps.d2, out, row0, false);
           } else {
             uint32_t r[32];
             tmem_ld32(t_row + acc * kMaxBN + c0, r);
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 8; ++j) out[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            store(out, (t / num_mn) * p.split_rows + row0);
+            if (w.dw) store(&maps.d2, out, row0, p.dw_add != 0);
+            else store(&maps.d, out, w.split * p.split_rows + row0, p.add != 0);
           }
         }
         release(acc);
@@ -678,8 +749,7 @@ __global__ void sum_parts_kernel(const float* __restrict__ src, int parts, int c
 }
 
 template <Mode M>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const Params& p, int dev,
-            cudaStream_t st) {
+void launch(const Maps& maps, const Params& p, int dev, cudaStream_t st) {
   static bool attr_set[64] = {};
   TORCH_CHECK(dev >= 0 && dev < 64, "head: device index");
   auto k = head_kernel<M>;
@@ -689,9 +759,11 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
                "cudaFuncSetAttribute(head smem)");
     attr_set[dev] = true;
   }
-  const long tiles = (long)((p.rows + 2 * BM - 1) / (2 * BM)) * ((p.cols + p.bn - 1) / p.bn) * p.splits;
-  const int grid = (int)std::min<long>(2 * tiles, num_sms(dev) & ~1);
-  launch_after("head launch", k, dim3(grid), dim3(kThreads), (size_t)smem, st, ta, tb, td, p);
+  const long num_n = (p.cols + p.bn - 1) / p.bn;
+  long items = (long)((p.rows + 2 * BM - 1) / (2 * BM)) * num_n * p.splits;
+  if (M == PRODS) items += (long)((p.K + 2 * BM - 1) / (2 * BM)) * num_n;
+  const int grid = (int)std::min<long>(2 * items, num_sms(dev) & ~1);
+  launch_after("head launch", k, dim3(grid), dim3(kThreads), (size_t)smem, st, maps, p);
 }
 
 template <int NT>
@@ -806,9 +878,10 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, at::Tensor> hea
       if (T == 1) launch_few<1>(xp, row_stride(x), wp, row_stride(w), p, few_blocks, dev, st);
       else launch_few<2>(xp, row_stride(x), wp, row_stride(w), p, few_blocks, dev, st);
     } else {
-      CUtensorMap tw = make_tmap_2d(w.data_ptr(), bf, 2, H, V, row_stride(w), BK, p.bn / 2);
-      CUtensorMap tx = make_tmap_2d(xp, bf, 2, H, p.rows, row_stride(x), BK, BM);
-      launch<STATS>(tx, tw, tx, p, dev, st);
+      Maps maps = {};
+      maps.a = make_tmap_2d(xp, bf, 2, H, p.rows, row_stride(x), BK, BM);
+      maps.b = make_tmap_2d(w.data_ptr(), bf, 2, H, V, row_stride(w), BK, p.bn / 2);
+      launch<STATS>(maps, p, dev, st);
     }
     launch_after("head join", head_join_kernel, dim3((p.rows + 31) / 32), dim3(1024), 0, st, p.stats, p.zt, p.targets,
                  parts, p.rows, V, logp ? logp->data_ptr<float>() + t0 : nullptr,
@@ -817,53 +890,60 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, at::Tensor> hea
   return {logp, entropy, lse};
 }
 
-void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
-              const at::Tensor& lse, const at::Tensor& coef, double inv_temp, at::Tensor& dx, at::Tensor& dw,
-              bool accumulate, int64_t piece) {
+// Returns dx (into `into` when it is given).
+at::Tensor head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& targets,
+                    const at::Tensor& lse, const at::Tensor& coef, double inv_temp,
+                    const c10::optional<at::Tensor>& into, at::Tensor& dw, bool accumulate, int64_t piece) {
   using namespace head;
   check_operands(x, w, targets, inv_temp);
   check_rows(lse, x, "lse");
   check_rows(coef, x, "coef");
   const int T = x.size(0), V = w.size(0), H = x.size(1);
-  TORCH_CHECK(dx.device() == x.device() && dx.scalar_type() == at::kBFloat16 && dx.dim() == 2 && dx.size(0) == T &&
-                  dx.size(1) == H && dx.stride(1) == 1 && (T <= 1 || dx.stride(0) % 8 == 0) &&
-                  reinterpret_cast<uintptr_t>(dx.data_ptr()) % 16 == 0,
-              "head: dx must be bf16 [T, H] with contiguous, 16-byte aligned rows");
-  TORCH_CHECK(dw.device() == x.device() && (dw.scalar_type() == at::kBFloat16 || dw.scalar_type() == at::kFloat) &&
-                  dw.dim() == 2 && dw.size(0) == V && dw.size(1) == H && dw.is_contiguous() &&
+  if (into)
+    TORCH_CHECK(into->device() == x.device() && into->scalar_type() == at::kBFloat16 && into->dim() == 2 &&
+                    into->size(0) == T && into->size(1) == H && into->stride(1) == 1 &&
+                    (T <= 1 || into->stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(into->data_ptr()) % 16 == 0,
+                "head: dx must be bf16 [T, H] with contiguous, 16-byte aligned rows");
+  const bool f32 = dw.scalar_type() == at::kFloat;
+  TORCH_CHECK(dw.device() == x.device() && (f32 || dw.scalar_type() == at::kBFloat16) && dw.dim() == 2 &&
+                  dw.size(0) == V && dw.size(1) == H && dw.is_contiguous() &&
                   reinterpret_cast<uintptr_t>(dw.data_ptr()) % 16 == 0,
               "head: dw must be contiguous bf16 or fp32 [V, H] on 16 bytes");
   TORCH_CHECK(piece >= 0, "head: piece must not be negative");
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor dx = into ? *into : at::empty({T, H}, x.options());
   if (T == 0) {
     if (!accumulate) dw.zero_();
-    return;
+    return dx;
   }
-  c10::cuda::CUDAGuard g(x.device());
-  const int dev = x.get_device();
+  const int dev = x.get_device(), sms = num_sms(dev);
   auto st = at::cuda::getCurrentCUDAStream();
-  // dz of one piece is the only [T, .] workspace: about 256 MB by default, in
-  // equal pieces of whole tiles
+  // dz of one piece is the only workspace as wide as the vocabulary: about 256 MB
+  // by default, in equal pieces of whole tiles
   int64_t width = piece;
   if (width == 0) width = std::max<int64_t>(4096, (int64_t(128) << 20) / T);
   const int64_t n_pieces = (V + width - 1) / width;
   if (piece == 0) width = ((V + n_pieces - 1) / n_pieces + kMaxBN - 1) / kMaxBN * kMaxBN;
   width = std::min<int64_t>((width + 7) / 8 * 8, ((int64_t)V + 7) / 8 * 8);
-  const int sms = num_sms(dev);
   // up to kTwoTerms rows dz is held as two bf16 terms, 2 T rows in all
   const int copies = T <= kTwoTerms ? 2 : 1, R = T * copies, r32 = (R + 31) / 32 * 32;
   const int splits = pick_splits((long)((R + 2 * BM - 1) / (2 * BM)) * ((H + kMaxBN - 1) / kMaxBN),
                                  (std::min<int64_t>(width, V) + BK - 1) / BK, (long)R * H, sms / 2);
-  at::Tensor dz = at::empty({R, width}, x.options());
-  at::Tensor xm = at::empty({R, H}, x.options());
-  at::Tensor acc = at::empty({(int64_t)splits * r32, H}, x.options().dtype(at::kFloat));
+  // workspace: dx parts fp32 [splits r32, H], dz bf16 [R, width], masked x bf16 [R, H]
+  const int64_t acc_bytes = (int64_t)splits * r32 * H * 4, dz_bytes = ((int64_t)R * width * 2 + 127) / 128 * 128;
+  at::Tensor ws = at::empty({acc_bytes + dz_bytes + (int64_t)R * H * 2}, x.options().dtype(at::kByte));
+  float* acc = reinterpret_cast<float*>(ws.data_ptr());
+  __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>((uint8_t*)ws.data_ptr() + acc_bytes);
+  __nv_bfloat16* xm = reinterpret_cast<__nv_bfloat16*>((uint8_t*)ws.data_ptr() + acc_bytes + dz_bytes);
   const long nvec = (long)T * H / 8;
   const int grid = (int)std::min<long>((nvec + 255) / 256, (long)sms * 8);
   launch_after("head mask rows", mask_rows_kernel, dim3(grid), dim3(256), 0, st, (const __nv_bfloat16*)x.data_ptr(),
-               row_stride(x), coef.data_ptr<float>(), (__nv_bfloat16*)xm.data_ptr(), T, H, copies);
-  auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap tx = make_tmap_2d(x.data_ptr(), bf, 2, H, T, row_stride(x), BK, BM);
-  CUtensorMap tacc = make_tmap_2d(acc.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, H, (uint64_t)splits * r32, H, 32,
-                                  32);
+               row_stride(x), coef.data_ptr<float>(), xm, T, H, copies);
+  const auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ff = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  Maps grad = {}, prods = {};
+  grad.a = make_tmap_2d(x.data_ptr(), bf, 2, H, T, row_stride(x), BK, BM);
+  prods.d = make_tmap_2d(acc, ff, 4, H, (uint64_t)splits * r32, H, 32, 32);
+  prods.b2 = make_tmap_2d(xm, bf, 2, H, R, H, 64, BK);
   Params p = {};
   p.rows = T; p.K = H;
   p.bn = kMaxBN;
@@ -873,31 +953,35 @@ void head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::
   p.targets = targets ? targets->data_ptr<long>() : nullptr;
   p.lse = lse.data_ptr<float>();
   p.coef = coef.data_ptr<float>();
-  p.low = copies == 2 ? (__nv_bfloat16*)dz.data_ptr() + (long)T * width : nullptr;
+  p.low = copies == 2 ? dz + (long)T * width : nullptr;
   p.low_ld = width;
   Params d = {};
   d.rows = R; d.cols = H;
   d.bn = kMaxBN;
   d.splits = splits;
   d.split_rows = r32;
+  d.dw_f32 = f32;
+  d.dw_add = accumulate;
   for (int64_t v0 = 0; v0 < V; v0 += width) {
     const int n = (int)std::min<int64_t>(width, V - v0);
-    at::Tensor wp = w.narrow(0, v0, n);
-    at::Tensor dwp = dw.narrow(0, v0, n);
+    const __nv_bfloat16* wp = (const __nv_bfloat16*)w.data_ptr() + v0 * row_stride(w);
     p.cols = n;
     p.v0 = (int)v0;
-    CUtensorMap tw = make_tmap_2d(wp.data_ptr(), bf, 2, H, n, row_stride(w), BK, kMaxBN / 2);
-    CUtensorMap td = make_tmap_2d(dz.data_ptr(), bf, 2, (n + 7) / 8 * 8, T, width, 64, 32);
-    launch<GRAD>(tx, tw, td, p, dev, st);
-    gemm_bf16(dz.narrow(1, 0, n), xm, dwp, true, true, 1.0, accumulate, c10::nullopt, 0);
-    CUtensorMap tz = make_tmap_2d(dz.data_ptr(), bf, 2, n, R, width, BK, BM);
-    CUtensorMap tk = make_tmap_2d(wp.data_ptr(), bf, 2, H, n, row_stride(w), 64, BK);
+    grad.b = make_tmap_2d(wp, bf, 2, H, n, row_stride(w), BK, kMaxBN / 2);
+    grad.d = make_tmap_2d(dz, bf, 2, (n + 7) / 8 * 8, T, width, 64, 32);
+    launch<GRAD>(grad, p, dev, st);
     d.K = n;
     d.add = v0 > 0;
-    launch<DX>(tz, tk, tacc, d, dev, st);
+    d.dw = (uint8_t*)dw.data_ptr() + v0 * H * (f32 ? 4 : 2);
+    prods.a = make_tmap_2d(dz, bf, 2, n, R, width, BK, BM);
+    prods.b = make_tmap_2d(wp, bf, 2, H, n, row_stride(w), 64, BK);
+    prods.a2 = make_tmap_2d(dz, bf, 2, n, R, width, 64, BK);
+    prods.d2 = f32 ? make_tmap_2d(d.dw, ff, 4, H, n, H, 32, 32) : make_tmap_2d(d.dw, bf, 2, H, n, H, 64, 32);
+    launch<PRODS>(prods, d, dev, st);
   }
-  launch_after("head sum parts", sum_parts_kernel, dim3(grid), dim3(256), 0, st, acc.data_ptr<float>(), splits, copies,
+  launch_after("head sum parts", sum_parts_kernel, dim3(grid), dim3(256), 0, st, (const float*)acc, splits, copies,
                (long)r32 * H, (__nv_bfloat16*)dx.data_ptr(), row_stride(dx), T, H);
+  return dx;
 }
 
 }  // namespace kore

@@ -733,7 +733,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_balance_fwd(const at::Tensor&
   auto st = at::cuda::getCurrentCUDAStream();
   // one block reads 128 KB in about the time that a second launch takes
   const bool one = (long)T * E <= 32768;
-  const int threads = one ? 1024 : 256;
+  const int threads = one ? 1024 : 512;
   const int per_block = threads / 32 * moe::kBalUnroll;
   const int blocks = one ? 1 : std::min((T + per_block - 1) / per_block, num_sms(probs.get_device()));
   at::Tensor part;

@@ -61,13 +61,12 @@ def head_bwd(x: torch.Tensor, w: torch.Tensor, targets: Optional[torch.Tensor], 
     inv = _inv_temp(temperature)
     if accumulate and dw is None:
         raise ValueError("accumulate needs dw")
-    if dx is None:
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     if dw is None:
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
     if x.is_cuda:
-        native().head_bwd(x, w, targets, lse, coef, inv, dx, dw, bool(accumulate), int(piece))
-        return dx, dw
+        return native().head_bwd(x, w, targets, lse, coef, inv, dx, dw, bool(accumulate), int(piece)), dw
+    if dx is None:
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     V = w.shape[0]
     live = (coef != 0).unsqueeze(1)
     xm = torch.where(live, x.float(), torch.zeros((), dtype=torch.float32))

@@ -209,22 +209,6 @@ def test_head_no_rows_and_refusals():
             f()
 
 
-@pytest.mark.parametrize("M,N,K,pad", [(77, 128, 200, 3), (300, 256, 131, 5), (1001, 512, 64, 7), (8, 64, 9, 7)])
-def test_gemm_ragged_contiguous_extents(M, N, K, pad):
-    """K (or M of a transposed A) need not be a multiple of 8 when the rows are padded."""
-    g = torch.Generator(device="cuda").manual_seed(M)
-    A = torch.full((M, K + pad + (-(K + pad)) % 8), float("nan"), device="cuda", dtype=torch.bfloat16)
-    A[:, :K] = torch.randn(M, K, generator=g, device="cuda")
-    B = torch.randn(K, N, generator=g, device="cuda").bfloat16()
-    want = A[:, :K].to(F8) @ B.to(F8)
-    tol = 2.0 ** -8 * (A[:, :K].to(F8).abs() @ B.to(F8).abs())
-    assert ((ops.mm(A[:, :K], B, b_t=False).to(F8) - want).abs() <= tol).all()
-    At = torch.full((K, M + pad + (-(M + pad)) % 8), float("nan"), device="cuda", dtype=torch.bfloat16)
-    At[:, :M] = A[:, :K].t()
-    assert ((ops.mm(At[:, :M], B, a_t=True, b_t=False).to(F8) - want).abs() <= tol).all()
-    assert ops.check_device_error() == 0
-
-
 # ------------------------------------------------------------------ embedding
 def _ids(T, V, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
