@@ -48,15 +48,14 @@ KORE_DEV float sum_pair(uint64_t v) {
   return lo + hi;
 }
 
-// Quantises the 8 values of this lane; the 16 lanes of a half warp share a
-// block. All lanes of the warp take part. Returns the bytes, sets the scale.
-KORE_DEV uint2 quantise(const uint4& raw, float& scale) {
-  // the largest magnitude, as bf16 bits in both halves (NaN > inf > finite)
-  uint32_t m = __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu),
-                        __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffff, m, o));
-  const uint32_t top = max(m & 0xffffu, m >> 16);
+// The largest magnitude of 8 values, as bf16 bits in both halves (NaN > inf > finite)
+KORE_DEV uint32_t magnitude2(const uint4& raw) {
+  return __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu),
+                  __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+}
+
+// Quantises 8 values of a block whose largest magnitude has the bf16 bits `top`.
+KORE_DEV uint2 quantise_by(const uint4& raw, uint32_t top, float& scale) {
   const float a = __uint_as_float(top << 16);
   float inv = 0.f;
   scale = 0.f;
@@ -88,6 +87,15 @@ KORE_DEV uint2 quantise(const uint4& raw, float& scale) {
   const uint32_t lo0 = __byte_perm(b[0], b[1], 0x0040), lo1 = __byte_perm(b[2], b[3], 0x0040);
   const uint32_t hi0 = __byte_perm(b[4], b[5], 0x0040), hi1 = __byte_perm(b[6], b[7], 0x0040);
   return make_uint2(__byte_perm(lo0, lo1, 0x5410), __byte_perm(hi0, hi1, 0x5410));
+}
+
+// Quantises the 8 values of this lane; the 16 lanes of a half warp share a
+// block. All lanes of the warp take part. Returns the bytes, sets the scale.
+KORE_DEV uint2 quantise(const uint4& raw, float& scale) {
+  uint32_t m = magnitude2(raw);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffff, m, o));
+  return quantise_by(raw, max(m & 0xffffu, m >> 16), scale);
 }
 
 // The 8 values that the bytes stand for. 0x4B000000 | (q + 128) is the float
@@ -339,6 +347,76 @@ __global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* __r
   }
 }
 
+// Any F: the blocks of up are not aligned to those of gate, and one block may
+// hold columns of both. One block of threads per row; a block's maximum is joined
+// in shared memory from the lanes that hold a part of it (at most three groups of
+// neighbouring lanes per warp).
+constexpr int kRowThreads = 512;
+constexpr int kMaxRowF = 5 * kRowThreads * 8;
+
+KORE_DEV void join_block_max(uint32_t* s_top, uint32_t mine, int blk, bool live) {
+  // lanes with the same block are neighbours: the first of them and their mask
+  const int lane = threadIdx.x & 31;
+  const int prev = __shfl_up_sync(0xffffffff, blk, 1), next = __shfl_down_sync(0xffffffff, blk, 1);
+  const uint32_t starts = __ballot_sync(0xffffffff, lane == 0 || prev != blk);
+  const uint32_t ends = __ballot_sync(0xffffffff, lane == 31 || next != blk);
+  const int lo = 31 - __clz(starts & (0xffffffffu >> (31 - lane)));
+  const int hi = __ffs(ends & (0xffffffffu << lane)) - 1;
+  const uint32_t group = (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+  const uint32_t top = __reduce_max_sync(group, live ? max(mine & 0xffffu, mine >> 16) : 0u);
+  if (lane == lo && top != 0) atomicMax(s_top + blk, top);
+}
+
+template <int VPT>
+__global__ void __launch_bounds__(kRowThreads) swiglu_row_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
+                                                                 __nv_bfloat16* __restrict__ a, Held h) {
+  __shared__ uint32_t s_top[2 * kMaxRowF / kBlock + 2];
+  const int F = h.H / 2, nvec = F / 8;
+  const long t = blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  uint4 g[VPT], u[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    g[i] = u[i] = make_uint4(0, 0, 0, 0);
+    if (j < nvec) {
+      g[i] = __ldg(reinterpret_cast<const uint4*>(gu + t * ldg) + j);
+      u[i] = __ldg(reinterpret_cast<const uint4*>(gu + t * ldg + F) + j);
+    }
+  }
+  for (int b = threadIdx.x; b < h.nb; b += blockDim.x) s_top[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    const bool live = j < nvec;
+    join_block_max(s_top, magnitude2(g[i]), live ? j / 16 : h.nb, live);
+    join_block_max(s_top, magnitude2(u[i]), live ? (nvec + j) / 16 : h.nb, live);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < h.nb; b += blockDim.x) {
+    float scale;
+    quantise_by(make_uint4(0, 0, 0, 0), s_top[b], scale);
+    h.s[t * h.nb + b] = scale;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    if (j < nvec) {
+      float scale;
+      reinterpret_cast<uint2*>(h.q + t * h.H)[j] = quantise_by(g[i], s_top[j / 16], scale);
+      reinterpret_cast<uint2*>(h.q + t * h.H + F)[j] = quantise_by(u[i], s_top[(nvec + j) / 16], scale);
+      uint64_t gf[4], uf[4];
+      unpack8(g[i], gf);
+      unpack8(u[i], uf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) gf[e] = f2_mul(f2_mul(gf[e], sigmoid(gf[e])), uf[e]);
+      reinterpret_cast<uint4*>(a + t * F)[j] = pack8(gf);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bfloat16* __restrict__ dout, long ldd,
                                                          __nv_bfloat16* __restrict__ dgu,
                                                          __nv_bfloat16* __restrict__ a, long T) {
@@ -525,8 +603,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_swiglu_save(const at::Tensor
   const Shape sh = shape_for(F / 8, T, kGluRows, dev);
   if (F % kBlock == 0) {
     launch_after("act8_swiglu_save", swiglu_kernel<true>, sh.grid, dim3(sh.threads), 0, st, gp, stride_of(gu), ap, h, T);
+  } else if (F <= kMaxRowF) {
+    const int nvec = F / 8, vpt = (nvec + kRowThreads - 1) / kRowThreads;
+    auto k = vpt == 1 ? swiglu_row_kernel<1> : vpt == 2 ? swiglu_row_kernel<2> : vpt == 3 ? swiglu_row_kernel<3>
+                                                                                         : swiglu_row_kernel<5>;
+    const int per = vpt == 4 ? 5 : vpt;
+    launch_after("act8_swiglu_save", k, dim3((unsigned)T), dim3(((nvec + per - 1) / per + 31) / 32 * 32), 0, st, gp,
+                 stride_of(gu), ap, h);
   } else {
-    // the block at the border holds columns of gate and of up: two passes
     const Shape ss = shape_for(h.H / 8, T, kSaveRows, dev);
     launch_after("act8_swiglu_save", save_kernel, ss.grid, dim3(ss.threads), 0, st, gp, stride_of(gu), h, T);
     launch_after("act8_swiglu_save", swiglu_kernel<false>, sh.grid, dim3(sh.threads), 0, st, gp, stride_of(gu), ap, h, T);

@@ -125,6 +125,19 @@ KORE_DEV void tma_reduce_add_2d(const CUtensorMap* d, const void* smem_src, int 
       : "memory");
 }
 
+// 64 accumulator columns of this lane's row, both loads in flight
+KORE_DEV void load64(float (&f)[64], uint32_t from) {
+  uint32_t a[32], b[32];
+  tmem_ld32(from, a);
+  tmem_ld32(from + 32, b);
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    f[i] = __uint_as_float(a[i]);
+    f[32 + i] = __uint_as_float(b[i]);
+  }
+}
+
 // groups of 8 row blocks walk the columns together, so a B tile is read
 // from HBM once per 2048 rows and the group's A rows stay in L2
 KORE_DEV void tile_coords(int t, int num_m, int num_n, int& tm, int& tn) {
@@ -344,70 +357,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_cluster(tempty_leader[acc]);
       };
       if (M == STATS) {
-        float v[kMaxBN / 2];
+        // the row's columns stay in registers: first the maximum, then the sums
+        // against it, each in four independent chains (two warps per scheduler
+        // cannot hide a serial one)
+        constexpr int kCols = kMaxBN / 2;
+        uint32_t v[kCols];
         bool ok = true;
         for (int c0 = w.k0; c0 < w.k1; c0 += part, ++it) {
           const int acc = it & 1;
           if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { ok = false; break; }
           tc_fence_after();
+          const uint32_t from = t_row + acc * kMaxBN;
+          if (c0 == w.k0) {
 #pragma unroll
-          for (int j = 0; j < kMaxBN / 64; ++j)
-            if (32 * j < cols) {
-              uint32_t r[32];
-              tmem_ld32(t_row + acc * kMaxBN + 32 * j, r);
-              tmem_wait_ld();
-              if (c0 == w.k0) {
+            for (int j = 0; j < kCols / 32; ++j)
+              if (32 * j < cols) tmem_ld32(from + 32 * j, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * j));
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[32 * j + i] = __uint_as_float(r[i]);
-              } else {
+            for (int j = 0; j < kCols / 32; ++j)
+              if (32 * j < cols) {
+                uint32_t r[32];
+                tmem_ld32(from + 32 * j, r);
+                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[32 * j + i] += __uint_as_float(r[i]);
+                for (int i = 0; i < 32; ++i)
+                  v[32 * j + i] = __float_as_uint(__uint_as_float(v[32 * j + i]) + __uint_as_float(r[i]));
               }
-            }
+          }
           release(acc);
         }
         if (!ok) { *abort_flag = 1; break; }
-        float m = -INFINITY, s = 0.f, u = 0.f;
+        if (cols < kCols) {
 #pragma unroll
-        for (int j = 0; j < kMaxBN / 64; ++j)
-          if (32 * j < cols) {
-            float* r = v + 32 * j;
-            if (32 * j + 32 > cols) {
+          for (int i = 0; i < kCols; ++i)
+            if (i >= cols) v[i] = 0xff800000u;  // -inf: not a column of the vocabulary
+        }
+        if (tc >= 0) {
+          uint32_t z = 0;
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * j + i >= cols) r[i] = -INFINITY;  // not a column of the vocabulary
-            }
-            const int ti = tc - 32 * j;
-            if (ti >= 0 && ti < 32) {
-              float z = 0.f;
+          for (int i = 0; i < kCols; ++i)
+            if (i == tc) z = v[i];
+          p.zt[row] = __uint_as_float(z) * p.scale;
+        }
+        float top[4];
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i == ti) z = r[i];
-              p.zt[row] = z * p.scale;
-            }
-            float cm = r[0];
+        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(v[i]);
 #pragma unroll
-            for (int i = 1; i < 32; ++i) cm = fmaxf(cm, r[i]);
-            const float nm = fmaxf(m, cm * p.scale);
-            const float base = nm == -INFINITY ? 0.f : nm;  // all columns so far -inf: keep their terms 0
-            const float d = m == -INFINITY ? 0.f : m - base;
-            const float corr = ex2(d);
-            u = corr * (u + d * s);
-            s *= corr;
-            m = nm;
-            if (p.entropy) {
+        for (int i = 4; i + 8 <= kCols; i += 8)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float zr = fmaf(r[i], p.scale, -base);
-                const float e = ex2(zr);
-                s += e;
-                u += e == 0.f ? 0.f : e * zr;
-              }
-            } else {
+          for (int e = 0; e < 4; ++e)
+            top[e] = fmax3f(top[e], __uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s += ex2(fmaf(r[i], p.scale, -base));
-            }
-          }
+        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(v[kCols - 4 + e]));
+        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
+        const float base = m == -INFINITY ? 0.f : m;  // all columns -inf: their terms are 0
+        const uint64_t scale2 = f2_pack(p.scale, p.scale), base2 = f2_pack(-base, -base);
+        uint64_t s2[4] = {0, 0, 0, 0}, u2[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kCols; i += 2) {
+          float z0, z1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, base2), z0, z1);
+          const uint64_t e = f2_pack(ex2(z0), ex2(z1));
+          s2[(i / 2) & 3] = f2_add(s2[(i / 2) & 3], e);
+          // (0 times -inf is 0 here)
+          if (p.entropy) u2[(i / 2) & 3] = f2_fma(e, f2_pack(fmaxf(z0, -1e30f), fmaxf(z1, -1e30f)), u2[(i / 2) & 3]);
+        }
+        float lo, hi;
+        f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), lo, hi);
+        const float s = lo + hi;
+        f2_unpack(f2_add(f2_add(u2[0], u2[1]), f2_add(u2[2], u2[3])), lo, hi);
+        const float u = lo + hi;
         if (live) {
           const size_t o = (size_t)(2 * w.tn + half) * p.rows + row, plane = (size_t)2 * num_n * p.rows;
           p.stats[o] = m;
@@ -439,17 +459,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint4 out[8];
           if (M == GRAD) {
             float f[64];
+            load64(f, t_row + acc * kMaxBN + c0);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t r[32];
-              tmem_ld32(t_row + acc * kMaxBN + c0 + 32 * h, r);
-              tmem_wait_ld();
+            for (int i = 0; i < 64; ++i) f[i] = -c * ex2(fmaf(f[i], p.scale, -lse2));
+            if (c == 0.f || c0 + 64 > cols) {
+              // coefficient 0, or past the piece's last column: 0
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float e = ex2(fmaf(__uint_as_float(r[i]), p.scale, -lse2));
-                // coefficient 0, or past the piece's last column: 0
-                f[32 * h + i] = c == 0.f || c0 + 32 * h + i >= cols ? 0.f : -c * e;
-              }
+              for (int i = 0; i < 64; ++i)
+                if (c == 0.f || c0 + i >= cols) f[i] = 0.f;
             }
             const int ti = tc - c0;
             if (ti >= 0 && ti < 64) {
@@ -477,14 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
           } else if (w.dw && !p.dw_f32) {
             float f[64];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t r[32];
-              tmem_ld32(t_row + acc * kMaxBN + c0 + 32 * h, r);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) f[32 * h + i] = __uint_as_float(r[i]);
-            }
+            load64(f, t_row + acc * kMaxBN + c0);
             if (p.dw_add && live) {  // one rounding of the sum: no bf16 reduction of a rounded tile
               const __nv_bfloat16* old = (const __nv_bfloat16*)p.dw + (size_t)row * p.cols + n0 + c0;
 #pragma unroll

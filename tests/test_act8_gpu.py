@@ -89,7 +89,8 @@ def test_rmsnorm_save_and_load(T, H):
     assert ((hn8.to(F8) - want).abs() <= (2.0 ** -8 * 1.01 + 2e-5) * want.abs()).all()
 
 
-@pytest.mark.parametrize("T,F", [(0, 8), (1, 8), (3, 64), (7, 128), (33, 256), (21, 200), (130, 2048), (5, 17408)])
+@pytest.mark.parametrize("T,F", [(0, 8), (1, 8), (3, 64), (7, 128), (33, 256), (21, 200), (130, 2048), (5, 17408),
+                                 (3, 5000), (9, 11112), (4, 15008), (2, 20488), (40, 1368)])
 @pytest.mark.parametrize("pad", [0, 8])
 def test_swiglu_save_and_backward(T, F, pad):
     g = torch.Generator(device="cuda").manual_seed(F)
