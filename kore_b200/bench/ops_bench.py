@@ -6,7 +6,10 @@ Times RMSNorm forward / backward (with the residual gradient), q/k RMSNorm +
 RoPE forward, SwiGLU forward / backward, the fused vocabulary log-prob +
 gradient (one 2,048-row chunk of the LM head's logits, overwritten in place
 by the gradient) and the AdamW step over one decoder layer's MLP weights
-(bf16 parameters and gradients, fp32 moments, stochastic rounding). Each is
+(bf16 parameters and gradients, fp32 moments, stochastic rounding); further the
+8-bit activation checkpoints with their RMSNorm and SwiGLU, the embedding with
+its sorted gradient, the router's balance loss, and the head in pieces of the
+vocabulary (bound by the tensor cores: read its time). Each is
 timed with CUDA events on the launching stream after warm-up, with L2
 flushed between iterations; the achieved figure is the kernel's compulsory
 HBM bytes (each operand read or written once) over the median time, also
@@ -17,11 +20,13 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import os
 
 import torch
 
 from .. import ops
+from ..ops import act8, moe, vocab
 from ..ops import reference as ref
 from .timing import median_ms, time_cuda
 
@@ -79,6 +84,31 @@ def cases(T: int, dev):
     g = torch.randn(n, **bf) * 1e-3
     m, v = torch.zeros(n, **f32), torch.zeros(n, **f32)
     yield ("adamw_bf16_sr", lambda: ops.adamw_step(p, g, m, v, lr=1e-5, wd=0.1, step=3), n * (2 * 2 + 2 + 2 * 8))
+    del p, g, m, v
+    x, w = torch.randn(T, H, **bf), 1 + 0.1 * torch.randn(H, **bf)
+    a = act8.save(x)
+    held = 1 + 4 / act8.BLOCK
+    yield ("act8_rmsnorm_save", lambda: act8.rmsnorm_save(x, w, 1e-6), T * H * (4 + held))
+    yield ("act8_rmsnorm_load", lambda: act8.rmsnorm_load(a, w, 1e-6), T * H * (4 + held))
+    gu, dh = torch.randn(T, 2 * FF, **bf), torch.randn(T, FF, **bf)
+    ag = act8.save(gu)
+    yield ("act8_swiglu_save", lambda: act8.swiglu_save(gu), T * FF * (6 + 2 * held))
+    yield ("act8_swiglu_bwd", lambda: act8.swiglu_bwd(dh, ag), T * FF * (8 + 2 * held))
+    del gu, dh, a, ag
+    probs = torch.softmax(torch.randn(T, 128, **f32), -1)
+    idx = probs.topk(8, -1).indices.int()
+    gain = moe.balance_loss(probs, idx)[2]
+    yield ("balance_loss", lambda: moe.balance_loss(probs, idx), T * (128 * 4 + 8 * 4))
+    yield ("balance_bwd", lambda: moe.balance_bwd(probs, gain), 2 * T * 128 * 4)
+    ids = torch.exp(torch.rand(T, device=dev, dtype=torch.float64) * math.log(V)).long().clamp_(1, V) - 1
+    table, dtable = torch.randn(V, H, **bf), torch.empty(V, H, **bf)
+    yield ("embed", lambda: vocab.embed(ids, table, 2.0), 2 * T * H * 2)
+    yield ("embed_grad_sorted", lambda: vocab.embed_grad(ids, x, dtable, accumulate=False), (T + V) * H * 2)
+    tg = torch.randint(0, V, (T,), device=dev)
+    coef = torch.full((T,), -1.0 / T, **f32)
+    lse = vocab.head_fwd(x, table, tg)[2]
+    yield ("head_pieces_fwd", lambda: vocab.head_fwd(x, table, tg), (T + V) * H * 2)
+    yield ("head_pieces_bwd", lambda: vocab.head_bwd(x, table, tg, lse, coef, dw=dtable), 2 * (T + V) * H * 2)
 
 
 def main(argv=None):

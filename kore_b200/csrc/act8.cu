@@ -10,7 +10,10 @@
 //
 // All kernels are one pass over HBM: 16 lanes hold a block (8 values each, one
 // 16-byte bf16 vector), its maximum is an integer maximum over the values'
-// magnitude bits. They are bound by HBM.
+// magnitude bits. They are bound by HBM (copy rate 6.5 TB/s), measured at
+//   16384 x 5120   RMSNorm + save 69 us, 6.1 TB/s; load + RMSNorm 66 us, 6.4 TB/s
+//                  save 42 us, 6.0 TB/s; load 44 us, 5.8 TB/s
+//   8192 x 17408   SwiGLU + save 193 us, 6.0 TB/s; SwiGLU backward 229 us, 6.3 TB/s
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -350,7 +353,8 @@ __global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* __r
 // Any F: the blocks of up are not aligned to those of gate, and one block may
 // hold columns of both. One block of threads per row; a block's maximum is joined
 // in shared memory from the lanes that hold a part of it (at most three groups of
-// neighbouring lanes per warp).
+// neighbouring lanes per warp). 8192 x 17400: 255 us, 4.5 TB/s (rows wait for the
+// slowest warp at each of the two barriers); 4877 x 4048: 34 us.
 constexpr int kRowThreads = 512;
 constexpr int kMaxRowF = 5 * kRowThreads * 8;
 

@@ -61,7 +61,8 @@ def _check_fwd(o, logp, ent, lse):
 
 
 SHAPES = [(1, 8, 8), (1, 1, 64), (3, 17, 72), (129, 1000, 256), (127, 32000, 256), (257, 4097, 264), (300, 513, 1032),
-          (1000, 9999, 640), (64, 151936, 128), (513, 20011, 5120)]
+          (1000, 9999, 640), (64, 151936, 128), (2, 5000, 5120),
+          (33001, 130, 64), (513, 20011, 5120)]
 
 
 @pytest.mark.parametrize("T,V,H", SHAPES)
@@ -181,6 +182,30 @@ def test_head_logits_of_minus_inf():
         assert torch.allclose(a, b, rtol=2e-5, atol=2e-5)
 
 
+def test_head_without_coefficients_and_into_given_outputs():
+    T, V, H = 150, 900, 128
+    x, w, y, coef = _inputs(T, V, H, seed=7)
+    _, _, lse = vocab.head_fwd(x, w, y)
+    dx, dw = vocab.head_bwd(x, w, y, lse, torch.zeros_like(coef))
+    assert (dx == 0).all() and (dw == 0).all()
+    dx, dw = vocab.head_bwd(x, w, y, lse, coef)
+    wide = torch.full((T, H + 8), 3.0, device="cuda", dtype=torch.bfloat16)
+    got, _ = vocab.head_bwd(x, w, y, lse, coef, dx=wide[:, :H], dw=torch.full_like(dw, float("nan")))
+    assert torch.equal(wide[:, :H], dx) and (wide[:, H:] == 3.0).all() and got.data_ptr() == wide.data_ptr()
+    # bf16 dW is added to with one rounding of the sum
+    base = torch.randn(V, H, device="cuda").bfloat16()
+    exact = torch.zeros(V, H, device="cuda")
+    vocab.head_bwd(x, w, y, lse, coef, dw=exact)
+    acc = base.clone()
+    vocab.head_bwd(x, w, y, lse, coef, dw=acc, accumulate=True)
+    assert torch.equal(acc, (base.float() + exact).bfloat16())
+    # no targets: the gradient of -coef lse
+    dx, _ = vocab.head_bwd(x, w, None, lse, coef)
+    p = torch.softmax(x.to(F8) @ w.to(F8).t(), -1)
+    want = -(coef.to(F8)[:, None] * p) @ w.to(F8)
+    assert ((dx.to(F8) - want).abs() <= 2.0 ** -7 * (coef.to(F8).abs()[:, None] * p) @ w.to(F8).abs() + 1e-9).all()
+
+
 def test_head_no_rows_and_refusals():
     x, w, y, coef = _inputs(4, 32, 16)
     e = torch.empty(0, 16, device="cuda", dtype=torch.bfloat16)
@@ -260,6 +285,21 @@ def test_embed_lookup(T, V, H):
         got = vocab.embed(ids, table, scale)
         want = torch.where(ok[:, None], table[torch.where(ok, ids, 0)].float() * scale, torch.zeros((), device="cuda")).bfloat16()
         assert torch.equal(got, want)
+        into = torch.full((T, H), 5.0, device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(vocab.embed(ids, table, scale, out=into), want) and torch.equal(into, want)
+
+
+def test_embed_grad_of_one_token_everywhere():
+    """A single id: every chunk is one segment; and its neighbours stay zero."""
+    for T in (1, 31, 32, 33, 255, 256, 257, 1024, 1025, 5000):
+        dy = torch.randn(T, 264, device="cuda").bfloat16()
+        ids = torch.full((T,), 2, dtype=torch.long, device="cuda")
+        got = vocab.embed_grad(ids, dy, torch.full((5, 264), float("nan"), device="cuda"), accumulate=False)
+        want = dy.to(F8).sum(0)
+        assert ((got[2].to(F8) - want).abs() <= (T + 2) * 2.0 ** -24 * dy.to(F8).abs().sum(0)).all()
+        assert (got[[0, 1, 3, 4]] == 0).all()
+        ids = torch.full((T,), 9, dtype=torch.long, device="cuda")          # none in the table
+        assert (vocab.embed_grad(ids, dy, torch.full((5, 264), 1.0, device="cuda"), accumulate=False) == 0).all()
 
 
 def test_embed_grad_keeps_rows_apart():
