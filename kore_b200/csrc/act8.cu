@@ -518,31 +518,48 @@ int norm_vpt(int nvec) { return nvec > 128 ? 4 : 1; }
 
 }  // namespace act8
 
-void act8_save(const at::Tensor& x, at::Tensor& q, at::Tensor& s) {
+// Returns (q, scales): the given ones (both or none), or new ones.
+std::tuple<at::Tensor, at::Tensor> act8_save(const at::Tensor& x, const c10::optional<at::Tensor>& q_into,
+                                             const c10::optional<at::Tensor>& s_into) {
   using namespace act8;
   check_bf16(x, "x");
-  Held h = check_held(q, s);
-  TORCH_CHECK(q.device() == x.device() && q.size(0) == x.size(0) && q.size(1) == x.size(1), "act8: q must match x");
   const long T = x.size(0);
-  if (T == 0) return;
+  TORCH_CHECK(q_into.has_value() == s_into.has_value(), "act8: give q and scales, or neither");
   c10::cuda::CUDAGuard g(x.device());
+  at::Tensor q, s;
+  if (q_into) {
+    q = *q_into;
+    s = *s_into;
+    check_held(q, s);
+    TORCH_CHECK(q.device() == x.device() && q.size(0) == T && q.size(1) == x.size(1), "act8: q must match x");
+  } else {
+    std::tie(q, s) = new_held(T, x.size(1), x);
+  }
+  if (T == 0) return {q, s};
+  const Held h = held_of(q, s);
   const Shape sh = shape_for(h.H / 8, T, kSaveRows, x.get_device());
   launch_after("act8_save", save_kernel, sh.grid, dim3(sh.threads), 0, at::cuda::getCurrentCUDAStream(),
                (const __nv_bfloat16*)x.data_ptr(), stride_of(x), h, T);
+  return {q, s};
 }
 
-void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out) {
+// Returns the values as bf16, in `into` when it is given.
+at::Tensor act8_load(const at::Tensor& q, const at::Tensor& s, const c10::optional<at::Tensor>& into) {
   using namespace act8;
   Held h = check_held(q, s);
-  check_bf16(out, "out");
-  TORCH_CHECK(q.device() == out.device() && q.size(0) == out.size(0) && q.size(1) == out.size(1),
-              "act8: out must match the held shape");
   const long T = q.size(0);
-  if (T == 0) return;
+  if (into) {
+    check_bf16(*into, "out");
+    TORCH_CHECK(q.device() == into->device() && q.size(0) == into->size(0) && q.size(1) == into->size(1),
+                "act8: out must match the held shape");
+  }
   c10::cuda::CUDAGuard g(q.device());
+  at::Tensor out = into ? *into : at::empty({T, h.H}, s.options().dtype(at::kBFloat16));
+  if (T == 0) return out;
   const Shape sh = shape_for(h.H / 8, T, kLoadRows, q.get_device());
   launch_after("act8_load", load_kernel, sh.grid, dim3(sh.threads), 0, at::cuda::getCurrentCUDAStream(), h,
                (__nv_bfloat16*)out.data_ptr(), stride_of(out), T);
+  return out;
 }
 
 // Returns (hn, rstd, q, scales).

@@ -126,8 +126,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_balance_fwd(const at::Tensor&
                                                                const c10::optional<at::Tensor>& mask, double coef);
 at::Tensor moe_balance_bwd(const at::Tensor& probs, const at::Tensor& gain, const c10::optional<at::Tensor>& mask,
                            double dloss, const c10::optional<at::Tensor>& dlogits);
-void act8_save(const at::Tensor& x, at::Tensor& q, at::Tensor& s);
-void act8_load(const at::Tensor& q, const at::Tensor& s, at::Tensor& out);
+std::tuple<at::Tensor, at::Tensor> act8_save(const at::Tensor& x, const c10::optional<at::Tensor>& q_into,
+                                             const c10::optional<at::Tensor>& s_into);
+at::Tensor act8_load(const at::Tensor& q, const at::Tensor& s, const c10::optional<at::Tensor>& into);
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_save(const at::Tensor& x,
                                                                              const at::Tensor& w, double eps);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_load(const at::Tensor& q, const at::Tensor& s,

@@ -71,23 +71,23 @@ def _values(a: Act8) -> torch.Tensor:
 
 def save(x: torch.Tensor, out: Optional[Act8] = None) -> Act8:
     """The 8-bit copy of x [T, H]."""
-    a = out if out is not None else empty(x.shape[0], x.shape[1], x.device)
     if x.is_cuda:
-        native().act8_save(x, a.q, a.s)
-    else:
-        _quantise(x, a)
+        q, s = native().act8_save(x, None if out is None else out.q, None if out is None else out.s)
+        return Act8(q, s)
+    a = out if out is not None else empty(x.shape[0], x.shape[1], x.device)
+    _quantise(x, a)
     return a
 
 
 def load(a: Act8, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that ``a`` stands for, rounded to bf16."""
-    if out is None:
-        out = torch.empty(a.shape, dtype=dtype, device=a.q.device)
+    """The values that ``a`` stands for, rounded to ``dtype`` (CUDA: bf16)."""
     if a.q.is_cuda:
-        native().act8_load(a.q, a.s, out)
-    else:
-        out.copy_(_values(a))
-    return out
+        if dtype != torch.bfloat16:
+            raise ValueError("act8: CUDA checkpoints load as bf16")
+        return native().act8_load(a.q, a.s, out)
+    if out is None:
+        out = torch.empty(a.shape, dtype=dtype)
+    return out.copy_(_values(a))
 
 
 def rmsnorm_save(x: torch.Tensor, w: torch.Tensor, eps: float):

@@ -41,6 +41,9 @@ def test_save_and_load(T, H, pad):
     wide = torch.full((T, H + 8), 7.0, device="cuda", dtype=torch.bfloat16)
     act8.load(a, out=wide[:, :H])
     assert torch.equal(wide[:, :H], back) and (wide[:, H:] == 7.0).all()
+    into = act8.empty(T, H, "cuda")
+    again = act8.save(x, out=into)
+    assert torch.equal(into.q, a.q) and torch.equal(into.s, a.s) and again.q.data_ptr() == into.q.data_ptr()
     if T:
         v, xd = _values(a), x.to(F8)
         amax = torch.nn.functional.pad(xd.abs(), (0, -H % 128)).view(T, -1, 128).amax(-1).repeat_interleave(128, 1)[:, :H]
@@ -153,7 +156,8 @@ def test_refusals():
     big = torch.zeros(2, 8200, device="cuda", dtype=torch.bfloat16)
     short = act8.Act8(a.q, a.s[:3])
     for f in (lambda: act8.save(x.float()), lambda: act8.save(x[:, :12]), lambda: act8.save(x.t()),
-              lambda: act8.save(x[:, 4:20]), lambda: act8.load(short), lambda: act8.load(act8.Act8(a.q.float(), a.s)),
+              lambda: act8.save(x[:, 4:20]), lambda: act8.load(short), lambda: act8.load(a, dtype=torch.float32),
+              lambda: act8.save(x, out=short), lambda: act8.load(act8.Act8(a.q.float(), a.s)),
               lambda: act8.load(a, out=torch.empty(4, 72, device="cuda", dtype=torch.bfloat16)),
               lambda: act8.rmsnorm_save(x, w[:32], 1e-6), lambda: act8.rmsnorm_save(x, w.float(), 1e-6),
               lambda: act8.rmsnorm_save(big, torch.ones(8200, device="cuda", dtype=torch.bfloat16), 1e-6),
