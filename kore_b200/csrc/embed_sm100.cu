@@ -274,7 +274,7 @@ __global__ void segments_kernel(const u64* __restrict__ keys, const __nv_bfloat1
     const bool beyond = at > first;     // (walk) only the segment that is still open
     if (!beyond) begins = s_id[0] != s_id[1];
     if (beyond && s_id[0] != s_id[1]) break;
-    bool done = false;
+    bool done = false, open = begins;   // open: the segment being summed begins in this chunk
     for (int i0 = 0; i0 < n && !done && mine; i0 += 8) {
       uint4 v[8];
       Old<G> old[8];
@@ -298,23 +298,25 @@ __global__ void segments_kernel(const u64* __restrict__ keys, const __nv_bfloat1
         for (int e = 0; e < 8; ++e) sum[e] += f[e];
         const bool ends = s_id[i + 2] != id;
         if (!ends && (walk || i + 1 < n)) continue;
-        if (begins && ends) {
+        if (open && ends) {
           write_row(dtable + (size_t)id * H, j, sum, scale, add != 0, old[u]);
         } else if (!walk) {
-          float4* p = reinterpret_cast<float4*>(part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * H) + 2 * j;
+          float4* p = reinterpret_cast<float4*>(part + ((size_t)blockIdx.x * 2 + (open ? 1 : 0)) * H) + 2 * j;
           p[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
           p[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-        begins = true;
+        open = true;
         if (beyond) done = true;
       }
     }
-    // walk on while the last segment is open and began in this block's chunk
+    // walk on while the last segment is open and began in this block's chunk; every test
+    // here is the same for all threads, those without columns load keys for the others
+    begins = begins || s_id[1] != s_id[n];
     if (!walk || s_id[n + 1] != s_id[n] || s_id[n] >= V) break;
     if (beyond && s_id[n] != s_id[0]) break;   // it has ended; what is open now began later
-    if (!begins && s_id[1] == s_id[n]) break;
+    if (!begins) break;
   }
 }
 

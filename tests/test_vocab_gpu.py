@@ -302,6 +302,41 @@ def test_embed_grad_of_one_token_everywhere():
         assert (vocab.embed_grad(ids, dy, torch.full((5, 264), 1.0, device="cuda"), accumulate=False) == 0).all()
 
 
+def _check_grad(ids, V, H, dt, seed=0):
+    T = len(ids)
+    g = torch.Generator(device="cuda").manual_seed(seed + T + H)
+    dy = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    ok = (ids >= 0) & (ids < V)
+    want, mag = torch.zeros(V, H, dtype=F8, device="cuda"), torch.zeros(V, H, dtype=F8, device="cuda")
+    want.index_put_((ids[ok],), dy[ok].to(F8), accumulate=True)
+    mag.index_put_((ids[ok],), dy[ok].to(F8).abs(), accumulate=True)
+    count = torch.bincount(ids[ok], minlength=V).to(F8)[:, None]
+    unit = 2.0 ** -24 if dt == torch.float32 else 2.0 ** -8
+    # an fp32 sum of n terms is off by at most n roundings of its magnitudes
+    tol = (count + 2) * 2.0 ** -24 * mag
+    got = vocab.embed_grad(ids, dy, torch.full((V, H), float("nan"), device="cuda", dtype=dt), accumulate=False)
+    assert ((got.to(F8) - want).abs() <= 1.001 * (tol + unit * want.abs()) + 1e-30).all()
+    base = torch.randn(V, H, generator=g, device="cuda").to(dt)
+    acc = vocab.embed_grad(ids, dy, base.clone())
+    assert ((acc.to(F8) - base.to(F8) - want).abs() <= 1.001 * (tol + 2 * unit * (base.to(F8).abs() + mag)) + 1e-30).all()
+    again = vocab.embed_grad(ids, dy, torch.empty(V, H, device="cuda", dtype=dt), accumulate=False)
+    assert torch.equal(again, got)
+
+
+# widths whose last 1024 columns (128 threads) leave threads of the block without columns, and their neighbours
+@pytest.mark.parametrize("H", [8, 16, 24, 32, 40, 48, 1024, 1032, 1040, 1064, 1072, 2056])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_embed_grad_of_few_tokens_with_long_runs(H, dt):
+    """Runs that begin inside four sorted positions and end several such groups later."""
+    for runs in ([6, 14, 3], [1, 13], [2, 3, 9, 1, 17], [5, 40, 1, 1, 30, 7], [3, 200, 53], [64, 65, 66, 61]):
+        ids = torch.repeat_interleave(torch.arange(len(runs), device="cuda"), torch.tensor(runs, device="cuda"))
+        ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(H)).cuda()]
+        _check_grad(ids, len(runs) + 2, H, dt)
+        _check_grad(ids, len(runs) - 1, H, dt)              # the last run lies outside the table
+    for T in (20, 100, 255, 256):
+        _check_grad(_ids(T, 1000, T), 1000, H, dt)
+
+
 def test_embed_grad_keeps_rows_apart():
     """inf and NaN stay in the rows of their own tokens."""
     T, V, H = 300, 40, 64
