@@ -337,13 +337,15 @@ __global__ void join_kernel(const u64* __restrict__ keys, const float* __restric
   const int chunks = (T + kChunk - 1) / kChunk;
   if (threadIdx.x == 0) s_last = chunks;
   __syncthreads();
+  int last;
   for (int d0 = c + 1;; d0 += blockDim.x) {
     const int d = d0 + threadIdx.x;
     if (d < chunks && key_id(keys[d * kChunk]) != id) atomicMin(&s_last, d);
     __syncthreads();
-    if (s_last < chunks || d0 + (int)blockDim.x >= chunks) break;
+    last = s_last;
+    if (last < chunks || d0 + (int)blockDim.x >= chunks) break;
+    __syncthreads();   // all have read it before the next turn lowers it
   }
-  const int last = s_last;
   const int j = blockIdx.y * blockDim.x + threadIdx.x;
   if (j * 8 >= H) return;
   float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};

@@ -337,6 +337,19 @@ def test_embed_grad_of_few_tokens_with_long_runs(H, dt):
         _check_grad(_ids(T, 1000, T), 1000, H, dt)
 
 
+@pytest.mark.parametrize("H,run", [(264, 4200), (512, 2300), (1024, 4300), (1024, 9000)])
+def test_embed_grad_of_a_long_run_before_others(H, run):
+    """One id on more positions than a block of threads looks at in one turn, and
+    many others behind it: its sum takes its own parts only, and repeats."""
+    g = torch.Generator(device="cuda").manual_seed(run)
+    ids = torch.cat([torch.full((run,), 3, dtype=torch.long, device="cuda"),
+                     torch.randint(0, 3, (700,), generator=g, device="cuda"),
+                     torch.randint(4, 500, (6000,), generator=g, device="cuda")])
+    ids = ids[torch.randperm(len(ids), generator=g, device="cuda")]
+    for seed in range(8):
+        _check_grad(ids, 500, H, torch.float32, seed)
+
+
 def test_embed_grad_keeps_rows_apart():
     """inf and NaN stay in the rows of their own tokens."""
     T, V, H = 300, 40, 64
