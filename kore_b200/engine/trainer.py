@@ -206,6 +206,11 @@ class CausalLMTrainer:
         self._planned_tokens = micro_tokens
         return keep
 
+    def share_balance_loss(self, n_micro: int) -> None:
+        """The routers' balance loss of a step is the mean over its micro-batches and
+        over ranks: every loop over micro-batches of :attr:`eng` calls this first."""
+        self.eng.aux_scale = 1.0 / (max(1, n_micro) * self.ctx.world)
+
     @torch.no_grad()
     def train_step_device(self, ids: torch.Tensor, loss_mask: Optional[torch.Tensor] = None
                           ) -> torch.Tensor:
@@ -221,7 +226,7 @@ class CausalLMTrainer:
         self.eng.zero_grad()
         loss = torch.zeros((), dtype=torch.float32, device=ids.device)
         starts = list(range(0, B, self.mbs))
-        self.eng.aux_scale = 1.0 / (max(1, len(starts)) * self.ctx.world)
+        self.share_balance_loss(len(starts))
         shuttle = self._moment_shuttle(len(starts), min(self.mbs, B) * S)
         for i, s in enumerate(starts):
             if shuttle is not None:
@@ -257,7 +262,7 @@ class CausalLMTrainer:
                 ntok = 0
             chunks[-1].append(j)
             ntok += len(seqs[j])
-        self.eng.aux_scale = 1.0 / (max(1, len(chunks)) * self.ctx.world)
+        self.share_balance_loss(len(chunks))
         for chunk in chunks:
             b = Batch.from_sequences([torch.as_tensor(seqs[j]) for j in chunk],
                                      [torch.as_tensor(label_masks[j]) for j in chunk], device=dev)

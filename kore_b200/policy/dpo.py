@@ -200,6 +200,7 @@ class DPOTrainer:
         total = 0.0
         starts = list(range(0, len(pairs), self.micro_pairs))
         batches = [self._batch([x for p in pairs[s0:s0 + self.micro_pairs] for x in p]) for s0 in starts]
+        self.tr.share_balance_loss(len(batches))
         if getattr(self, "_ref_stream", None) is not None:
             # streamed / gathered reference: each layer moves once for the whole step
             ref_lps = [lp for lp, _ in self.ref.token_logprobs_many(batches)]

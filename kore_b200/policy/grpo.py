@@ -531,7 +531,9 @@ class GRPOTrainer:
         loss_sum = 0.0
         kl_sum, kl_n = 0.0, 0
         trainer_old = cfg.old_logp_source == "trainer"
-        for chunk in self._pack(self._rows(train), budget):
+        chunks = list(self._pack(self._rows(train), budget))
+        self.trainer.share_balance_loss(len(chunks))
+        for chunk in chunks:
             b, flat, seg = self._batch(chunk)
 
             def coef_fn(lp_full, seg=seg, flat=flat):

@@ -125,3 +125,57 @@ def test_options_are_checked():
     for kw in (dict(head="rows"), dict(embed_grad="hash"), dict(router_aux_coef=-1.0)):
         with pytest.raises(ValueError):
             _engine(cfg, **kw)
+
+
+def _moe_weights(coef=0.5):
+    cfg = _cfg(moe=True)
+    cfg.router_aux_loss_coef = coef
+    return cfg, Qwen3Weights(cfg, device=torch.device("cpu"), dtype=torch.float32, seed=3)
+
+
+def _same_aux(runs):
+    """Equal micro-batches: their mean is the balance loss of all of them at once."""
+    (aux, grads), (aux2, grads2) = runs
+    assert aux > 0 and abs(aux - aux2) <= 1e-5 * aux
+    for a, b in zip(grads, grads2):
+        assert torch.allclose(a, b, rtol=1e-3, atol=1e-6)
+
+
+def test_balance_loss_weight_in_dpo():
+    from kore_b200.policy.configs import DPOConfig
+    from kore_b200.policy.dpo import DPOTrainer
+    g = torch.Generator().manual_seed(5)
+    cfg, _ = _moe_weights()
+    ids = torch.randint(0, cfg.vocab_size, (30,), generator=g).tolist()
+    pair = [(ids[:19], 9), (ids[:9] + ids[19:26], 9)]
+    runs = []
+    for micro in (4, 1):
+        dt = DPOTrainer(DPOConfig(beta=0.1, learning_rate=1e-3, use_lora=False, bf16=False, micro_pairs=micro,
+                                  router_aux=True), get_context(), _moe_weights()[1])
+        dt.tr.opt.step = lambda *a, **k: None
+        dt.step([pair] * 4)
+        runs.append((float(dt.tr.eng.aux_loss), [x.clone() for x in dt.tr.eng.grads]))
+    _same_aux(runs)
+
+
+def test_balance_loss_weight_in_grpo():
+    from kore_b200.env.base import SyntheticRewardEnv
+    from kore_b200.policy.configs import GRPOConfig
+    from kore_b200.policy.grpo import GRPOTrainer, TrainSample
+    g = torch.Generator().manual_seed(6)
+    cfg, _ = _moe_weights()
+    ids = torch.randint(0, cfg.vocab_size, (24,), generator=g).tolist()
+    runs = []
+    for budget in (4096, 24):
+        tr = GRPOTrainer(GRPOConfig(num_trajectories=4, num_turns=1, tasks_per_step=1, max_response_length=8,
+                                    max_prompt_length=64, learning_rate=1e-3, bf16=False, total_steps=2,
+                                    overlong_mask=False, pack_trajectories=False, router_aux=True),
+                         weights=_moe_weights()[1],
+                         env=SyntheticRewardEnv(seed=0, prompt_len=16, feedback_len=4, vocab_size=cfg.vocab_size),
+                         rollout_kwargs=dict(num_pages=64, page_size=16, max_seq_len=128))
+        tr.trainer.opt.step = lambda *a, **k: None
+        samples = [TrainSample(list(ids), 8, ret=0.0, adv=0.5, old_logp=-5.0, ref_logp=-5.0) for _ in range(4)]
+        assert len(list(tr._pack(tr._rows(samples), budget))) == (1 if budget == 4096 else 4)
+        tr.update(samples, budget)
+        runs.append((float(tr.trainer.eng.aux_loss), [x.clone() for x in tr.trainer.eng.grads]))
+    _same_aux(runs)
