@@ -77,7 +77,7 @@ void symm_adamw_bcast(int64_t id, int64_t param_offset, int64_t grad_offset, int
 void gemm_grouped_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out,
                        const std::vector<int64_t>& offsets, bool b_mn, bool accumulate);
 void moe_route_fwd(const at::Tensor& logits, int64_t k, bool norm, at::Tensor& probs, at::Tensor& idx,
-                   at::Tensor& w);
+                   at::Tensor& w, bool given);
 void moe_route_bwd(const at::Tensor& probs, const at::Tensor& idx, const at::Tensor& w, const at::Tensor& dw,
                    bool norm, at::Tensor& dlogits);
 void moe_combine(const at::Tensor& src, const at::Tensor& pos, const c10::optional<at::Tensor>& w,

@@ -1,6 +1,6 @@
 // Mixture-of-experts kernels for sm_100a (Qwen3-MoE: 128 experts, top-8).
 //   * moe_route_fwd: softmax over experts, top-k selection by k rounds of a
-//                    warp argmax, optional renormalisation of the k weights
+//                    warp argmax (or the choices given), optional renormalisation of the k weights
 //   * moe_route_bwd: gradient of the router logits from d(weights)
 //   * moe_combine:   y[t] = sum_j w[t,j] * src[pos[t,j]] (+ residual); with
 //                    w == nullptr it is the un-permute sum used by the backward
@@ -25,8 +25,9 @@ namespace moe {
 constexpr int kMaxE = 256;
 constexpr int kMaxK = 16;
 
-// one warp per token; E <= 256 (E / 32 values per lane)
-__global__ void route_fwd_kernel(const float* __restrict__ logits, int T, int E, int k, int norm,
+// one warp per token; E <= 256 (E / 32 values per lane). given: idx holds the
+// choices already; one outside [0, E) has weight 0.
+__global__ void route_fwd_kernel(const float* __restrict__ logits, int T, int E, int k, int norm, int given,
                                  float* __restrict__ probs, int* __restrict__ idx, float* __restrict__ w) {
   const long tok = (long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   const int lane = threadIdx.x & 31;
@@ -63,6 +64,17 @@ __global__ void route_fwd_kernel(const float* __restrict__ logits, int T, int E,
   for (int j = 0; j < k; ++j) {
     float best = -1.f;
     int bi = 0x7fffffff;
+    if (given) {
+      bi = idx[tok * k + j];
+      best = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMaxE / 32; ++i)
+        if (i < per && lane + 32 * i == bi && bi < E) best = v[i];
+      best = __shfl_sync(0xffffffff, best, bi & 31);
+      sel[j] = best;
+      tot += best;
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < kMaxE / 32; ++i) {
       const int e = lane + 32 * i;
@@ -84,7 +96,7 @@ __global__ void route_fwd_kernel(const float* __restrict__ logits, int T, int E,
   }
   if (lane == 0) {
     for (int j = 0; j < k; ++j) {
-      idx[tok * k + j] = sid[j];
+      if (!given) idx[tok * k + j] = sid[j];
       w[tok * k + j] = norm ? sel[j] / tot : sel[j];
     }
   }
@@ -652,15 +664,20 @@ void moe_gather_rows(const at::Tensor& x, const at::Tensor& src_row, at::Tensor&
   check_cuda(cudaGetLastError(), "moe gather rows");
 }
 
+// given: idx holds the choices and only their weights are computed.
 void moe_route_fwd(const at::Tensor& logits, int64_t k, bool norm, at::Tensor& probs, at::Tensor& idx,
-                   at::Tensor& w) {
+                   at::Tensor& w, bool given) {
   TORCH_CHECK(logits.scalar_type() == at::kFloat && logits.is_contiguous(), "logits fp32 contiguous [T,E]");
   const int T = logits.size(0), E = logits.size(1);
   TORCH_CHECK(E <= moe::kMaxE && k <= moe::kMaxK && k <= E, "E <= 256 and k <= 16");
+  if (given)
+    TORCH_CHECK(idx.device() == logits.device() && idx.scalar_type() == at::kInt && idx.is_contiguous() &&
+                    idx.dim() == 2 && idx.size(0) == T && idx.size(1) == k,
+                "route: given choices must be contiguous int32 [T, k]");
   if (T == 0) return;
   c10::cuda::CUDAGuard g(logits.device());
   moe::route_fwd_kernel<<<moe::warps_grid(T), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      logits.data_ptr<float>(), T, E, k, norm ? 1 : 0, probs.data_ptr<float>(), idx.data_ptr<int>(),
+      logits.data_ptr<float>(), T, E, k, norm ? 1 : 0, given ? 1 : 0, probs.data_ptr<float>(), idx.data_ptr<int>(),
       w.data_ptr<float>());
   check_cuda(cudaGetLastError(), "moe_route_fwd");
 }

@@ -196,11 +196,14 @@ class Qwen3Engine:
 
     # ------------------------------------------------------------------ layer
     def _layer_fwd(self, u: int, x, b: Batch, keep: bool, attn_saved=None,
-                   save_attn: Optional[list] = None, hold: Optional[dict] = None, hold_all: bool = False):
+                   save_attn: Optional[list] = None, hold: Optional[dict] = None, hold_all: bool = False,
+                   routing: Optional[dict] = None):
         """``x``: the layer's input, or its 8-bit copy (backward recompute).
         ``hold`` receives 8-bit copies: of the input ("x"), and with
         ``hold_all`` of everything that ``_held_ctx`` rebuilds the layer's
-        context from without a GEMM."""
+        context from without a GEMM; a MoE layer's choice of experts goes there
+        as "routing", which the recompute takes back: routed again from the
+        8-bit input, a few percent of the tokens would change experts."""
         W = self.w.views(u)
         T = x.shape[0]
         qd, kd = self.hq * self.D, self.hkv * self.D
@@ -236,7 +239,11 @@ class Qwen3Engine:
         hn2 = ops.rmsnorm_fwd(x2, W["ln2"], self.eps, rstd=rstd2)
         ctx = None
         if self.w.layouts[u].kind == "moe_layer":
-            x3, mctx = self._moe_fwd(W, hn2, x2, u if keep else None)
+            # the balance loss is counted once per step: where the routing is decided for good
+            count = hold is not None or (keep and routing is None)
+            x3, mctx = self._moe_fwd(W, hn2, x2, u if count else None, routing)
+            if hold is not None:
+                hold["routing"] = {k: mctx[k] for k in ("idx", "gain") if k in mctx}
             if keep:
                 ctx = dict(x=x, rstd1=rstd1, hn=hn, qkv=qkv, qk=qk, o=o, lse=lse, x2=x2, rstd2=rstd2, hn2=hn2)
                 ctx.update(mctx)             # the expert-parallel context may carry its own hn2
@@ -262,16 +269,19 @@ class Qwen3Engine:
                     hn2=hn2, gu8=held["gu"])
 
     # ------------------------------------------------------------------ MoE
-    def _moe_fwd(self, W, hn2, x2, u=None):
+    def _moe_fwd(self, W, hn2, x2, u=None, routing=None):
         """Router -> top-k -> expert-major permutation -> grouped SwiGLU experts
         -> weighted combine (+ residual). Experts outside this rank's range (EP)
-        are handled by the expert-parallel dispatcher when one is attached."""
+        are handled by the expert-parallel dispatcher when one is attached.
+        ``u``: count this pass's routing in the balance loss of layer u;
+        ``routing``: choices (and gain) of an earlier pass."""
         from ..ops import moe
         c = self.cfg
         logits = ops.mm(hn2, W["router"], out_dtype=torch.float32)
-        probs, idx, wts = moe.route(logits, c.num_experts_per_tok, c.norm_topk_prob)
-        balance = {}
-        if u is not None and self.router_aux_coef > 0:     # (the backward's pass over the layer)
+        routing = routing or {}
+        probs, idx, wts = moe.route(logits, c.num_experts_per_tok, c.norm_topk_prob, idx=routing.get("idx"))
+        balance = {"gain": routing["gain"]} if "gain" in routing else {}
+        if u is not None and self.router_aux_coef > 0:
             aux, counts, gain = moe.balance_loss(probs, idx, None, self.router_aux_coef / self.moe_layers)
             self.aux_loss.add_(aux, alpha=self.aux_scale)
             self.expert_counts[u] = counts if u not in self.expert_counts else self.expert_counts[u] + counts
@@ -471,12 +481,14 @@ class Qwen3Engine:
 
     @torch.no_grad()
     def forward_hidden(self, b: Batch, checkpoints: Optional[list] = None,
-                       attn_saves: Optional[list] = None, contexts: Optional[dict] = None) -> torch.Tensor:
+                       attn_saves: Optional[list] = None, contexts: Optional[dict] = None,
+                       routings: Optional[dict] = None) -> torch.Tensor:
         """Forward to the last hidden state. ``checkpoints`` collects each
         layer's input; ``attn_saves`` (selective checkpointing) also keeps each
         layer's attention output and logsumexp so the backward does not
         recompute attention; ``contexts`` receives the whole forward context of
-        the layers selected by ``keep_layers`` (no recompute at all)."""
+        the layers selected by ``keep_layers`` (no recompute at all);
+        ``routings`` the MoE layers' choices where the checkpoints are 8-bit."""
         x = ops.embed_fwd(b.ids, self.w.views(0)["embed"])
         hook = self.param_hook
         last = self.w.num_units - 2
@@ -491,6 +503,8 @@ class Qwen3Engine:
                 x, _ = self._layer_fwd(u, x, b, keep=False, save_attn=None if kept else attn_saves, hold=hold,
                                        hold_all=kept)
                 checkpoints.append(hold["x"])
+                if "routing" in hold:
+                    routings[u] = hold["routing"]
                 if kept:
                     contexts[u] = hold
                     if attn_saves is not None:
@@ -560,7 +574,8 @@ class Qwen3Engine:
         ckpts: list = []
         asaves: Optional[list] = [] if self.save_attention else None
         kept: dict = {}
-        x = self.forward_hidden(b, ckpts, asaves, kept)
+        routings: dict = {}
+        x = self.forward_hidden(b, ckpts, asaves, kept, routings)
         uh = self.w.num_units - 1
         Wn = self.w.views(uh)["norm"]
         T = b.num_tokens
@@ -606,7 +621,7 @@ class Qwen3Engine:
                 self.param_hook.begin_bwd(u)
             ctx = kept.pop(u, None)
             if ctx is None:
-                _, ctx = self._layer_fwd(u, xin, b, keep=True, attn_saved=saved)
+                _, ctx = self._layer_fwd(u, xin, b, keep=True, attn_saved=saved, routing=routings.pop(u, None))
             elif self.act8:
                 ctx = self._held_ctx(u, ctx, b)
             dx = self._layer_bwd(u, ctx["x"], dx, ctx, b)

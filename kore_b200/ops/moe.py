@@ -13,18 +13,26 @@ from . import embed_fwd
 from ._lib import native
 
 
-def route(logits: torch.Tensor, k: int, norm: bool = True):
+def route(logits: torch.Tensor, k: int, norm: bool = True, idx: Optional[torch.Tensor] = None):
     """softmax over experts -> top-k -> optional renormalisation.
-    Returns (probs [T,E] fp32, idx [T,k] int32, w [T,k] fp32)."""
+    Returns (probs [T,E] fp32, idx [T,k] int32, w [T,k] fp32). With ``idx`` the
+    choices are those given (a recompute from inexact inputs must not choose
+    again) and only their weights are computed."""
     T, E = logits.shape
     if logits.is_cuda:
         probs = torch.empty(T, E, dtype=torch.float32, device=logits.device)
-        idx = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+        given = idx is not None
+        if not given:
+            idx = torch.empty(T, k, dtype=torch.int32, device=logits.device)
         w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
-        native().moe_route_fwd(logits.float().contiguous(), k, bool(norm), probs, idx, w)
+        native().moe_route_fwd(logits.float().contiguous(), k, bool(norm), probs, idx, w, given)
         return probs, idx, w
     probs = torch.softmax(logits.float(), -1)
-    w, idx = probs.topk(k, -1)
+    if idx is None:
+        w, idx = probs.topk(k, -1)
+    else:
+        ok = (idx >= 0) & (idx < E)
+        w = torch.where(ok, probs.gather(-1, torch.where(ok, idx, 0).long()), torch.zeros(()))
     if norm:
         w = w / w.sum(-1, keepdim=True)
     return probs, idx.int(), w

@@ -179,3 +179,48 @@ def test_balance_loss_weight_in_grpo():
         tr.update(samples, budget)
         runs.append((float(tr.trainer.eng.aux_loss), [x.clone() for x in tr.trainer.eng.grads]))
     _same_aux(runs)
+
+
+def _wide_moe():
+    cfg = Qwen3Config(vocab_size=211, hidden_size=128, intermediate_size=128, num_hidden_layers=3, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=32, max_position_embeddings=512, model_type="qwen3_moe",
+                      num_experts=64, num_experts_per_tok=8, moe_intermediate_size=32)
+    g = torch.Generator().manual_seed(8)
+    return cfg, Batch.from_sequences([torch.randint(0, 211, (n,), generator=g) for n in (301, 99)])
+
+
+def test_act8_backward_takes_the_forwards_routing(monkeypatch):
+    """The 8-bit input moves some tokens over the edge between two experts; the
+    backward, the counts and the balance loss follow the forward's choices."""
+    from kore_b200.ops import moe
+    cfg, b = _wide_moe()
+    seen = []
+    real = moe.plan
+    monkeypatch.setattr(moe, "plan", lambda idx, *a, **k: (seen.append(idx.clone()), real(idx, *a, **k))[1])
+    plain, held = _engine(cfg, router_aux_coef=0.1), _engine(cfg, router_aux_coef=0.1, act8=True)
+    (_, ga), (_, gc) = _step(plain, b), _step(held, b)
+    assert len(seen) == 12
+    forward, backward = seen[6:9], seen[9:][::-1]
+    for f, r, p in zip(forward, backward, seen[:3]):
+        assert torch.equal(f, r) and torch.equal(f, p)
+    assert sorted(held.expert_counts) == [1, 2, 3]
+    for u in held.expert_counts:
+        assert torch.equal(held.expert_counts[u], plain.expert_counts[u])
+    assert torch.equal(held.aux_loss, plain.aux_loss)
+    for u, (x, y) in enumerate(zip(ga, gc)):
+        assert (x - y).norm() <= 0.03 * x.norm(), u
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_route_with_given_choices(norm):
+    from kore_b200.ops import moe
+    logits = torch.randn(9, 12, generator=torch.Generator().manual_seed(4))
+    probs, idx, w = moe.route(logits, 3, norm)
+    same = moe.route(logits, 3, norm, idx=idx)
+    assert all(torch.equal(a, b) for a, b in zip(same, (probs, idx, w)))
+    other = (idx + 1) % 12
+    p2, i2, w2 = moe.route(logits, 3, norm, idx=other)
+    want = torch.softmax(logits.double(), -1).gather(1, other.long())
+    if norm:
+        want = want / want.sum(-1, keepdim=True)
+    assert torch.equal(i2, other) and torch.equal(p2, probs) and torch.allclose(w2.double(), want, rtol=1e-5)

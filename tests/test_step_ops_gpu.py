@@ -81,3 +81,51 @@ def test_training_with_all_of_them(moe):
         # 4 micro-batches of 128 tokens, 2 choices each, in every layer
         assert all(int(c.sum()) == 4 * 128 * 2 for c in tr.eng.expert_counts.values())
         assert len(tr.eng.expert_counts) == 3
+
+
+@pytest.mark.parametrize("T,E,k", [(0, 8, 2), (1, 8, 8), (77, 60, 4), (513, 128, 8), (40, 256, 16)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_route_with_given_choices(T, E, k, norm):
+    from kore_b200.ops import moe
+    logits = torch.randn(T, E, device="cuda", generator=torch.Generator(device="cuda").manual_seed(E))
+    probs, idx, w = moe.route(logits, k, norm)
+    p2, i2, w2 = moe.route(logits, k, norm, idx=idx.clone())
+    assert torch.equal(p2, probs) and torch.equal(i2, idx) and torch.equal(w2, w)
+    other = torch.argsort(torch.rand(T, E, device="cuda"), -1)[:, :k].int().contiguous()
+    _, i3, w3 = moe.route(logits, k, norm, idx=other)
+    want = torch.softmax(logits.double(), -1).gather(1, other.long())
+    if norm:
+        want = want / want.sum(-1, keepdim=True)
+    assert torch.equal(i3, other)
+    # the exponential is off by up to 2 + |x| / 2 units of 2^-24, twice (entry and sum)
+    assert ((w3.double() - want).abs() <= 1e-5 * want).all()
+    if T:
+        none = other.clone()
+        none[:, 0] = -1 if T % 2 else E
+        _, _, w4 = moe.route(logits, k, False, idx=none)
+        assert (w4[:, 0] == 0).all()
+        for bad in (other[:, :k - 1], other.long(), other[:T - 1] if T > 1 else other.float()):
+            with pytest.raises(RuntimeError):
+                moe.route(logits, k, norm, idx=bad)
+
+
+def test_act8_backward_takes_the_forwards_routing(monkeypatch):
+    from kore_b200.ops import moe
+    kw = dict(vocab_size=2048, hidden_size=512, intermediate_size=1024, num_hidden_layers=3, num_attention_heads=4,
+              num_key_value_heads=2, head_dim=128, max_position_embeddings=1024, model_type="qwen3_moe",
+              num_experts=64, num_experts_per_tok=8, moe_intermediate_size=128)
+    cfg = Qwen3Config(**kw)
+    b = _batch(cfg)
+    seen = []
+    real = moe.plan
+    monkeypatch.setattr(moe, "plan", lambda idx, *a, **k: (seen.append(idx.clone()), real(idx, *a, **k))[1])
+    a, ga, plain = _grads(cfg, b, router_aux_coef=0.1)
+    c, gc, held = _grads(cfg, b, router_aux_coef=0.1, act8=True)
+    assert len(seen) == 12
+    for f, r in zip(seen[6:9], seen[9:][::-1]):
+        assert torch.equal(f, r)
+    assert torch.equal(a["logp"], c["logp"])
+    for u in plain.expert_counts:
+        assert torch.equal(held.expert_counts[u], plain.expert_counts[u])
+    for u, (x, y) in enumerate(zip(ga, gc)):
+        assert (x - y).norm() <= 0.04 * x.norm(), (u, float((x - y).norm() / x.norm()))
