@@ -98,7 +98,7 @@ class DPOTrainer:
                                   warmup_steps=int(config.warmup_ratio * total_steps), total_steps=total_steps,
                                   weights=weights, comm=config.comm, **step_kwargs(config))
         self.ref_placement = self._choose_placement(getattr(config, "ref_placement", "auto"))
-        self.ref = Qwen3Engine(self._build_ref(ref_weights), allocate_grads=False)
+        self.ref = Qwen3Engine(self._build_ref(ref_weights), allocate_grads=False, head=self.tr.eng.head)
         if self.ref_placement != "resident":
             self.ref.param_hook = self._ref_stream
         self.micro_pairs = max(1, int(getattr(config, "micro_pairs", 1)))

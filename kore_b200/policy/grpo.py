@@ -106,7 +106,8 @@ class GRPOTrainer:
         self.ref_placement = "none"
         if ref_weights is not None or config.ref_anchor_coef:
             self.ref_w, self.ref_placement = self._build_ref(ref_weights, getattr(config, "ref_placement", "auto"))
-        self.ref_eng = (Qwen3Engine(self.ref_w, allocate_grads=False, temperature=config.temperature)
+        self.ref_eng = (Qwen3Engine(self.ref_w, allocate_grads=False, temperature=config.temperature,
+                                    head=self.trainer.eng.head)
                         if self.ref_w is not None else None)
         if self.ref_eng is not None and self.ref_stream is not None:
             self.ref_eng.param_hook = self.ref_stream

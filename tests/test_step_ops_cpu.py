@@ -224,3 +224,22 @@ def test_route_with_given_choices(norm):
     if norm:
         want = want / want.sum(-1, keepdim=True)
     assert torch.equal(i2, other) and torch.equal(p2, probs) and torch.allclose(w2.double(), want, rtol=1e-5)
+
+
+def test_reference_model_uses_the_policys_head():
+    """Equal weights have equal log-probs: the frozen reference scores with the same head."""
+    from kore_b200.env.base import SyntheticRewardEnv
+    from kore_b200.policy.configs import DPOConfig, GRPOConfig
+    from kore_b200.policy.dpo import DPOTrainer
+    from kore_b200.policy.grpo import GRPOTrainer
+    cfg = _cfg()
+    b = _batch(cfg)
+    for head in ("chunks", "pieces"):
+        w = Qwen3Weights(cfg, device=torch.device("cpu"), dtype=torch.float32, seed=3)
+        dt = DPOTrainer(DPOConfig(use_lora=False, bf16=False, head=head), get_context(), w.clone())
+        gt = GRPOTrainer(GRPOConfig(bf16=False, head=head, ref_anchor_coef=1e-2), weights=w.clone(),
+                         env=SyntheticRewardEnv(seed=0, prompt_len=16, feedback_len=4, vocab_size=cfg.vocab_size),
+                         rollout_kwargs=dict(num_pages=64, page_size=16, max_seq_len=128))
+        for policy, ref in ((dt.tr.eng, dt.ref), (gt.trainer.eng, gt.ref_eng)):
+            assert policy.head == ref.head == head and policy.temperature == ref.temperature
+            assert torch.equal(policy.token_logprobs(b)[0], ref.token_logprobs(b)[0])
