@@ -473,7 +473,17 @@ class Qwen3Engine:
         H, F = c.hidden_size, c.intermediate_size
         if self.act8:                                                # qkv x2 gu in 8 bits, a scale per 128
             return int(tokens * (qd + 2 * kd + H + 2 * F) * (1 + 4 / a8.BLOCK))
+        return self.layer_context_bytes(tokens)
+
+    def layer_context_bytes(self, tokens: int) -> int:
+        """HBM of the context that a dense layer's backward works on, beyond the
+        checkpoints: in the weights' type, however the checkpoints are held."""
+        c = self.cfg
+        qd, kd = self.hq * self.D, self.hkv * self.D
+        H, F = c.hidden_size, c.intermediate_size
         elems = H + (qd + 2 * kd) + (qd + kd) + H + H + 2 * F + F   # hn qkv qk x2 hn2 gu a
+        if self.act8:
+            elems += H                                               # x out of its 8 bits
         return tokens * (elems * self.w.dtype.itemsize + 8)           # + two fp32 rstd
 
     def _kept(self, u: int) -> bool:

@@ -196,7 +196,7 @@ class CausalLMTrainer:
             free, _ = torch.cuda.mem_get_info(self.ctx.device)
             free += torch.cuda.memory_reserved(self.ctx.device) - torch.cuda.memory_allocated(self.ctx.device)
             per = self.eng.activation_bytes_per_layer(micro_tokens)
-            budget = free - self.reserve_bytes - per
+            budget = free - self.reserve_bytes - self.eng.layer_context_bytes(micro_tokens)
             keep = int(max(0, min(L, budget // per)))
         if self.ctx.world > 1:
             t = torch.tensor([float(keep)], device=self.ctx.device)

@@ -243,3 +243,24 @@ def test_reference_model_uses_the_policys_head():
         for policy, ref in ((dt.tr.eng, dt.ref), (gt.trainer.eng, gt.ref_eng)):
             assert policy.head == ref.head == head and policy.temperature == ref.temperature
             assert torch.equal(policy.token_logprobs(b)[0], ref.token_logprobs(b)[0])
+
+
+@pytest.mark.parametrize("act8", [False, True])
+def test_plan_leaves_room_for_the_layer_in_flight(monkeypatch, act8):
+    """The layer that the backward works on is held in the weights' type, whatever its checkpoint is held in."""
+    from types import SimpleNamespace
+    cfg = _cfg()
+    tr = CausalLMTrainer(cfg, get_context(), dtype=torch.float32, act8=act8, activation_reserve_gb=0.0)
+    tokens = 1000
+    _, ctx = tr.eng._layer_fwd(1, torch.randn(40, cfg.hidden_size), Batch.from_sequences([torch.arange(40)]), keep=True)
+    held = ("o", "lse", "rstd1", "rstd2") + (() if act8 else ("x",))       # from 8 bits, x is another tensor
+    flight = sum(t.numel() * t.element_size() for k, t in ctx.items() if k not in held) * tokens // 40 + 8 * tokens
+    per = tr.eng.activation_bytes_per_layer(tokens)
+    free = flight + 2 * per
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (free, free))
+    monkeypatch.setattr(torch.cuda, "memory_reserved", lambda *a: 0)
+    monkeypatch.setattr(torch.cuda, "memory_allocated", lambda *a: 0)
+    tr.ctx = SimpleNamespace(device=torch.device("cuda"), world=1)
+    assert tr.plan_activations(tokens) == 2
+    free -= 1
+    assert tr.plan_activations(tokens) == 1
