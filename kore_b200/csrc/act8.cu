@@ -130,7 +130,7 @@ constexpr int kSaveRows = 2;
 constexpr int kLoadRows = 4;
 
 // ---------------------------------------------------------------- save / load
-__global__ void __launch_bounds__(256) save_kernel(const __nv_bfloat16* __restrict__ x, long ldx, Held h, long T) {
+__global__ void __launch_bounds__(256) save_kernel(const __nv_bfloat16* x, long ldx, Held h, long T) {
   const int j = blockIdx.x * blockDim.x + threadIdx.x;
   const bool live = j * 8 < h.H;
   pdl_wait();
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256) save_kernel(const __nv_bfloat16* __restri
 #pragma unroll
     for (int r = 0; r < kSaveRows; ++r) {
       raw[r] = make_uint4(0, 0, 0, 0);
-      if (live && t0 + r < T) raw[r] = __ldg(reinterpret_cast<const uint4*>(x + (t0 + r) * ldx) + j);
+      if (live && t0 + r < T) raw[r] = reinterpret_cast<const uint4*>(x + (t0 + r) * ldx)[j];
     }
 #pragma unroll
     for (int r = 0; r < kSaveRows; ++r) {
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(256) load_kernel(Held h, __nv_bfloat16* __rest
 #pragma unroll
     for (int r = 0; r < kLoadRows; ++r)
       if (t0 + r < T) {
-        q[r] = __ldg(reinterpret_cast<const uint2*>(h.q + (t0 + r) * h.H) + j);
-        s[r] = __ldg(h.s + (t0 + r) * h.nb + j / 16);
+        q[r] = reinterpret_cast<const uint2*>(h.q + (t0 + r) * h.H)[j];
+        s[r] = h.s[(t0 + r) * h.nb + j / 16];
       }
 #pragma unroll
     for (int r = 0; r < kLoadRows; ++r)
@@ -193,8 +193,7 @@ KORE_DEV float block_sum(float v, float* red) {
 // hn = x rstd w and the 8-bit copy of x, one read of x
 // (5 blocks of 256 threads: 48 registers; 16384 x 5120: 69 us, 74 with 62 registers)
 template <int VPT>
-__global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
-                                                        const __nv_bfloat16* __restrict__ w,
+__global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* x, long ldx, const __nv_bfloat16* w,
                                                         __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
                                                         Held h, float eps) {
   __shared__ float red[8];
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* 
   for (int i = 0; i < VPT; ++i) {
     const int j = threadIdx.x + i * blockDim.x;
     raw[i] = make_uint4(0, 0, 0, 0);
-    if (j < nvec) raw[i] = __ldg(reinterpret_cast<const uint4*>(x + t * ldx) + j);
+    if (j < nvec) raw[i] = reinterpret_cast<const uint4*>(x + t * ldx)[j];
   }
   uint64_t ss = 0;
 #pragma unroll
@@ -236,7 +235,7 @@ __global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* 
     if (j < nvec) {
       uint64_t f[4], g[4];
       unpack8(raw[i], f);
-      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
+      unpack8(reinterpret_cast<const uint4*>(w)[j], g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = f2_mul(f2_mul(f[e], rs2), g[e]);
       reinterpret_cast<uint4*>(hn + t * h.H)[j] = pack8(f);
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(256, 5) norm_save_kernel(const __nv_bfloat16* 
 
 // x back from 8 bits (bf16), and its RMSNorm from the unrounded values
 template <int VPT>
-__global__ void __launch_bounds__(256) norm_load_kernel(Held h, const __nv_bfloat16* __restrict__ w,
+__global__ void __launch_bounds__(256) norm_load_kernel(Held h, const __nv_bfloat16* w,
                                                         __nv_bfloat16* __restrict__ x,
                                                         __nv_bfloat16* __restrict__ hn, float* __restrict__ rstd,
                                                         float eps) {
@@ -263,8 +262,8 @@ __global__ void __launch_bounds__(256) norm_load_kernel(Held h, const __nv_bfloa
     q[i] = make_uint2(0, 0);
     s[i] = 0.f;
     if (j < nvec) {
-      q[i] = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H) + j);
-      s[i] = __ldg(h.s + t * h.nb + j / 16);
+      q[i] = reinterpret_cast<const uint2*>(h.q + t * h.H)[j];
+      s[i] = h.s[t * h.nb + j / 16];
     }
   }
   uint64_t ss = 0;
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(256) norm_load_kernel(Held h, const __nv_bfloa
     if (j < nvec) {
       uint64_t f[4], g[4];
       restore(q[i], s[i], f);
-      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), g);
+      unpack8(reinterpret_cast<const uint4*>(w)[j], g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = f2_mul(f2_mul(f[e], rs2), g[e]);
       reinterpret_cast<uint4*>(hn + t * h.H)[j] = pack8(f);
@@ -307,7 +306,7 @@ KORE_DEV uint64_t sigmoid(uint64_t x) {
 // HOLD (F % 128 == 0, so that a block lies wholly in gate or in up): also
 // writes the 8-bit copy (4 blocks of 256 threads per SM: 193 us at 8192 x 17408, 211 without)
 template <bool HOLD>
-__global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
+__global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* gu, long ldg,
                                                      __nv_bfloat16* __restrict__ a, Held h, long T) {
   const int F = h.H / 2;
   const int j = blockIdx.x * blockDim.x + threadIdx.x;
@@ -320,8 +319,8 @@ __global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* __r
     for (int r = 0; r < kGluRows; ++r) {
       g[r] = u[r] = make_uint4(0, 0, 0, 0);
       if (live && t0 + r < T) {
-        g[r] = __ldg(reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg) + j);
-        u[r] = __ldg(reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg + F) + j);
+        g[r] = reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg)[j];
+        u[r] = reinterpret_cast<const uint4*>(gu + (t0 + r) * ldg + F)[j];
       }
     }
 #pragma unroll
@@ -372,7 +371,7 @@ KORE_DEV void join_block_max(uint32_t* s_top, uint32_t mine, int blk, bool live)
 }
 
 template <int VPT>
-__global__ void __launch_bounds__(kRowThreads) swiglu_row_kernel(const __nv_bfloat16* __restrict__ gu, long ldg,
+__global__ void __launch_bounds__(kRowThreads) swiglu_row_kernel(const __nv_bfloat16* gu, long ldg,
                                                                  __nv_bfloat16* __restrict__ a, Held h) {
   __shared__ uint32_t s_top[2 * kMaxRowF / kBlock + 2];
   const int F = h.H / 2, nvec = F / 8;
@@ -385,8 +384,8 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_row_kernel(const __nv_bflo
     const int j = threadIdx.x + i * blockDim.x;
     g[i] = u[i] = make_uint4(0, 0, 0, 0);
     if (j < nvec) {
-      g[i] = __ldg(reinterpret_cast<const uint4*>(gu + t * ldg) + j);
-      u[i] = __ldg(reinterpret_cast<const uint4*>(gu + t * ldg + F) + j);
+      g[i] = reinterpret_cast<const uint4*>(gu + t * ldg)[j];
+      u[i] = reinterpret_cast<const uint4*>(gu + t * ldg + F)[j];
     }
   }
   for (int b = threadIdx.x; b < h.nb; b += blockDim.x) s_top[b] = 0;
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_row_kernel(const __nv_bflo
   }
 }
 
-__global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bfloat16* __restrict__ dout, long ldd,
+__global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bfloat16* dout, long ldd,
                                                          __nv_bfloat16* __restrict__ dgu,
                                                          __nv_bfloat16* __restrict__ a, long T) {
   const int F = h.H / 2;
@@ -430,10 +429,10 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bflo
   pdl_trigger();
   if (j * 8 >= F) return;
   for (long t = blockIdx.y; t < T; t += gridDim.y) {
-    const uint2 qg = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H) + j);
-    const uint2 qu = __ldg(reinterpret_cast<const uint2*>(h.q + t * h.H + F) + j);
-    const uint4 dv = __ldg(reinterpret_cast<const uint4*>(dout + t * ldd) + j);
-    const float sg = __ldg(h.s + t * h.nb + j / 16), su = __ldg(h.s + t * h.nb + (F / 8 + j) / 16);
+    const uint2 qg = reinterpret_cast<const uint2*>(h.q + t * h.H)[j];
+    const uint2 qu = reinterpret_cast<const uint2*>(h.q + t * h.H + F)[j];
+    const uint4 dv = reinterpret_cast<const uint4*>(dout + t * ldd)[j];
+    const float sg = h.s[t * h.nb + j / 16], su = h.s[t * h.nb + (F / 8 + j) / 16];
     uint64_t g[4], u[4], d[4], dg[4];
     restore(qg, sg, g);
     restore(qu, su, u);

@@ -70,7 +70,9 @@ KORE_DEV bool elect_one() {
 // A kernel launched with launch_after() may start while the kernel before it in
 // the stream still runs: pdl_wait() returns when that one has finished and its
 // writes are visible, so nothing that it wrote or still reads may be touched
-// earlier. pdl_trigger() lets the next such kernel start once all blocks are here.
+// earlier. Read-only loads (__ldg, const __restrict__ parameters) are defined only
+// for memory that nobody writes while the kernel runs, and a compiler may move them
+// above the wait: such kernels read global memory with plain loads. pdl_trigger() lets the next such kernel start once all blocks are here.
 KORE_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 KORE_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

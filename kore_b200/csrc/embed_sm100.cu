@@ -62,7 +62,7 @@ KORE_DEV uint4 pack8(const float (&f)[8]) {
 // first store (rows of 1024 columns and more: four per thread, 40 us at 16384 x 5120,
 // 65 us with one)
 template <int VPT>
-__global__ void lookup_kernel(const long* __restrict__ ids, const __nv_bfloat16* __restrict__ table, long ldt,
+__global__ void lookup_kernel(const long* ids, const __nv_bfloat16* table, long ldt,
                               __nv_bfloat16* __restrict__ out, float scale, int V, int H) {
   const int nvec = H / 8;
   const long t = blockIdx.x;
@@ -76,7 +76,7 @@ __global__ void lookup_kernel(const long* __restrict__ ids, const __nv_bfloat16*
     for (int i = 0; i < VPT; ++i) {
       const int j = j0 + i * blockDim.x;
       u[i] = make_uint4(0, 0, 0, 0);
-      if (ok && j < nvec) u[i] = __ldg(reinterpret_cast<const uint4*>(table + id * ldt) + j);
+      if (ok && j < nvec) u[i] = reinterpret_cast<const uint4*>(table + id * ldt)[j];
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -95,8 +95,8 @@ __global__ void lookup_kernel(const long* __restrict__ ids, const __nv_bfloat16*
 
 // Places of kRankThreads tokens within their tile of kTile: the key (id << 32 |
 // position) goes to that place. ids outside the table count as V, behind all others.
-__global__ void __launch_bounds__(kRankThreads) rank_in_tile_kernel(const long* __restrict__ ids,
-                                                                    u64* __restrict__ keys, int T, int V) {
+__global__ void __launch_bounds__(kRankThreads) rank_in_tile_kernel(const long* ids, u64* __restrict__ keys, int T,
+                                                                    int V) {
   __shared__ __align__(16) int s_id[kTile];
   const int i = blockIdx.x * kRankThreads + threadIdx.x;
   const int base = i / kTile * kTile;            // the same for all threads of the block
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kRankThreads) rank_in_tile_kernel(const long* 
 
 // Places among all tiles: 8 tiles are searched at once, without branches, so
 // that their loads overlap.
-__global__ void rank_kernel(const u64* __restrict__ tiles, u64* __restrict__ keys, int T) {
+__global__ void rank_kernel(const u64* tiles, u64* __restrict__ keys, int T) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   pdl_wait();
   pdl_trigger();
@@ -159,7 +159,7 @@ __global__ void rank_kernel(const u64* __restrict__ tiles, u64* __restrict__ key
     for (int s = kTile; s > 0; s >>= 1) {
       u64 k[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) k[u] = pos[u] + s <= n[u] ? __ldg(tiles + (size_t)(j0 + u) * kTile + pos[u] + s - 1) : ~0ull;
+      for (int u = 0; u < 8; ++u) k[u] = pos[u] + s <= n[u] ? tiles[(size_t)(j0 + u) * kTile + pos[u] + s - 1] : ~0ull;
 #pragma unroll
       for (int u = 0; u < 8; ++u) pos[u] += k[u] < key ? s : 0;
     }
@@ -174,7 +174,7 @@ KORE_DEV int key_id(u64 k) { return (int)(k >> 32); }
 // Zeros in the rows [r0, r0 + kZeroRows) of the table that no sorted key names:
 // a thread per row sends copies of a zeroed piece of shared memory.
 template <typename G>
-KORE_DEV void zero_rows(const u64* __restrict__ keys, G* __restrict__ dtable, int r0, int T, int V, int H) {
+KORE_DEV void zero_rows(const u64* keys, G* __restrict__ dtable, int r0, int T, int V, int H) {
   __shared__ __align__(128) uint4 s_zero[kZeroBytes / 16];
   for (int i = threadIdx.x; i < kZeroBytes / 16; i += blockDim.x) s_zero[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
@@ -242,7 +242,7 @@ KORE_DEV void write_row(__nv_bfloat16* row, int j, const float (&sum)[8], float 
 // walk: a block sums the segments that begin in its chunk to their ends and
 // passes over what began before (no workspace, no second launch).
 template <typename G>
-__global__ void segments_kernel(const u64* __restrict__ keys, const __nv_bfloat16* __restrict__ dy, long ldy,
+__global__ void segments_kernel(const u64* keys, const __nv_bfloat16* dy, long ldy,
                                 G* __restrict__ dtable, float* __restrict__ part, float scale, int add, int chunk,
                                 int chunks, int walk, int T, int V, int H) {
   __shared__ int s_id[kChunk + 2];
@@ -282,7 +282,7 @@ __global__ void segments_kernel(const u64* __restrict__ keys, const __nv_bfloat1
       for (int u = 0; u < 8; ++u) {
         const int i = i0 + u;
         if (i < n && s_id[i + 1] < V) {
-          v[u] = __ldg(src + s_pos[i] * ld);
+          v[u] = src[s_pos[i] * ld];
           if (add && s_id[i + 2] != s_id[i + 1]) read_old(old[u], dtable + (size_t)s_id[i + 1] * H, j);
         }
       }
@@ -322,7 +322,7 @@ __global__ void segments_kernel(const u64* __restrict__ keys, const __nv_bfloat1
 
 // The chunk in which a border-crossing segment begins joins its parts.
 template <typename G>
-__global__ void join_kernel(const u64* __restrict__ keys, const float* __restrict__ part, G* __restrict__ dtable,
+__global__ void join_kernel(const u64* keys, const float* part, G* __restrict__ dtable,
                             float scale, int add, int T, int V, int H) {
   __shared__ int s_last;
   const int c = blockIdx.x;

@@ -573,8 +573,8 @@ KORE_DEV uint64_t bf2_to_f2(uint32_t v) {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
-                                                               const __nv_bfloat16* __restrict__ w, long ldw,
+__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat16* x, long ldx,
+                                                               const __nv_bfloat16* w, long ldw,
                                                                const Params p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint4* sx = reinterpret_cast<uint4*>(smem_raw);  // [NT][H / 8]
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat
       uint4 wv[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        wv[r] = r0 + r < V ? __ldg(reinterpret_cast<const uint4*>(w + (r0 + r) * ldw) + j) : make_uint4(0, 0, 0, 0);
+        wv[r] = r0 + r < V ? reinterpret_cast<const uint4*>(w + (r0 + r) * ldw)[j] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const uint4 xv = sx[t * nvec + j];
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat
 
 // Joins the parts (half tiles, or blocks of few_rows_kernel) of each row: 32 rows per block, 32 threads per row.
 __global__ void __launch_bounds__(1024) head_join_kernel(
-    const float* __restrict__ stats, const float* __restrict__ zt, const long* __restrict__ targets, int parts,
+    const float* stats, const float* zt, const long* targets, int parts,
     int T, int V, float* __restrict__ logp, float* __restrict__ ent, float* __restrict__ lse) {
   __shared__ float sm[32][33], ss[32][33], su[32][33];
   pdl_wait();
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(1024) head_join_kernel(
 }
 
 // out = x with the rows of coefficient 0 set to zero, once or twice (8 elements per thread)
-__global__ void mask_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const float* __restrict__ coef,
+__global__ void mask_rows_kernel(const __nv_bfloat16* x, long ldx, const float* coef,
                                  __nv_bfloat16* __restrict__ out, int T, int H, int copies) {
   pdl_wait();
   pdl_trigger();
@@ -744,7 +744,7 @@ __global__ void mask_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, 
 }
 
 // dx = the sum of the K parts (and of dz's two terms, T rows apart), rounded once
-__global__ void sum_parts_kernel(const float* __restrict__ src, int parts, int copies, long part_stride,
+__global__ void sum_parts_kernel(const float* src, int parts, int copies, long part_stride,
                                  __nv_bfloat16* __restrict__ dst, long ld, int T, int H) {
   pdl_wait();
   pdl_trigger();

@@ -421,8 +421,8 @@ constexpr int kBalUnroll = 4;   // tokens that a warp has in flight
 // Sums of this block's tokens (warps take kBalUnroll consecutive tokens at a
 // time): s_sum [warps][32 NI], s_cnt [E + 1] (counts, then tokens).
 template <int NI>
-KORE_DEV void balance_sums(const float* __restrict__ probs, const int* __restrict__ idx,
-                           const bool* __restrict__ mask, int T, int E, int k, float* s_sum, int* s_cnt) {
+KORE_DEV void balance_sums(const float* probs, const int* idx, const bool* mask, int T, int E, int k, float* s_sum,
+                           int* s_cnt) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32;
   pdl_wait();
   pdl_trigger();
@@ -440,7 +440,7 @@ KORE_DEV void balance_sums(const float* __restrict__ probs, const int* __restric
       live[r] = t0 + r < T && (mask == nullptr || mask[t0 + r]);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        v[r][i] = live[r] && lane + 32 * i < E ? __ldg(probs + (t0 + r) * E + lane + 32 * i) : 0.f;
+        v[r][i] = live[r] && lane + 32 * i < E ? probs[(t0 + r) * E + lane + 32 * i] : 0.f;
     }
     for (int j = lane; j < kBalUnroll * k; j += 32) {
       const int r = j / k;
@@ -487,7 +487,7 @@ KORE_DEV void balance_finish(int e, int E, int c, float sum, int n, float coef, 
 // one block finishes by itself (part == nullptr).
 template <int NI>
 __global__ void __launch_bounds__(1024) balance_part_kernel(
-    const float* __restrict__ probs, const int* __restrict__ idx, const bool* __restrict__ mask, int T, int E, int k,
+    const float* probs, const int* idx, const bool* mask, int T, int E, int k,
     float* __restrict__ part, int* __restrict__ cnt, float coef, float* __restrict__ loss, int* __restrict__ counts,
     float* __restrict__ gain) {
   __shared__ float s_sum[32 * 32 * NI];
@@ -508,9 +508,8 @@ __global__ void __launch_bounds__(1024) balance_part_kernel(
 
 // One block: lane groups of E' = E rounded up to a warp each sum every
 // (1024 / E')-th block; the groups are added in order.
-__global__ void __launch_bounds__(1024) balance_join_kernel(const float* __restrict__ part,
-                                                            const int* __restrict__ cnt, int blocks, int E,
-                                                            float coef, float* __restrict__ loss,
+__global__ void __launch_bounds__(1024) balance_join_kernel(const float* part, const int* cnt, int blocks,
+                                                            int E, float coef, float* __restrict__ loss,
                                                             int* __restrict__ counts, float* __restrict__ gain) {
   __shared__ float s_sum[1024];
   __shared__ int s_cnt[1024];
@@ -546,10 +545,9 @@ __global__ void __launch_bounds__(1024) balance_join_kernel(const float* __restr
 }
 
 template <int NI>
-__global__ void __launch_bounds__(256) balance_bwd_kernel(const float* __restrict__ probs,
-                                                          const float* __restrict__ gain,
-                                                          const bool* __restrict__ mask, int T, int E, float dloss,
-                                                          int add, float* __restrict__ dlogits) {
+__global__ void __launch_bounds__(256) balance_bwd_kernel(const float* probs, const float* gain,
+                                                          const bool* mask, int T, int E, float dloss, int add,
+                                                          float* __restrict__ dlogits) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
@@ -565,7 +563,7 @@ __global__ void __launch_bounds__(256) balance_bwd_kernel(const float* __restric
       dot[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        p[r][i] = live[r] && lane + 32 * i < E ? __ldg(probs + (t0 + r) * E + lane + 32 * i) : 0.f;
+        p[r][i] = live[r] && lane + 32 * i < E ? probs[(t0 + r) * E + lane + 32 * i] : 0.f;
         dot[r] += p[r][i] * g[i];
       }
     }

@@ -155,3 +155,28 @@ def test_act8_in_the_forward_and_backward():
     want, = torch.autograd.grad(act, v, dout.to(F8))
     assert torch.allclose(dgu.to(F8), want, rtol=2.0 ** -8, atol=1e-5)
     assert torch.allclose(again.to(F8), act.detach(), rtol=2.0 ** -8, atol=1e-6)
+
+
+def test_dependent_launches_read_with_plain_loads():
+    """A kernel that starts while the one before it runs may not use read-only
+    loads: they are defined only for memory that nobody writes meanwhile."""
+    import re
+    from pathlib import Path
+    waiting = 0
+    for f in sorted((Path(moe.__file__).resolve().parents[1] / "csrc").glob("*.cu")):
+        text = re.sub(r"__(launch_bounds|cluster_dims)__\([^)]*\)", "", f.read_text())
+        funcs = {}                     # device functions: from their qualifier to a brace in the first column
+        for m in re.finditer(r"^(?:__global__|KORE_DEV) .*?^}", text, re.M | re.S):
+            body = m.group(0)
+            funcs[re.search(r"(\w+)\(", body).group(1)] = body
+        todo = [n for n, body in funcs.items() if "pdl_wait()" in body]
+        waiting += len(todo)
+        reach = set()
+        while todo:
+            n = todo.pop()
+            if n not in reach:
+                reach.add(n)
+                todo += [c for c in re.findall(r"(\w+)(?:<\w+>)?\(", funcs[n]) if c in funcs]
+        for n in reach:
+            assert "__ldg" not in funcs[n] and not re.search(r"const \w+\s*\*\s*__restrict__", funcs[n]), (f.name, n)
+    assert waiting >= 18
