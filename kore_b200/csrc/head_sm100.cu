@@ -59,6 +59,13 @@ constexpr int kStoreBytes = 32 * 128;  // one store box: 32 rows x 128 bytes
 // 720). With parts of 8, 12, 16 k-blocks the error was 2.2e-7, 3.3e-7, 4.7e-7 and
 // the time 11.8, 11.0, 10.3 ms (T = 8192, V = 151936); unsplit 10.3 ms. Short
 // sums take a few parts too: 8.6e-7 with one at H = 1024.
+// The gradient's logits are summed in the same parts. Where the label is well
+// predicted, its entry c (p - 1) is what is left of the difference of its logit and
+// the forward's lse: summed over all of K at once the logit is off by 1e-4 at H = 5120,
+// always to one side, which was half of such a row's dx at 1 - p = 2e-4 (0.6% with the
+// parts). All of head_bwd, ms, one part / parts: T = 8192, H = 2048 11.9 / 12.4; H = 5120
+// about 2% more. With one or two rows the forward's sums are exact and the parts' error
+// (3e-7 of the logit) is left.
 __host__ __device__ constexpr int k_parts(int kblocks) {
   return kblocks <= 8 ? 1 : kblocks <= 16 ? 2 : kblocks <= 48 ? 3 : (kblocks + 15) / 16;
 }
@@ -75,10 +82,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // What a launch does with its tiles of A B^T:
 //   STATS  A = x, B = W piece: row statistics      (columns: vocabulary, K = H)
-//   GRAD   A = x, B = W piece: dz, bf16            (columns: vocabulary, K = H)
+//   GRAD   A = x, B = W piece: dz, bf16            (columns: vocabulary, K = H in one part)
+//   GRADK  the same where K has several parts
 //   PRODS  first A = dz, B = W piece^T: fp32 parts of dx   (columns: H, K = vocabulary, split)
 //          then  A = dz^T, B = x^T: dW of the piece        (rows: vocabulary, columns: H, K = dz's rows)
-enum Mode { STATS, GRAD, PRODS };
+enum Mode { STATS, GRAD, GRADK, PRODS };
 
 template <Mode M>
 struct Layout {
@@ -91,7 +99,7 @@ struct Layout {
 struct Params {
   int rows, cols, K;    // A rows, B rows (columns of the product), contraction
   int bn;               // columns per tile (multiple of 16, <= 256)
-  const long* targets;  // STATS, GRAD; may be null
+  const long* targets;  // STATS, GRAD(K); may be null
   int v0;               // vocabulary id of column 0
   float scale;          // log2(e) / tau: the epilogue works in powers of two
   float inv_temp;
@@ -99,7 +107,7 @@ struct Params {
   float* stats;         // [planes][2 num_n][rows]: m, s, (u)
   float* zt;            // [rows] label logit in units of log2
   int entropy;
-  // GRAD
+  // GRAD, GRADK
   const float* lse;
   const float* coef;
   __nv_bfloat16* low;   // not null: what bf16 leaves of dz goes here, row stride low_ld
@@ -179,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int num_n = (p.cols + bn - 1) / bn;
   const int num_mn = num_m * num_n;
   const int kblocks = (p.K + BK - 1) / BK;
-  const int part = (kblocks + k_parts(kblocks) - 1) / k_parts(kblocks);  // STATS: k-blocks per part
+  const int part = (kblocks + k_parts(kblocks) - 1) / k_parts(kblocks);  // k-blocks per part of a logit's sum
   const int dw_m = M == PRODS ? (p.K + 2 * BM - 1) / (2 * BM) : 0;
   const int first_dw = M == PRODS ? num_mn * p.splits : num_mn;          // work items before dW's
   const int num_items = first_dw + dw_m * num_n;
@@ -298,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Item w = item(t);
         const uint32_t idesc = w.dw ? idesc_w : idesc_x;
         for (int c0 = w.k0; c0 < w.k1; ++it) {
-          const int c1 = M == STATS ? min(c0 + part, w.k1) : w.k1;
+          const int c1 = M == STATS || M == GRADK ? min(c0 + part, w.k1) : w.k1;
           const int acc = it & 1;
           if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1)) { *abort_flag = 1; break; }
           tc_fence_after();
@@ -351,7 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const long y = p.targets[row] - p.v0 - n0;
         if (y >= 0 && y < cols) tc = (int)y;
       }
-      if (M == GRAD && live) {
+      if ((M == GRAD || M == GRADK) && live) {
         lse2 = p.lse[row] * kLog2e;
         c = p.coef[row] * p.inv_temp;
       }
@@ -361,6 +369,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(tempty_leader[acc]);
+      };
+      // sends a box of the warp's 32 rows x 128 bytes, a lane's row in eight vectors, to
+      // column x and row y; add: into what is there
+      auto store_begin = [&]() {
+        if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
+        __syncwarp();
+      };
+      auto store_put = [&](int j, const uint4& u) {
+        *reinterpret_cast<uint4*>(stage_buf + lane * 128 + ((j ^ (lane & 7)) * 16)) = u;
+      };
+      auto store_end = [&](const CUtensorMap* map, int x, int y, bool add) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (add) tma_reduce_add_2d(map, stage_buf, x, y);
+          else tma_store_2d(map, stage_buf, x, y);
+          tma_store_commit();
+        }
+      };
+      auto store = [&](const CUtensorMap* map, const uint4 (&out)[8], int x, int y, bool add) {
+        store_begin();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) store_put(j, out[j]);
+        store_end(map, x, y, add);
+      };
+      // 64 logits of the row, from the warp's column c0 on: dz is made in place and sent
+      auto send_dz = [&](float (&f)[64], int c0) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) f[i] = -c * ex2(fmaf(f[i], p.scale, -lse2));
+        if (c == 0.f || c0 + 64 > cols) {
+          // coefficient 0, or past the piece's last column: 0
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (c == 0.f || c0 + i >= cols) f[i] = 0.f;
+        }
+        const int ti = tc - c0;
+        if (ti >= 0 && ti < 64) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i == ti) f[i] += c;
+        }
+        store_begin();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          store_put(j, make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
+                                  pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7])));
+        store_end(&maps.d, n0 + c0, row0, false);
+        if (p.low != nullptr && live) {
+          __nv_bfloat16* low = p.low + row * p.low_ld + n0 + c0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float a = f[8 * j + 2 * e], b = f[8 * j + 2 * e + 1];
+              const uint32_t hi = pack_bf16(a, b);
+              l[e] = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+            }
+            if (c0 + 8 * j < cols) *reinterpret_cast<uint4*>(low + 8 * j) = make_uint4(l[0], l[1], l[2], l[3]);
+          }
+        }
       };
       if (M == STATS) {
         // the row's columns stay in registers: first the maximum, then the sums
@@ -440,65 +509,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           p.stats[o + plane] = s;
           if (p.entropy) p.stats[o + 2 * plane] = u;
         }
+      } else if (M == GRADK) {
+        // the sum of the parts, as the forward sums them; the row's logits stay in registers
+        float v[2][64];
+        bool ok = true;
+        for (int k = w.k0; k < w.k1; k += part, ++it) {
+          const int acc = it & 1;
+          if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (32 * j < cols) {
+              uint32_t r[32];
+              tmem_ld32(t_row + acc * kMaxBN + 32 * j, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float& z = v[j / 2][32 * (j & 1) + i];
+                z = k == w.k0 ? __uint_as_float(r[i]) : z + __uint_as_float(r[i]);
+              }
+            }
+          release(acc);
+        }
+        if (!ok) { *abort_flag = 1; break; }
+        if (cols > 0) send_dz(v[0], 0);
+        // the second half's arithmetic stays behind the first half's stores (registers)
+#pragma unroll
+        for (int i = 0; i < 64; ++i) asm volatile("" : "+f"(v[1][i]));
+        if (cols > 64) send_dz(v[1], 64);
+      } else if (M == GRAD) {
+        const int acc = it & 1;
+        if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { *abort_flag = 1; break; }
+        ++it;
+        tc_fence_after();
+        for (int c0 = 0; c0 < cols; c0 += 64) {
+          float f[64];
+          load64(f, t_row + acc * kMaxBN + c0);
+          send_dz(f, c0);
+        }
+        release(acc);
       } else {
         const int acc = it & 1;
         if (!mbar_wait(&tfull_bar[acc], (it >> 1) & 1)) { *abort_flag = 1; break; }
         ++it;
         tc_fence_after();
-        const int box = M == GRAD || (w.dw && !p.dw_f32) ? 64 : 32;  // columns of 128 bytes
+        const int box = w.dw && !p.dw_f32 ? 64 : 32;  // columns of 128 bytes
         for (int c0 = 0; c0 < cols; c0 += box) {
-          // sends the warp's 32 rows x 128 bytes; add: into what is there
-          auto store = [&](const CUtensorMap* map, const uint4 (&out)[8], int y, bool add) {
-            if (lane == 0) tma_store_wait_read<0>();  // the last store has read the buffer
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(stage_buf + lane * 128 + ((j ^ (lane & 7)) * 16)) = out[j];
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (add) tma_reduce_add_2d(map, stage_buf, n0 + c0, y);
-              else tma_store_2d(map, stage_buf, n0 + c0, y);
-              tma_store_commit();
-            }
-          };
           uint4 out[8];
-          if (M == GRAD) {
-            float f[64];
-            load64(f, t_row + acc * kMaxBN + c0);
-#pragma unroll
-            for (int i = 0; i < 64; ++i) f[i] = -c * ex2(fmaf(f[i], p.scale, -lse2));
-            if (c == 0.f || c0 + 64 > cols) {
-              // coefficient 0, or past the piece's last column: 0
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (c == 0.f || c0 + i >= cols) f[i] = 0.f;
-            }
-            const int ti = tc - c0;
-            if (ti >= 0 && ti < 64) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i == ti) f[i] += c;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              out[j] = make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
-                                  pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7]));
-            store(&maps.d, out, row0, false);
-            if (p.low != nullptr && live) {
-              __nv_bfloat16* low = p.low + row * p.low_ld + n0 + c0;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const uint32_t hi[4] = {out[j].x, out[j].y, out[j].z, out[j].w};
-                uint32_t l[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  l[e] = pack_bf16(f[8 * j + 2 * e] - __uint_as_float(hi[e] << 16),
-                                   f[8 * j + 2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
-                if (c0 + 8 * j < cols) *reinterpret_cast<uint4*>(low + 8 * j) = make_uint4(l[0], l[1], l[2], l[3]);
-              }
-            }
-          } else if (w.dw && !p.dw_f32) {
+          if (w.dw && !p.dw_f32) {
             float f[64];
             load64(f, t_row + acc * kMaxBN + c0);
             if (p.dw_add && live) {  // one rounding of the sum: no bf16 reduction of a rounded tile
@@ -520,15 +578,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 8; ++j)
               out[j] = make_uint4(pack_bf16(f[8 * j], f[8 * j + 1]), pack_bf16(f[8 * j + 2], f[8 * j + 3]),
                                   pack_bf16(f[8 * j + 4], f[8 * j + 5]), pack_bf16(f[8 * j + 6], f[8 * j + 7]));
-            store(&maps.d2, out, row0, false);
+            store(&maps.d2, out, n0 + c0, row0, false);
           } else {
             uint32_t r[32];
             tmem_ld32(t_row + acc * kMaxBN + c0, r);
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 8; ++j) out[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            if (w.dw) store(&maps.d2, out, row0, p.dw_add != 0);
-            else store(&maps.d, out, w.split * p.split_rows + row0, p.add != 0);
+            if (w.dw) store(&maps.d2, out, n0 + c0, row0, p.dw_add != 0);
+            else store(&maps.d, out, n0 + c0, w.split * p.split_rows + row0, p.add != 0);
           }
         }
         release(acc);
@@ -985,7 +1043,8 @@ at::Tensor head_bwd(const at::Tensor& x, const at::Tensor& w, const c10::optiona
     p.v0 = (int)v0;
     grad.b = make_tmap_2d(wp, bf, 2, H, n, row_stride(w), BK, kMaxBN / 2);
     grad.d = make_tmap_2d(dz, bf, 2, (n + 7) / 8 * 8, T, width, 64, 32);
-    launch<GRAD>(grad, p, dev, st);
+    if (k_parts((H + BK - 1) / BK) == 1) launch<GRAD>(grad, p, dev, st);
+    else launch<GRADK>(grad, p, dev, st);
     d.K = n;
     d.add = v0 > 0;
     d.dw = (uint8_t*)dw.data_ptr() + v0 * H * (f32 ? 4 : 2);

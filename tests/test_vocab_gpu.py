@@ -129,6 +129,39 @@ def test_head_backward_is_the_gradient():
             assert abs(num - (d.to(F8) * v).sum()) <= 6 * 2.0 ** -8 * (d.to(F8) * v).norm() + 1e-6
 
 
+@pytest.mark.parametrize("T,H", [(100, 1024), (300, 1024), (300, 2048), (100, 5120), (300, 5120)])
+def test_head_backward_of_well_predicted_labels(T, H):
+    """The label's entry c (p - 1) with p near 1: it is the difference of the logit, summed
+    as the forward summed it, and the forward's lse, so only their last roundings show."""
+    V = 6000
+    g = torch.Generator(device="cuda").manual_seed(H)
+    w = (torch.randn(V, H, generator=g, device="cuda") * 0.02).bfloat16()
+    y = torch.randperm(V, generator=g, device="cuda")[:T]
+    wy = w[y].float()
+    lean = torch.linspace(6.0, 30.0, T, device="cuda")[:, None]         # 1 - p from near 1 down to 1e-9
+    x = (torch.randn(T, H, generator=g, device="cuda") + lean * wy / wy.square().sum(-1, keepdim=True)).bfloat16()
+    coef = torch.full((T,), -1.0, device="cuda")
+    _, _, lse = vocab.head_fwd(x, w, y)
+    dx, dw = vocab.head_bwd(x, w, y, lse, coef)
+    assert ops.check_device_error() == 0
+    z = x.to(F8) @ w.to(F8).t()
+    l = torch.logsumexp(z, -1, keepdim=True)
+    p = (z - l).exp()
+    rows = torch.arange(T, device="cuda")
+    mag = (x.to(F8).abs() @ w.to(F8).abs().t()).amax(-1, keepdim=True)
+    delta = (H / 16 + 2) * 2.0 ** -23 * mag + 2e-6 * (1 + l.abs())      # of another entry's logit
+    slack = (2.0 ** -8 + 2 * delta) * p
+    dz = p.clone()
+    dz[rows, y] = torch.expm1(z[rows, y] - l[:, 0])
+    # eight roundings of 2^-24 of lse between the logit and the exponent, and the exponential's own
+    slack[rows, y] = 2.0 ** -8 * dz[rows, y].abs() + 2.0 ** -21 * (1 + l[:, 0].abs())
+    slack += 2.0 ** -18 * dz.abs()
+    want = dz @ w.to(F8)
+    assert ((dx.to(F8) - want).abs() <= slack @ w.to(F8).abs() + 2.0 ** -8 * want.abs() + 1e-30).all()
+    want = dz.t() @ x.to(F8)
+    assert ((dw.to(F8) - want).abs() <= slack.t() @ x.to(F8).abs() + 2.0 ** -8 * want.abs() + 1e-30).all()
+
+
 def test_head_strides_streams_and_repeats():
     T, V, H = 200, 3001, 136
     x, w, y, coef = _inputs(T, V, H, seed=4)
