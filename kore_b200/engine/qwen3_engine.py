@@ -22,7 +22,8 @@ Options of the step (defaults leave it as described above):
   head="pieces"       the head runs in pieces of the vocabulary without logits
                       (ops.vocab): fp32 log-probs, dW written once
   embed_grad="sorted" the embedding gradient sums each token's rows in fp32 in
-                      a fixed order instead of with bf16 atomics
+                      a fixed order instead of with bf16 atomics; ids outside
+                      the table read a zero row and have no gradient
   act8=True           layer inputs, and the contexts of layers that skip the
                       recompute, are kept in 8 bits (ops.act8): about a third of
                       a bf16 context, so three times the layers keep theirs
@@ -489,6 +490,10 @@ class Qwen3Engine:
     def _kept(self, u: int) -> bool:
         return self.keep_layers > 0 and u > self.w.num_units - 2 - self.keep_layers
 
+    def _embed(self, ids: torch.Tensor) -> torch.Tensor:
+        table = self.w.views(0)["embed"]
+        return vocab.embed(ids, table) if self.embed_grad == "sorted" else ops.embed_fwd(ids, table)
+
     @torch.no_grad()
     def forward_hidden(self, b: Batch, checkpoints: Optional[list] = None,
                        attn_saves: Optional[list] = None, contexts: Optional[dict] = None,
@@ -499,7 +504,7 @@ class Qwen3Engine:
         recompute attention; ``contexts`` receives the whole forward context of
         the layers selected by ``keep_layers`` (no recompute at all);
         ``routings`` the MoE layers' choices where the checkpoints are 8-bit."""
-        x = ops.embed_fwd(b.ids, self.w.views(0)["embed"])
+        x = self._embed(b.ids)
         hook = self.param_hook
         last = self.w.num_units - 2
         for u in range(1, self.w.num_units - 1):
@@ -537,7 +542,7 @@ class Qwen3Engine:
         layers from host memory or gathers them over ranks, the weights then
         move once per call instead of once per micro-batch (the hidden states
         of all batches stay resident)."""
-        xs = [ops.embed_fwd(b.ids, self.w.views(0)["embed"]) for b in batches]
+        xs = [self._embed(b.ids) for b in batches]
         hook = self.param_hook
         last = self.w.num_units - 2
         for u in range(1, self.w.num_units - 1):

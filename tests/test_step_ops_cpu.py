@@ -264,3 +264,21 @@ def test_plan_leaves_room_for_the_layer_in_flight(monkeypatch, act8):
     assert tr.plan_activations(tokens) == 2
     free -= 1
     assert tr.plan_activations(tokens) == 1
+
+
+def test_ids_outside_the_table_with_the_sorted_gradient():
+    """They read a zero row, as their gradient says: no row of the table changes what they give."""
+    cfg = _cfg()
+    g = torch.Generator().manual_seed(0)
+    b = Batch.from_sequences([torch.randint(0, cfg.vocab_size - 1, (21,), generator=g)])
+    b.ids[4], b.ids[9] = -1, cfg.vocab_size
+    b.targets[3] = b.targets[8] = -1                          # the tokens before them have no label
+    eng = _engine(cfg, embed_grad="sorted")
+    eng.zero_grad()
+    eng.forward_backward(b, coef=eng.sft_coef(b))
+    table, grad = eng.w.views(0)["embed"], eng.grad_views(0)["embed"]
+    assert (grad[-1] == 0).all()
+    lp = eng.token_logprobs(b)[0]
+    many = eng.token_logprobs_many([b])[0][0]
+    table[-1] += 1.0
+    assert torch.equal(eng.token_logprobs(b)[0], lp) and torch.equal(many, lp)
