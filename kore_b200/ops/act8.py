@@ -37,11 +37,6 @@ class Act8:
     def nbytes(self) -> int:
         return self.q.numel() + 4 * self.s.numel()
 
-    def record_stream(self, stream) -> None:
-        """For a checkpoint that another stream than its own reads (as torch's own)."""
-        self.q.record_stream(stream)
-        self.s.record_stream(stream)
-
 
 def empty(T: int, H: int, device) -> Act8:
     if H <= 0 or H % 8:
