@@ -429,9 +429,9 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(Held h, const __nv_bflo
   pdl_trigger();
   if (j * 8 >= F) return;
   for (long t = blockIdx.y; t < T; t += gridDim.y) {
-    const uint2 qg = reinterpret_cast<const uint2*>(h.q + t * h.H)[j];
-    const uint2 qu = reinterpret_cast<const uint2*>(h.q + t * h.H + F)[j];
-    const uint4 dv = reinterpret_cast<const uint4*>(dout + t * ldd)[j];
+    const uint2 qg = load_once(reinterpret_cast<const uint2*>(h.q + t * h.H) + j);
+    const uint2 qu = load_once(reinterpret_cast<const uint2*>(h.q + t * h.H + F) + j);
+    const uint4 dv = load_once(reinterpret_cast<const uint4*>(dout + t * ldd) + j);
     const float sg = h.s[t * h.nb + j / 16], su = h.s[t * h.nb + (F / 8 + j) / 16];
     uint64_t g[4], u[4], d[4], dg[4];
     restore(qg, sg, g);

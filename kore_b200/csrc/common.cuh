@@ -73,6 +73,17 @@ KORE_DEV bool elect_one() {
 // earlier. Read-only loads (__ldg, const __restrict__ parameters) are defined only
 // for memory that nobody writes while the kernel runs, and a compiler may move them
 // above the wait: such kernels read global memory with plain loads. pdl_trigger() lets the next such kernel start once all blocks are here.
+KORE_DEV uint4 load_once(const uint4* p) {  // a plain load of what is read once: not kept in L1
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+KORE_DEV uint2 load_once(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
 KORE_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 KORE_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

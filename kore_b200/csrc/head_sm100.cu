@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __nv_bfloat
       uint4 wv[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        wv[r] = r0 + r < V ? reinterpret_cast<const uint4*>(w + (r0 + r) * ldw)[j] : make_uint4(0, 0, 0, 0);
+        wv[r] = r0 + r < V ? load_once(reinterpret_cast<const uint4*>(w + (r0 + r) * ldw) + j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const uint4 xv = sx[t * nvec + j];
