@@ -13,7 +13,7 @@
 // magnitude bits. They are bound by HBM (copy rate 6.5 TB/s), measured at
 //   16384 x 5120   RMSNorm + save 69 us, 6.1 TB/s; load + RMSNorm 66 us, 6.4 TB/s
 //                  save 42 us, 6.0 TB/s; load 44 us, 5.8 TB/s
-//   8192 x 17408   SwiGLU + save 193 us, 6.0 TB/s; SwiGLU backward 229 us, 6.3 TB/s
+//   8192 x 17408   SwiGLU + save 194 us, 5.9 TB/s; SwiGLU backward 237 us, 6.1 TB/s
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -123,9 +123,9 @@ struct Held {
 
 // Element-wise kernels: a thread owns one 8-column vector j and walks rows with
 // the grid's y; the loads of a few rows are issued before the first is used.
-// More rows cost registers and so resident warps (5003 x 5120 and 8192 x 17408, us,
-// with 1, 2, 4 rows: save -, 41, 49; load -, 49, 45; SwiGLU save 208, 185, -;
-// backward 229, 246, -).
+// More rows cost registers and so resident warps (us, L2 flushed, with 1, 2, 4 rows:
+// 16384 x 5120 save -, 49, 57; load -, 49, 49; 8192 x 17408 SwiGLU save 217, 197, -;
+// its backward, when it was tried, 229, 246, -).
 constexpr int kSaveRows = 2;
 constexpr int kLoadRows = 4;
 
@@ -304,7 +304,7 @@ KORE_DEV uint64_t sigmoid(uint64_t x) {
 }
 
 // HOLD (F % 128 == 0, so that a block lies wholly in gate or in up): also
-// writes the 8-bit copy (4 blocks of 256 threads per SM: 193 us at 8192 x 17408, 211 without)
+// writes the 8-bit copy (4 blocks of 256 threads per SM: 194 us at 8192 x 17408, 211 without)
 template <bool HOLD>
 __global__ void __launch_bounds__(256, 4) swiglu_kernel(const __nv_bfloat16* gu, long ldg,
                                                      __nv_bfloat16* __restrict__ a, Held h, long T) {

@@ -23,10 +23,11 @@
 //
 // Bound by the tensor cores: at T = 8192, V = 151936, H = 5120 the forward takes 9.1 ms
 // in a short run (1.40 PFLOP/s) and 10.0 ms under the power cap (1.28; a library
-// GEMM sustains 1.38), forward and gradients 39 ms over four products of 2 T V H.
-// Few rows are bound by W (T = 1: 266 us, 5.9 TB/s); small H by the epilogue, which
-// reads 256 columns a row from TMEM and takes as many exponentials (T = 1065,
-// V = 124357, H = 136: 117 us, 3.6 us a tile).
+// GEMM sustains 1.38), forward and gradients 40 ms over four products of 2 T V H.
+// One row is bound by W (255 us, 6.1 TB/s); small H by the latency of the epilogue,
+// which reads 256 columns a row from TMEM and takes as many exponentials with two
+// warps per scheduler (T = 1065, V = 124357, H = 136: 117 us, 3.6 us a tile; issue
+// slots 35% busy, the exponential unit 34%, the tensor pipe 26%).
 //
 // Reference parity: kore/policy/grpo.py:2728-2743 (log-softmax and gather over
 // the full vocabulary), kore/policy/sft.py:346-399 (mean cross-entropy).
@@ -607,7 +608,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------- few rows
 // One or two rows are bound by reading W once. Fused multiply-adds keep up with
 // that, and start and finish sooner than the tensor-core pipeline (a pass, us, this
-// kernel / the 256-row tiles: T = 1, V = 151936, H = 5120: 266 / 300; T = 2: 306 / 300;
+// kernel / the 256-row tiles: T = 1, V = 151936, H = 5120: 255 / 300; T = 2: 310 / 300;
 // T = 1, V = 32000, H = 256: 13.5 / 24; T = 2: 17.6 / 24; four rows here: 338 at H = 5120).
 // A warp takes 4 vocabulary entries at a time, lanes stride H, x stays in
 // shared memory; products and sums are fp32 (two per instruction).
@@ -856,7 +857,8 @@ void launch_few(const __nv_bfloat16* x, long ldx, const __nv_bfloat16* w, long l
 
 // Parts of dx's contraction (the piece's vocabulary): as many as fill the pairs
 // when T x H has few tiles; each part costs a pass over [T, H] in fp32. In units
-// of one k-block of a tile (0.27 us): 1.5 MB of HBM traffic.
+// of one k-block of a tile (0.27 us at the nominal rate, 0.37 at the 720 clocks it
+// takes): 1.5 MB of HBM traffic.
 int pick_splits(long tiles, long kblocks, long dx_elems, int pairs) {
   int best = 1;
   double best_cost = -1;

@@ -414,7 +414,7 @@ inline int warps_grid(long n, int warps_per_block = 8) {
 // Counts are integers; P sums in fp32 in an order that only T and E fix: a
 // warp's tokens, a block's warps, then the blocks. Masked tokens are not read.
 // Small: 17 MB at T = 32768, E = 128 stay in L2; the three launches take 5.5, 3 and
-// 6.5 us (5.3 us is what HBM would need), a pass 20 us with its host side. Small
+// 6.5 us (5.3 us is what HBM would need), a pass 18.5 us with its host side. Small
 // batches finish in one block (T = 64, E = 8: 3.4 us).
 constexpr int kBalUnroll = 4;   // tokens that a warp has in flight
 

@@ -55,7 +55,7 @@ def head_bwd(x: torch.Tensor, w: torch.Tensor, targets: Optional[torch.Tensor], 
     dx [T, H] is overwritten; dw [V, H] (bf16 or fp32) is overwritten, or added
     to with ``accumulate``. The logits are computed again for ``piece``
     vocabulary entries at a time (0: the size whose dz, [T, piece] bf16, takes
-    about 256 MB), so no [T, V] tensor exists. Rows with coefficient 0
+    about 256 MB, and 4,096 at least), so no [T, V] tensor exists. Rows with coefficient 0
     contribute nothing, even if x holds inf or NaN there. A row whose target is
     outside [0, V) has no label: its gradient is that of -coef_t * lse_t."""
     inv = _inv_temp(temperature)
