@@ -135,6 +135,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_rmsnorm_load(const at::Tenso
                                                                  const at::Tensor& w, double eps);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_swiglu_save(const at::Tensor& gu);
 std::tuple<at::Tensor, at::Tensor> act8_swiglu_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& s);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>> paged_plan(
+    const at::Tensor& ctx, const at::Tensor& new_toks, at::Tensor& table, int64_t page_size, int64_t rows,
+    const c10::optional<at::Tensor>& held, const c10::optional<at::Tensor>& free_stack,
+    const c10::optional<at::Tensor>& free_count);
+void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& table,
+                            const at::Tensor& lens, const at::Tensor& q_start, int64_t page_size, int64_t max_q,
+                            double scale, const c10::optional<at::Tensor>& group_start,
+                            const c10::optional<at::Tensor>& prefix_len, at::Tensor& out,
+                            const c10::optional<at::Tensor>& lse);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& logits, const at::Tensor& tokens,
+                                                           const at::Tensor& q_start, const at::Tensor& u,
+                                                           double temperature, const c10::optional<at::Tensor>& probs);
 int read_and_clear_device_error();
 }  // namespace kore
 
@@ -210,5 +222,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_rmsnorm_load", &kore::act8_rmsnorm_load);
   m.def("act8_swiglu_save", &kore::act8_swiglu_save);
   m.def("act8_swiglu_bwd", &kore::act8_swiglu_bwd);
+  m.def("paged_plan", &kore::paged_plan, "block tables and slot maps from request lengths");
+  m.def("paged_prefix_attention", &kore::paged_prefix_attention, "paged attention with shared prefixes");
+  m.def("spec_verify", &kore::spec_verify, "verification of drafted tokens");
   m.def("read_and_clear_device_error", &kore::read_and_clear_device_error);
 }

@@ -20,6 +20,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "tma_host.h"
 
@@ -32,14 +34,16 @@ constexpr int D = 128;
 // slot[t] = page * page_size + offset (precomputed on host side of the engine).
 __global__ void kv_append_kernel(const __nv_bfloat16* __restrict__ k, int ldk,
                                  const __nv_bfloat16* __restrict__ v, int ldv,
-                                 const int* __restrict__ slots, __nv_bfloat16* __restrict__ kc,
+                                 const int* __restrict__ slots, long nslots, __nv_bfloat16* __restrict__ kc,
                                  __nv_bfloat16* __restrict__ vc, int T, int Hkv) {
   const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;  // one thread per 8 elements
   const long per_tok = (long)Hkv * D / 8;
   if (i >= (long)T * per_tok) return;
   const long t = i / per_tok;
   const int r = (int)(i % per_tok) * 8;
-  const long dst = (long)slots[t] * Hkv * D + r;
+  const long slot = slots[t];
+  if (slot < 0 || slot >= nslots) return;   // a row that has no place in the cache
+  const long dst = slot * Hkv * D + r;
   *reinterpret_cast<uint4*>(kc + dst) = *reinterpret_cast<const uint4*>(k + t * ldk + r);
   *reinterpret_cast<uint4*>(vc + dst) = *reinterpret_cast<const uint4*>(v + t * ldv + r);
 }
@@ -678,7 +682,7 @@ void kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots
   const long n = (long)T * Hkv * D / 8;
   kv_append_kernel<<<(int)((n + 255) / 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
       (const __nv_bfloat16*)k.data_ptr(), k.stride(0), (const __nv_bfloat16*)v.data_ptr(), v.stride(0),
-      slots.data_ptr<int>(), (__nv_bfloat16*)kc.data_ptr(), (__nv_bfloat16*)vc.data_ptr(), T, Hkv);
+      slots.data_ptr<int>(), std::min(kc.size(0), vc.size(0)), (__nv_bfloat16*)kc.data_ptr(), (__nv_bfloat16*)vc.data_ptr(), T, Hkv);
   check_cuda(cudaGetLastError(), "kv_append");
 }
 
