@@ -16,8 +16,6 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-
 #include <tuple>
 
 #include "common.cuh"
