@@ -118,23 +118,34 @@ __global__ void plan_rows_kernel(PlanParams p) {
 // -------------------------------------------------------- prefix attention
 // A unit of work is the prefix of a group (all query rows of its sequences against
 // the shared keys) or a sequence's own keys (its rows against what follows the
-// prefix). A unit is cut into items, one for each kv head and each block of at most
-// 128 rows (row = token x query head of the kv head), and an item into tiles of 64
-// keys. All tiles of a call, in one order, are dealt to the blocks in equal runs, so
-// that a long prefix is split over as many blocks as it needs and no host value
-// depends on the lengths. A block that has an item's every tile and no other part to
-// join it with writes the result; all else goes to fp32 partials (running maximum,
-// sum and unnormalised output), which a second kernel joins in a fixed order:
+// prefix). A unit is cut into items, one for each kv head and each block of query
+// rows (row = token x query head of the kv head), and an item into tiles of 64 keys.
+// All tiles, in one order, are dealt to the blocks in equal runs, so that a long
+// prefix is split over as many blocks as it needs and no host value depends on the
+// lengths. An item that one block has whole, and that no other unit's part joins, is
+// written as the result; all else goes to fp32 partials (reference exponent, sum and
+// unnormalised output), which a second kernel joins in a fixed order:
 //   m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l.
+//
+// Items come in two forms, each with its own runs:
+//   wide   S[128 rows x 64 keys] = Q K^T, O[128 x 128] += P V: prefixes, and own keys
+//          when a sequence has more than 64 rows. One softmax thread owns a row.
+//   narrow S^T[64 keys x N rows] = K Q^T, O^T[128 x N] += V^T P^T with N = 16, 32 or
+//          64: own keys under few rows. The products cost N / 64 of the wide form's
+//          and a tile's exponentials are spread over its keys, not over the few rows.
+// Half of the blocks begin with their wide run, the other half with their narrow one:
+// two blocks share an SM, and the first is bound by the tensor cores where the second
+// is bound by HBM.
 constexpr int D = 128;
 constexpr int BK = 64;                            // keys of a tile
 constexpr int kStages = 2;
 constexpr int kTileBytes = BK * D * 2;            // 16 KB: 64 keys as two 8 KB swizzle atoms
 constexpr int kQBytes = 128 * D * 2;
 constexpr int kAttnThreads = 192;                 // producer, MMA, four softmax warps
-constexpr int kTmemCols = 256;                    // two S / P buffers of 64 columns, O of 128
-constexpr int kMaxSeqs = 1024;
-constexpr int kMinTiles = 4;                      // of a block: fewer cost more in partials than they save
+constexpr int kTmemCols = 256;                    // wide: two S / P buffers of 64 columns, O of 128; narrow: two S of 64, two O of 64
+constexpr uint32_t kTmemO = 128;
+constexpr int kMaxSeqs = 512;
+constexpr int kMinTiles = 4;                      // of a run: fewer cost more in partials than they save
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttnParams {
@@ -142,150 +153,730 @@ struct AttnParams {
   long ld_table;
   int M, page_size, B, T, Hq, Hkv, G;
   int tokens_prefix, tokens_own;                  // tokens of a row block, for a group's prefix and a sequence's own keys
+  int nwide;                                      // units in wide form: the first nwide
   int box;                                        // keys of one TMA box: gcd(64, page_size)
   const int *group_start, *prefix;                // null: no groups
   int ngroups;
   float scale_log2;
   __nv_bfloat16* out;
   float* lse;
-  float *whole_prefix, *whole_own;                // [T * Hq][D + 2]: o, then m and l, of items that one block had whole
-  float* split;                                   // [2 * blocks][128][D + 2]: a block's first and last, part-done items
-  int* meta;                                      // [units + 1] running sum of tiles
+  // Partial rows: o, then m and l. Items that one block had whole, by their result's
+  // row; what the runs cut, two items (a run's first and last) for each run.
+  float *whole_prefix, *whole_own, *split_wide, *split_narrow;
+  int4* where;                                    // [T][2] for the join: where the token's parts begin
+  int* runs;                                      // wide tiles, wide runs, narrow tiles, narrow runs
 };
 constexpr int kPart = D + 4;                      // floats of a partial row (16-byte aligned)
 
+// mbar_wait with its clock out of line: the kernel below has many waits, and what it
+// executes has to stay in the instruction cache.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t phase) { return mbar_wait(bar, phase); }
+KORE_DEV bool wait_on(uint64_t* bar, uint32_t phase) { return mbar_try_wait(smem_u32(bar), phase) || wait_long(bar, phase); }
 // A whole warp's wait: the lanes go on together or give up together.
-KORE_DEV bool warp_wait(uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffff, mbar_wait(bar, phase)); }
+KORE_DEV bool warp_wait(uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffff, wait_on(bar, phase)); }
 
 struct AttnSmem {
-  static constexpr int Q_OFF = 0;
+  static constexpr int Q_OFF = 0;                                    // wide: Q; narrow: two Q, then two P buffers
   static constexpr int K_OFF = kQBytes;
   static constexpr int V_OFF = K_OFF + kStages * kTileBytes;
   static constexpr int BAR_OFF = V_OFF + kStages * kTileBytes;
-  static constexpr int QS_OFF = BAR_OFF + 256;                       // int [kMaxSeqs + 1]
-  static constexpr int CUM_OFF = QS_OFF + 4 * (kMaxSeqs + 2);        // int [2 * kMaxSeqs + 1]
-  static constexpr int GS_OFF = CUM_OFF + 4 * (2 * kMaxSeqs + 2);    // uint16 [kMaxSeqs + 1]
-  static constexpr int TOTAL = GS_OFF + 2 * (kMaxSeqs + 2) + 1024;
+  static constexpr int X_OFF = BAR_OFF + 256;                        // NarrowSmem
+  static constexpr int UNITS_OFF = X_OFF + 6 * 64 * 4;               // Units
+  static constexpr int TOTAL = UNITS_OFF + 4 * 7 * kMaxSeqs + 1024;
 };
 static_assert(2 * (AttnSmem::TOTAL + 1024) <= 228 * 1024, "two blocks share an SM");
 
-// 128 x 128 tile as two K-major 64-column atoms of 16 KB, at K-step kk; 64 x 128 tile
-// (two atoms of 8 KB) K-major and MN-major (rows = K) at K-step kk.
-KORE_DEV uint64_t q_desc(uint32_t base, int kk) { return make_sw128_desc(base + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024); }
-KORE_DEV uint64_t k_desc(uint32_t base, int kk) { return make_sw128_desc(base + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024); }
-KORE_DEV uint64_t v_desc(uint32_t base, int kk) { return make_sw128_desc(base + kk * 2048, 8192, 1024); }
+// Shared-memory layouts, all of 64-column (128-byte) swizzled atoms: Q 128 x 128 in two
+// atoms of 16 KB; K and V 64 x 128 in two of 8 KB (V as an MN-major operand: rows = K);
+// narrow Q N x 128 in two of N * 128 bytes and P^T N x 64 in one.
+KORE_DEV void tma_load_4d(void* dst, const CUtensorMap* d, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(d)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 KORE_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   tmem_st16(taddr, *reinterpret_cast<const uint32_t(*)[16]>(&r[0]));
   tmem_st16(taddr + 16, *reinterpret_cast<const uint32_t(*)[16]>(&r[16]));
 }
+// Warp-wide maximum (NaN is passed over) and a vote and a barrier of the four softmax warps.
+KORE_DEV float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+KORE_DEV bool softmax_any(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred P, Q;\nsetp.ne.u32 P, %1, 0;\n"
+      "barrier.cta.red.or.pred Q, 1, 128, P;\n"
+      "selp.u32 %0, 1, 0, Q;\n}\n"
+      : "=r"(r) : "r"((uint32_t)v) : "memory");
+  return r != 0;
+}
+// The four warps' wait: they meet at named barriers, so they give up together too.
+KORE_DEV bool softmax_wait(uint64_t* bar, uint32_t phase) { return !softmax_any(!warp_wait(bar, phase)); }
+KORE_DEV void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-// The units as every block sees them: unit u < ngroups is a prefix, unit ngroups + b sequence b.
+// The units as every block sees them, in shared memory: unit u < ngroups is a prefix,
+// unit ngroups + b sequence b.
 struct Units {
   const AttnParams& p;
-  const int* qs;          // [B + 1] clamped to [0, T]
-  const int* cum;         // [units + 1] tiles before the unit
-  const uint16_t* gs;     // [ngroups + 1] clamped to [0, B]
-  KORE_DEV int cap() const { return p.M * p.page_size; }
-  KORE_DEV int group_of(int b) const {              // -1: none
-    int lo = 0, hi = p.ngroups;                     // first group that starts behind b
+  int *qs, *gs, *cum;     // [B + 1] rows, [ngroups + 1] sequences (both clamped to what exists), [units + 1] tiles before the unit
+  int *len, *prefix;      // [B], [ngroups] keys, clamped to the table
+  short* grp;             // [B] group, -1: none
+  KORE_DEV Units(const AttnParams& p_, uint8_t* at) : p(p_) {
+    qs = reinterpret_cast<int*>(at);
+    gs = qs + kMaxSeqs + 4;
+    cum = gs + kMaxSeqs + 4;
+    len = cum + 2 * kMaxSeqs + 4;
+    prefix = len + kMaxSeqs;
+    grp = reinterpret_cast<short*>(prefix + kMaxSeqs);
+    static_assert(3 * (kMaxSeqs + 4) + 3 * kMaxSeqs + kMaxSeqs / 2 <= 7 * kMaxSeqs, "the units fit");
+  }
+  KORE_DEV int seq_of(int t, int lo, int hi) const {  // the sequence in [lo, hi] that holds row t
+#pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (gs[mid] <= b) lo = mid + 1; else hi = mid;
+      if (qs[mid + 1] <= t) lo = mid + 1; else hi = mid;
     }
-    return lo > 0 && b < gs[lo] ? lo - 1 : -1;
+    return lo;
   }
-  KORE_DEV int prefix_of(int g) const { return min(max(p.prefix[g], 0), cap()); }
   KORE_DEV int row0(int u) const { return u < p.ngroups ? qs[gs[u]] : qs[u - p.ngroups]; }
   KORE_DEV int tokens(int u) const {
     return u < p.ngroups ? qs[gs[u + 1]] - qs[gs[u]] : qs[u - p.ngroups + 1] - qs[u - p.ngroups];
   }
   KORE_DEV int block_tokens(int u) const { return u < p.ngroups ? p.tokens_prefix : p.tokens_own; }
-  KORE_DEV int blocks(int u) const { return (tokens(u) + block_tokens(u) - 1) / block_tokens(u); }
+  KORE_DEV int blocks(int u) const {
+    const int tb = block_tokens(u), n = tokens(u);
+    return n <= tb ? 1 : (n + tb - 1) / tb;
+  }
   KORE_DEV void keys(int u, int& lo, int& hi) const {      // the unit's keys
     if (u < p.ngroups) {
       lo = 0;
-      hi = prefix_of(u);
+      hi = prefix[u];
     } else {
-      const int g = p.ngroups ? group_of(u - p.ngroups) : -1;
-      lo = g < 0 ? 0 : prefix_of(g);
-      hi = min(max(p.lens[u - p.ngroups], 0), cap());
+      const int g = grp[u - p.ngroups];
+      lo = g < 0 ? 0 : prefix[g];
+      hi = len[u - p.ngroups];
     }
   }
-  KORE_DEV int tiles(int u) const {
-    if (tokens(u) <= 0) return 0;
+  KORE_DEV int item_tiles(int u) const {
     int lo, hi;
     keys(u, lo, hi);
-    return hi > lo ? ((hi + BK - 1) / BK - lo / BK) * blocks(u) * p.Hkv : 0;
+    return hi > lo ? (hi + BK - 1) / BK - lo / BK : 0;
+  }
+  KORE_DEV int tiles(int u) const { return tokens(u) > 0 ? item_tiles(u) * blocks(u) * p.Hkv : 0; }
+  KORE_DEV bool shared(int b) const {                      // sequence b has a part that a group's unit computes
+    const int g = grp[b];
+    return g >= 0 && cum[g + 1] > cum[g];
   }
 };
 
 struct Item {
-  int u, h, rb, n, j0, j1;       // unit, kv head, row block, tiles of the item, this block's tiles of it
+  int u, h, rb, n, j0, j1;       // unit, kv head, row block, tiles of the item, this run's tiles of it
 };
-// The item at tile x of [x, hi); advances x past this block's part of it. False at the end.
-KORE_DEV bool next_item(const Units& w, int& x, int hi, int& u, Item& it) {
-  if (x >= hi) return false;
-  while (w.cum[u + 1] <= x) ++u;
-  const int nb = w.blocks(u);
-  it.u = u;
-  it.n = (w.cum[u + 1] - w.cum[u]) / (nb * w.p.Hkv);
-  const int r = x - w.cum[u], i = r / it.n;
-  it.h = i / nb;
-  it.rb = i % nb;
-  it.j0 = r % it.n;
-  it.j1 = min(it.n, it.j0 + hi - x);
-  x += it.j1 - it.j0;
+struct Walk {                    // what is left of a run: tiles [x, end), x in unit u or behind it
+  int x, end, u;
+};
+// The run's next item; false at its end.
+KORE_DEV bool next_item(const Units& w, Walk& r, Item& it) {
+  if (r.x >= r.end) return false;
+#pragma unroll 1
+  while (w.cum[r.u + 1] <= r.x) ++r.u;
+  const int nb = w.blocks(r.u), d = r.x - w.cum[r.u];
+  it.u = r.u;
+  it.n = w.item_tiles(r.u);
+  const int i = d / it.n;
+  it.h = nb == 1 ? i : i / nb;
+  it.rb = i - it.h * nb;
+  it.j0 = d - i * it.n;
+  it.j1 = min(it.n, it.j0 + r.end - r.x);
+  r.x += it.j1 - it.j0;
   return true;
 }
-KORE_DEV int run_start(long c, long W, long C) { return (int)(c * W / C); }
-KORE_DEV int block_of(long x, long W, long C) { return (int)(((x + 1) * C - 1) / W); }   // whose run holds tile x
-KORE_DEV int used_blocks(int W, int grid) { return max(1, min(grid, (W + kMinTiles - 1) / kMinTiles)); }
+// Quotients of numbers below 2^40 and 2^30: exact in fp64, whose quotient cannot round up
+// to an integer that it is at least 2^-30 short of.
+KORE_DEV int quotient(long a, int b) { return (int)((double)a / (double)b); }
+KORE_DEV int run_start(int c, int W, int C) { return quotient((long)c * W, C); }
+KORE_DEV int run_of(int x, int W, int C) { return quotient((long)(x + 1) * C - 1, W); }   // which run holds tile x
+KORE_DEV int num_runs(int W, int grid) { return min(grid, (W + kMinTiles - 1) / kMinTiles); }
+KORE_DEV Walk make_walk(const int* cum, int nu, int base, int W, int C, int c) {
+  Walk r = {0, 0, 0};
+  if (c < C) {
+    r.x = base + run_start(c, W, C);
+    r.end = base + run_start(c + 1, W, C);
+    int lo = 0, hi = nu;         // the unit that holds r.x
+#pragma unroll 1
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cum[mid + 1] <= r.x) lo = mid + 1; else hi = mid;
+    }
+    r.u = lo;
+  }
+  return r;
+}
 
+// Narrow form: Q buffers (by the item's number) and, behind them, two P buffers (by the tile's parity).
+constexpr int q_bufs(int N) { return N <= 32 ? 2 : 1; }
+constexpr int p_off(int N) { return AttnSmem::Q_OFF + q_bufs(N) * N * 256; }
+static_assert(p_off(64) + 2 * 64 * 128 <= AttnSmem::K_OFF && p_off(32) + 2 * 32 * 128 <= AttnSmem::K_OFF, "narrow Q and P");
+
+struct Bars {
+  uint64_t *k_full, *k_empty, *v_full, *v_empty;     // [kStages]
+  uint64_t *s_full, *p_full;                         // [2]
+  uint64_t *o_done, *o_final;                        // one phase per tile, per item
+  uint64_t *q_full, *q_empty, *o_free;               // wide: one buffer each
+  uint64_t *qn_full, *qn_empty, *on_free;            // narrow: by the Q or O buffer
+  volatile int* aborted;
+};
+
+// ---- producer warp: Q of each item, K and V of each tile
+template <int N>
+KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, int& cnt,
+                      const CUtensorMap* tmQp, const CUtensorMap* tmQo, const CUtensorMap* tmK, const CUtensorMap* tmV) {
+  using S = AttnSmem;
+  constexpr int QB = q_bufs(N);
+  const int lane = threadIdx.x & 31, nbox = BK / p.box;
+  Item it;
+#pragma unroll 1
+  for (int k = 0; next_item(w, r, it); ++k) {
+    const bool pre = it.u < p.ngroups;
+    const int tb = w.block_tokens(it.u), t0 = w.row0(it.u) + it.rb * tb;
+    int klo, khi;
+    w.keys(it.u, klo, khi);
+    const int* bt = p.table + (pre ? (long)w.gs[it.u] : (long)(it.u - p.ngroups)) * p.ld_table;
+    const int tile0 = klo / BK;
+    auto slot_of = [&](int key) {               // the cache slot where the box at `key` begins
+      const int page = (unsigned)key / (unsigned)p.page_size;
+      return key + p.box > klo && key < khi ? (int)((unsigned)bt[page] * (unsigned)p.page_size + (unsigned)(key - page * p.page_size)) : 0;
+    };
+    int slot = slot_of((tile0 + it.j0) * BK + lane * p.box), window = 0;     // lane i: of the item's box window + i
+    bool ok = true;
+    if (lane == 0) {
+      const int nq = wide ? 1 : QB, qi = wide ? 0 : k % QB, ph = wide ? k : k / QB;
+      uint64_t* full = (wide ? bar.q_full : bar.qn_full) + qi;
+      ok = !*bar.aborted && (k < nq || wait_on((wide ? bar.q_empty : bar.qn_empty) + qi, (ph - 1) & 1));
+      if (ok) {
+        const CUtensorMap* tm = pre ? tmQp : tmQo;
+        uint8_t* q = smem + S::Q_OFF + qi * N * 256;
+        mbar_arrive_expect_tx(full, 2 * 128 * p.G * tb);
+        tma_load_3d(q, tm, full, 0, it.h * p.G, t0);
+        tma_load_3d(q + (wide ? 16384 : N * 128), tm, full, 64, it.h * p.G, t0);
+      }
+    }
+    int first = 0;                              // the tile's first box, from the item's first on
+#pragma unroll 1
+    for (int j = it.j0; j < it.j1; ++j, ++cnt, first += nbox) {
+      const int st = cnt % kStages, key0 = (tile0 + j) * BK;
+      const uint32_t ph = (cnt / kStages) & 1;
+      if (first == window + 32) {               // 32 is a multiple of nbox: a tile's boxes lie in one window
+        window = first;
+        slot = slot_of(key0 + lane * p.box);
+      }
+      // boxes that hold keys of the unit; the others are not loaded
+      const unsigned held = __ballot_sync(0xffffffff, key0 + lane * p.box < khi && key0 + (lane + 1) * p.box > klo && lane < nbox);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        const CUtensorMap* tm = kv ? tmV : tmK;
+        uint64_t* full = (kv ? bar.v_full : bar.k_full) + st;
+        uint8_t* dst = smem + (kv ? S::V_OFF : S::K_OFF) + st * kTileBytes;
+        if (lane == 0 && ok) {
+          ok = wait_on((kv ? bar.v_empty : bar.k_empty) + st, ph ^ 1);
+          if (ok) mbar_arrive_expect_tx(full, __popc(held) * p.box * 256);
+        }
+        if (nbox == 1) {                        // one box of 64 keys x two 64-column halves
+          const int z = __shfl_sync(0xffffffff, slot, first - window);
+          if (lane == 0 && ok) tma_load_4d(dst, tm, full, 0, z, 0, it.h);
+        } else {
+#pragma unroll 1
+          for (int b = 0; b < nbox; ++b) {
+            const int z = __shfl_sync(0xffffffff, slot, first - window + b);
+            if (lane == 0 && ok && (held >> b & 1)) {
+              tma_load_4d(dst + b * p.box * 128, tm, full, 0, z, 0, it.h);
+              tma_load_4d(dst + 8192 + b * p.box * 128, tm, full, 0, z, 1, it.h);
+            }
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffff, ok && !*bar.aborted, 0);
+      if (!ok) return false;
+    }
+  }
+  return true;
+}
+
+// ---- one thread: the products. S of the next tile is issued before O of this one, so
+// that the softmax warps find it ready. One in-order pipe: S_{i+1} overwrites S_{i-1}'s
+// buffer (wide: P_{i-1}, which PV_{i-1}, issued before, has read by then). The thread
+// issues twelve products a tile; their descriptors are sums of what it keeps, because
+// building them anew took longer (0.8 us a tile) than the products themselves.
+constexpr uint64_t step16(int kk, int half) { return (uint64_t)(((kk >> 2) * half + (kk & 3) * 32) >> 4); }   // K-step kk of K-major atoms `half` bytes apart
+template <bool WIDE, int N>
+KORE_DEV bool multiply(const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt) {
+  using S = AttnSmem;
+  constexpr uint32_t idesc_s = WIDE ? make_idesc_bf16(128, BK, false, false) : make_idesc_bf16(128, N, false, false);
+  constexpr uint32_t idesc_o = WIDE ? make_idesc_bf16(128, D, false, true) : make_idesc_bf16(128, N, true, false);
+  constexpr int QB = WIDE ? 1 : q_bufs(N);
+  const uint64_t q0 = make_sw128_desc(smem_u32(smem + S::Q_OFF), 16, 1024), k0 = make_sw128_desc(smem_u32(smem + S::K_OFF), 16, 1024),
+                 v0 = make_sw128_desc(smem_u32(smem + S::V_OFF), 8192, 1024), p0 = make_sw128_desc(smem_u32(smem + p_off(N)), 16, 1024);
+  Item it;
+  bool ok = true;
+#pragma unroll 1
+  for (int k = 0; ok && next_item(w, r, it); ++k) {
+    const int qi = k % QB, qp = k / QB;
+    const uint64_t qd = q0 + (uint64_t)(qi * N * 16);
+    const uint32_t to = tmem + kTmemO + (WIDE ? 0 : (k & 1) * 64);
+    const int n = it.j1 - it.j0;
+    uint64_t *const q_full = WIDE ? bar.q_full : bar.qn_full + qi, *const q_empty = WIDE ? bar.q_empty : bar.qn_empty + qi;
+    uint64_t* const o_free = WIDE ? bar.o_free : bar.on_free + (k & 1);
+    ok = wait_on(q_full, qp & 1);
+#pragma unroll 1
+    for (int j = -1; j < n && ok; ++j) {        // S of tile j + 1, then O of tile j
+      const int i = cnt + j;
+      if (j + 1 < n) {
+        const int st = (i + 1) % kStages;
+        if (!(ok = wait_on(&bar.k_full[st], ((i + 1) / kStages) & 1))) break;
+        tc_fence_after();
+        const uint64_t kd = k0 + (uint64_t)(st * (kTileBytes >> 4));
+        const uint32_t ts = tmem + ((i + 1) & 1) * 64;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          // narrow: K is the left operand; its rows 64..127 are whatever lies behind the 64 of the tile, and nobody reads their result
+          if (WIDE) umma_f16_ss(ts, qd + step16(kk, 16384), kd + step16(kk, 8192), idesc_s, kk > 0);
+          else umma_f16_ss(ts, kd + step16(kk, 8192), qd + step16(kk, N * 128), idesc_s, kk > 0);
+        }
+        umma_commit(&bar.k_empty[st]);
+        umma_commit(&bar.s_full[(i + 1) & 1]);
+        if (j + 2 == n) umma_commit(q_empty);   // the item's last S is issued
+      }
+      if (j < 0) continue;
+      const int st = i % kStages, ob = WIDE ? 1 : 2;
+      if (j == 0 && k >= ob) ok = wait_on(o_free, (WIDE ? k - 1 : (k >> 1) - 1) & 1);   // the last item in this O has been read
+      ok = ok && wait_on(&bar.p_full[i & 1], (i >> 1) & 1) && wait_on(&bar.v_full[st], (i / kStages) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t vd = v0 + (uint64_t)(st * (kTileBytes >> 4)), pd = p0 + (uint64_t)((i & 1) * N * 8);
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk) {
+        if (WIDE) umma_f16_ts(to, tmem + (i & 1) * 64 + kk * 8, vd + kk * 128, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+        else umma_f16_ss(to, vd + kk * 128, pd + step16(kk, 0), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+      }
+      umma_commit(&bar.v_empty[st]);
+      umma_commit(bar.o_done);
+    }
+    if (ok) umma_commit(bar.o_final);
+    cnt += n;
+  }
+  return ok;
+}
+
+// What lies outside a unit's keys in the cache may be anything, NaN included, and
+// 0 x NaN is not 0: those rows of a V tile are cleared before the product reads them.
+__device__ __noinline__ bool clear_v(uint8_t* smem, const Bars& bar, int cnt, int kv0, int klo, int khi) {
+  const int lane = threadIdx.x & 31, vs = cnt % kStages, r = (threadIdx.x / 32 & 3) * 16 + (lane >> 1);
+  if (!warp_wait(&bar.v_full[vs], (cnt / kStages) & 1)) return false;
+  if (kv0 + r < klo || kv0 + r >= khi) {
+    uint4* dst = reinterpret_cast<uint4*>(smem + AttnSmem::V_OFF + vs * kTileBytes + (lane & 1) * 8192 + r * 128);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  return true;
+}
+
+// ---- four warps, wide form: a thread owns a row
+KORE_DEV bool softmax_wide(const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt, int& items, int run) {
+  const int lane = threadIdx.x & 31, q4 = threadIdx.x / 32 & 3, row = q4 * 32 + lane;
+  const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
+  Item it;
+  int tile = cnt;
+#pragma unroll 1
+  for (int k = 0; next_item(w, r, it); ++k) {
+    const bool pre = it.u < p.ngroups;
+    const int tb = w.block_tokens(it.u), rt = it.rb * tb + row / p.G;      // token within the unit
+    const bool live = row < tb * p.G && rt < w.tokens(it.u);
+    const bool warp_live = __any_sync(0xffffffff, live);
+    const int t = w.row0(it.u) + rt, h = it.h * p.G + row % p.G;
+    int klo, khi, limit = 0;                    // the row sees keys [klo, limit)
+    w.keys(it.u, klo, khi);
+    bool joined = pre;                          // another part of the row's keys is another unit's
+    if (live) {
+      const int b = pre ? w.seq_of(t, w.gs[it.u], w.gs[it.u + 1] - 1) : it.u - p.ngroups;
+      if (!pre) joined = w.shared(b);
+      limit = min(w.len[b] - (w.qs[b + 1] - t) + 1, khi);
+    }
+    const int tile0 = klo / BK;
+    float m = -INFINITY, l = 0.f, sv[BK];
+#pragma unroll 1
+    for (int j = it.j0; j < it.j1; ++j, ++tile) {
+      const int st = tile & 1, kv0 = (tile0 + j) * BK;
+      if (!warp_wait(&bar.s_full[st], (tile >> 1) & 1)) return false;
+      if ((kv0 < klo || kv0 + BK > khi) && !clear_v(smem, bar, tile, kv0, klo, khi)) return false;
+      if (warp_live) {
+        tc_fence_after();
+        {
+          uint32_t x[2][32];
+          tmem_ld32(tmem + lane_base + st * 64, x[0]);
+          tmem_ld32(tmem + lane_base + st * 64 + 32, x[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < BK; ++i) sv[i] = __uint_as_float(x[i / 32][i % 32]);
+        }
+        if (kv0 + BK > limit || kv0 < klo) {
+#pragma unroll
+          for (int i = 0; i < BK; ++i)
+            if (kv0 + i >= limit || kv0 + i < klo) sv[i] = -INFINITY;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < BK; i += 8) {
+          mx4[0] = fmax3f(mx4[0], sv[i], sv[i + 1]);
+          mx4[1] = fmax3f(mx4[1], sv[i + 2], sv[i + 3]);
+          mx4[2] = fmax3f(mx4[2], sv[i + 4], sv[i + 5]);
+          mx4[3] = fmax3f(mx4[3], sv[i + 6], sv[i + 7]);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        const float m_new = fmaxf(m, mx);
+        // O follows the running maximum only when that grew by more than 2^8 (fp32 has the room)
+        const bool need = m == -INFINITY || m_new > m + 8.f;
+        if (j > it.j0) {
+          const float alpha = need && m != -INFINITY ? exp2f(m - m_new) : 1.f;
+          if (__any_sync(0xffffffff, need && m != -INFINITY)) {
+            // S of this tile is committed, so PV of the tile two before is done and PV of this one not issued: the parity is clear
+            if (!warp_wait(bar.o_done, (tile - 1) & 1)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+              uint32_t x[32];
+              const uint32_t a = tmem + lane_base + kTmemO + i4 * 32;
+              tmem_ld32(a, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+              tmem_st32(a, x);
+            }
+            tmem_wait_st();
+          }
+          l *= alpha;
+        }
+        if (need) m = m_new;
+        const float mref = m == -INFINITY ? 0.f : m;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-mref, -mref);
+        uint64_t rs2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < BK; i += 2) {
+          float a, b;
+          f2_unpack(f2_fma(f2_pack(sv[i], sv[i + 1]), sc2, nm2), a, b);
+          sv[i] = exp2f(a);
+          sv[i + 1] = exp2f(b);
+          rs2[(i >> 1) & 1] = f2_add(rs2[(i >> 1) & 1], f2_pack(sv[i], sv[i + 1]));
+        }
+        float a0, b0, a1, b1;
+        f2_unpack(rs2[0], a0, b0);
+        f2_unpack(rs2[1], a1, b1);
+        l += (a0 + b0) + (a1 + b1);
+        // P in bf16 (the operand type of V): a probability is off by up to 2^-8 of itself, the sum l is not rounded
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(sv[2 * i], sv[2 * i + 1]);
+        tmem_st32(tmem + lane_base + st * 64, pk);
+        tmem_wait_st();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full[st]);
+    }
+    if (!warp_wait(bar.o_final, items++ & 1)) return false;
+    if (warp_live) {
+      tc_fence_after();
+      const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
+      const size_t at = (size_t)t * p.Hq + h;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* part = whole ? (pre ? p.whole_prefix : p.whole_own) + at * kPart
+                          : p.split_wide + ((size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 128 + row) * kPart;
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        uint32_t x[32];
+        tmem_ld32(tmem + lane_base + kTmemO + i4 * 32, x);
+        tmem_wait_ld();
+        if (live && direct) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(x[8 * i + 0]) * inv, __uint_as_float(x[8 * i + 1]) * inv);
+            v.y = pack_bf16(__uint_as_float(x[8 * i + 2]) * inv, __uint_as_float(x[8 * i + 3]) * inv);
+            v.z = pack_bf16(__uint_as_float(x[8 * i + 4]) * inv, __uint_as_float(x[8 * i + 5]) * inv);
+            v.w = pack_bf16(__uint_as_float(x[8 * i + 6]) * inv, __uint_as_float(x[8 * i + 7]) * inv);
+            *reinterpret_cast<uint4*>(p.out + at * D + i4 * 32 + 8 * i) = v;
+          }
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(part + i4 * 32 + 4 * i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        }
+      }
+      if (live && direct && p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      if (live && !direct) {
+        part[D] = m;
+        part[D + 1] = l;
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar.o_free);
+  }
+  cnt = tile;
+  return true;
+}
+
+// ---- four warps, narrow form, NL >= the block's rows: threads of the first two own a
+// key of S^T, all own a column of O^T. The rows' reference exponents are common to
+// the keys and kept in shared memory; they move only when some score passes its row's
+// by more than 2^8.
+template <int NL>
+KORE_DEV void tmem_ld(uint32_t taddr, float (&v)[NL]) {
+  uint32_t x[NL];
+  if constexpr (NL == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]) : "r"(taddr));
+  } else if constexpr (NL == 16) {
+    tmem_ld16(taddr, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; i += 32) tmem_ld32(taddr + i, *reinterpret_cast<uint32_t(*)[32]>(&x[i]));
+  }
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < NL; ++i) v[i] = __uint_as_float(x[i]);
+}
+template <int NL>
+KORE_DEV void tmem_st(uint32_t taddr, const float (&v)[NL]) {
+  uint32_t x[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) x[i] = __float_as_uint(v[i]);
+  if constexpr (NL == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+                 "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; i += 16) tmem_st16(taddr + i, *reinterpret_cast<const uint32_t(*)[16]>(&x[i]));
+  }
+  tmem_wait_st();
+}
+// Sums of v[i] over the warp's lanes, by halving: NL - 1 exchanges. Lane's sums are
+// those of the columns (its upper bits) * max(NL / 32, 1) onwards; they end in v[0..].
+template <int NL>
+KORE_DEV void warp_sums(float (&v)[NL]) {
+  const int lane = threadIdx.x & 31;
+  int n = NL;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+#pragma unroll
+      for (int i = 0; i < NL / 2; ++i)
+        if (i < n) {
+          const float keep = lane & o ? v[i + n] : v[i], give = lane & o ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffff, give, o);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffff, v[0], o);
+    }
+  }
+}
+
+struct NarrowSmem {               // per row of the block
+  float ref[64], factor[64], mine[2][64];       // reference exponent; factor when it moves, later 1 / sum; the two key warps' values
+  int limit[64], at[64];                        // the row sees keys [klo, limit); row of the result
+};
+
+template <int N, int NL>
+KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt, int& items, int run) {
+  const int lane = threadIdx.x & 31, q4 = threadIdx.x / 32 & 3, tid = q4 * 32 + lane;
+  const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
+  NarrowSmem& x = *reinterpret_cast<NarrowSmem*>(smem + AttnSmem::X_OFF);
+  Item it;
+  int tile = cnt;
+#pragma unroll 1
+  for (int k = 0; next_item(w, r, it); ++k) {
+    const int b = it.u - p.ngroups, tb = p.tokens_own, rt0 = it.rb * tb, t0 = w.row0(it.u) + rt0;
+    const int rows = min(tb, w.tokens(it.u) - rt0) * p.G;                  // live rows of the block
+    int klo, khi;
+    w.keys(it.u, klo, khi);
+    const bool joined = w.shared(b);
+    if (tid < NL) {
+      const int i = tid / p.G;
+      x.limit[tid] = tid < rows ? min(w.len[b] - (w.qs[b + 1] - t0 - i) + 1, khi) : -1;    // behind the block's rows Q is not defined
+      x.at[tid] = (t0 + i) * p.Hq + it.h * p.G + tid % p.G;
+    }
+    softmax_sync();
+    const int tile0 = klo / BK;
+    const uint32_t to = tmem + lane_base + kTmemO + (k & 1) * 64;
+    float l[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) l[i] = 0.f;
+#pragma unroll 1
+    for (int j = it.j0; j < it.j1; ++j, ++tile) {
+      const int st = tile & 1, kv0 = (tile0 + j) * BK;
+      if (!softmax_wait(&bar.s_full[st], (tile >> 1) & 1)) return false;
+      if ((kv0 < klo || kv0 + BK > khi) && softmax_any(!clear_v(smem, bar, tile, kv0, klo, khi))) return false;
+      float s[NL];
+      bool over = false;
+      if (q4 < 2) {
+        tc_fence_after();
+        tmem_ld<NL>(tmem + lane_base + st * 64, s);
+        const int key = kv0 + tid >= klo ? kv0 + tid : 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          s[i] = key < x.limit[i] ? s[i] * p.scale_log2 : -INFINITY;
+          over = over || s[i] > x.ref[i] + 8.f;
+        }
+      }
+      if (softmax_any(over || j == it.j0)) {
+        if (q4 < 2) {
+          float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const float v = warp_max(s[i]);
+            if (lane == (i & 31)) (i < 32 ? top : top2) = v;
+          }
+          if (lane < NL) x.mine[q4][lane] = top;
+          if (NL > 32) x.mine[q4][lane + 32] = top2;
+        }
+        softmax_sync();
+        if (tid < NL) {
+          const float old = j == it.j0 ? -INFINITY : x.ref[tid], v = fmaxf(x.mine[0][tid], x.mine[1][tid]);
+          const bool need = v > old + 8.f || old == -INFINITY;
+          const float now = need ? fmaxf(v, old) : old;
+          x.factor[tid] = need && old != -INFINITY ? exp2f(old - now) : 1.f;
+          x.ref[tid] = now;
+        }
+        softmax_sync();
+        if (j > it.j0) {
+          if (!softmax_wait(bar.o_done, (tile - 1) & 1)) return false;
+          tc_fence_after();
+          float o[NL];
+          tmem_ld<NL>(to, o);
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            l[i] *= x.factor[i];
+            o[i] *= x.factor[i];
+          }
+          tmem_st<NL>(to, o);
+        }
+      }
+      if (q4 < 2) {
+        // P^T as the right operand: row i of the block is 64 keys, 128 bytes, swizzled in 16-byte pieces by the row
+        uint8_t* pt = smem + p_off(N) + st * N * 128 + (tid & 7) * 2;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const float m = x.ref[i], e = exp2f(s[i] - (m == -INFINITY ? 0.f : m));
+          l[i] += e;
+          *reinterpret_cast<__nv_bfloat16*>(pt + i * 128 + (((tid >> 3) ^ (i & 7)) << 4)) = __float2bfloat16(e);
+        }
+        fence_proxy_async_smem();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full[st]);
+    }
+    if (q4 < 2) {
+      warp_sums<NL>(l);
+      constexpr int per = NL > 32 ? NL / 32 : 1, same = NL < 32 ? 32 / NL : 1;   // sums of a lane, lanes with the same one
+      if (lane % same == 0)
+#pragma unroll
+        for (int i = 0; i < per; ++i) x.mine[q4][lane / same * per + i] = l[i];
+    }
+    if (!softmax_wait(bar.o_final, items++ & 1)) return false;             // also: `mine` is there
+    tc_fence_after();
+    float o[NL];
+    tmem_ld<NL>(to, o);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar.on_free + (k & 1));
+    const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
+    float* split = p.split_narrow + (size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 64 * kPart;
+    if (tid < rows) {
+      const float sum = x.mine[0][tid] + x.mine[1][tid], m = x.ref[tid];
+      if (direct) {
+        if (p.lse) p.lse[x.at[tid]] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+        x.factor[tid] = sum == 0.f ? 0.f : 1.f / sum;
+      } else {
+        float* part = whole ? p.whole_own + (size_t)x.at[tid] * kPart : split + tid * kPart;
+        part[D] = m;
+        part[D + 1] = sum;
+      }
+    }
+    softmax_sync();
+    if (direct) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (i < rows) p.out[(size_t)x.at[i] * D + tid] = __float2bfloat16(x.factor[i] == 0.f ? 0.f : o[i] * x.factor[i]);
+    } else {
+      float* part = (whole ? p.whole_own : split) + tid;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (i < rows) part[(size_t)(whole ? x.at[i] : i) * kPart] = o[i];
+    }
+    softmax_sync();                             // the rows' values have been read
+  }
+  cnt = tile;
+  return true;
+}
+
+template <int NL>
 __global__ void __launch_bounds__(kAttnThreads, 2)
     attn_kernel(const __grid_constant__ CUtensorMap tmQp, const __grid_constant__ CUtensorMap tmQo,
-                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, AttnParams p) {
+                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnParams p) {
   using S = AttnSmem;
+  constexpr int N = NL < 16 ? 16 : NL;           // the narrow products' width: rows in multiples of 16
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
-  uint64_t *q_full = bars, *q_empty = bars + 1, *o_done = bars + 2, *o_final = bars + 3, *o_free = bars + 4;
-  uint64_t *k_full = bars + 5, *k_empty = k_full + kStages, *v_full = k_empty + kStages, *v_empty = v_full + kStages;
-  uint64_t *s_full = v_empty + kStages, *p_full = s_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   int* warp_sum = reinterpret_cast<int*>(tmem_slot + 2);             // [6]
-  int* qs = reinterpret_cast<int*>(smem + S::QS_OFF);
-  int* cum = reinterpret_cast<int*>(smem + S::CUM_OFF);
-  uint16_t* gs = reinterpret_cast<uint16_t*>(smem + S::GS_OFF);
+  const Bars bar = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 12, bars + 13, bars + 14,
+                    bars + 15, bars + 16, bars + 17, bars + 19, bars + 21, reinterpret_cast<volatile int*>(tmem_slot + 1)};
+  static_assert(kStages == 2, "barrier layout");
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const Units w{p, qs, cum, gs};
+  const Units w(p, smem + S::UNITS_OFF);
+  int* const cum = w.cum;
 
   pdl_trigger();
   // ---- the units' tiles, summed
-  for (int i = threadIdx.x; i <= p.B; i += kAttnThreads) qs[i] = min(max(p.q_start[i], 0), p.T);
-  for (int i = threadIdx.x; i <= p.ngroups; i += kAttnThreads)
-    gs[i] = (uint16_t)(p.ngroups ? min(max(p.group_start[i], 0), p.B) : 0);
+#pragma unroll 1
+  for (int i = threadIdx.x; i <= p.B; i += kAttnThreads) {
+    w.qs[i] = min(max(p.q_start[i], 0), p.T);
+    if (i < p.B) w.len[i] = min(max(p.lens[i], 0), p.M * p.page_size);
+    if (i <= p.ngroups) w.gs[i] = p.ngroups ? min(max(p.group_start[i], 0), p.B) : 0;
+    if (i < p.ngroups) w.prefix[i] = min(max(p.prefix[i], 0), p.M * p.page_size);
+  }
   if (threadIdx.x == 0) {
-    for (uint64_t* b : {q_full, q_empty, o_done, o_final}) mbar_init(b, 1);
-    mbar_init(o_free, 4);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-    }
-    *abort_flag = 0;
+#pragma unroll 1
+    for (int i = 0; i < 23; ++i) mbar_init(bars + i, i == 10 || i == 11 || i == 16 || i == 21 || i == 22 ? 4 : 1);   // p_full, o_free: a warp's lane each
+    *bar.aborted = 0;
     fence_barrier_init();
   }
+  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   __syncthreads();
   const int nu = p.ngroups + p.B, per = (nu + kAttnThreads - 1) / kAttnThreads;
+#pragma unroll 1
+  for (int b = threadIdx.x; b < p.B; b += kAttnThreads) {
+    int lo = 0, hi = p.ngroups;      // the first group that starts behind b
+#pragma unroll 1
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (w.gs[mid] <= b) lo = mid + 1; else hi = mid;
+    }
+    w.grp[b] = (short)(lo > 0 && b < w.gs[lo] ? lo - 1 : -1);
+  }
+  __syncthreads();
   {
     const int u0 = min((int)threadIdx.x * per, nu), u1 = min(u0 + per, nu);
     int mine = 0;
+#pragma unroll 1
     for (int u = u0; u < u1; ++u) mine += w.tiles(u);
     int upto = mine;
 #pragma unroll
@@ -296,390 +887,148 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
     int at = upto - mine;
+#pragma unroll 1
     for (int i = 0; i < warp; ++i) at += warp_sum[i];
+#pragma unroll 1
     for (int u = u0; u < u1; ++u) {
       cum[u] = at;
       at += w.tiles(u);
     }
     if (u1 == nu) cum[nu] = at;      // the same from every thread that ends there
   }
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= nu; i += kAttnThreads) p.meta[i] = cum[i];
-  const int W = cum[nu], C = used_blocks(W, gridDim.x), c = blockIdx.x;
-  if (W == 0 || c >= C) return;
-  const int x0 = run_start(c, W, C), x1 = run_start(c + 1, W, C);
-  int u_first = 0;
-  {
-    int lo = 0, hi = nu;             // the last unit that starts at or before x0
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid + 1] <= x0) lo = mid + 1; else hi = mid;
-    }
-    u_first = lo;
-  }
-  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const int Ww = cum[p.nwide], Wn = cum[nu] - Ww, Cw = num_runs(Ww, gridDim.x), Cn = num_runs(Wn, gridDim.x);
+  if (warp >= 2) {
+    // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
+    const int id = blockIdx.x * 128 + threadIdx.x - 64;
+    if (id == 0) *reinterpret_cast<int4*>(p.runs) = make_int4(Ww, Cw, Wn, Cn);
+#pragma unroll 1
+    for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 128) {
+      const int t = i >> 1, b = w.seq_of(t, 0, p.B - 1), u = i & 1 ? p.ngroups + b : w.grp[b];
+      int4 e = make_int4(0, 0, 0, 0);
+      if (u >= 0 && cum[u + 1] > cum[u]) {
+        const int tb = w.block_tokens(u), d = t - w.row0(u), rb = d / tb;
+        e.y = w.item_tiles(u);
+        e.x = cum[u] - (u < p.nwide ? 0 : Ww) + rb * e.y;
+        e.z = w.blocks(u) * e.y;
+        e.w = (d - rb * tb) * p.G;
+      }
+      p.where[i] = e;
+    }
+  }
   const uint32_t tmem = *tmem_slot;
-  constexpr uint32_t T_O = 128;
-  int x = x0, u = u_first, k = 0, cnt = 0;        // tile, unit, items done, tiles done
-  Item it;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    while (next_item(w, x, x1, u, it)) {
-      const bool pre = it.u < p.ngroups;
-      const int tb = w.block_tokens(it.u), t0 = w.row0(it.u) + it.rb * tb;
-      int klo, khi;
-      w.keys(it.u, klo, khi);
-      const int* bt = p.table + (pre ? (long)gs[it.u] : (long)(it.u - p.ngroups)) * p.ld_table;
-      bool ok = true;
-      if (lane == 0) {
-        ok = !*abort_flag && (k == 0 || mbar_wait(q_empty, (k - 1) & 1));
-        if (ok) {
-          const CUtensorMap* tm = pre ? &tmQp : &tmQo;
-          mbar_arrive_expect_tx(q_full, 2 * 128 * p.G * tb);
-          tma_load_3d(smem + S::Q_OFF, tm, q_full, 0, it.h * p.G, t0);
-          tma_load_3d(smem + S::Q_OFF + 16384, tm, q_full, 64, it.h * p.G, t0);
-        }
-      }
-      const int tile0 = klo / BK, nbox = BK / p.box;
-      int page = 0, window = -32;                 // lane i holds the page of the item's box window + i
-      for (int j = it.j0; j < it.j1; ++j, ++cnt) {
-        const int st = cnt % kStages;
-        const uint32_t ph = (cnt / kStages) & 1;
-        const int key0 = (tile0 + j) * BK;
-        const int b0 = min(max((klo - key0) / p.box, 0), nbox), b1 = min((khi - key0 + p.box - 1) / p.box, nbox);  // boxes with keys of the unit
-        const int first = (j - it.j0) * nbox;
-        if (first >= window + 32) {               // 32 is a multiple of nbox: a tile's boxes lie in one window
-          window = first;
-          const int key = key0 + lane * p.box;
-          page = key >= klo - (klo % p.box) && key < khi ? bt[key / p.page_size] : 0;
-        }
-        if (lane == 0 && ok) ok = mbar_wait(&k_empty[st], ph ^ 1);
-        uint8_t* kt = smem + S::K_OFF + st * kTileBytes;
-        uint8_t* vt = smem + S::V_OFF + st * kTileBytes;
-        const uint32_t bytes = (uint32_t)(b1 - b0) * p.box * 256;
-        if (lane == 0 && ok) mbar_arrive_expect_tx(&k_full[st], bytes);
-        for (int b = b0; b < b1; ++b) {
-          const int key = key0 + b * p.box;
-          const int z = (int)((unsigned)__shfl_sync(0xffffffff, page, first - window + b) * (unsigned)p.page_size + key % p.page_size);
-          if (lane == 0 && ok) {
-            tma_load_3d(kt + b * p.box * 128, &tmK, &k_full[st], 0, it.h, z);
-            tma_load_3d(kt + 8192 + b * p.box * 128, &tmK, &k_full[st], 64, it.h, z);
-          }
-        }
-        if (lane == 0 && ok) ok = mbar_wait(&v_empty[st], ph ^ 1);
-        if (lane == 0 && ok) mbar_arrive_expect_tx(&v_full[st], bytes);
-        for (int b = b0; b < b1; ++b) {
-          const int key = key0 + b * p.box;
-          const int z = (int)((unsigned)__shfl_sync(0xffffffff, page, first - window + b) * (unsigned)p.page_size + key % p.page_size);
-          if (lane == 0 && ok) {
-            tma_load_3d(vt + b * p.box * 128, &tmV, &v_full[st], 0, it.h, z);
-            tma_load_3d(vt + 8192 + b * p.box * 128, &tmV, &v_full[st], 64, it.h, z);
-          }
-        }
-        ok = __shfl_sync(0xffffffff, ok && !*abort_flag, 0);
-        if (!ok) break;
-      }
-      if (!ok) { *abort_flag = 1; break; }
-      ++k;
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA
-    constexpr uint32_t idesc_qk = make_idesc_bf16(128, BK, false, false);
-    constexpr uint32_t idesc_pv = make_idesc_bf16(128, D, false, true);
-    if (elect_one()) {
-      const uint32_t qa = smem_u32(smem + S::Q_OFF);
-      bool ok = true;
-      auto issue_s = [&](int i) -> bool {         // i: tile of this block
-        const int st = i % kStages;
-        if (!mbar_wait(&k_full[st], (i / kStages) & 1)) return false;
-        tc_fence_after();
-        const uint32_t ka = smem_u32(smem + S::K_OFF + st * kTileBytes);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16_ss(tmem + (i & 1) * BK, q_desc(qa, kk), k_desc(ka, kk), idesc_qk, kk > 0);
-        umma_commit(&k_empty[st]);
-        umma_commit(&s_full[i & 1]);
-        return true;
-      };
-      while (ok && next_item(w, x, x1, u, it)) {
-        const int n = it.j1 - it.j0;
-        ok = mbar_wait(q_full, k & 1);
-        if (ok) ok = issue_s(cnt);
-        for (int j = 0; j < n && ok; ++j) {
-          const int i = cnt + j;
-          // the buffer of S_{i+1} held P_{i-1}, which PV_{i-1}, issued before, has read by then (one in-order pipe)
-          if (j + 1 < n) ok = issue_s(i + 1);
-          if (ok && j + 1 == n) umma_commit(q_empty);              // the item's last S is issued
-          const int st = i % kStages;
-          if (ok && j == 0 && k > 0) ok = mbar_wait(o_free, (k - 1) & 1);   // the last item's O has been read
-          if (ok) ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1);
-          if (ok) ok = mbar_wait(&v_full[st], (i / kStages) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = smem_u32(smem + S::V_OFF + st * kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            umma_f16_ts(tmem + T_O, tmem + (i & 1) * BK + kk * 8, v_desc(va, kk), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&v_empty[st]);
-          umma_commit(o_done);
-        }
-        if (ok) umma_commit(o_final);
-        cnt += n;
-        ++k;
-      }
-      if (!ok) *abort_flag = 1;
-    }
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------ softmax
-    const int q4 = warp & 3, row = q4 * 32 + lane;
-    const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
-    bool ok = true;
-    while (ok && next_item(w, x, x1, u, it)) {
-      const bool pre = it.u < p.ngroups;
-      const int tb = w.block_tokens(it.u), rt = it.rb * tb + row / p.G;      // token within the unit
-      const bool live = row < tb * p.G && rt < w.tokens(it.u);
-      const bool warp_live = __any_sync(0xffffffff, live);
-      const int t = w.row0(it.u) + rt, h = it.h * p.G + row % p.G;
-      int klo, khi, limit = 0;                    // the row sees keys [klo, limit)
-      w.keys(it.u, klo, khi);
-      bool joined = pre;                          // another part of the row's keys is another unit's
-      if (live) {
-        int b = it.u - p.ngroups;
-        if (pre) {
-          int lo = gs[it.u], hi = gs[it.u + 1] - 1;
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (qs[mid + 1] <= t) lo = mid + 1; else hi = mid;
-          }
-          b = lo;
-        } else if (p.ngroups) {
-          const int g = w.group_of(b);
-          joined = g >= 0 && cum[g + 1] > cum[g];
-        }
-        limit = min(p.lens[b] - (qs[b + 1] - t) + 1, khi);
-      }
-      const int tile0 = klo / BK;
-      float m = -INFINITY, l = 0.f, sv[BK];
-      for (int j = it.j0; j < it.j1; ++j, ++cnt) {
-        const int st = cnt & 1, kv0 = (tile0 + j) * BK;
-        if (!warp_wait(&s_full[st], (cnt >> 1) & 1)) { ok = false; break; }
-        if (kv0 < klo || kv0 + BK > khi) {
-          // What lies outside the unit's keys may be anything, NaN included, and
-          // 0 x NaN is not 0: these rows of V are cleared before the product reads them.
-          const int vs = cnt % kStages;
-          if (!warp_wait(&v_full[vs], (cnt / kStages) & 1)) { ok = false; break; }
-          const int r = q4 * 16 + (lane >> 1);
-          if (kv0 + r < klo || kv0 + r >= khi) {
-            uint4* dst = reinterpret_cast<uint4*>(smem + S::V_OFF + vs * kTileBytes + (lane & 1) * 8192 + r * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        if (warp_live) {
-          tc_fence_after();
-          {
-            uint32_t r[2][32];
-            tmem_ld32(tmem + lane_base + st * BK, r[0]);
-            tmem_ld32(tmem + lane_base + st * BK + 32, r[1]);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < BK; ++i) sv[i] = __uint_as_float(r[i / 32][i % 32]);
-          }
-          if (kv0 + BK > limit || kv0 < klo) {
-#pragma unroll
-            for (int i = 0; i < BK; ++i)
-              if (kv0 + i >= limit || kv0 + i < klo) sv[i] = -INFINITY;
-          }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < BK; i += 8) {
-            mx4[0] = fmax3f(mx4[0], sv[i], sv[i + 1]);
-            mx4[1] = fmax3f(mx4[1], sv[i + 2], sv[i + 3]);
-            mx4[2] = fmax3f(mx4[2], sv[i + 4], sv[i + 5]);
-            mx4[3] = fmax3f(mx4[3], sv[i + 6], sv[i + 7]);
-          }
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-          const float m_new = fmaxf(m, mx);
-          // O follows the running maximum only when that grew by more than 2^8 (fp32 has the room)
-          const bool need = m == -INFINITY || m_new > m + 8.f;
-          if (j > it.j0) {
-            const float alpha = need && m != -INFINITY ? exp2f(m - m_new) : 1.f;
-            if (__any_sync(0xffffffff, need && m != -INFINITY)) {
-              if (!warp_wait(o_done, (cnt - 1) & 1)) { ok = false; break; }
-              tc_fence_after();
-#pragma unroll
-              for (int i4 = 0; i4 < 4; ++i4) {
-                uint32_t r[32];
-                const uint32_t a = tmem + lane_base + T_O + i4 * 32;
-                tmem_ld32(a, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                tmem_st32(a, r);
-              }
-              tmem_wait_st();
-            }
-            l *= alpha;
-          }
-          if (need) m = m_new;
-          const float mref = m == -INFINITY ? 0.f : m;
-          const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-mref, -mref);
-          uint64_t rs2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-#pragma unroll
-          for (int i = 0; i < BK; i += 2) {
-            float a, b;
-            f2_unpack(f2_fma(f2_pack(sv[i], sv[i + 1]), sc2, nm2), a, b);
-            sv[i] = exp2f(a);
-            sv[i + 1] = exp2f(b);
-            rs2[(i >> 1) & 1] = f2_add(rs2[(i >> 1) & 1], f2_pack(sv[i], sv[i + 1]));
-          }
-          float a0, b0, a1, b1;
-          f2_unpack(rs2[0], a0, b0);
-          f2_unpack(rs2[1], a1, b1);
-          l += (a0 + b0) + (a1 + b1);
-          // P in bf16 (the operand type of V): each probability is off by 2^-9 of itself, the sum l is not rounded
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(sv[2 * i], sv[2 * i + 1]);
-          tmem_st32(tmem + lane_base + st * BK, pk);
-          tmem_wait_st();
-          tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[st]);
-      }
-      if (!ok || !warp_wait(o_final, k & 1)) { ok = false; break; }
-      if (warp_live) {
-        tc_fence_after();
-        const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
-        const size_t at = (size_t)t * p.Hq + h;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        float* part = whole ? (pre ? p.whole_prefix : p.whole_own) + at * kPart
-                            : p.split + ((size_t)(2 * c + (it.j0 == 0 ? 1 : 0)) * 128 + row) * kPart;
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          uint32_t r[32];
-          tmem_ld32(tmem + lane_base + T_O + i4 * 32, r);
-          tmem_wait_ld();
-          if (live && direct) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4 v;
-              v.x = pack_bf16(__uint_as_float(r[8 * i + 0]) * inv, __uint_as_float(r[8 * i + 1]) * inv);
-              v.y = pack_bf16(__uint_as_float(r[8 * i + 2]) * inv, __uint_as_float(r[8 * i + 3]) * inv);
-              v.z = pack_bf16(__uint_as_float(r[8 * i + 4]) * inv, __uint_as_float(r[8 * i + 5]) * inv);
-              v.w = pack_bf16(__uint_as_float(r[8 * i + 6]) * inv, __uint_as_float(r[8 * i + 7]) * inv);
-              *reinterpret_cast<uint4*>(p.out + at * D + i4 * 32 + 8 * i) = v;
-            }
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(part + i4 * 32 + 4 * i) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-          }
-        }
-        if (live && direct && p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-        if (live && !direct) {
-          part[D] = m;
-          part[D + 1] = l;
-        }
-        tc_fence_before();
-      }
+  const int cw = blockIdx.x, cn = gridDim.x - 1 - blockIdx.x;       // few runs of both forms land on different blocks
+  const Walk wide = make_walk(cum, nu, 0, Ww, Cw, cw), narrow = make_walk(cum, nu, Ww, Wn, Cn, cn);
+  const bool wide_first = blockIdx.x < gridDim.x / 2;
+  const bool leader = warp == 1 && elect_one();
+  int cnt = 0, items = 0;          // tiles and items so far, in both turns
+  bool ok = true;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    const bool is_wide = (turn == 0) == wide_first;
+    if (warp == 0) {
+      if (ok) ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, &tmQp, &tmQo, &tmK, &tmV);
+    } else if (warp == 1) {
+      if (leader && ok) ok = is_wide ? multiply<true, N>(w, wide, smem, bar, tmem, cnt) : multiply<false, N>(w, narrow, smem, bar, tmem, cnt);
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_free);
-      ++k;
+    } else {
+      if (ok) ok = is_wide ? softmax_wide(p, w, wide, smem, bar, tmem, cnt, items, cw) : softmax_narrow<N, NL>(p, w, narrow, smem, bar, tmem, cnt, items, cn);
     }
-    if (!ok) *abort_flag = 1;
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
+    if (!ok) *bar.aborted = 1;
+    tc_fence_before();
+    __syncthreads();               // both forms use the same buffers
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    if (*bar.aborted) break;
+    __syncthreads();
   }
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the partials of a token's rows: one block per token, one warp per head.
-// Parts are added in the order prefix, own keys, ascending tiles.
-__global__ void __launch_bounds__(256) join_kernel(AttnParams p, int grid) {
+// Joins the partials of a (token, head): one block each, its warps take every fourth part.
+// Parts are the prefix's and the own keys' runs, in the order of their tiles.
+__global__ void __launch_bounds__(128) join_kernel(AttnParams p) {
   pdl_wait();
-  const int t = blockIdx.x, lane = threadIdx.x & 31;
+  __shared__ float4 acc[4][32];
+  __shared__ float2 ml[4];
+  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int4 runs = *reinterpret_cast<const int4*>(p.runs), e0 = p.where[2 * t], e1 = p.where[2 * t + 1];
   if (t >= min(p.q_start[p.B], p.T)) return;
-  // the last i in [0, n] with v[i] <= key (v[0] <= key), 32 probes at a time
-  auto last_at_most = [&](const int* v, int n, int key) {
-    int lo = 0, hi = n;
-    while (hi > lo) {
-      const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
-      const unsigned m = __ballot_sync(0xffffffff, i <= hi && v[i] <= key);
-      const int k = __popc(m);       // probes are ascending: the first k hold
-      lo += k * step;
-      hi = min(hi, lo + step - 1);
-    }
-    return lo;
+  const size_t at = (size_t)t * p.Hq + h;
+  const bool own_wide = p.nwide > p.ngroups;
+  int first0 = 0, first1 = 0, n0 = 0, n1 = 0;
+  if (e0.y) {
+    const int x = e0.x + h / p.G * e0.z;
+    first0 = run_of(x, runs.x, runs.y);
+    n0 = run_of(x + e0.y - 1, runs.x, runs.y) - first0 + 1;
+  }
+  if (e1.y) {
+    const int W = own_wide ? runs.x : runs.z, C = own_wide ? runs.y : runs.w, x = e1.x + h / p.G * e1.z;
+    first1 = run_of(x, W, C);
+    n1 = run_of(x + e1.y - 1, W, C) - first1 + 1;
+  }
+  if (n0 == 0 && n1 == 1) return;                    // written by the block that had it all
+  const int g = h % p.G;
+  auto part = [&](int j) -> const float* {           // part j of n0 + n1
+    const bool own = j >= n0;
+    j -= own ? n0 : 0;
+    if ((own ? n1 : n0) == 1) return (own ? p.whole_own : p.whole_prefix) + at * kPart;
+    const size_t slot = 2 * ((own ? first1 : first0) + j) + (j == 0 ? 1 : 0);
+    return own && !own_wide ? p.split_narrow + (slot * 64 + e1.w + g) * kPart
+                            : p.split_wide + (slot * 128 + (own ? e1.w : e0.w) + g) * kPart;
   };
-  auto start = [&](int i) { return min(max(p.q_start[i], 0), p.T); };
-  auto group = [&](int i) { return min(max(p.group_start[i], 0), p.B); };
-  const int b = min(last_at_most(p.q_start, p.B, t), p.B - 1);
-  const int nu = p.ngroups + p.B, W = p.meta[nu], C = used_blocks(W, grid);
-  int g = -1;
-  if (p.ngroups && p.group_start[0] <= b) {
-    g = last_at_most(p.group_start, p.ngroups, b);
-    if (g >= p.ngroups || p.meta[g + 1] == p.meta[g]) g = -1;          // in no group, or nothing shared
-  }
-  for (int h = threadIdx.x / 32; h < p.Hq; h += blockDim.x / 32) {
-    const size_t at = (size_t)t * p.Hq + h;
-    // up to two units: first partial row and the distance to the next
-    const float* first[2] = {nullptr, nullptr};
-    int count[2] = {0, 0}, c0[2] = {0, 0}, row[2] = {0, 0};
-    bool whole_own = false;
-    for (int i = 0; i < 2; ++i) {
-      const int u = i == 0 ? g : p.ngroups + b;
-      if (u < 0) continue;
-      const int tiles = p.meta[u + 1] - p.meta[u];
-      if (tiles == 0) continue;
-      const int s0 = i == 0 ? group(g) : b, s1 = i == 0 ? group(g + 1) : b + 1;
-      const int tb = i == 0 ? p.tokens_prefix : p.tokens_own, q0 = start(s0);
-      const int nb = (start(s1) - q0 + tb - 1) / tb, rb = (t - q0) / tb;
-      if (nb <= 0 || t < q0 || rb >= nb) continue;   // starts that do not ascend: nothing is read out of range
-      const int n = tiles / (nb * p.Hkv), x = p.meta[u] + ((h / p.G) * nb + rb) * n;
-      const int ca = block_of(x, W, C), cb = block_of(x + n - 1, W, C);
-      row[i] = (t - q0 - rb * tb) * p.G + h % p.G;
-      c0[i] = ca;
-      count[i] = cb - ca + 1;
-      if (count[i] == 1) {
-        first[i] = (i == 0 ? p.whole_prefix : p.whole_own) + at * kPart;
-        whole_own = whole_own || i == 1;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float mj, float lj, float4 v) {
+    if (mj == -INFINITY) return;                     // no key of this part was visible
+    const float now = fmaxf(m, mj), a = exp2f(m - now), b = exp2f(mj - now);     // m = -inf: a = 0
+    l = l * a + lj * b;
+    o.x = o.x * a + v.x * b; o.y = o.y * a + v.y * b; o.z = o.z * a + v.z * b; o.w = o.w * a + v.w * b;
+    m = now;
+  };
+#pragma unroll 1
+  for (int j = warp; j < n0 + n1; j += 16) {         // four parts' loads in flight
+    float2 s[4];
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = make_float2(-INFINITY, 0.f);
+      if (j + 4 * i < n0 + n1) {
+        const float* r = part(j + 4 * i);
+        s[i] = *reinterpret_cast<const float2*>(r + D);
+        v[i] = *reinterpret_cast<const float4*>(r + lane * 4);
       }
     }
-    if (whole_own && count[0] == 0) continue;        // written by the block that had it all
-    auto part = [&](int i, int j) -> const float* {
-      if (first[i]) return first[i];
-      return p.split + ((size_t)(2 * (c0[i] + j) + (j == 0 ? 1 : 0)) * 128 + row[i]) * kPart;
-    };
-    float m = -INFINITY;
-    for (int i = 0; i < 2; ++i)
-      for (int j = 0; j < count[i]; ++j) m = fmaxf(m, part(i, j)[D]);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < 2; ++i)
-      for (int j = 0; j < count[i]; ++j) {
-        const float* r = part(i, j);
-        if (r[D] == -INFINITY) continue;             // no key of this part was visible
-        const float f = exp2f(r[D] - m);
-        const float4 v = *reinterpret_cast<const float4*>(r + lane * 4);
-        l += r[D + 1] * f;
-        o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
-      }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-    if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(s[i].x, s[i].y, v[i]);
   }
+  if (n0 + n1 > 1) {
+    acc[warp][lane] = o;
+    if (lane == 0) ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp) return;
+    for (int i = 1; i < 4; ++i) add(ml[i].x, ml[i].y, acc[i][lane]);
+  } else if (warp) {
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// A cache as [64 columns, slots, 2 halves, heads]: a box of 64 keys holds both halves of a
+// head, one of fewer keys (small pages) a half of it.
+CUtensorMap cache_map(const at::Tensor& c, int box) {
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {64, (cuuint64_t)c.size(0), 2, (cuuint64_t)c.size(1)};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.stride(0) * 2, 128, (cuuint64_t)c.stride(1) * 2};
+  const cuuint32_t b[4] = {64, (cuuint32_t)box, box == BK ? 2u : 1u, 1}, unit[4] = {1, 1, 1, 1};
+  const CUresult r = get_encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, c.data_ptr(), dims, strides, b, unit,
+                                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "prefix_attention: the cache's strides cannot be described to the TMA unit (code ", std::to_string((int)r), ")");
+  return m;
 }
 
 void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
@@ -767,8 +1116,9 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
                     (uintptr_t)c->data_ptr() % 16 == 0 && c->sizes() == kc.sizes(),
                 "prefix_attention: caches must be bf16 [slots, Hkv, 128] with 16-byte aligned heads, of one shape");
   const int64_t T = q.size(0), Hq = q.size(1), Hkv = kc.size(1), B = lens.numel();
-  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 128, "prefix_attention: Hq must be a multiple (up to 128) of Hkv");
-  TORCH_CHECK(B <= 1024, "prefix_attention: at most 1024 sequences a call");
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 128 && Hq <= 65535, "prefix_attention: Hq must be a multiple (up to 128) of Hkv");
+  static_assert(kMaxSeqs == 512, "the message below");
+  TORCH_CHECK(B <= kMaxSeqs, "prefix_attention: at most 512 sequences a call");
   TORCH_CHECK(page_size % 8 == 0, "prefix_attention: page_size must be a multiple of 8");
   TORCH_CHECK(max_q >= 1, "prefix_attention: max_q must be positive");
   check_ints(lens, q, B, "lens");
@@ -803,7 +1153,10 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   p.Hkv = (int)Hkv;
   p.G = G;
   p.tokens_prefix = 128 / G;
+  // The narrow form up to 64 rows of a sequence; what max_q leaves out is further row blocks.
+  const bool narrow = max_q * G <= 64;
   p.tokens_own = (int)std::min<int64_t>(128 / G, max_q);
+  p.nwide = narrow ? ngroups : ngroups + (int)B;
   p.box = (int)std::gcd<int64_t, int64_t>(page_size, BK);
   p.group_start = group_start ? group_start->data_ptr<int>() : nullptr;
   p.prefix = prefix_len ? prefix_len->data_ptr<int>() : nullptr;
@@ -814,30 +1167,31 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   const int64_t tiles = (table.size(1) * page_size + BK - 1) / BK + 1;
   TORCH_CHECK(tiles * Hkv * (T / p.tokens_prefix + ngroups + T / p.tokens_own + B) < (int64_t)1 << 30,
               "prefix_attention: rows x table length out of range");
-  // Partials: whole items of rows that have a shared prefix, one row each; what the
-  // blocks' runs cut, two row blocks for each of them.
   const int grid = 2 * num_sms(q.get_device());
-  const int64_t rows = ngroups ? T * Hq * kPart : 0, split = (int64_t)2 * grid * 128 * kPart;
-  at::Tensor ws = at::empty({2 * rows + split + ngroups + B + 1}, q.options().dtype(at::kFloat));
-  p.whole_prefix = ws.data_ptr<float>();
+  const int64_t rows = ngroups ? T * Hq * kPart : 0, wide = (int64_t)2 * grid * 128 * kPart, thin = wide / 2;
+  at::Tensor ws = at::empty({8 * T + 4 + 2 * rows + wide + thin}, q.options().dtype(at::kFloat));
+  p.where = reinterpret_cast<int4*>(ws.data_ptr<float>());
+  p.runs = reinterpret_cast<int*>(p.where + 2 * T);
+  p.whole_prefix = reinterpret_cast<float*>(p.runs + 4);
   p.whole_own = p.whole_prefix + rows;
-  p.split = p.whole_own + rows;
-  p.meta = reinterpret_cast<int*>(p.split + split);
+  p.split_wide = p.whole_own + rows;
+  p.split_narrow = p.split_wide + wide;
   const auto bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMap tq = make_tmap_3d(q.data_ptr(), bf, 2, D, Hq, T, D, q.stride(0), 64, G, p.tokens_prefix);
   const CUtensorMap to = make_tmap_3d(q.data_ptr(), bf, 2, D, Hq, T, D, q.stride(0), 64, G, p.tokens_own);
-  const CUtensorMap tk = make_tmap_3d(kc.data_ptr(), bf, 2, D, Hkv, kc.size(0), kc.stride(1), kc.stride(0), 64, 1, p.box);
-  const CUtensorMap tv = make_tmap_3d(vc.data_ptr(), bf, 2, D, Hkv, vc.size(0), vc.stride(1), vc.stride(0), 64, 1, p.box);
-  static bool attr[64] = {};
+  const CUtensorMap tk = cache_map(kc, p.box), tv = cache_map(vc, p.box);
+  const int form = !narrow || p.tokens_own * G <= 8 ? 0 : p.tokens_own * G <= 16 ? 1 : p.tokens_own * G <= 32 ? 2 : 3;
+  void (*const kernels[])(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnParams) = {attn_kernel<8>, attn_kernel<16>, attn_kernel<32>, attn_kernel<64>};
+  static bool attr[64][4] = {};
   const int dev = q.get_device();
-  if (!attr[dev]) {
-    check_cuda(cudaFuncSetAttribute(attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnSmem::TOTAL), "prefix_attention smem");
-    attr[dev] = true;
+  if (!attr[dev][form]) {
+    check_cuda(cudaFuncSetAttribute(kernels[form], cudaFuncAttributeMaxDynamicSharedMemorySize, AttnSmem::TOTAL), "prefix_attention smem");
+    attr[dev][form] = true;
   }
   auto st = at::cuda::getCurrentCUDAStream();
-  attn_kernel<<<grid, kAttnThreads, AttnSmem::TOTAL, st>>>(tq, to, tk, tv, p);
+  kernels[form]<<<grid, kAttnThreads, AttnSmem::TOTAL, st>>>(tq, to, tk, tv, p);
   check_cuda(cudaGetLastError(), "prefix_attention");
-  launch_after("prefix_attention join", join_kernel, dim3((unsigned)T), dim3(256), 0, st, p, grid);
+  launch_after("prefix_attention join", join_kernel, dim3((unsigned)T, (unsigned)Hq), dim3(128), 0, st, p);
 }
 
 }  // namespace kore

@@ -106,7 +106,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     ``max_q`` is the largest number of rows of a sequence as far as the host knows
     (it chooses the split, not the result). CUDA: bf16, D = 128, page_size a
-    multiple of 8, at most 1024 sequences. What the cache holds behind a
+    multiple of 8, at most 512 sequences. What the cache holds behind a
     sequence's last token does not matter, NaN included; among the tokens of a
     call, a row's value that is not finite reaches the sequence's earlier rows too."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])

@@ -134,11 +134,11 @@ def test_without_groups(groups, ps, hq, hkv):
 
 
 def test_many_sequences():
-    """1024 sequences in 300 groups, some groups empty of shared keys, some of sequences."""
+    """512 sequences in 300 groups, some groups empty of shared keys, some of sequences."""
     g = torch.Generator().manual_seed(5)
-    cut = sorted(torch.randint(0, 1025, (299,), generator=g).tolist())
+    cut = sorted(torch.randint(0, 513, (299,), generator=g).tolist())
     groups = []
-    for a, b in zip([0] + cut, cut + [1024]):
+    for a, b in zip([0] + cut, cut + [512]):
         P = int(torch.randint(0, 90, (1,), generator=g))
         groups.append((P, [(P + 1 + int(torch.randint(0, 60, (1,), generator=g)), 1) for _ in range(b - a)]))
     a = build_cache(groups, 16, 4, 2, device="cuda", seed=2)
@@ -328,7 +328,7 @@ def test_refusals():
     for b in bad:
         with pytest.raises(RuntimeError):
             paged.prefix_attention(**{**dict(max_q=2), **a, **b})
-    many = build_cache([(0, [(1, 1)] * 1025)], 8, 1, 1, device="cuda")
+    many = build_cache([(0, [(1, 1)] * 513)], 8, 1, 1, device="cuda")
     with pytest.raises(RuntimeError):
         paged.prefix_attention(**many)
 
