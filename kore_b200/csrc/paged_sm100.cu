@@ -215,8 +215,6 @@ KORE_DEV bool softmax_any(bool v) {
       : "=r"(r) : "r"((uint32_t)v) : "memory");
   return r != 0;
 }
-// The four warps' wait: they meet at named barriers, so they give up together too.
-KORE_DEV bool softmax_wait(uint64_t* bar, uint32_t phase) { return !softmax_any(!warp_wait(bar, phase)); }
 KORE_DEV void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
 // The units as every block sees them, in shared memory: unit u < ngroups is a prefix,
@@ -697,6 +695,9 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
   const int lane = threadIdx.x & 31, q4 = threadIdx.x / 32 & 3, tid = q4 * 32 + lane;
   const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
   NarrowSmem& x = *reinterpret_cast<NarrowSmem*>(smem + AttnSmem::X_OFF);
+  // The four warps meet at named barriers, whose waits have no limit: one whose wait on an
+  // mbarrier ran out goes through the rest of the run without waiting, so that all meet.
+  bool ok = true;
   Item it;
   int tile = cnt;
 #pragma unroll 1
@@ -720,8 +721,8 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
 #pragma unroll 1
     for (int j = it.j0; j < it.j1; ++j, ++tile) {
       const int st = tile & 1, kv0 = (tile0 + j) * BK;
-      if (!softmax_wait(&bar.s_full[st], (tile >> 1) & 1)) return false;
-      if ((kv0 < klo || kv0 + BK > khi) && softmax_any(!clear_v(smem, bar, tile, kv0, klo, khi))) return false;
+      ok = ok && warp_wait(&bar.s_full[st], (tile >> 1) & 1);
+      if (kv0 < klo || kv0 + BK > khi) ok = ok && clear_v(smem, bar, tile, kv0, klo, khi);
       float s[NL];
       bool over = false;
       if (q4 < 2) {
@@ -755,7 +756,7 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
         }
         softmax_sync();
         if (j > it.j0) {
-          if (!softmax_wait(bar.o_done, (tile - 1) & 1)) return false;
+          ok = ok && warp_wait(bar.o_done, (tile - 1) & 1);
           tc_fence_after();
           float o[NL];
           tmem_ld<NL>(to, o);
@@ -789,13 +790,14 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
 #pragma unroll
         for (int i = 0; i < per; ++i) x.mine[q4][lane / same * per + i] = l[i];
     }
-    if (!softmax_wait(bar.o_final, items++ & 1)) return false;             // also: `mine` is there
+    ok = ok && warp_wait(bar.o_final, items++ & 1);
     tc_fence_after();
     float o[NL];
     tmem_ld<NL>(to, o);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar.on_free + (k & 1));
+    softmax_sync();                             // `mine` is there
     const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
     float* split = p.split_narrow + (size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 64 * kPart;
     if (tid < rows) {
@@ -823,7 +825,7 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
     softmax_sync();                             // the rows' values have been read
   }
   cnt = tile;
-  return true;
+  return ok;
 }
 
 template <int NL>
@@ -846,12 +848,26 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 
   pdl_trigger();
   // ---- the units' tiles, summed
-#pragma unroll 1
-  for (int i = threadIdx.x; i <= p.B; i += kAttnThreads) {
-    w.qs[i] = min(max(p.q_start[i], 0), p.T);
-    if (i < p.B) w.len[i] = min(max(p.lens[i], 0), p.M * p.page_size);
-    if (i <= p.ngroups) w.gs[i] = p.ngroups ? min(max(p.group_start[i], 0), p.B) : 0;
-    if (i < p.ngroups) w.prefix[i] = min(max(p.prefix[i], 0), p.M * p.page_size);
+  {
+    constexpr int R = (kMaxSeqs + kAttnThreads) / kAttnThreads;      // all loads in flight together
+    int q[R], n[R], g[R], x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = threadIdx.x + r * kAttnThreads;
+      q[r] = i <= p.B ? p.q_start[i] : 0;
+      n[r] = i < p.B ? p.lens[i] : 0;
+      g[r] = p.ngroups && i <= p.ngroups ? p.group_start[i] : 0;
+      x[r] = i < p.ngroups ? p.prefix[i] : 0;
+    }
+    const int cap = p.M * p.page_size;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = threadIdx.x + r * kAttnThreads;
+      if (i <= p.B) w.qs[i] = min(max(q[r], 0), p.T);
+      if (i < p.B) w.len[i] = min(max(n[r], 0), cap);
+      if (i <= p.ngroups) w.gs[i] = min(max(g[r], 0), p.B);
+      if (i < p.ngroups) w.prefix[i] = min(max(x[r], 0), cap);
+    }
   }
   if (threadIdx.x == 0) {
 #pragma unroll 1
