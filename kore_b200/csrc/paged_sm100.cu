@@ -129,10 +129,10 @@ __global__ void plan_rows_kernel(PlanParams p) {
 //
 // Items come in two forms, each with its own runs:
 //   wide   S[128 rows x 64 keys] = Q K^T, O[128 x 128] += P V: prefixes, and own keys
-//          when a sequence has more than 64 rows. One softmax thread owns a row.
-//   narrow S^T[64 keys x N rows] = K Q^T, O^T[128 x N] += V^T P^T with N = 16, 32 or
-//          64: own keys under few rows. The products cost N / 64 of the wide form's
-//          and a tile's exponentials are spread over its keys, not over the few rows.
+//          when a sequence has more than 32 rows. One softmax thread owns a row.
+//   narrow S^T[64 keys x N rows] = K Q^T, O^T[128 x N] += V^T P^T with N = 16 or 32:
+//          own keys under few rows. A tile's exponentials are spread over its keys,
+//          where the wide form would have one thread to a row do all of them.
 // Half of the blocks begin with their wide run, the other half with their narrow one:
 // two blocks share an SM, and the first is bound by the tensor cores where the second
 // is bound by HBM.
@@ -141,8 +141,8 @@ constexpr int BK = 64;                            // keys of a tile
 constexpr int kStages = 2;
 constexpr int kTileBytes = BK * D * 2;            // 16 KB: 64 keys as two 8 KB swizzle atoms
 constexpr int kQBytes = 128 * D * 2;
-constexpr int kAttnThreads = 192;                 // producer, MMA, four softmax warps
-constexpr int kTmemCols = 256;                    // wide: two S / P buffers of 64 columns, O of 128; narrow: two S of 64, two O of 64
+constexpr int kAttnThreads = 256;                 // producer, S products, O products, one more, four softmax warps
+constexpr int kTmemCols = 256;                    // wide: two S / P buffers of 64 columns, O of 128; narrow: the same S buffers, two O
 constexpr uint32_t kTmemO = 128;
 constexpr int kMaxSeqs = 512;
 constexpr int kMinTiles = 4;                      // of a run: fewer cost more in partials than they save
@@ -168,10 +168,8 @@ struct AttnParams {
 };
 constexpr int kPart = D + 4;                      // floats of a partial row (16-byte aligned)
 
-// mbar_wait with its clock out of line: the kernel below has many waits, and what it
-// executes has to stay in the instruction cache.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t phase) { return mbar_wait(bar, phase); }
-KORE_DEV bool wait_on(uint64_t* bar, uint32_t phase) { return mbar_try_wait(smem_u32(bar), phase) || wait_long(bar, phase); }
+// mbar_wait without its limit's clock on the way in.
+KORE_DEV bool wait_on(uint64_t* bar, uint32_t phase) { return mbar_try_wait(smem_u32(bar), phase) || mbar_wait(bar, phase); }
 // A whole warp's wait: the lanes go on together or give up together.
 KORE_DEV bool warp_wait(uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffff, wait_on(bar, phase)); }
 
@@ -181,7 +179,7 @@ struct AttnSmem {
   static constexpr int V_OFF = K_OFF + kStages * kTileBytes;
   static constexpr int BAR_OFF = V_OFF + kStages * kTileBytes;
   static constexpr int X_OFF = BAR_OFF + 256;                        // NarrowSmem
-  static constexpr int UNITS_OFF = X_OFF + 6 * 64 * 4;               // Units
+  static constexpr int UNITS_OFF = X_OFF + 6 * 32 * 4;               // Units
   static constexpr int TOTAL = UNITS_OFF + 4 * 7 * kMaxSeqs + 1024;
 };
 static_assert(2 * (AttnSmem::TOTAL + 1024) <= 228 * 1024, "two blocks share an SM");
@@ -317,14 +315,13 @@ KORE_DEV Walk make_walk(const int* cum, int nu, int base, int W, int C, int c) {
 }
 
 // Narrow form: Q buffers (by the item's number) and, behind them, two P buffers (by the tile's parity).
-constexpr int q_bufs(int N) { return N <= 32 ? 2 : 1; }
-constexpr int p_off(int N) { return AttnSmem::Q_OFF + q_bufs(N) * N * 256; }
-static_assert(p_off(64) + 2 * 64 * 128 <= AttnSmem::K_OFF && p_off(32) + 2 * 32 * 128 <= AttnSmem::K_OFF, "narrow Q and P");
+constexpr int p_off(int N) { return AttnSmem::Q_OFF + 2 * N * 256; }
+static_assert(kStages == 2 && p_off(32) + 2 * 32 * 128 <= AttnSmem::K_OFF, "narrow Q and P");
 
 struct Bars {
   uint64_t *k_full, *k_empty, *v_full, *v_empty;     // [kStages]
   uint64_t *s_full, *p_full;                         // [2]
-  uint64_t *o_done, *o_final;                        // one phase per tile, per item
+  uint64_t *o_done, *o_final;                        // [2] by the tile's parity; one phase per item
   uint64_t *q_full, *q_empty, *o_free;               // wide: one buffer each
   uint64_t *qn_full, *qn_empty, *on_free;            // narrow: by the Q or O buffer
   volatile int* aborted;
@@ -335,7 +332,7 @@ template <int N>
 KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, int& cnt,
                       const CUtensorMap* tmQp, const CUtensorMap* tmQo, const CUtensorMap* tmK, const CUtensorMap* tmV) {
   using S = AttnSmem;
-  constexpr int QB = q_bufs(N);
+  constexpr int QB = 2;
   const int lane = threadIdx.x & 31, nbox = BK / p.box;
   Item it;
 #pragma unroll 1
@@ -405,74 +402,78 @@ KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk
   return true;
 }
 
-// ---- one thread: the products. S of the next tile is issued before O of this one, so
-// that the softmax warps find it ready. One in-order pipe: S_{i+1} overwrites S_{i-1}'s
-// buffer (wide: P_{i-1}, which PV_{i-1}, issued before, has read by then). The thread
-// issues twelve products a tile; their descriptors are sums of what it keeps, because
-// building them anew took longer (0.8 us a tile) than the products themselves.
+// ---- the products, one thread of a warp each for S and for O. A product of this size
+// takes about 98 cycles in its chain (measured; 32 to 64 at full rate), and the issuing
+// thread goes along with it: the eight products of an S and the four of an O, issued by
+// one thread, were 1,100 of a tile's 2,200 cycles. From two threads they overlap.
 constexpr uint64_t step16(int kk, int half) { return (uint64_t)(((kk >> 2) * half + (kk & 3) * 32) >> 4); }   // K-step kk of K-major atoms `half` bytes apart
+
 template <bool WIDE, int N>
-KORE_DEV bool multiply(const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt) {
+KORE_DEV bool multiply_s(const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt) {
   using S = AttnSmem;
-  constexpr uint32_t idesc_s = WIDE ? make_idesc_bf16(128, BK, false, false) : make_idesc_bf16(128, N, false, false);
-  constexpr uint32_t idesc_o = WIDE ? make_idesc_bf16(128, D, false, true) : make_idesc_bf16(128, N, true, false);
-  constexpr int QB = WIDE ? 1 : q_bufs(N);
-  const uint64_t q0 = make_sw128_desc(smem_u32(smem + S::Q_OFF), 16, 1024), k0 = make_sw128_desc(smem_u32(smem + S::K_OFF), 16, 1024),
-                 v0 = make_sw128_desc(smem_u32(smem + S::V_OFF), 8192, 1024), p0 = make_sw128_desc(smem_u32(smem + p_off(N)), 16, 1024);
+  constexpr uint32_t idesc = WIDE ? make_idesc_bf16(128, BK, false, false) : make_idesc_bf16(128, N, false, false);
+  constexpr int QB = WIDE ? 1 : 2;
+  const uint64_t q0 = make_sw128_desc(smem_u32(smem + S::Q_OFF), 16, 1024), k0 = make_sw128_desc(smem_u32(smem + S::K_OFF), 16, 1024);
   Item it;
-  bool ok = true;
 #pragma unroll 1
-  for (int k = 0; ok && next_item(w, r, it); ++k) {
-    const int qi = k % QB, qp = k / QB;
+  for (int k = 0; next_item(w, r, it); ++k) {
+    const int qi = k % QB, last = cnt + it.j1 - it.j0 - 1;
     const uint64_t qd = q0 + (uint64_t)(qi * N * 16);
-    const uint32_t to = tmem + kTmemO + (WIDE ? 0 : (k & 1) * 64);
-    const int n = it.j1 - it.j0;
-    uint64_t *const q_full = WIDE ? bar.q_full : bar.qn_full + qi, *const q_empty = WIDE ? bar.q_empty : bar.qn_empty + qi;
-    uint64_t* const o_free = WIDE ? bar.o_free : bar.on_free + (k & 1);
-    ok = wait_on(q_full, qp & 1);
+    if (!wait_on(WIDE ? bar.q_full : bar.qn_full + qi, (k / QB) & 1)) return false;
 #pragma unroll 1
-    for (int j = -1; j < n && ok; ++j) {        // S of tile j + 1, then O of tile j
-      const int i = cnt + j;
-      if (j + 1 < n) {
-        const int st = (i + 1) % kStages;
-        if (!(ok = wait_on(&bar.k_full[st], ((i + 1) / kStages) & 1))) break;
-        tc_fence_after();
-        const uint64_t kd = k0 + (uint64_t)(st * (kTileBytes >> 4));
-        const uint32_t ts = tmem + ((i + 1) & 1) * 64;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          // narrow: K is the left operand; its rows 64..127 are whatever lies behind the 64 of the tile, and nobody reads their result
-          if (WIDE) umma_f16_ss(ts, qd + step16(kk, 16384), kd + step16(kk, 8192), idesc_s, kk > 0);
-          else umma_f16_ss(ts, kd + step16(kk, 8192), qd + step16(kk, N * 128), idesc_s, kk > 0);
-        }
-        umma_commit(&bar.k_empty[st]);
-        umma_commit(&bar.s_full[(i + 1) & 1]);
-        if (j + 2 == n) umma_commit(q_empty);   // the item's last S is issued
-      }
-      if (j < 0) continue;
-      const int st = i % kStages, ob = WIDE ? 1 : 2;
-      if (j == 0 && k >= ob) ok = wait_on(o_free, (WIDE ? k - 1 : (k >> 1) - 1) & 1);   // the last item in this O has been read
-      ok = ok && wait_on(&bar.p_full[i & 1], (i >> 1) & 1) && wait_on(&bar.v_full[st], (i / kStages) & 1);
-      if (!ok) break;
+    for (; cnt <= last; ++cnt) {
+      const int st = cnt & 1;
+      if (!wait_on(&bar.k_full[st], (cnt >> 1) & 1)) return false;
+      if (cnt >= 2 && !wait_on(&bar.o_done[st], ((cnt >> 1) - 1) & 1)) return false;   // this S buffer's last tile is through
       tc_fence_after();
-      const uint64_t vd = v0 + (uint64_t)(st * (kTileBytes >> 4)), pd = p0 + (uint64_t)((i & 1) * N * 8);
+      const uint64_t kd = k0 + (uint64_t)(st * (kTileBytes >> 4));
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        // narrow: K is the left operand; its rows 64..127 are whatever lies behind the 64 of the tile, and nobody reads their result
+        if (WIDE) umma_f16_ss(tmem + st * 64, qd + step16(kk, 16384), kd + step16(kk, 8192), idesc, kk > 0);
+        else umma_f16_ss(tmem + st * 64, kd + step16(kk, 8192), qd + step16(kk, N * 128), idesc, kk > 0);
+      }
+      umma_commit(&bar.k_empty[st]);
+      umma_commit(&bar.s_full[st]);
+    }
+    if (!WIDE) umma_commit(bar.qn_empty + qi);
+  }
+  return true;
+}
+
+template <bool WIDE, int N>
+KORE_DEV bool multiply_o(const Units& w, Walk r, uint8_t* smem, const Bars& bar, uint32_t tmem, int& cnt) {
+  constexpr uint32_t idesc = WIDE ? make_idesc_bf16(128, D, false, true) : make_idesc_bf16(128, N, true, false);
+  const uint64_t v0 = make_sw128_desc(smem_u32(smem + AttnSmem::V_OFF), 8192, 1024), p0 = make_sw128_desc(smem_u32(smem + p_off(N)), 16, 1024);
+  Item it;
+#pragma unroll 1
+  for (int k = 0; next_item(w, r, it); ++k) {
+    const int first = cnt, last = cnt + it.j1 - it.j0 - 1, ob = WIDE ? 1 : 2;
+    const uint32_t to = tmem + kTmemO + (WIDE ? 0 : (k & 1) * 64);
+    // the last item in this O has been read
+    if (k >= ob && !wait_on(WIDE ? bar.o_free : bar.on_free + (k & 1), (WIDE ? k - 1 : (k >> 1) - 1) & 1)) return false;
+#pragma unroll 1
+    for (; cnt <= last; ++cnt) {
+      const int st = cnt & 1;
+      if (!wait_on(&bar.v_full[st], (cnt >> 1) & 1) || !wait_on(&bar.p_full[st], (cnt >> 1) & 1)) return false;
+      tc_fence_after();
+      const uint64_t vd = v0 + (uint64_t)(st * (kTileBytes >> 4)), pd = p0 + (uint64_t)(st * N * 8);
 #pragma unroll
       for (int kk = 0; kk < BK / 16; ++kk) {
-        if (WIDE) umma_f16_ts(to, tmem + (i & 1) * 64 + kk * 8, vd + kk * 128, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-        else umma_f16_ss(to, vd + kk * 128, pd + step16(kk, 0), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+        if (WIDE) umma_f16_ts(to, tmem + st * 64 + kk * 8, vd + kk * 128, idesc, (cnt > first || kk > 0) ? 1u : 0u);
+        else umma_f16_ss(to, vd + kk * 128, pd + step16(kk, 0), idesc, (cnt > first || kk > 0) ? 1u : 0u);
       }
       umma_commit(&bar.v_empty[st]);
-      umma_commit(bar.o_done);
+      umma_commit(&bar.o_done[st]);
     }
-    if (ok) umma_commit(bar.o_final);
-    cnt += n;
+    umma_commit(bar.o_final);
   }
-  return ok;
+  return true;
 }
 
 // What lies outside a unit's keys in the cache may be anything, NaN included, and
 // 0 x NaN is not 0: those rows of a V tile are cleared before the product reads them.
-__device__ __noinline__ bool clear_v(uint8_t* smem, const Bars& bar, int cnt, int kv0, int klo, int khi) {
+KORE_DEV bool clear_v(uint8_t* smem, const Bars& bar, int cnt, int kv0, int klo, int khi) {
   const int lane = threadIdx.x & 31, vs = cnt % kStages, r = (threadIdx.x / 32 & 3) * 16 + (lane >> 1);
   if (!warp_wait(&bar.v_full[vs], (cnt / kStages) & 1)) return false;
   if (kv0 + r < klo || kv0 + r >= khi) {
@@ -542,8 +543,7 @@ KORE_DEV bool softmax_wide(const AttnParams& p, const Units& w, Walk r, uint8_t*
         if (j > it.j0) {
           const float alpha = need && m != -INFINITY ? exp2f(m - m_new) : 1.f;
           if (__any_sync(0xffffffff, need && m != -INFINITY)) {
-            // S of this tile is committed, so PV of the tile two before is done and PV of this one not issued: the parity is clear
-            if (!warp_wait(bar.o_done, (tile - 1) & 1)) return false;
+            if (!warp_wait(&bar.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1)) return false;
             tc_fence_after();
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
@@ -588,41 +588,50 @@ KORE_DEV bool softmax_wide(const AttnParams& p, const Units& w, Walk r, uint8_t*
     }
     if (!warp_wait(bar.o_final, items++ & 1)) return false;
     if (warp_live) {
+      // Rows go out through this warp's 8 KB of the Q buffer, which the item needs no
+      // more, 64 columns at a time (16-byte pieces swizzled by the row): a store
+      // instruction then covers two whole row halves, not 16 bytes of 32 rows.
       tc_fence_after();
       const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
-      const size_t at = (size_t)t * p.Hq + h;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* part = whole ? (pre ? p.whole_prefix : p.whole_own) + at * kPart
-                          : p.split_wide + ((size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 128 + row) * kPart;
+      const int at = t * p.Hq + h, dst = whole ? at : (2 * run + (it.j0 == 0 ? 1 : 0)) * 128 + row;
+      float* const part = whole ? (pre ? p.whole_prefix : p.whole_own) : p.split_wide;
+      const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const unsigned rows = __ballot_sync(0xffffffff, live), joins = __ballot_sync(0xffffffff, !direct);
+      uint8_t* const stage = smem + AttnSmem::Q_OFF + q4 * 8192;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        uint32_t x[32];
-        tmem_ld32(tmem + lane_base + kTmemO + i4 * 32, x);
-        tmem_wait_ld();
-        if (live && direct) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 v;
-            v.x = pack_bf16(__uint_as_float(x[8 * i + 0]) * inv, __uint_as_float(x[8 * i + 1]) * inv);
-            v.y = pack_bf16(__uint_as_float(x[8 * i + 2]) * inv, __uint_as_float(x[8 * i + 3]) * inv);
-            v.z = pack_bf16(__uint_as_float(x[8 * i + 4]) * inv, __uint_as_float(x[8 * i + 5]) * inv);
-            v.w = pack_bf16(__uint_as_float(x[8 * i + 6]) * inv, __uint_as_float(x[8 * i + 7]) * inv);
-            *reinterpret_cast<uint4*>(p.out + at * D + i4 * 32 + 8 * i) = v;
-          }
-        } else if (live) {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t x[32];
+          tmem_ld32(tmem + lane_base + kTmemO + half * 64 + c * 32, x);
+          tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(part + i4 * 32 + 4 * i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            *reinterpret_cast<float4*>(stage + lane * 256 + (((c * 8 + i) ^ (lane & 7)) << 4)) =
+                make_float4(__uint_as_float(x[4 * i]) * inv, __uint_as_float(x[4 * i + 1]) * inv, __uint_as_float(x[4 * i + 2]) * inv,
+                            __uint_as_float(x[4 * i + 3]) * inv);
         }
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int rr = 2 * i + (lane >> 4), c = lane & 15;
+          const float4 v = *reinterpret_cast<const float4*>(stage + rr * 256 + ((c ^ (rr & 7)) << 4));
+          const int to = __shfl_sync(0xffffffff, dst, rr);
+          if (!(rows >> rr & 1)) continue;
+          if (joins >> rr & 1)
+            *reinterpret_cast<float4*>(part + (size_t)to * kPart + half * 64 + c * 4) = v;
+          else
+            *reinterpret_cast<uint2*>(p.out + (size_t)to * D + half * 64 + c * 4) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+        }
+        __syncwarp();
       }
       if (live && direct && p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-      if (live && !direct) {
-        part[D] = m;
-        part[D + 1] = l;
-      }
+      if (live && !direct) *reinterpret_cast<float2*>(part + (size_t)dst * kPart + D) = make_float2(m, l);
       tc_fence_before();
+      fence_proxy_async_smem();                 // the next Q is written by the TMA unit
     }
     __syncwarp();
+    if (lane == 0) mbar_arrive(bar.q_empty);
     if (lane == 0) mbar_arrive(bar.o_free);
   }
   cnt = tile;
@@ -663,8 +672,8 @@ KORE_DEV void tmem_st(uint32_t taddr, const float (&v)[NL]) {
   }
   tmem_wait_st();
 }
-// Sums of v[i] over the warp's lanes, by halving: NL - 1 exchanges. Lane's sums are
-// those of the columns (its upper bits) * max(NL / 32, 1) onwards; they end in v[0..].
+// Sums of v[i] over the warp's lanes, by halving: a lane ends with that of column
+// lane / (32 / NL), in v[0].
 template <int NL>
 KORE_DEV void warp_sums(float (&v)[NL]) {
   const int lane = threadIdx.x & 31;
@@ -686,8 +695,8 @@ KORE_DEV void warp_sums(float (&v)[NL]) {
 }
 
 struct NarrowSmem {               // per row of the block
-  float ref[64], factor[64], mine[2][64];       // reference exponent; factor when it moves, later 1 / sum; the two key warps' values
-  int limit[64], at[64];                        // the row sees keys [klo, limit); row of the result
+  float ref[32], factor[32], mine[2][32];       // reference exponent; factor when it moves, later 1 / sum; the two key warps' values
+  int limit[32], at[32];                        // the row sees keys [klo, limit); row of the result
 };
 
 template <int N, int NL>
@@ -737,14 +746,13 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
       }
       if (softmax_any(over || j == it.j0)) {
         if (q4 < 2) {
-          float top = -INFINITY, top2 = -INFINITY;
+          float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < NL; ++i) {
             const float v = warp_max(s[i]);
-            if (lane == (i & 31)) (i < 32 ? top : top2) = v;
+            if (lane == i) top = v;
           }
           if (lane < NL) x.mine[q4][lane] = top;
-          if (NL > 32) x.mine[q4][lane + 32] = top2;
         }
         softmax_sync();
         if (tid < NL) {
@@ -756,16 +764,20 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
         }
         softmax_sync();
         if (j > it.j0) {
-          ok = ok && warp_wait(bar.o_done, (tile - 1) & 1);
+          ok = ok && warp_wait(&bar.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1);
           tc_fence_after();
-          float o[NL];
-          tmem_ld<NL>(to, o);
+          constexpr int step = NL < 16 ? NL : 16;
 #pragma unroll
-          for (int i = 0; i < NL; ++i) {
-            l[i] *= x.factor[i];
-            o[i] *= x.factor[i];
+          for (int i0 = 0; i0 < NL; i0 += step) {
+            float o[step];
+            tmem_ld<step>(to + i0, o);
+#pragma unroll
+            for (int i = 0; i < step; ++i) {
+              l[i0 + i] *= x.factor[i0 + i];
+              o[i] *= x.factor[i0 + i];
+            }
+            tmem_st<step>(to + i0, o);
           }
-          tmem_st<NL>(to, o);
         }
       }
       if (q4 < 2) {
@@ -785,10 +797,7 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
     }
     if (q4 < 2) {
       warp_sums<NL>(l);
-      constexpr int per = NL > 32 ? NL / 32 : 1, same = NL < 32 ? 32 / NL : 1;   // sums of a lane, lanes with the same one
-      if (lane % same == 0)
-#pragma unroll
-        for (int i = 0; i < per; ++i) x.mine[q4][lane / same * per + i] = l[i];
+      if (lane % (32 / NL) == 0) x.mine[q4][lane / (32 / NL)] = l[0];
     }
     ok = ok && warp_wait(bar.o_final, items++ & 1);
     tc_fence_after();
@@ -799,7 +808,7 @@ KORE_DEV bool softmax_narrow(const AttnParams& p, const Units& w, Walk r, uint8_
     if (lane == 0) mbar_arrive(bar.on_free + (k & 1));
     softmax_sync();                             // `mine` is there
     const bool whole = it.j0 == 0 && it.j1 == it.n, direct = whole && !joined;
-    float* split = p.split_narrow + (size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 64 * kPart;
+    float* split = p.split_narrow + (size_t)(2 * run + (it.j0 == 0 ? 1 : 0)) * 32 * kPart;
     if (tid < rows) {
       const float sum = x.mine[0][tid] + x.mine[1][tid], m = x.ref[tid];
       if (direct) {
@@ -838,9 +847,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
-  int* warp_sum = reinterpret_cast<int*>(tmem_slot + 2);             // [6]
-  const Bars bar = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 12, bars + 13, bars + 14,
-                    bars + 15, bars + 16, bars + 17, bars + 19, bars + 21, reinterpret_cast<volatile int*>(tmem_slot + 1)};
+  int* warp_sum = reinterpret_cast<int*>(tmem_slot + 2);             // [8]
+  const Bars bar = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 12, bars + 14, bars + 15,
+                    bars + 16, bars + 17, bars + 18, bars + 20, bars + 22, reinterpret_cast<volatile int*>(tmem_slot + 1)};
   static_assert(kStages == 2, "barrier layout");
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Units w(p, smem + S::UNITS_OFF);
@@ -871,7 +880,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   }
   if (threadIdx.x == 0) {
 #pragma unroll 1
-    for (int i = 0; i < 23; ++i) mbar_init(bars + i, i == 10 || i == 11 || i == 16 || i == 21 || i == 22 ? 4 : 1);   // p_full, o_free: a warp's lane each
+    for (int i = 0; i < 24; ++i)     // p_full, wide q_empty, o_free, on_free: a lane of each softmax warp
+      mbar_init(bars + i, i == 10 || i == 11 || i == 16 || i == 17 || i >= 22 ? 4 : 1);
     *bar.aborted = 0;
     fence_barrier_init();
   }
@@ -916,12 +926,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   __syncthreads();
   tc_fence_after();
   const int Ww = cum[p.nwide], Wn = cum[nu] - Ww, Cw = num_runs(Ww, gridDim.x), Cn = num_runs(Wn, gridDim.x);
-  if (warp >= 2) {
+  if (warp == 3) {
     // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
-    const int id = blockIdx.x * 128 + threadIdx.x - 64;
+    const int id = blockIdx.x * 32 + lane;
     if (id == 0) *reinterpret_cast<int4*>(p.runs) = make_int4(Ww, Cw, Wn, Cn);
 #pragma unroll 1
-    for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 128) {
+    for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 32) {
       const int t = i >> 1, b = w.seq_of(t, 0, p.B - 1), u = i & 1 ? p.ngroups + b : w.grp[b];
       int4 e = make_int4(0, 0, 0, 0);
       if (u >= 0 && cum[u + 1] > cum[u]) {
@@ -938,60 +948,81 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   const int cw = blockIdx.x, cn = gridDim.x - 1 - blockIdx.x;       // few runs of both forms land on different blocks
   const Walk wide = make_walk(cum, nu, 0, Ww, Cw, cw), narrow = make_walk(cum, nu, Ww, Wn, Cn, cn);
   const bool wide_first = blockIdx.x < gridDim.x / 2;
-  const bool leader = warp == 1 && elect_one();
-  int cnt = 0, items = 0;          // tiles and items so far, in both turns
-  bool ok = true;
-#pragma unroll 1
-  for (int turn = 0; turn < 2; ++turn) {
-    const bool is_wide = (turn == 0) == wide_first;
-    if (warp == 0) {
-      if (ok) ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, &tmQp, &tmQo, &tmK, &tmV);
-    } else if (warp == 1) {
-      if (leader && ok) ok = is_wide ? multiply<true, N>(w, wide, smem, bar, tmem, cnt) : multiply<false, N>(w, narrow, smem, bar, tmem, cnt);
-      __syncwarp();
-    } else {
-      if (ok) ok = is_wide ? softmax_wide(p, w, wide, smem, bar, tmem, cnt, items, cw) : softmax_narrow<N, NL>(p, w, narrow, smem, bar, tmem, cnt, items, cn);
-    }
+  // The end of a turn: both forms use the same buffers. True: give up.
+  auto turned = [&](bool ok) {
     if (!ok) *bar.aborted = 1;
     tc_fence_before();
-    __syncthreads();               // both forms use the same buffers
-    tc_fence_after();
-    if (*bar.aborted) break;
     __syncthreads();
+    tc_fence_after();
+    const bool stop = *bar.aborted;
+    __syncthreads();
+    return stop;
+  };
+  int cnt = 0;                     // tiles so far, in both turns
+  // 56 and 200 registers for four warps each: together the 256 x 128 of the launch (the
+  // host checks that it has these: an increase beyond them would wait for good).
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const bool lead = elect_one();
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+      const bool is_wide = (turn == 0) == wide_first;
+      bool ok = true;
+      if (warp == 0) {
+        ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, &tmQp, &tmQo, &tmK, &tmV);
+      } else if (warp == 1) {
+        if (lead) ok = is_wide ? multiply_s<true, N>(w, wide, smem, bar, tmem, cnt) : multiply_s<false, N>(w, narrow, smem, bar, tmem, cnt);
+      } else if (warp == 2) {
+        if (lead) ok = is_wide ? multiply_o<true, N>(w, wide, smem, bar, tmem, cnt) : multiply_o<false, N>(w, narrow, smem, bar, tmem, cnt);
+      }
+      __syncwarp();
+      if (turned(ok)) break;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    int items = 0;                 // items so far
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+      const bool is_wide = (turn == 0) == wide_first;
+      const bool ok = is_wide ? softmax_wide(p, w, wide, smem, bar, tmem, cnt, items, cw) : softmax_narrow<N, NL>(p, w, narrow, smem, bar, tmem, cnt, items, cn);
+      if (turned(ok)) break;
+    }
   }
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the partials of a (token, head): one block each, its warps take every fourth part.
-// Parts are the prefix's and the own keys' runs, in the order of their tiles.
+// Joins the partials of a (token, head), WPR warps for each: their every WPR-th part, four
+// at a time. Parts are the prefix's and the own keys' runs, in the order of their tiles.
+template <int WPR>
 __global__ void __launch_bounds__(128) join_kernel(AttnParams p) {
   pdl_wait();
   __shared__ float4 acc[4][32];
   __shared__ float2 ml[4];
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, sub = warp % WPR;
+  const int at = blockIdx.x * (4 / WPR) + warp / WPR, t = at / p.Hq, h = at - t * p.Hq;
+  if (t >= p.T) return;                              // whole warps, and whole blocks where they meet
   const int4 runs = *reinterpret_cast<const int4*>(p.runs), e0 = p.where[2 * t], e1 = p.where[2 * t + 1];
-  if (t >= min(p.q_start[p.B], p.T)) return;
-  const size_t at = (size_t)t * p.Hq + h;
+  if (t >= p.q_start[p.B]) return;
   const bool own_wide = p.nwide > p.ngroups;
+  const int kvh = h / p.G, g = h - kvh * p.G;
   int first0 = 0, first1 = 0, n0 = 0, n1 = 0;
   if (e0.y) {
-    const int x = e0.x + h / p.G * e0.z;
+    const int x = e0.x + kvh * e0.z;
     first0 = run_of(x, runs.x, runs.y);
     n0 = run_of(x + e0.y - 1, runs.x, runs.y) - first0 + 1;
   }
   if (e1.y) {
-    const int W = own_wide ? runs.x : runs.z, C = own_wide ? runs.y : runs.w, x = e1.x + h / p.G * e1.z;
+    const int W = own_wide ? runs.x : runs.z, C = own_wide ? runs.y : runs.w, x = e1.x + kvh * e1.z;
     first1 = run_of(x, W, C);
     n1 = run_of(x + e1.y - 1, W, C) - first1 + 1;
   }
   if (n0 == 0 && n1 == 1) return;                    // written by the block that had it all
-  const int g = h % p.G;
   auto part = [&](int j) -> const float* {           // part j of n0 + n1
     const bool own = j >= n0;
     j -= own ? n0 : 0;
-    if ((own ? n1 : n0) == 1) return (own ? p.whole_own : p.whole_prefix) + at * kPart;
+    if ((own ? n1 : n0) == 1) return (own ? p.whole_own : p.whole_prefix) + (size_t)at * kPart;
     const size_t slot = 2 * ((own ? first1 : first0) + j) + (j == 0 ? 1 : 0);
-    return own && !own_wide ? p.split_narrow + (slot * 64 + e1.w + g) * kPart
+    return own && !own_wide ? p.split_narrow + (slot * 32 + e1.w + g) * kPart
                             : p.split_wide + (slot * 128 + (own ? e1.w : e0.w) + g) * kPart;
   };
   float m = -INFINITY, l = 0.f;
@@ -1004,14 +1035,14 @@ __global__ void __launch_bounds__(128) join_kernel(AttnParams p) {
     m = now;
   };
 #pragma unroll 1
-  for (int j = warp; j < n0 + n1; j += 16) {         // four parts' loads in flight
+  for (int j = sub; j < n0 + n1; j += 4 * WPR) {
     float2 s[4];
     float4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s[i] = make_float2(-INFINITY, 0.f);
-      if (j + 4 * i < n0 + n1) {
-        const float* r = part(j + 4 * i);
+      if (j + WPR * i < n0 + n1) {
+        const float* r = part(j + WPR * i);
         s[i] = *reinterpret_cast<const float2*>(r + D);
         v[i] = *reinterpret_cast<const float4*>(r + lane * 4);
       }
@@ -1019,17 +1050,15 @@ __global__ void __launch_bounds__(128) join_kernel(AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) add(s[i].x, s[i].y, v[i]);
   }
-  if (n0 + n1 > 1) {
+  if constexpr (WPR > 1) {
     acc[warp][lane] = o;
     if (lane == 0) ml[warp] = make_float2(m, l);
     __syncthreads();
-    if (warp) return;
-    for (int i = 1; i < 4; ++i) add(ml[i].x, ml[i].y, acc[i][lane]);
-  } else if (warp) {
-    return;
+    if (sub) return;
+    for (int i = 1; i < WPR; ++i) add(ml[i].x, ml[i].y, acc[i][lane]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(p.out + (size_t)at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -1132,7 +1161,7 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
                     (uintptr_t)c->data_ptr() % 16 == 0 && c->sizes() == kc.sizes(),
                 "prefix_attention: caches must be bf16 [slots, Hkv, 128] with 16-byte aligned heads, of one shape");
   const int64_t T = q.size(0), Hq = q.size(1), Hkv = kc.size(1), B = lens.numel();
-  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 128 && Hq <= 65535, "prefix_attention: Hq must be a multiple (up to 128) of Hkv");
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 128, "prefix_attention: Hq must be a multiple (up to 128) of Hkv");
   static_assert(kMaxSeqs == 512, "the message below");
   TORCH_CHECK(B <= kMaxSeqs, "prefix_attention: at most 512 sequences a call");
   TORCH_CHECK(page_size % 8 == 0, "prefix_attention: page_size must be a multiple of 8");
@@ -1169,8 +1198,8 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   p.Hkv = (int)Hkv;
   p.G = G;
   p.tokens_prefix = 128 / G;
-  // The narrow form up to 64 rows of a sequence; what max_q leaves out is further row blocks.
-  const bool narrow = max_q * G <= 64;
+  // The narrow form up to 32 rows of a sequence; what max_q leaves out is further row blocks.
+  const bool narrow = max_q * G <= 32;
   p.tokens_own = (int)std::min<int64_t>(128 / G, max_q);
   p.nwide = narrow ? ngroups : ngroups + (int)B;
   p.box = (int)std::gcd<int64_t, int64_t>(page_size, BK);
@@ -1181,10 +1210,11 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   p.out = (__nv_bfloat16*)out.data_ptr();
   p.lse = lse ? lse->data_ptr<float>() : nullptr;
   const int64_t tiles = (table.size(1) * page_size + BK - 1) / BK + 1;
+  TORCH_CHECK(T * Hq < (int64_t)1 << 31, "prefix_attention: too many rows");
   TORCH_CHECK(tiles * Hkv * (T / p.tokens_prefix + ngroups + T / p.tokens_own + B) < (int64_t)1 << 30,
               "prefix_attention: rows x table length out of range");
   const int grid = 2 * num_sms(q.get_device());
-  const int64_t rows = ngroups ? T * Hq * kPart : 0, wide = (int64_t)2 * grid * 128 * kPart, thin = wide / 2;
+  const int64_t rows = ngroups ? T * Hq * kPart : 0, wide = (int64_t)2 * grid * 128 * kPart, thin = wide / 4;
   at::Tensor ws = at::empty({8 * T + 4 + 2 * rows + wide + thin}, q.options().dtype(at::kFloat));
   p.where = reinterpret_cast<int4*>(ws.data_ptr<float>());
   p.runs = reinterpret_cast<int*>(p.where + 2 * T);
@@ -1196,18 +1226,27 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   const CUtensorMap tq = make_tmap_3d(q.data_ptr(), bf, 2, D, Hq, T, D, q.stride(0), 64, G, p.tokens_prefix);
   const CUtensorMap to = make_tmap_3d(q.data_ptr(), bf, 2, D, Hq, T, D, q.stride(0), 64, G, p.tokens_own);
   const CUtensorMap tk = cache_map(kc, p.box), tv = cache_map(vc, p.box);
-  const int form = !narrow || p.tokens_own * G <= 8 ? 0 : p.tokens_own * G <= 16 ? 1 : p.tokens_own * G <= 32 ? 2 : 3;
-  void (*const kernels[])(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnParams) = {attn_kernel<8>, attn_kernel<16>, attn_kernel<32>, attn_kernel<64>};
-  static bool attr[64][4] = {};
+  const int form = !narrow || p.tokens_own * G <= 8 ? 0 : p.tokens_own * G <= 16 ? 1 : 2;
+  void (*const kernels[])(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnParams) = {attn_kernel<8>, attn_kernel<16>, attn_kernel<32>};
+  static bool attr[64][3] = {};
   const int dev = q.get_device();
   if (!attr[dev][form]) {
+    cudaFuncAttributes fa;
+    check_cuda(cudaFuncGetAttributes(&fa, kernels[form]), "prefix_attention attributes");
+    TORCH_CHECK(fa.numRegs == 128, "prefix_attention: built with another register count than its warps share out");
     check_cuda(cudaFuncSetAttribute(kernels[form], cudaFuncAttributeMaxDynamicSharedMemorySize, AttnSmem::TOTAL), "prefix_attention smem");
     attr[dev][form] = true;
   }
   auto st = at::cuda::getCurrentCUDAStream();
   kernels[form]<<<grid, kAttnThreads, AttnSmem::TOTAL, st>>>(tq, to, tk, tv, p);
   check_cuda(cudaGetLastError(), "prefix_attention");
-  launch_after("prefix_attention join", join_kernel, dim3((unsigned)T, (unsigned)Hq), dim3(128), 0, st, p);
+  // A row to a warp when the rows fill the SMs by themselves (64 warps each), else to four:
+  // few rows may have their parts on all blocks.
+  const int64_t all = T * Hq;
+  if (all >= 32 * grid)
+    launch_after("prefix_attention join", join_kernel<1>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, st, p);
+  else
+    launch_after("prefix_attention join", join_kernel<4>, dim3((unsigned)all), dim3(128), 0, st, p);
 }
 
 }  // namespace kore
