@@ -133,9 +133,9 @@ __global__ void plan_rows_kernel(PlanParams p) {
 //   narrow S^T[64 keys x N rows] = K Q^T, O^T[128 x N] += V^T P^T with N = 16 or 32:
 //          own keys under few rows. A tile's exponentials are spread over its keys,
 //          where the wide form would have one thread to a row do all of them.
-// Half of the blocks begin with their wide run, the other half with their narrow one:
-// two blocks share an SM, and the first is bound by the tensor cores where the second
-// is bound by HBM.
+// Every block has a run of each form, the narrow one first. (Half of them the other way
+// round, so that one form's products overlap the other's loads, was slower by a third:
+// the code of both does not fit the instruction cache.)
 constexpr int D = 128;
 constexpr int BK = 64;                            // keys of a tile
 constexpr int kStages = 2;
@@ -145,7 +145,6 @@ constexpr int kAttnThreads = 256;                 // producer, S products, O pro
 constexpr int kTmemCols = 256;                    // wide: two S / P buffers of 64 columns, O of 128; narrow: the same S buffers, two O
 constexpr uint32_t kTmemO = 128;
 constexpr int kMaxSeqs = 512;
-constexpr int kMinTiles = 4;                      // of a run: fewer cost more in partials than they save
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttnParams {
@@ -297,7 +296,6 @@ KORE_DEV bool next_item(const Units& w, Walk& r, Item& it) {
 KORE_DEV int quotient(long a, int b) { return (int)((double)a / (double)b); }
 KORE_DEV int run_start(int c, int W, int C) { return quotient((long)c * W, C); }
 KORE_DEV int run_of(int x, int W, int C) { return quotient((long)(x + 1) * C - 1, W); }   // which run holds tile x
-KORE_DEV int num_runs(int W, int grid) { return min(grid, (W + kMinTiles - 1) / kMinTiles); }
 KORE_DEV Walk make_walk(const int* cum, int nu, int base, int W, int C, int c) {
   Walk r = {0, 0, 0};
   if (c < C) {
@@ -925,7 +923,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int Ww = cum[p.nwide], Wn = cum[nu] - Ww, Cw = num_runs(Ww, gridDim.x), Cn = num_runs(Wn, gridDim.x);
+  const int Ww = cum[p.nwide], Wn = cum[nu] - Ww, Cw = min(Ww, (int)gridDim.x), Cn = min(Wn, (int)gridDim.x);
   if (warp == 3) {
     // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
     const int id = blockIdx.x * 32 + lane;
@@ -947,7 +945,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const int cw = blockIdx.x, cn = gridDim.x - 1 - blockIdx.x;       // few runs of both forms land on different blocks
   const Walk wide = make_walk(cum, nu, 0, Ww, Cw, cw), narrow = make_walk(cum, nu, Ww, Wn, Cn, cn);
-  const bool wide_first = blockIdx.x < gridDim.x / 2;
   // The end of a turn: both forms use the same buffers. True: give up.
   auto turned = [&](bool ok) {
     if (!ok) *bar.aborted = 1;
@@ -966,7 +963,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const bool lead = elect_one();
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
-      const bool is_wide = (turn == 0) == wide_first;
+      const bool is_wide = turn == 1;
       bool ok = true;
       if (warp == 0) {
         ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, &tmQp, &tmQo, &tmK, &tmV);
@@ -983,7 +980,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     int items = 0;                 // items so far
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
-      const bool is_wide = (turn == 0) == wide_first;
+      const bool is_wide = turn == 1;
       const bool ok = is_wide ? softmax_wide(p, w, wide, smem, bar, tmem, cnt, items, cw) : softmax_narrow<N, NL>(p, w, narrow, smem, bar, tmem, cnt, items, cn);
       if (turned(ok)) break;
     }
