@@ -163,7 +163,7 @@ struct AttnParams {
   // row; what the runs cut, two items (a run's first and last) for each run.
   float *whole_prefix, *whole_own, *split_wide, *split_narrow;
   int4* where;                                    // [T][2] for the join: where the token's parts begin
-  int* runs;                                      // wide tiles, wide runs, narrow tiles, narrow runs
+  int* runs;                                      // wide tiles, narrow tiles
 };
 constexpr int kPart = D + 4;                      // floats of a partial row (16-byte aligned)
 
@@ -291,25 +291,35 @@ KORE_DEV bool next_item(const Units& w, Walk& r, Item& it) {
   r.x += it.j1 - it.j0;
   return true;
 }
-// Quotients of numbers below 2^40 and 2^30: exact in fp64, whose quotient cannot round up
-// to an integer that it is at least 2^-30 short of.
-KORE_DEV int quotient(long a, int b) { return (int)((double)a / (double)b); }
-KORE_DEV int run_start(int c, int W, int C) { return quotient((long)c * W, C); }
-KORE_DEV int run_of(int x, int W, int C) { return quotient((long)(x + 1) * C - 1, W); }   // which run holds tile x
-KORE_DEV Walk make_walk(const int* cum, int nu, int base, int W, int C, int c) {
-  Walk r = {0, 0, 0};
-  if (c < C) {
-    r.x = base + run_start(c, W, C);
-    r.end = base + run_start(c + 1, W, C);
-    int lo = 0, hi = nu;         // the unit that holds r.x
+// W tiles dealt to C runs: run c is [start(c), start(c + 1)), start(c) = floor(c W / C).
+struct Runs {
+  int W, C, q, r;                // q = W / C, r = W % C
+  KORE_DEV Runs(int W_, int grid) : W(W_), C(min(W_, grid)) {
+    q = C ? W / C : 0;
+    r = W - q * C;
+  }
+  KORE_DEV int start(int c) const { return c * q + (r ? (unsigned)(c * r) / (unsigned)C : 0); }
+  KORE_DEV int of(int x) const { // whose run holds tile x
+    int c = min((int)((float)x * (float)C / (float)W), C - 1);     // within one of it
+    if (start(c) > x) --c;
+    else if (start(c + 1) <= x) ++c;
+    return c;
+  }
+};
+KORE_DEV Walk make_walk(const int* cum, int nu, int base, const Runs& runs, int c) {
+  Walk w = {0, 0, 0};
+  if (c < runs.C) {
+    w.x = base + runs.start(c);
+    w.end = base + runs.start(c + 1);
+    int lo = 0, hi = nu;         // the unit that holds w.x
 #pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (cum[mid + 1] <= r.x) lo = mid + 1; else hi = mid;
+      if (cum[mid + 1] <= w.x) lo = mid + 1; else hi = mid;
     }
-    r.u = lo;
+    w.u = lo;
   }
-  return r;
+  return w;
 }
 
 // Narrow form: Q buffers (by the item's number) and, behind them, two P buffers (by the tile's parity).
@@ -901,7 +911,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const int u0 = min((int)threadIdx.x * per, nu), u1 = min(u0 + per, nu);
     int mine = 0;
 #pragma unroll 1
-    for (int u = u0; u < u1; ++u) mine += w.tiles(u);
+    for (int u = u0; u < u1; ++u) {
+      cum[u] = mine;
+      mine += w.tiles(u);
+    }
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -914,37 +927,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll 1
     for (int i = 0; i < warp; ++i) at += warp_sum[i];
 #pragma unroll 1
-    for (int u = u0; u < u1; ++u) {
-      cum[u] = at;
-      at += w.tiles(u);
-    }
-    if (u1 == nu) cum[nu] = at;      // the same from every thread that ends there
+    for (int u = u0; u < u1; ++u) cum[u] += at;
+    if (u1 == nu) cum[nu] = at + mine;      // the same from every thread that ends there
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int Ww = cum[p.nwide], Wn = cum[nu] - Ww, Cw = min(Ww, (int)gridDim.x), Cn = min(Wn, (int)gridDim.x);
-  if (warp == 3) {
-    // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
-    const int id = blockIdx.x * 32 + lane;
-    if (id == 0) *reinterpret_cast<int4*>(p.runs) = make_int4(Ww, Cw, Wn, Cn);
-#pragma unroll 1
-    for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 32) {
-      const int t = i >> 1, b = w.seq_of(t, 0, p.B - 1), u = i & 1 ? p.ngroups + b : w.grp[b];
-      int4 e = make_int4(0, 0, 0, 0);
-      if (u >= 0 && cum[u + 1] > cum[u]) {
-        const int tb = w.block_tokens(u), d = t - w.row0(u), rb = d / tb;
-        e.y = w.item_tiles(u);
-        e.x = cum[u] - (u < p.nwide ? 0 : Ww) + rb * e.y;
-        e.z = w.blocks(u) * e.y;
-        e.w = (d - rb * tb) * p.G;
-      }
-      p.where[i] = e;
-    }
-  }
+  const int Ww = cum[p.nwide];
+  const Runs wides(Ww, gridDim.x), narrows(cum[nu] - Ww, gridDim.x);
   const uint32_t tmem = *tmem_slot;
   const int cw = blockIdx.x, cn = gridDim.x - 1 - blockIdx.x;       // few runs of both forms land on different blocks
-  const Walk wide = make_walk(cum, nu, 0, Ww, Cw, cw), narrow = make_walk(cum, nu, Ww, Wn, Cn, cn);
+  const Walk wide = make_walk(cum, nu, 0, wides, cw), narrow = make_walk(cum, nu, Ww, narrows, cn);
   // The end of a turn: both forms use the same buffers. True: give up.
   auto turned = [&](bool ok) {
     if (!ok) *bar.aborted = 1;
@@ -961,6 +954,24 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const bool lead = elect_one();
+    if (warp == 3) {
+      // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
+      const int id = blockIdx.x * 32 + lane;
+      if (id == 0) *reinterpret_cast<int2*>(p.runs) = make_int2(Ww, narrows.W);
+#pragma unroll 1
+      for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 32) {
+        const int t = i >> 1, b = w.seq_of(t, 0, p.B - 1), u = i & 1 ? p.ngroups + b : w.grp[b];
+        int4 e = make_int4(0, 0, 0, 0);
+        if (u >= 0 && cum[u + 1] > cum[u]) {
+          const int tb = w.block_tokens(u), d = t - w.row0(u), rb = d / tb;
+          e.y = w.item_tiles(u);
+          e.x = cum[u] - (u < p.nwide ? 0 : Ww) + rb * e.y;
+          e.z = w.blocks(u) * e.y;
+          e.w = (d - rb * tb) * p.G;
+        }
+        p.where[i] = e;
+      }
+    }
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
       const bool is_wide = turn == 1;
@@ -991,27 +1002,30 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 // Joins the partials of a (token, head), WPR warps for each: their every WPR-th part, four
 // at a time. Parts are the prefix's and the own keys' runs, in the order of their tiles.
 template <int WPR>
-__global__ void __launch_bounds__(128) join_kernel(AttnParams p) {
+__global__ void __launch_bounds__(128) join_kernel(AttnParams p, int grid) {
   pdl_wait();
   __shared__ float4 acc[4][32];
   __shared__ float2 ml[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, sub = warp % WPR;
   const int at = blockIdx.x * (4 / WPR) + warp / WPR, t = at / p.Hq, h = at - t * p.Hq;
   if (t >= p.T) return;                              // whole warps, and whole blocks where they meet
-  const int4 runs = *reinterpret_cast<const int4*>(p.runs), e0 = p.where[2 * t], e1 = p.where[2 * t + 1];
+  const int2 tiles = *reinterpret_cast<const int2*>(p.runs);
+  const int4 e0 = p.where[2 * t], e1 = p.where[2 * t + 1];
   if (t >= p.q_start[p.B]) return;
   const bool own_wide = p.nwide > p.ngroups;
   const int kvh = h / p.G, g = h - kvh * p.G;
   int first0 = 0, first1 = 0, n0 = 0, n1 = 0;
+  const Runs wides(tiles.x, grid), narrows(tiles.y, grid);
   if (e0.y) {
     const int x = e0.x + kvh * e0.z;
-    first0 = run_of(x, runs.x, runs.y);
-    n0 = run_of(x + e0.y - 1, runs.x, runs.y) - first0 + 1;
+    first0 = wides.of(x);
+    n0 = wides.of(x + e0.y - 1) - first0 + 1;
   }
   if (e1.y) {
-    const int W = own_wide ? runs.x : runs.z, C = own_wide ? runs.y : runs.w, x = e1.x + kvh * e1.z;
-    first1 = run_of(x, W, C);
-    n1 = run_of(x + e1.y - 1, W, C) - first1 + 1;
+    const Runs& r = own_wide ? wides : narrows;
+    const int x = e1.x + kvh * e1.z;
+    first1 = r.of(x);
+    n1 = r.of(x + e1.y - 1) - first1 + 1;
   }
   if (n0 == 0 && n1 == 1) return;                    // written by the block that had it all
   auto part = [&](int j) -> const float* {           // part j of n0 + n1
@@ -1241,9 +1255,9 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   // few rows may have their parts on all blocks.
   const int64_t all = T * Hq;
   if (all >= 32 * grid)
-    launch_after("prefix_attention join", join_kernel<1>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, st, p);
+    launch_after("prefix_attention join", join_kernel<1>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, st, p, grid);
   else
-    launch_after("prefix_attention join", join_kernel<4>, dim3((unsigned)all), dim3(128), 0, st, p);
+    launch_after("prefix_attention join", join_kernel<4>, dim3((unsigned)all), dim3(128), 0, st, p, grid);
 }
 
 }  // namespace kore
