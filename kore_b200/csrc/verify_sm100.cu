@@ -61,35 +61,49 @@ struct RowView {
     nvec = (V + off + VE - 1) / VE;
   }
   KORE_DEV long elem(long j) const { return j * VE - off; }
-  KORE_DEV void load(long j, float (&f)[VE]) const;
+  KORE_DEV bool whole(long j) const { return elem(j) >= 0 && elem(j) + VE <= V; }
+  KORE_DEV uint4 raw(long j) const;
 };
 template <>
-KORE_DEV void RowView<__nv_bfloat16>::load(long j, float (&f)[8]) const {
-  const long e0 = elem(j);
-  if (e0 >= 0 && e0 + 8 <= V) {
-    const uint4 u = *reinterpret_cast<const uint4*>(base + j * 8);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+KORE_DEV uint4 RowView<__nv_bfloat16>::raw(long j) const {
+  if (whole(j)) return *reinterpret_cast<const uint4*>(base + j * 8);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = __bfloat1622float2(h[i]);
-      f[2 * i] = x.x;
-      f[2 * i + 1] = x.y;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long e = elem(j) + 2 * i + k;
+      h[k] = e >= 0 && e < V ? *reinterpret_cast<const uint16_t*>(base + j * 8 + 2 * i + k) : 0xff80u;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = e0 + i >= 0 && e0 + i < V ? __bfloat162float(base[j * 8 + i]) : -INFINITY;
+    w[i] = h[0] | h[1] << 16;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <>
-KORE_DEV void RowView<float>::load(long j, float (&f)[4]) const {
-  const long e0 = elem(j);
-  if (e0 >= 0 && e0 + 4 <= V) {
-    const float4 u = *reinterpret_cast<const float4*>(base + j * 4);
-    f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
-  } else {
+KORE_DEV uint4 RowView<float>::raw(long j) const {
+  if (whole(j)) return *reinterpret_cast<const uint4*>(base + j * 4);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = e0 + i >= 0 && e0 + i < V ? base[j * 4 + i] : -INFINITY;
+  for (int i = 0; i < 4; ++i) {
+    const long e = elem(j) + i;
+    w[i] = e >= 0 && e < V ? __float_as_uint(base[j * 4 + i]) : 0xff800000u;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+KORE_DEV void unpack(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+KORE_DEV void unpack(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x);
+  f[1] = __uint_as_float(u.y);
+  f[2] = __uint_as_float(u.z);
+  f[3] = __uint_as_float(u.w);
 }
 KORE_DEV float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 KORE_DEV float to_float(float x) { return x; }
@@ -168,41 +182,40 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   int turn = 0;
   for (long r0 = t0; r0 < t1; r0 += kRows, turn ^= 1) {
     const int n = (int)min((long)kRows, t1 - r0);
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
+    // the rows side by side: a share of the warps to each, so that all are on their way together
+    const int wpr = kWarps / n, i = warp / wpr, sub = warp - i * wpr;
+    if (i < n) {
       const RowView<T> v(logits + (r0 + i) * p.ld, p.V);
       Stat a = {-INFINITY, 0.f, 0x7fffffff};
-      constexpr int U = 4;        // loads in flight
+      constexpr int U = 8;        // loads in flight
+      const long step = nblk * wpr * 32;
+      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
 #pragma unroll 1
-      for (long j0 = rank * kThreads + threadIdx.x; j0 < v.nvec; j0 += U * nblk * kThreads) {
-        float f[U][VE];
+      for (long j0 = (rank * wpr + sub) * 32 + lane; j0 < v.nvec; j0 += U * step) {
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = j0 + u * step < v.nvec ? v.raw(j0 + u * step) : make_uint4(none, none, none, none);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const long j = j0 + u * nblk * kThreads;
-          if (j < v.nvec) {
-            v.load(j, f[u]);
-          } else {
+          float f[VE];
+          unpack(x[u], f);
+          float mx = f[0];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) f[u][e] = -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float mx = f[u][0];
-#pragma unroll
-          for (int e = 1; e < VE; ++e) mx = fmaxf(mx, f[u][e]);
+          for (int e = 1; e < VE; ++e) mx = fmaxf(mx, f[e]);
           if (mx > a.m) {         // rare after the first vectors
             int at = 0;
 #pragma unroll
             for (int e = VE - 1; e >= 0; --e)
-              if (f[u][e] == mx) at = e;
+              if (f[e] == mx) at = e;
             a.s = a.m == -INFINITY ? a.s : a.s * exp2f((a.m - mx) * c);
             a.m = mx;
-            a.at = (int)v.elem(j0 + u * nblk * kThreads) + at;
+            a.at = (int)v.elem(j0 + u * step) + at;
           }
           const float mref = a.m == -INFINITY ? 0.f : a.m;
+          float add[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < VE; ++e) a.s += exp2f((f[u][e] - mref) * c);   // a NaN or +inf makes the sum NaN
+          for (int e = 0; e < VE; ++e) add[e & 1] += exp2f((f[e] - mref) * c);   // a NaN or +inf makes the sum NaN
+          a.s += add[0] + add[1];
         }
       }
 #pragma unroll
@@ -210,12 +223,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
         Stat x = {__shfl_xor_sync(0xffffffff, a.m, o), __shfl_xor_sync(0xffffffff, a.s, o), __shfl_xor_sync(0xffffffff, a.at, o)};
         join(a, x, c);
       }
-      if (lane == 0) part[i][warp] = a;
+      if (lane == 0) part[i][sub] = a;
     }
     __syncthreads();
     if (warp < n && lane == 0) {
       Stat a = part[warp][0];
-      for (int w = 1; w < kWarps; ++w) join(a, part[warp][w], c);
+      for (int w = 1; w < wpr; ++w) join(a, part[warp][w], c);
       mine[turn][warp] = a;
     }
     __syncthreads();
@@ -279,32 +292,56 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   const float* qrow = p.probs && over ? p.probs + row * p.ld_probs : nullptr;
   const double m = rs.m;
   const Exp ex = {tab};
-  auto weight = [&](float z, long e, int mode, double inv_s) -> double {  // mode 0: p s, 1: without the draft, 2: max(0, p - q)
+  auto weight = [&](float z, float q, long e, int mode, double inv_s) -> double {  // mode 0: p s, 1: without the draft, 2: max(0, p - q)
     double w = ex(((double)z - m) * p.inv_tau);
     if (mode == 1 && e == x) w = 0.0;
-    if (mode == 2) w = fmax(w * inv_s - (double)qrow[e], 0.0);
+    if (mode == 2) w = fmax(w * inv_s - (double)q, 0.0);
     return w;
+  };
+  auto draft = [&](long j, float (&q)[VE]) {               // the draft's probabilities of vector j
+    const float* at = qrow + v.elem(j);
+    if (v.whole(j) && ((uintptr_t)at & 15) == 0) {
+#pragma unroll
+      for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(&q[e]) = *reinterpret_cast<const float4*>(at + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) q[e] = v.elem(j) + e >= 0 && v.elem(j) + e < p.V ? at[e] : 0.f;
+    }
   };
   // The cluster's total and the sum of the blocks before this one; group[] gets each warp's part of each step.
   auto sums = [&](int mode, double inv_s, int slot, double& before) -> double {
     double own = 0;
     int step = 0;
+    constexpr int U = 2;          // vectors of a thread in flight
 #pragma unroll 1
-    for (long j0 = lo; j0 < hi; j0 += kThreads, ++step) {
-      const long j = j0 + threadIdx.x;
-      double w = 0;
-      if (j < hi) {
-        float f[VE];
-        v.load(j, f);
+    for (long j0 = lo; j0 < hi; j0 += U * kThreads, step += U) {
+      uint4 z[U];
+      float q[U][VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (f[e] != -INFINITY) w += weight(f[e], v.elem(j) + e, mode, inv_s);
+      for (int u = 0; u < U; ++u) {
+        const long j = j0 + u * kThreads + threadIdx.x;
+        if (j < hi) {
+          z[u] = v.raw(j);
+          if (mode == 2) draft(j, q[u]);
+        }
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffff, w, o);
-      if (lane == 0) {
-        group[step * kWarps + warp] = w;
-        own += w;
+      for (int u = 0; u < U; ++u) {
+        const long j = j0 + u * kThreads + threadIdx.x;
+        double w = 0;
+        if (j < hi) {
+          float f[VE];
+          unpack(z[u], f);
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if (f[e] != -INFINITY) w += weight(f[e], q[u][e], v.elem(j) + e, mode, inv_s);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffff, w, o);
+        if (lane == 0 && j0 + u * kThreads < hi) {
+          group[(step + u) * kWarps + warp] = w;
+          own += w;
+        }
       }
     }
     if (lane == 0) red[warp] = own;
@@ -378,11 +415,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) w[e] = 0;
     if (j < hi) {
-      float f[VE];
-      v.load(j, f);
+      float f[VE], q[VE];
+      unpack(v.raw(j), f);
+      if (mode == 2) draft(j, q);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        w[e] = f[e] != -INFINITY ? weight(f[e], v.elem(j) + e, mode, inv_s) : 0.0;
+        w[e] = f[e] != -INFINITY ? weight(f[e], q[e], v.elem(j) + e, mode, inv_s) : 0.0;
         own += w[e];
       }
     }
