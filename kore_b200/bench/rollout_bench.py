@@ -1,12 +1,13 @@
 """Decode-step benchmark of the rollout engine (CUDA-graph decode loop).
 
-    python -m kore_b200.bench.rollout_bench [--batch 64] [--ctx 4096] [--layers 0]
+    python -m kore_b200.bench.rollout_bench [--batch 64] [--ctx 4096] [--layers 0] [--shared 0]
 
 Times one replay of the captured decode step for ``batch`` sequences whose KV
 history is ``ctx`` tokens, plus its parts in isolation (the decode GEMMs at
 M = batch, the paged attention, the sampler). Prints one JSON line with the
 step time, the bytes a step must read (weights + KV history) and the achieved
-fraction of the measured HBM bandwidth (MEASURED_PEAKS.json).
+fraction of the measured HBM bandwidth (MEASURED_PEAKS.json). ``--shared N``: all
+rows share their first N tokens' pages and the attention reads those once.
 """
 from __future__ import annotations
 
@@ -32,6 +33,7 @@ def main(argv=None):
     ap.add_argument("--ctx", type=int, default=4096)
     ap.add_argument("--nsplit", type=int, default=4)
     ap.add_argument("--iters", type=int, default=20)
+    ap.add_argument("--shared", type=int, default=0)
     args = ap.parse_args(argv)
     cfg = PRESETS[args.model]()
     if args.layers:
@@ -40,21 +42,28 @@ def main(argv=None):
     w = Qwen3Weights(cfg, device="cuda", dtype=torch.bfloat16, seed=0)
     B, L, ps = args.batch, args.ctx, 64
     pages_per = (L + 1 + ps - 1) // ps + 1
-    eng = RolloutEngine(w, max_batch=B, page_size=ps, num_pages=B * pages_per, max_seq_len=L + 2 * ps)
+    eng = RolloutEngine(w, max_batch=B, page_size=ps, num_pages=B * pages_per, max_seq_len=L + 2 * ps,
+                        shared_attention=args.shared > 0)
     for t in eng.cache.k + eng.cache.v:
         t.normal_(0, 1)
     g = DecodeGraph(eng, B, 1 << 20, nsplit=args.nsplit, temperature=1.0)
     for i in range(B):
         g.bt[i, :pages_per] = torch.arange(i * pages_per, (i + 1) * pages_per, dtype=torch.int32)
+    if args.shared:
+        whole = min(args.shared, L) // ps
+        g.bt[:, :whole] = g.bt[:1, :whole]
+        g.groups[0].fill_(B)
+        g.groups[0][0] = 0
+        g.groups[1][0] = whole * ps
     g.pos.fill_(L)
     g.active.fill_(False)   # keep the position fixed: every replay decodes at context L
     g.budget.fill_(1 << 30)
     g.tok.random_(0, cfg.vocab_size)
     g.step()                # capture
-    out = {"batch": B, "ctx": L, "layers": cfg.num_hidden_layers, "nsplit": args.nsplit}
+    out = {"batch": B, "ctx": L, "layers": cfg.num_hidden_layers, "nsplit": args.nsplit, "shared": args.shared}
     out["step_ms"] = median_ms(time_cuda(g.step, args.iters, flush_l2=False))
     wbytes = sum(b.numel() * b.element_size() for b in w.bufs)
-    kvbytes = B * (L + 1) * eng.kv_bytes_per_token()
+    kvbytes = (B * (L + 1) - (B - 1) * (min(args.shared, L) // ps * ps)) * eng.kv_bytes_per_token()
     out["weights_gb"] = round(wbytes / 1e9, 2)
     out["kv_gb"] = round(kvbytes / 1e9, 2)
     peaks = measured_peaks() or {}
@@ -75,9 +84,9 @@ def main(argv=None):
     q = torch.randn(B, eng.hq, eng.D, device="cuda").bfloat16()
     lens = torch.full((B,), L + 1, dtype=torch.int32, device="cuda")
     ms = median_ms(time_cuda(lambda: eng._paged_attention(q, 0, g.bt, lens, g.qs, 1, 1 / math.sqrt(eng.D),
-                                                          g.nsplit, g.part_o, g.part_ml), args.iters))
+                                                          g.nsplit, g.part_o, g.part_ml, g.groups), args.iters))
     parts["attention_ms"] = round(ms, 4)
-    parts["attention_gbs"] = round(B * (L + 1) * eng.kv_bytes_per_token() / cfg.num_hidden_layers / ms / 1e6, 1)
+    parts["attention_gbs"] = round(kvbytes / cfg.num_hidden_layers / ms / 1e6, 1)
     logits = torch.randn(B, cfg.vocab_size, device="cuda").bfloat16()
     tok = torch.empty(B, dtype=torch.long, device="cuda")
     lp = torch.empty(B, device="cuda")

@@ -31,6 +31,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..ops import paged
 from .rollout import GenRequest, RolloutEngine, _Seq
 
 
@@ -64,6 +65,13 @@ class DecodeGraph:
         self.out_tok = torch.zeros(B, max_new, dtype=torch.long, device=dev)
         self.out_lp = torch.zeros(B, max_new, dtype=torch.float32, device=dev)
         self.qs = torch.arange(B + 1, **i32)
+        self.one = torch.ones(B, **i32)
+        self.groups = None                           # shared-prefix attention: (group_start [B + 1], prefix_len [B])
+        if eng.shared_attention:
+            if B > paged.MAX_SEQUENCES:
+                raise ValueError(f"shared_attention: at most {paged.MAX_SEQUENCES} trajectories in a batch")
+            self.groups = (torch.full((B + 1,), B, **i32), torch.zeros(B, **i32))
+            self.groups[0][0] = 0
         self.eos = torch.tensor(sorted(set(int(e) for e in eos_ids)) or [-1], dtype=torch.long, device=dev)
         T, hq, D = B, eng.hq, eng.D
         self.part_o = self.part_ml = None
@@ -80,9 +88,8 @@ class DecodeGraph:
         ps = eng.page_size
         B = self.B
         pos = self.pos
-        page = self.bt.gather(1, torch.div(pos, ps, rounding_mode="floor").long().unsqueeze(1)).squeeze(1)
-        slots = page * ps + torch.remainder(pos, ps)
-        lens = pos + 1
+        step = paged.plan(pos, self.one, self.bt, ps, B)
+        slots, lens = step.slots, step.lens
         qd, kd = eng.hq * eng.D, eng.hkv * eng.D
         x = ops.embed_fwd(self.tok, eng.w.views(0)["embed"])
         scale = 1.0 / math.sqrt(eng.D)
@@ -97,7 +104,7 @@ class DecodeGraph:
             v = qkv[:, qd + kd:].view(B, eng.hkv, eng.D)
             eng._kv_append(k, v, slots, li)
             o = eng._paged_attention(q, li, self.bt, lens, self.qs, 1, scale, self.nsplit, self.part_o,
-                                     self.part_ml)
+                                     self.part_ml, self.groups)
             x = ops.mm(o.reshape(B, qd), W["o"], residual=x)
             hn2 = ops.rmsnorm_fwd(x, W["ln2"], eng.eps)
             a = ops.swiglu_fwd(ops.mm(hn2, W["gate_up"]))
@@ -207,6 +214,9 @@ class MultiTurnRollout:
         g.bt.zero_()
         for i, s in enumerate(seqs):
             g.bt[i, : len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
+        if g.groups is not None:
+            for t, v in zip(g.groups, eng.prefix_groups(seqs, n)):
+                t.copy_(v)
         try:
             for turn in range(num_turns):
                 for i in range(n):

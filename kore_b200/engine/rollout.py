@@ -12,6 +12,12 @@
   paged split-KV attention kernel. Every GEMM is the tcgen05 GEMM.
 * Sampling (temperature, top-p, Gumbel-max) and the sampled token's
   log-prob come from one fused kernel per step.
+* Where a step's rows go (positions, cache slots, row starts) is planned on the
+  device from the sequences' lengths (``ops.paged.plan``).
+* ``shared_attention=True``: multi-token and decode attention read the pages that
+  consecutive sequences share once for all of them (``ops.paged.prefix_attention``).
+* ``generate(draft_tokens=k)``: up to k tokens a sequence are drafted by look-up in
+  its own transcript and verified against the model in one step (``ops.spec``).
 
 The engine reads weights from a :class:`Qwen3Weights` (on one GPU the
 trainer's own buffers, so weight sync is free; with tensor parallelism the
@@ -32,6 +38,7 @@ import torch
 from .. import ops
 from ..models.qwen3 import Qwen3Weights
 from ..ops import attention as attn
+from ..ops import paged, spec
 from ..ops import reference as ref
 
 
@@ -101,7 +108,7 @@ class PagedKVCache:
 class RolloutEngine:
     def __init__(self, weights: Qwen3Weights, *, max_batch: int = 256, page_size: int = 64,
                  num_pages: Optional[int] = None, kv_fraction: float = 0.35, max_seq_len: int = 32768,
-                 split_kv_min: int = 2048):
+                 split_kv_min: int = 2048, shared_attention: bool = False):
         self.w = weights
         c = weights.cfg
         self.cfg = c
@@ -113,11 +120,18 @@ class RolloutEngine:
         self.max_pages_per_seq = (max_seq_len + page_size - 1) // page_size
         self.split_kv_min = split_kv_min
         self.kv_fraction = kv_fraction
+        self.shared_attention = bool(shared_attention)
+        if self.shared_attention:
+            self._check_paged("shared_attention")
         self._num_pages = num_pages
         self._cache: Optional[PagedKVCache] = None
         self.cos, self.sin = ref.rope_tables(c.max_position_embeddings, self.D, c.rope_theta, self.dev)
         self._step = 0
         self._prefix: Dict[object, tuple] = {}
+
+    def _check_paged(self, what: str) -> None:
+        if self.page_size % 8 or self.max_batch > paged.MAX_SEQUENCES:
+            raise ValueError(f"{what}: needs a page_size that is a multiple of 8 and max_batch <= {paged.MAX_SEQUENCES}")
 
     # ------------------------------------------------------------------ KV pool
     def kv_bytes_per_token(self) -> int:
@@ -156,30 +170,25 @@ class RolloutEngine:
         self._cache = None
 
     # ------------------------------------------------------------------ model
-    def _forward(self, seqs: List[_Seq], fresh: bool, want_logits: bool = True):
-        """Feed each sequence's pending tokens; returns last-token logits [B, V]."""
+    def _forward(self, seqs: List[_Seq], fresh: bool, want_logits: bool = True, all_rows: bool = False):
+        """Feed each sequence's pending tokens; returns last-token logits [B, V], or
+        those of every fed token [T, V] and the row starts with ``all_rows``."""
         dev = self.dev
-        toks, pos, slots, q_start, lens = [], [], [], [0], []
-        for s in seqs:
-            n = len(s.pending)
-            toks.extend(s.pending)
-            for j in range(n):
-                p = s.length + j
-                pos.append(p)
-                slots.append(s.pages[p // self.page_size] * self.page_size + p % self.page_size)
-            q_start.append(q_start[-1] + n)
-            lens.append(s.length + n)
-        T = len(toks)
+        toks = [t for s in seqs for t in s.pending]
+        new = [len(s.pending) for s in seqs]
+        lens = [s.length + n for s, n in zip(seqs, new)]
+        T, max_q = len(toks), max(new)
         ids = torch.tensor(toks, dtype=torch.long, device=dev)
-        pos_t = torch.tensor(pos, dtype=torch.int32, device=dev)
-        slots_t = torch.tensor(slots, dtype=torch.int32, device=dev)
-        qs_t = torch.tensor(q_start, dtype=torch.int32, device=dev)
-        lens_t = torch.tensor(lens, dtype=torch.int32, device=dev)
-        max_q = max(len(s.pending) for s in seqs)
         bt = torch.zeros(len(seqs), self.max_pages_per_seq, dtype=torch.int32)
         for i, s in enumerate(seqs):
             bt[i, : len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
         bt = bt.to(dev)
+        ctx, new_t = torch.tensor([[s.length for s in seqs], new], dtype=torch.int32).to(dev)
+        step = paged.plan(ctx, new_t, bt, self.page_size, T)
+        pos_t, slots_t, qs_t, lens_t = step.pos, step.slots, step.q_start, step.lens
+        groups = None
+        if not fresh and (self.shared_attention or all_rows):
+            groups = self.prefix_groups(seqs) if self.shared_attention else (None, None)
         max_len = max(lens)
         nsplit = max(1, min(16, max_len // self.split_kv_min)) if max_q == 1 else 1
         part_o = part_ml = None
@@ -202,7 +211,7 @@ class RolloutEngine:
             if fresh:
                 o, _ = attn.attn_fwd(q, k, v, qs_t, max_q, scale)
             else:
-                o = self._paged_attention(q, li, bt, lens_t, qs_t, max_q, scale, nsplit, part_o, part_ml)
+                o = self._paged_attention(q, li, bt, lens_t, qs_t, max_q, scale, nsplit, part_o, part_ml, groups)
             x = ops.mm(o.reshape(T, qd), W["o"], residual=x)
             hn2 = ops.rmsnorm_fwd(x, W["ln2"], self.eps)
             a = ops.swiglu_fwd(ops.mm(hn2, W["gate_up"]))
@@ -212,19 +221,45 @@ class RolloutEngine:
             s.pending = []
         if not want_logits:
             return None
-        last = qs_t[1:] - 1
-        hl = ops.rmsnorm_fwd(x.index_select(0, last), self.w.views(self.w.num_units - 1)["norm"], self.eps)
-        return ops.mm(hl, self.w.lm_head_weight())
+        if not all_rows:
+            x = x.index_select(0, qs_t[1:] - 1)
+        hl = ops.rmsnorm_fwd(x, self.w.views(self.w.num_units - 1)["norm"], self.eps)
+        logits = ops.mm(hl, self.w.lm_head_weight())
+        return (logits, ids, qs_t) if all_rows else logits
+
+    def prefix_groups(self, seqs: Sequence[_Seq], rows: Optional[int] = None):
+        """(group_start, prefix_len) of consecutive sequences whose tables begin with
+        the same shared pages, for :func:`ops.paged.prefix_attention`; padded to
+        ``rows`` groups (the last ones empty)."""
+        start, length = [], []
+        for i, s in enumerate(seqs):
+            lead = seqs[start[-1]] if start else None
+            n = s.shared_pages
+            if lead is not None and n and lead.pages[:n] == s.pages[:n]:
+                length[-1] = min(length[-1], n) if length[-1] else n
+            else:
+                start.append(i)
+                length.append(0)
+        pad = (rows if rows is not None else len(start)) - len(start)
+        i32 = dict(dtype=torch.int32)
+        return (torch.tensor(start + [len(seqs)] * (pad + 1), **i32).to(self.dev),
+                torch.tensor([n * self.page_size for n in length] + [0] * pad, **i32).to(self.dev))
 
     def _kv_append(self, k, v, slots, li):
         if k.is_cuda:
             ops.native().kv_append(k, v, slots, self.cache.k[li], self.cache.v[li])
         else:
-            self.cache.k[li][slots.long()] = k
-            self.cache.v[li][slots.long()] = v
+            rows = (slots >= 0).nonzero()[:, 0]
+            at = slots[rows].long()
+            self.cache.k[li][at] = k[rows]
+            self.cache.v[li][at] = v[rows]
 
-    def _paged_attention(self, q, li, bt, lens, qs, max_q, scale, nsplit, part_o, part_ml):
+    def _paged_attention(self, q, li, bt, lens, qs, max_q, scale, nsplit, part_o, part_ml, groups=None):
+        """``groups``: (group_start, prefix_len), possibly (None, None), runs the shared-prefix attention."""
         T = q.shape[0]
+        if groups is not None:
+            return paged.prefix_attention(q, self.cache.k[li], self.cache.v[li], bt, lens, qs, self.page_size, max_q=max_q,
+                                          scale=scale, group_start=groups[0], prefix_len=groups[1])[0]
         if q.is_cuda:
             out = torch.empty(T, self.hq, self.D, dtype=q.dtype, device=q.device)
             ops.native().paged_attention(q, self.cache.k[li], self.cache.v[li], bt, lens, qs, int(max_q),
@@ -247,8 +282,21 @@ class RolloutEngine:
     # ------------------------------------------------------------------ public
     @torch.no_grad()
     def generate(self, requests: List[GenRequest], *, temperature: float = 1.0, top_p: float = 1.0,
-                 eos_ids: Sequence[int] = (), seed: int = 0) -> List[GenResult]:
-        """Continuous-batching generation of every request."""
+                 eos_ids: Sequence[int] = (), seed: int = 0, draft_tokens: int = 0, draft_ngram: int = 3
+                 ) -> List[GenResult]:
+        """Continuous-batching generation of every request.
+
+        ``draft_tokens``: a decode step feeds up to that many drafted tokens more per
+        sequence (the continuation of the last earlier place in its transcript that
+        ends in the same ``draft_ngram`` tokens) and keeps those that the model
+        accepts: the tokens are distributed as without, in fewer steps where the
+        transcript repeats itself. Needs top_p = 1."""
+        if draft_tokens < 0 or draft_ngram < 1:
+            raise ValueError("generate: draft_tokens must not be negative and draft_ngram positive")
+        if draft_tokens:
+            if top_p < 1.0:
+                raise ValueError("generate: drafted tokens are verified against the whole distribution (top_p = 1)")
+            self._check_paged("draft_tokens")
         waiting = list(requests)
         active: List[_Seq] = []
         done: Dict[int, GenResult] = {}
@@ -268,7 +316,9 @@ class RolloutEngine:
                     raise RuntimeError("KV cache too small for the next request")
                 break
             decoding = [s for s in active if s.pending and s not in admitted]
-            if decoding:
+            if decoding and draft_tokens:
+                self._drafted_step(decoding, temperature, seed, eos, draft_tokens, draft_ngram)
+            elif decoding:
                 logits = self._forward(decoding, fresh=False)
                 self._emit(decoding, logits, temperature, top_p, seed, eos)
             for s in list(active):
@@ -284,21 +334,58 @@ class RolloutEngine:
         tok_l = tok.tolist()
         lp_l = lp.tolist()
         for s, t, l in zip(seqs, tok_l, lp_l):
-            s.out.append(int(t))
-            s.logps.append(float(l))
-            if int(t) in eos:
-                s.done, s.reason = True, "stop"
-            elif len(s.out) >= s.req.max_new_tokens:
-                s.done, s.reason = True, "length"
-            else:
-                s.pending = [int(t)]
-                need = (s.length + 1 + self.page_size - 1) // self.page_size
-                if need > len(s.pages):
-                    p = self.cache.alloc(need - len(s.pages))
-                    if p is None:       # out of pages: stop this sequence
-                        s.done, s.reason = True, "kv_full"
-                    else:
-                        s.pages.extend(p)
+            self._take(s, int(t), float(l), eos)
+
+    def _take(self, s: _Seq, t: int, l: float, eos) -> None:
+        """Append one generated token: the sequence ends, or feeds it next."""
+        s.out.append(t)
+        s.logps.append(l)
+        if t in eos:
+            s.done, s.reason = True, "stop"
+        elif len(s.out) >= s.req.max_new_tokens:
+            s.done, s.reason = True, "length"
+        else:
+            s.pending = [t]
+            need = (s.length + 1 + self.page_size - 1) // self.page_size
+            if need > len(s.pages):
+                p = self.cache.alloc(need - len(s.pages))
+                if p is None:       # out of pages: stop this sequence
+                    s.done, s.reason = True, "kv_full"
+                else:
+                    s.pages.extend(p)
+
+    def _drafted_step(self, seqs, temperature, seed, eos, k, ngram):
+        """One decode step with drafts: feed the pending token and its drafts, verify,
+        keep what was accepted (the cache's length goes back behind it)."""
+        start = []
+        for s in seqs:
+            room = min(k, s.req.max_new_tokens - len(s.out) - 1, self.max_pages_per_seq * self.page_size - s.length - 1)
+            drafts = spec.lookup(s.req.prompt + s.out, room, ngram)
+            need = -(-(s.length + 1 + len(drafts)) // self.page_size) - len(s.pages)
+            if need > 0:
+                got = self.cache.alloc(need)
+                if got is None:
+                    drafts = drafts[: len(s.pages) * self.page_size - s.length - 1]
+                else:
+                    s.pages.extend(got)
+            s.pending = s.pending + drafts
+            start.append((s.length, list(s.pending)))
+        logits, ids, q_start = self._forward(seqs, fresh=False, all_rows=True)
+        self._step += 1
+        g = torch.Generator(device=self.dev).manual_seed((int(seed) * 1000003 + self._step) & 0x7FFFFFFF)
+        u = torch.rand(ids.numel(), 2, generator=g, device=self.dev)
+        v = spec.verify(logits, ids, q_start, u, max(float(temperature), 0.0))
+        acc, nxt, lp = v.accepted.tolist(), v.next.tolist(), v.logp.tolist()
+        row = 0
+        for s, a, y, (length, fed) in zip(seqs, acc, nxt, start):
+            if y < 0:
+                raise RuntimeError("generate: a row of logits has no distribution (NaN or infinite)")
+            for j, t in enumerate(fed[1: 1 + a] + [y]):
+                s.length, s.pending = length + 1 + j, []
+                self._take(s, int(t), float(lp[row + j]), eos)
+                if s.done:
+                    break
+            row += len(fed)
 
     def _admit(self, waiting: List[GenRequest], active: List[_Seq]) -> List[_Seq]:
         out = []

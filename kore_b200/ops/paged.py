@@ -15,6 +15,8 @@ import torch
 
 from ._lib import native
 
+MAX_SEQUENCES = 512                    # of one prefix_attention call on CUDA
+
 
 @dataclass
 class Plan:

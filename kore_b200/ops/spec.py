@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -17,6 +17,19 @@ class Verdict:
     accepted: torch.Tensor   # [B] int32: drafts accepted
     next: torch.Tensor       # [B] int64: the token after them
     logp: torch.Tensor       # [T] fp32: log-probs of the accepted drafts and of ``next``, row by row
+
+
+def lookup(tokens: Sequence[int], k: int, ngram: int = 3) -> List[int]:
+    """Up to k draft tokens for the end of ``tokens``: what followed the last earlier
+    place with the same ``ngram`` last tokens (fewer, down to one, where none has)."""
+    if k <= 0:
+        return []
+    for n in range(min(ngram, len(tokens) - 1), 0, -1):
+        tail = list(tokens[-n:])
+        for i in range(len(tokens) - n - 1, -1, -1):
+            if tokens[i] == tail[0] and list(tokens[i:i + n]) == tail:
+                return list(tokens[i + n:i + n + k])
+    return []
 
 
 def verify(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, u: torch.Tensor,

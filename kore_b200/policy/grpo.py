@@ -112,7 +112,8 @@ class GRPOTrainer:
         if self.ref_eng is not None and self.ref_stream is not None:
             self.ref_eng.param_hook = self.ref_stream
         rk = dict(max_batch=config.rollout_max_batch, page_size=min(config.kv_page_size, 128),
-                  kv_fraction=config.kv_cache_fraction)
+                  kv_fraction=config.kv_cache_fraction,
+                  shared_attention=getattr(config, "rollout_shared_attention", False))
         rk.update(rollout_kwargs or {})
         self.rollout = RolloutEngine(self.w, **rk)
         self.step_idx = 0
@@ -193,7 +194,8 @@ class GRPOTrainer:
                 for j in range(ncand):
                     reqs.append(GenRequest(prompt=c, max_new_tokens=max_new, rid=i * ncand + j, share_key=key))
             outs = self.rollout.generate(reqs, temperature=cfg.temperature, top_p=cfg.top_p,
-                                         eos_ids=self.eos, seed=cfg.seed * 1000003 + self.step_idx * 97 + turn)
+                                         eos_ids=self.eos, seed=cfg.seed * 1000003 + self.step_idx * 97 + turn,
+                                         draft_tokens=getattr(cfg, "rollout_draft_tokens", 0))
             for i, tr in enumerate(trajs):
                 cands = outs[i * ncand:(i + 1) * ncand]
                 if ncand == 1:

@@ -21,7 +21,7 @@ from typing import Callable, List, Optional, Sequence
 
 class KorePolicy:
     def __init__(self, model_path: str, *, device: str = "cuda", max_batch: int = 64, temperature: float = 0.0,
-                 top_p: float = 1.0, max_new_tokens: int = 2048, weights=None, tokenizer=None):
+                 top_p: float = 1.0, max_new_tokens: int = 2048, weights=None, tokenizer=None, draft_tokens: int = 0):
         import torch
         from ..data.tokenizer import eos_ids, load_tokenizer
         from ..engine.rollout import RolloutEngine
@@ -30,12 +30,13 @@ class KorePolicy:
         self.w = weights if weights is not None else from_pretrained(model_path, device=device, dtype=torch.bfloat16)
         self.eng = RolloutEngine(self.w, max_batch=max_batch)
         self.eos = eos_ids(self.tok)
-        self.temperature, self.top_p, self.max_new = temperature, top_p, max_new_tokens
+        self.temperature, self.top_p, self.max_new, self.draft_tokens = temperature, top_p, max_new_tokens, draft_tokens
 
     def generate_ids(self, prompts: Sequence[List[int]], max_new_tokens: Optional[int] = None, seed: int = 0):
         from ..engine.rollout import GenRequest
         reqs = [GenRequest(list(p), max_new_tokens or self.max_new) for p in prompts]
-        return self.eng.generate(reqs, temperature=self.temperature, top_p=self.top_p, eos_ids=self.eos, seed=seed)
+        return self.eng.generate(reqs, temperature=self.temperature, top_p=self.top_p, eos_ids=self.eos, seed=seed,
+                                 draft_tokens=self.draft_tokens)
 
     def chat(self, conversations: Sequence[List[dict]], **kw) -> List[str]:
         from ..data.tokenizer import render_chat
