@@ -47,6 +47,16 @@ def test_plan_sizes(B, new, ps, short):
     assert wide[:, :M].tolist() == want["table"] and (wide[:, M:] == -7).all()
 
 
+def test_plan_without_sequences_and_with_wide_numbers():
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    p = paged.plan(none, none, torch.empty(0, 4, dtype=torch.int32, device="cuda"), 16, 3)
+    assert p.q_start.tolist() == [0] and p.pos.tolist() == [0] * 3 and p.slots.tolist() == [-1] * 3 and p.lens.numel() == 0
+    big = 2 ** 31 - 1                                  # lengths that fit no table
+    p = paged.plan(_i([big, 5, big]), _i([1, 1, big]), torch.zeros(3, 4, dtype=torch.int32, device="cuda"), 16, 4)
+    assert p.ok.tolist() == [False, True, False] and p.lens.tolist() == [big, 6, big]
+    assert p.q_start.tolist() == [0, 1, 2, 4] and p.slots.tolist() == [-1, 5, -1, -1]
+
+
 def test_plan_captured():
     """Captured and replayed over its own results: each replay appends a token to every sequence."""
     ps, B, steps = 16, 5, 40
@@ -321,7 +331,7 @@ def test_refusals():
     bad = [dict(q=a["q"].float()), dict(q=a["q"][:, :7]), dict(q=a["q"][..., :64]), dict(q=a["q"].cpu().cuda()[:, ::2]),
            dict(k_cache=a["k_cache"][:, :1]), dict(v_cache=a["v_cache"].half()), dict(k_cache=a["k_cache"].cpu()),
            dict(table=a["table"].long()), dict(table=a["table"][:1]), dict(table=a["table"].t().contiguous().t()),
-           dict(lens=a["lens"].long()), dict(q_start=a["q_start"][1:]), dict(page_size=12), dict(page_size=0), dict(max_q=0),
+           dict(lens=a["lens"].long()), dict(q_start=a["q_start"][1:]), dict(page_size=12), dict(page_size=0), dict(max_q=0), dict(scale=0.0), dict(scale=-1.0),
            dict(group_start=None), dict(prefix_len=None), dict(prefix_len=_i([1, 2])),
            dict(group_start=_i([0, 1, 2, 3, 3]), prefix_len=_i([0] * 4)),
            dict(out=torch.empty(3, 8, 128, device="cuda")), dict(out=torch.empty(2, 8, 128, dtype=torch.bfloat16, device="cuda"))]

@@ -148,6 +148,12 @@ def test_refusals():
         spec.verify(z, tokens, qs, u, -0.5)
 
 
+def test_sequences_without_any_rows():
+    z, tokens, _, u, _ = verify_case(9, 50, [2], device="cuda")
+    v = spec.verify(z[:0], tokens[:0], _i([0, 0, 0]), u[:0])
+    assert v.accepted.tolist() == [0, 0] and v.next.tolist() == [-1, -1] and v.logp.numel() == 0
+
+
 def test_no_sequences():
     z, tokens, qs, u, _ = verify_case(9, 50, [2], device="cuda")
     v = spec.verify(z, tokens, qs[:1].contiguous(), u)
