@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <algorithm>
 #include <tuple>
 
 #include "common.cuh"
@@ -27,9 +28,11 @@ namespace verify {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 8;     // of a sequence: a cluster, each with a part of the vocabulary
-constexpr int kRows = 8;          // rows whose statistics are taken together
+constexpr int kStatThreads = 256;
+constexpr int kMaxParts = 16;     // of a row's statistics
 constexpr int kMaxSteps = 257;    // vectors of a thread in the drawing pass, by one block alone
 
+struct Stat;
 struct Params {
   const void* logits;
   long ld, V;
@@ -39,12 +42,13 @@ struct Params {
   const float* probs;             // [T, V] or null
   long ld_probs;
   long B, T;
-  int blocks;                     // of a sequence
+  int blocks, parts;              // blocks of a sequence in the draw, of a row in the statistics
   double inv_tau;                 // 1 when greedy
   bool greedy;
   int* accepted;
   long* next;
   float* logp;
+  Stat* stats;             // [T, parts]
 };
 
 // A row as vectors of VE elements that start on 16-byte boundaries: the first
@@ -151,17 +155,75 @@ struct Exp {
   }
 };
 
-// One cluster of p.blocks blocks per sequence.
+// Statistics of the rows, p.parts blocks to each (all rows at once: a pass over the logits
+// that fills the SMs whatever the shape of the batch).
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) stats_kernel(Params p) {
+  constexpr int VE = RowView<T>::VE;
+  constexpr int U = sizeof(T) == 2 ? 4 : 8;     // loads of a thread in flight
+  __shared__ Stat part[kStatThreads / 32];
+  pdl_trigger();
+  const long row = blockIdx.x / p.parts;
+  const int own = blockIdx.x - (int)(row * p.parts), warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const float c = (float)(p.inv_tau * 1.4426950408889634);
+  const RowView<T> v(static_cast<const T*>(p.logits) + row * p.ld, p.V);
+  const long step = (long)p.parts * kStatThreads;
+  const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
+  Stat a = {-INFINITY, 0.f, 0x7fffffff};
+#pragma unroll 1
+  for (long j0 = own * kStatThreads + threadIdx.x; j0 < v.nvec; j0 += U * step) {
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = j0 + u * step < v.nvec ? v.raw(j0 + u * step) : make_uint4(none, none, none, none);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VE];
+      unpack(x[u], f);
+      float mx = f[0];
+#pragma unroll
+      for (int e = 1; e < VE; ++e) mx = fmaxf(mx, f[e]);
+      if (mx > a.m) {             // rare after the first vectors
+        int at = 0;
+#pragma unroll
+        for (int e = VE - 1; e >= 0; --e)
+          if (f[e] == mx) at = e;
+        a.s = a.m == -INFINITY ? a.s : a.s * exp2f((a.m - mx) * c);
+        a.m = mx;
+        a.at = (int)v.elem(j0 + u * step) + at;
+      }
+      const float mref = a.m == -INFINITY ? 0.f : a.m;
+      float add[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < VE; ++e) add[e & 1] += exp2f((f[e] - mref) * c);   // a NaN or +inf makes the sum NaN
+      a.s += add[0] + add[1];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat x = {__shfl_xor_sync(0xffffffff, a.m, o), __shfl_xor_sync(0xffffffff, a.s, o), __shfl_xor_sync(0xffffffff, a.at, o)};
+    join(a, x, c);
+  }
+  if (lane == 0) part[warp] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kStatThreads / 32; ++w) join(a, part[w], c);
+    p.stats[blockIdx.x] = a;
+  }
+}
+
+// One cluster of p.blocks blocks per sequence: accepts, then draws.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   constexpr int VE = RowView<T>::VE;
-  __shared__ Stat part[kRows][kWarps], mine[2][kRows], stat[kRows];
+  __shared__ Stat s_stat;
   __shared__ double red[kWarps], group[kMaxSteps * kWarps], total_of[3], tab[32];
-  __shared__ int s_stop;
+  __shared__ long s_row;
   const int nblk = p.blocks;
   const long b = blockIdx.x / nblk;
   const uint32_t rank = cluster_ctarank();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) tab[threadIdx.x] = exp2((double)threadIdx.x / 32);
+  pdl_wait();
   const long t0 = min(max((long)p.q_start[b], 0L), p.T), t1 = min(max((long)p.q_start[b + 1], t0), p.T);
   const T* logits = static_cast<const T*>(p.logits);
   const float c = (float)(p.inv_tau * 1.4426950408889634);
@@ -175,78 +237,16 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
     }
     return;
   }
-  if (threadIdx.x < 32) tab[threadIdx.x] = exp2((double)threadIdx.x / 32);
-  long row = t1;                  // the row that gives the next token
-  Stat rs = {-INFINITY, 0.f, 0};
-  bool good = false;
-  int turn = 0;
-  for (long r0 = t0; r0 < t1; r0 += kRows, turn ^= 1) {
-    const int n = (int)min((long)kRows, t1 - r0);
-    // the rows side by side: a share of the warps to each, so that all are on their way together
-    const int wpr = kWarps / n, i = warp / wpr, sub = warp - i * wpr;
-    if (i < n) {
-      const RowView<T> v(logits + (r0 + i) * p.ld, p.V);
+  if (warp == 0) {                // a row to a lane, 32 rows at a time, until one stops
+    long row = -1;
+    for (long r0 = t0; r0 < t1 && row < 0; r0 += 32) {
+      const long t = r0 + lane;
       Stat a = {-INFINITY, 0.f, 0x7fffffff};
-      constexpr int U = 8;        // loads in flight
-      const long step = nblk * wpr * 32;
-      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
-#pragma unroll 1
-      for (long j0 = (rank * wpr + sub) * 32 + lane; j0 < v.nvec; j0 += U * step) {
-        uint4 x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = j0 + u * step < v.nvec ? v.raw(j0 + u * step) : make_uint4(none, none, none, none);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float f[VE];
-          unpack(x[u], f);
-          float mx = f[0];
-#pragma unroll
-          for (int e = 1; e < VE; ++e) mx = fmaxf(mx, f[e]);
-          if (mx > a.m) {         // rare after the first vectors
-            int at = 0;
-#pragma unroll
-            for (int e = VE - 1; e >= 0; --e)
-              if (f[e] == mx) at = e;
-            a.s = a.m == -INFINITY ? a.s : a.s * exp2f((a.m - mx) * c);
-            a.m = mx;
-            a.at = (int)v.elem(j0 + u * step) + at;
-          }
-          const float mref = a.m == -INFINITY ? 0.f : a.m;
-          float add[2] = {0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < VE; ++e) add[e & 1] += exp2f((f[e] - mref) * c);   // a NaN or +inf makes the sum NaN
-          a.s += add[0] + add[1];
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        Stat x = {__shfl_xor_sync(0xffffffff, a.m, o), __shfl_xor_sync(0xffffffff, a.s, o), __shfl_xor_sync(0xffffffff, a.at, o)};
-        join(a, x, c);
-      }
-      if (lane == 0) part[i][sub] = a;
-    }
-    __syncthreads();
-    if (warp < n && lane == 0) {
-      Stat a = part[warp][0];
-      for (int w = 1; w < wpr; ++w) join(a, part[warp][w], c);
-      mine[turn][warp] = a;
-    }
-    __syncthreads();
-    cluster_sync();               // `mine` of the turn before the last is read by nobody any more
-    if (warp == 0) {
-      bool stop = false;
-      if (lane < n) {
-        Stat a = {-INFINITY, 0.f, 0x7fffffff};
-#pragma unroll 1
-        for (int k = 0; k < nblk; ++k) {
-          const Stat* s = &mine[turn][lane];
-          const Stat x = {__uint_as_float(peer_u32(&s->m, k)), __uint_as_float(peer_u32(&s->s, k)), (int)peer_u32(&s->at, k)};
-          join(a, x, c);
-        }
-        stat[lane] = a;
-        const long t = r0 + lane;
+      bool stop = t < t1;
+      float logp = 0.f;
+      if (t < t1) {
+        for (int k = 0; k < p.parts; ++k) join(a, p.stats[t * p.parts + k], c);
         const bool fine = a.s > 0.f && a.s < INFINITY;     // a distribution: neither empty nor NaN nor +inf
-        stop = true;
         if (fine && t + 1 < t1) {
           const long x = p.tokens[t + 1];
           if (x >= 0 && x < p.V) {
@@ -255,26 +255,26 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
             const double qx = p.probs ? (double)p.probs[t * p.ld_probs + x] : 1.0;
             if (p.greedy ? x == a.at : (double)p.u[2 * t] * qx < px) {
               stop = false;
-              if (first) part[lane][0].s = (float)(zx - log((double)a.s));   // its log-prob, if no row before it stops
+              logp = (float)(zx - log((double)a.s));
             }
           }
         }
       }
       const unsigned bad = __ballot_sync(0xffffffff, stop);
-      const int end = bad ? __ffs(bad) - 1 : n;
-      if (first && lane < end) p.logp[r0 + lane] = part[lane][0].s;
-      if (lane == 0) s_stop = bad ? end : -1;
+      const int end = bad ? __ffs(bad) - 1 : 32;
+      if (first && lane < end && t < t1) p.logp[t] = logp;
+      if (bad) {
+        row = r0 + end;
+        if (lane == end) s_stat = a;
+      }
     }
-    __syncthreads();
-    if (s_stop >= 0) {
-      row = r0 + s_stop;
-      rs = stat[s_stop];
-      good = rs.s > 0.f && rs.s < INFINITY;
-      break;
-    }
+    if (lane == 0) s_row = row;
   }
-  if (first)
-    for (long t = row + 1 + threadIdx.x; t < t1; t += kThreads) p.logp[t] = 0.f;
+  __syncthreads();
+  const long row = s_row;         // the row that gives the next token
+  const Stat rs = s_stat;
+  const bool good = rs.s > 0.f && rs.s < INFINITY;
+  for (long t = row + 1 + threadIdx.x; t < t1; t += kThreads) p.logp[t] = 0.f;
   const bool over = row + 1 < t1;                          // a draft was rejected
   const long x = over ? p.tokens[row + 1] : -1;
   if (!good || p.greedy) {
@@ -283,17 +283,16 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
       p.next[b] = good ? rs.at : -1;
       p.logp[row] = good ? (float)-log((double)rs.s) : NAN;
     }
-    cluster_sync();                                        // peers have read this block's statistics
     return;
   }
   // ---- the draw: weights in fp64, summed in the order of the vocabulary, a part to a block
   const RowView<T> v(logits + row * p.ld, p.V);
   const long per = (v.nvec + nblk - 1) / nblk, lo = min(rank * per, v.nvec), hi = min(lo + per, v.nvec);
   const float* qrow = p.probs && over ? p.probs + row * p.ld_probs : nullptr;
-  const double m = rs.m;
+  const double m = rs.m, shift = -m * p.inv_tau;
   const Exp ex = {tab};
   auto weight = [&](float z, float q, long e, int mode, double inv_s) -> double {  // mode 0: p s, 1: without the draft, 2: max(0, p - q)
-    double w = ex(((double)z - m) * p.inv_tau);
+    double w = ex(fma((double)z, p.inv_tau, shift));
     if (mode == 1 && e == x) w = 0.0;
     if (mode == 2) w = fmax(w * inv_s - (double)q, 0.0);
     return w;
@@ -363,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   };
   int mode = over && !qrow ? 1 : 0, slot = 0;
   double before, total = sums(mode, 1.0, slot, before), s64 = total;
-  if (mode == 1 && x >= 0 && x < p.V) s64 += ex(((double)to_float(logits[row * p.ld + x]) - m) * p.inv_tau);
+  if (mode == 1 && x >= 0 && x < p.V) s64 += ex(fma((double)to_float(logits[row * p.ld + x]), p.inv_tau, shift));
   const double inv_s = 1.0 / s64;
   if (qrow) {
     mode = 2;
@@ -484,6 +483,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
   at::Tensor accepted = at::empty({B}, q_start.options()), next = at::empty({B}, tokens.options()),
              logp = at::empty({T}, u.options());
   if (B == 0) return {accepted, next, logp.zero_()};
+  if (T == 0) return {accepted.zero_(), next.fill_(-1), logp};
+  TORCH_CHECK(T < (int64_t)1 << 27, "verify: too many rows");
   Params p;
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
@@ -505,17 +506,26 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
   const int room = 2 * num_sms(logits.get_device());
   p.blocks = 1;
   while (p.blocks < kMaxBlocks && B * p.blocks * 2 <= room) p.blocks *= 2;
+  // Statistics: eight blocks to an SM, each thread with a vector at least.
+  p.parts = (int)std::min<int64_t>(kMaxParts, std::max<int64_t>(1, std::min<int64_t>(4 * room / T, V / (8 * kStatThreads))));
+  at::Tensor stats = at::empty({T * p.parts, 3}, u.options());
+  p.stats = reinterpret_cast<Stat*>(stats.data_ptr<float>());
+  const bool f32 = logits.scalar_type() == at::kFloat;
+  auto st = at::cuda::getCurrentCUDAStream();
+  (f32 ? stats_kernel<float> : stats_kernel<__nv_bfloat16>)<<<(unsigned)(T * p.parts), kStatThreads, 0, st>>>(p);
+  check_cuda(cudaGetLastError(), "verify statistics");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * p.blocks));
   cfg.blockDim = dim3(kThreads);
-  cfg.stream = at::cuda::getCurrentCUDAStream();
-  cudaLaunchAttribute attr[1];
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const bool f32 = logits.scalar_type() == at::kFloat;
+  cfg.numAttrs = 2;
   check_cuda(cudaLaunchKernelEx(&cfg, f32 ? verify_kernel<float> : verify_kernel<__nv_bfloat16>, p), "verify");
   return {accepted, next, logp};
 }
