@@ -7,8 +7,8 @@
 //                       shares are read and scored once for all their rows
 //
 // Measured on one B200 (bf16, D = 128, 40 query and 8 kv heads; times of whole calls):
-//   plan, 64 x 1 rows: 4.6 us on the device, 14 with its host side; 523k rows of 256
-//   prompts: 20 us. prefix_attention, 8 groups x 8 sequences, prefixes of 512 to 1024 and
+//   plan, 64 x 1 rows: 5 us on the device, 14 with its host side; 523k rows of 256
+//   prompts: 16 us. prefix_attention, 8 groups x 8 sequences, prefixes of 512 to 1024 and
 //   own keys of 432 to 6912 tokens: 127 us = 4.9 TB/s of the keys read once; one group of
 //   256 on 16,384 shared tokens: 221 us = 400 TFLOP/s; 4 sequences of 260 tokens: 14 us.
 #include <ATen/ATen.h>
@@ -63,34 +63,45 @@ KORE_DEV long block_scan(long v, long* part, long& total) {
   return v + (w ? before : 0);
 }
 
-// Row t's position and slot; q_start in global or shared memory.
-KORE_DEV void plan_row(const PlanParams& p, const int* q_start, long t) {
-  long lo = 0, hi = p.B;                // the sequence with q_start[b] <= t < q_start[b + 1]
-  while (lo < hi) {
-    const long mid = (lo + hi) >> 1;
-    if (q_start[mid + 1] <= t) lo = mid + 1; else hi = mid;
+// Positions and slots of rows t .. t + N - 1; q_start in global or shared memory.
+template <int N>
+KORE_DEV void plan_rows(const PlanParams& p, const int* q_start, long t) {
+  int b = 0, hi = (int)p.B;             // the sequence with q_start[b] <= t < q_start[b + 1]
+  while (b < hi) {
+    const int mid = (int)(((unsigned)b + (unsigned)hi) >> 1);
+    if (q_start[mid + 1] <= t) b = mid + 1; else hi = mid;
   }
-  if (lo == p.B) {                      // behind the last sequence
-    p.pos[t] = 0;
-    p.slots[t] = -1;
-    return;
+  int pos[N], slot[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    while (b < p.B && q_start[b + 1] <= t + i) ++b;
+    pos[i] = 0;                         // behind the last sequence
+    slot[i] = -1;
+    if (b == p.B || t + i >= p.rows) continue;
+    pos[i] = max(p.ctx[b], 0) + (int)(t + i - q_start[b]);
+    if (!p.ok[b]) continue;
+    const int at = (unsigned)pos[i] / (unsigned)p.page_size, page = p.table[b * p.ld_table + at];
+    const long s = (long)page * p.page_size + (pos[i] - at * p.page_size);
+    if (page >= 0 && s <= 0x7fffffffL) slot[i] = (int)s;
   }
-  const int pos = max(p.ctx[lo], 0) + (int)(t - q_start[lo]), at = (unsigned)pos / (unsigned)p.page_size;
-  p.pos[t] = pos;
-  long slot = -1;
-  if (p.ok[lo]) {
-    const int page = p.table[lo * p.ld_table + at];
-    slot = (long)page * p.page_size + (pos - at * p.page_size);
-    if (page < 0 || slot > 0x7fffffffL) slot = -1;
+  if (N == 4 && t + 4 <= p.rows) {
+    *reinterpret_cast<int4*>(p.pos + t) = make_int4(pos[0], pos[N / 4], pos[N / 2], pos[N - 1]);
+    *reinterpret_cast<int4*>(p.slots + t) = make_int4(slot[0], slot[N / 4], slot[N / 2], slot[N - 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (t + i < p.rows) {
+        p.pos[t + i] = pos[i];
+        p.slots[t + i] = slot[i];
+      }
   }
-  p.slots[t] = (int)slot;
 }
 
 // One block: rows' starts and granted pages are running sums over the sequences. With
 // `map_rows` (B <= 1024) it goes on to the rows.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p, bool map_rows) {
   __shared__ long part[32];
-  __shared__ int starts[kPlanThreads + 1], granted;
+  __shared__ int starts[kPlanThreads + 1], granted, asks[kPlanThreads], holds[kPlanThreads];
   pdl_trigger();
   const int count = p.free_stack ? (int)min((long)max(*p.free_count, 0), p.nfree) : 0;
   long rows = 0, asked = 0, total;
@@ -114,29 +125,46 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p, bool m
       upto = block_scan(take, part, total) + asked;
       asked += total;
     }
-    if (!in) continue;
     const bool ok = fits && upto <= count;
     const int got = ok ? (int)take : 0;
-    if (got) atomicMax(&granted, (int)upto);         // granted sequences are a prefix of those that ask
-    for (int j = 0; j < got; ++j)
-      p.table[b * p.ld_table + held + j] = p.free_stack[count - 1 - (upto - take) - j];
-    const int end = (int)min(to, p.rows);
-    p.q_start[b + 1] = end;
-    if (b0 == 0) starts[b + 1] = end;
-    p.lens[b] = ok ? (int)(ctx + n) : ctx;
-    p.ok[b] = ok;
-    p.held_out[b] = (int)held + got;
+    if (in) {
+      if (got) atomicMax(&granted, (int)upto);       // granted sequences are a prefix of those that ask
+      const int end = (int)min(to, p.rows);
+      p.q_start[b + 1] = end;
+      if (b0 == 0) starts[b + 1] = end;
+      p.lens[b] = ok ? (int)(ctx + n) : ctx;
+      p.ok[b] = ok;
+      p.held_out[b] = (int)held + got;
+    }
+    if (p.free_stack) {
+      // pages to threads, not sequences to threads: a long prompt alone may ask for hundreds
+      const long before = asked - total;
+      asks[threadIdx.x] = (int)min(upto - before, (long)count + 1);
+      holds[threadIdx.x] = (int)held;
+      __syncthreads();
+      const int most = (int)min(total, count - before);
+      for (int k = threadIdx.x; k < most; k += kPlanThreads) {
+        int lo = 0, hi = kPlanThreads - 1;           // whose page k of this round is
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (asks[mid] <= k) lo = mid + 1; else hi = mid;
+        }
+        if (before + asks[lo] > count) continue;     // not granted
+        const int j = k - (lo ? asks[lo - 1] : 0);
+        p.table[(b0 + lo) * p.ld_table + holds[lo] + j] = p.free_stack[count - 1 - before - k];
+      }
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0 && p.count_out) *p.count_out = count - granted;
   if (map_rows)
-    for (long t = threadIdx.x; t < p.rows; t += kPlanThreads) plan_row(p, starts, t);
+    for (long t = threadIdx.x; t < p.rows; t += kPlanThreads) plan_rows<1>(p, starts, t);
 }
 
 __global__ void __launch_bounds__(256) plan_rows_kernel(PlanParams p) {
   pdl_wait();
-  const long t = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (t < p.rows) plan_row(p, p.q_start, t);
+  const long t = 4 * ((long)blockIdx.x * blockDim.x + threadIdx.x);      // four rows to a search
+  if (t < p.rows) plan_rows<4>(p, p.q_start, t);
 }
 
 // -------------------------------------------------------- prefix attention
@@ -1175,7 +1203,7 @@ paged_plan(const at::Tensor& ctx, const at::Tensor& new_toks, at::Tensor& table,
   const bool map_rows = B <= kPlanThreads && rows <= kPlanRows;
   plan_kernel<<<1, kPlanThreads, 0, st>>>(p, map_rows);
   check_cuda(cudaGetLastError(), "paged_plan");
-  if (!map_rows) launch_after("paged_plan rows", plan_rows_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, p);
+  if (!map_rows) launch_after("paged_plan rows", plan_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), 0, st, p);
   return {q_start, lens, pos, slots, ok, held_out, count_out};
 }
 
