@@ -151,7 +151,7 @@ struct Exp {
     const int n = __double2loint(t);
     const double r = fma(t - 6755399441055744.0, -0.6931471805599453 / 32, x);
     const double e = fma(fma(fma(fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0) * tab[n & 31];
-    return __hiloint2double(__double2hiint(e) + (n >> 5) * (1 << 20), __double2loint(e));
+    return __hiloint2double(__double2hiint(e) + (int)((unsigned)(n & ~31) << 15), __double2loint(e));
   }
 };
 
@@ -291,11 +291,22 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   const float* qrow = p.probs && over ? p.probs + row * p.ld_probs : nullptr;
   const double m = rs.m, shift = -m * p.inv_tau;
   const Exp ex = {tab};
-  auto weight = [&](float z, float q, long e, int mode, double inv_s) -> double {  // mode 0: p s, 1: without the draft, 2: max(0, p - q)
-    double w = ex(fma((double)z, p.inv_tau, shift));
-    if (mode == 1 && e == x) w = 0.0;
-    if (mode == 2) w = fmax(w * inv_s - (double)q, 0.0);
-    return w;
+  const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
+  // Weights of a vector's tokens: p s (mode 0), without the draft (1), max(0, p - q) (2).
+  auto weights = [&](long j, const uint4& z, const float (&q)[VE], int mode, double inv_s, double (&w)[VE]) {
+    float f[VE];
+    unpack(z, f);
+    if (mode == 1 && x >= v.elem(j) && x < v.elem(j) + VE) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (v.elem(j) + e == x) f[e] = -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) w[e] = ex(fma((double)f[e], p.inv_tau, shift));   // 0 at -inf
+    if (mode == 2) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) w[e] = fmax(__dmul_rn(w[e], inv_s) - (double)q[e], 0.0);
+    }
   };
   auto draft = [&](long j, float (&q)[VE]) {               // the draft's probabilities of vector j
     const float* at = qrow + v.elem(j);
@@ -319,27 +330,28 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long j = j0 + u * kThreads + threadIdx.x;
+        z[u] = make_uint4(none, none, none, none);
+        if (j < hi) z[u] = v.raw(j);
+        if (mode != 2) continue;
         if (j < hi) {
-          z[u] = v.raw(j);
-          if (mode == 2) draft(j, q[u]);
+          draft(j, q[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) q[u][e] = 0.f;
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const long j = j0 + u * kThreads + threadIdx.x;
-        double w = 0;
-        if (j < hi) {
-          float f[VE];
-          unpack(z[u], f);
+        double w[VE];
+        weights(j0 + u * kThreads + threadIdx.x, z[u], q[u], mode, inv_s, w);
+        double sum = 0;
 #pragma unroll
-          for (int e = 0; e < VE; ++e)
-            if (f[e] != -INFINITY) w += weight(f[e], q[u][e], v.elem(j) + e, mode, inv_s);
-        }
+        for (int e = 0; e < VE; ++e) sum += w[e];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffff, w, o);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
         if (lane == 0 && j0 + u * kThreads < hi) {
-          group[(step + u) * kWarps + warp] = w;
-          own += w;
+          group[(step + u) * kWarps + warp] = sum;
+          own += sum;
         }
       }
     }
@@ -411,18 +423,11 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
     if (found < 0) found = lastpos;
     const long j = lo + (long)(found / kWarps) * kThreads + (found % kWarps) * 32 + lane;
     double w[VE], own = 0;
+    float q[VE] = {};
+    if (mode == 2 && j < hi) draft(j, q);
+    weights(j, j < hi ? v.raw(j) : make_uint4(none, none, none, none), q, mode, inv_s, w);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) w[e] = 0;
-    if (j < hi) {
-      float f[VE], q[VE];
-      unpack(v.raw(j), f);
-      if (mode == 2) draft(j, q);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        w[e] = f[e] != -INFINITY ? weight(f[e], q[e], v.elem(j) + e, mode, inv_s) : 0.0;
-        own += w[e];
-      }
-    }
+    for (int e = 0; e < VE; ++e) own += w[e];
     double cum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
