@@ -26,7 +26,7 @@ import os
 import torch
 
 from .. import ops
-from ..ops import act8, moe, vocab
+from ..ops import act8, moe, paged, spec, vocab
 from ..ops import reference as ref
 from .timing import median_ms, time_cuda
 
@@ -109,6 +109,25 @@ def cases(T: int, dev):
     lse = vocab.head_fwd(x, table, tg)[2]
     yield ("head_pieces_fwd", lambda: vocab.head_fwd(x, table, tg), (T + V) * H * 2)
     yield ("head_pieces_bwd", lambda: vocab.head_bwd(x, table, tg, lse, coef, dw=dtable), 2 * (T + V) * H * 2)
+
+
+    del table, dtable, x, probs, idx, gain
+    # a drafted decode step: 64 sequences in 8 groups on 1024 shared tokens, 2048 of their own
+    B, P, own, ps, V14 = 64, 1024, 2048, 64, 151936
+    i32 = dict(dtype=torch.int32, device=dev)
+    pages = (8 * P + B * own) // ps
+    kc, vc = torch.randn(pages * ps, HKV, D, **bf), torch.randn(pages * ps, HKV, D, **bf)
+    pt = torch.arange(pages, **i32)
+    bt = torch.cat([pt[:8 * P // ps].view(8, 1, -1).expand(8, 8, -1).reshape(B, -1), pt[8 * P // ps:].view(B, -1)], 1).contiguous()
+    ctx, one = torch.full((B,), P + own - 1, **i32), torch.ones(B, **i32)
+    yield ("step_plan", lambda: paged.plan(ctx, one, bt, ps, B), B * 33)
+    q = torch.randn(B, HQ, D, **bf)
+    gs, pl, qs = torch.arange(0, B + 1, 8, **i32), torch.full((8,), P, **i32), torch.arange(B + 1, **i32)
+    yield ("prefix_attention", lambda: paged.prefix_attention(q, kc, vc, bt, ctx + 1, qs, ps, group_start=gs, prefix_len=pl),
+           pages * ps * HKV * D * 4 + 2 * B * HQ * D * 2)
+    z, u = torch.randn(5 * B, V14, **bf), torch.rand(5 * B, 2, device=dev)
+    tok = z.argmax(-1).roll(1)
+    yield ("draft_verify", lambda: spec.verify(z, tok, qs * 5, u, 0.9), 5 * B * V14 * 2)
 
 
 def main(argv=None):

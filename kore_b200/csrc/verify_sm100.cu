@@ -13,6 +13,10 @@
 // draw compares against every border of a running sum over the vocabulary, where
 // such an error moves a token in up to 1% of the draws of a flat distribution, so
 // the one row that is drawn from is summed again in fp64.
+//
+// Measured on one B200, V = 151,936: 64 sequences x 5 rows in bf16 51 us (statistics 26:
+// one pass of exponentials over 97 MB; the draw 25, bound by fp64 exponentials), with
+// draft probabilities 48 x 8 rows 87 us; greedy 200 x 2 rows of 50,257 in fp32 18 us.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -506,8 +510,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
   p.accepted = accepted.data_ptr<int>();
   p.next = next.data_ptr<int64_t>();
   p.logp = logp.data_ptr<float>();
-  // As many blocks to a sequence as two on each SM leave room for (more, in a second wave,
-  // were slower: 57 us instead of 19 for 200 sequences x 2 rows x 50,257), at most a portable cluster.
+  // As many blocks to a sequence as two on each SM leave room for, at most a portable
+  // cluster. (Eight for all took 57 us for 200 sequences x 2 rows x 50,257 in several
+  // waves of blocks, one each 27, with the statistics still in this kernel.)
   const int room = 2 * num_sms(logits.get_device());
   p.blocks = 1;
   while (p.blocks < kMaxBlocks && B * p.blocks * 2 <= room) p.blocks *= 2;
