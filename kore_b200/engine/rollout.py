@@ -69,6 +69,7 @@ class _Seq:
     logps: List[float] = field(default_factory=list)
     done: bool = False
     reason: str = ""
+    lookup: Optional[spec.Lookup] = None
 
 
 class PagedKVCache:
@@ -360,7 +361,10 @@ class RolloutEngine:
         start = []
         for s in seqs:
             room = min(k, s.req.max_new_tokens - len(s.out) - 1, self.max_pages_per_seq * self.page_size - s.length - 1)
-            drafts = spec.lookup(s.req.prompt + s.out, room, ngram)
+            if s.lookup is None:
+                s.lookup = spec.Lookup(s.req.prompt, ngram)
+            s.lookup.extend(s.out[len(s.lookup.tokens) - len(s.req.prompt):])
+            drafts = s.lookup.draft(room)
             need = -(-(s.length + 1 + len(drafts)) // self.page_size) - len(s.pages)
             if need > 0:
                 got = self.cache.alloc(need)

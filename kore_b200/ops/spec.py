@@ -19,17 +19,30 @@ class Verdict:
     logp: torch.Tensor       # [T] fp32: log-probs of the accepted drafts and of ``next``, row by row
 
 
-def lookup(tokens: Sequence[int], k: int, ngram: int = 3) -> List[int]:
-    """Up to k draft tokens for the end of ``tokens``: what followed the last earlier
-    place with the same ``ngram`` last tokens (fewer, down to one, where none has)."""
-    if k <= 0:
+class Lookup:
+    """Drafts for a growing sequence by look-up in itself: what followed the last
+    earlier place with the same ``ngram`` last tokens (fewer, down to one, where no
+    place has them). A token costs ``ngram`` dictionary entries, a draft as many look-ups."""
+
+    def __init__(self, tokens: Sequence[int] = (), ngram: int = 3):
+        self.tokens: List[int] = []
+        self.after = [{} for _ in range(ngram)]      # the last n tokens -> where what followed them begins
+        self.extend(tokens)
+
+    def extend(self, tokens: Sequence[int]) -> None:
+        for t in tokens:
+            j = len(self.tokens)
+            for n in range(1, min(len(self.after), j) + 1):
+                self.after[n - 1][tuple(self.tokens[j - n:])] = j
+            self.tokens.append(t)
+
+    def draft(self, k: int) -> List[int]:
+        """Up to k tokens."""
+        for n in range(min(len(self.after), len(self.tokens)), 0, -1):
+            at = self.after[n - 1].get(tuple(self.tokens[-n:]))
+            if at is not None:
+                return self.tokens[at:at + max(k, 0)]
         return []
-    for n in range(min(ngram, len(tokens) - 1), 0, -1):
-        tail = list(tokens[-n:])
-        for i in range(len(tokens) - n - 1, -1, -1):
-            if tokens[i] == tail[0] and list(tokens[i:i + n]) == tail:
-                return list(tokens[i + n:i + n + k])
-    return []
 
 
 def verify(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, u: torch.Tensor,

@@ -102,11 +102,28 @@ def test_groups_of_a_batch():
 
 
 def test_lookup():
-    assert spec.lookup([1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
-    assert spec.lookup([1, 2, 3, 8, 1, 2, 3, 9, 1, 2, 3], 5) == [9, 1, 2, 3]        # the last earlier place
-    assert spec.lookup([4, 3, 7, 5, 3], 2) == [7, 5]                                # one token matches
-    assert spec.lookup([1, 2, 3], 4) == [] and spec.lookup([], 3) == [] and spec.lookup([1, 1], 0) == []
-    assert spec.lookup([1, 1], 3) == [1]
+    draft = lambda tokens, k, n=3: spec.Lookup(tokens, n).draft(k)
+    assert draft([1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
+    assert draft([1, 2, 3, 8, 1, 2, 3, 9, 1, 2, 3], 5) == [9, 1, 2, 3]        # the last earlier place
+    assert draft([4, 3, 7, 5, 3], 2) == [7, 5]                                # one token matches
+    assert draft([1, 2, 3], 4) == [] and draft([], 3) == [] and draft([1, 1], 0) == [] and draft([1, 1], -2) == []
+    assert draft([1, 1], 3) == [1]
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 5])
+def test_lookup_against_a_search(n):
+    g = torch.Generator().manual_seed(n)
+    tokens = torch.randint(0, 4, (120,), generator=g).tolist()
+    look = spec.Lookup(tokens[:7], n)
+    for end in range(7, len(tokens)):
+        have, want = tokens[:end], []
+        for m in range(min(n, end), 0, -1):
+            places = [i for i in range(end - m) if have[i:i + m] == have[end - m:]]
+            if places:
+                want = have[places[-1] + m:places[-1] + m + 4]
+                break
+        assert look.draft(4) == want
+        look.extend(tokens[end:end + 1])
 
 
 def test_refusals():
