@@ -1011,7 +1011,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const int id = blockIdx.x * 32 + lane;
       if (id == 0) *reinterpret_cast<int2*>(p.runs) = make_int2(Ww, narrows.W);
 #pragma unroll 1
-      for (int i = id; i < 2 * min(p.T, w.qs[p.B]); i += gridDim.x * 32) {
+      for (int i = 2 * w.qs[0] + id; i < 2 * w.qs[p.B]; i += gridDim.x * 32) {
         const int t = i >> 1, b = w.seq_of(t, 0, p.B - 1), u = i & 1 ? p.ngroups + b : w.grp[b];
         int4 e = make_int4(0, 0, 0, 0);
         if (u >= 0 && cum[u + 1] > cum[u]) {
@@ -1063,7 +1063,7 @@ __global__ void __launch_bounds__(128) join_kernel(AttnParams p, int grid) {
   if (t >= p.T) return;                              // whole warps, and whole blocks where they meet
   const int2 tiles = *reinterpret_cast<const int2*>(p.runs);
   const int4 e0 = p.where[2 * t], e1 = p.where[2 * t + 1];
-  if (t >= p.q_start[p.B]) return;
+  if (t < p.q_start[0] || t >= p.q_start[p.B]) return;       // a row of no sequence: it has no entry, and its result stays
   const bool own_wide = p.nwide > p.ngroups;
   const int kvh = h / p.G, g = h - kvh * p.G;
   int first0 = 0, first1 = 0, n0 = 0, n1 = 0;

@@ -98,8 +98,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Rows q_start[b] .. q_start[b + 1] of q [T, Hq, D] are the last tokens of
     sequence b, whose ``lens[b]`` tokens (these included) are in the cache. Returns
     (out [T, Hq, D], lse [T, Hq] fp32 or None). A row without keys gives zeros and
-    lse -inf; rows behind the last sequence are left as they were in ``out`` (their
-    lse is not defined).
+    lse -inf; rows before the first sequence (q_start[0] need not be 0) and behind the
+    last one are left as they were in ``out`` (their lse is not defined).
 
     Sequences group_start[g] .. group_start[g + 1] share their first
     ``prefix_len[g]`` tokens (int32 [groups + 1] and [groups]; any length, also one

@@ -1,0 +1,33 @@
+"""Edges of the step plan, shared-prefix attention and draft verification on the GPU."""
+import math
+
+import pytest
+import torch
+from paged_oracle import build_cache, check_attention
+
+from kore_b200.ops import check_device_error, paged
+
+pytestmark = pytest.mark.gpu
+
+
+def _i(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("groups,hq,hkv,max_q", [
+    ([(0, [(1000, 1), (1000, 1)])], 40, 8, 1),
+    ([(0, [(4096, 1)])], 40, 8, 1),
+    ([(300, [(301, 1), (900, 3), (20, 2)]), (0, [(0, 1), (65, 4)])], 16, 2, 4),
+    ([(0, [(400, 300)]), (333, [(600, 130), (340, 5)])], 10, 2, 300),
+])
+@pytest.mark.parametrize("lead", [1, 5, 63])
+def test_rows_before_the_first_sequence(groups, hq, hkv, max_q, lead):
+    """A batch that begins behind other rows: those stay, the others are what the batch gives by itself."""
+    a = build_cache(groups, 64, hq, hkv, device="cuda", seed=lead)
+    want, wl = paged.prefix_attention(**a, max_q=max_q, want_lse=True)
+    check_attention(want, wl, a)
+    q = torch.cat([torch.full((lead, hq, 128), math.nan, dtype=torch.bfloat16, device="cuda"), a["q"]])
+    out = torch.full_like(q, 7.0)
+    got, lse = paged.prefix_attention(**{**a, "q": q, "q_start": a["q_start"] + lead}, max_q=max_q, want_lse=True, out=out)
+    assert check_device_error() == 0
+    assert (got[:lead] == 7).all() and torch.equal(got[lead:], want) and torch.equal(lse[lead:], wl)
