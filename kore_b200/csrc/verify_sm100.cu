@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   const T* logits = static_cast<const T*>(p.logits);
   const float c = (float)(p.inv_tau * 1.4426950408889634);
   const bool first = rank == 0;   // the block that writes what all know
-  if (b == p.B - 1 && first)      // rows behind the last sequence
+  if (b == 0 && first)            // rows before the first sequence
+    for (long t = threadIdx.x; t < t0; t += kThreads) p.logp[t] = 0.f;
+  if (b == p.B - 1 && first)      // rows behind the last one
     for (long t = t1 + threadIdx.x; t < p.T; t += kThreads) p.logp[t] = 0.f;
   if (t0 == t1) {                 // the whole cluster
     if (first && threadIdx.x == 0) {

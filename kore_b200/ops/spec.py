@@ -63,8 +63,8 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, u:
 
     The emitted tokens are distributed as if drawn from p one by one. Temperature
     0 is greedy: a draft is accepted while it is the (lowest) argmax, log-probs are
-    those at temperature 1. ``logp`` is 0 in rows behind r and behind the last
-    sequence. Logits of -inf are masked tokens; at a row that has no distribution
+    those at temperature 1. ``logp`` is 0 in rows behind r, before the first sequence
+    and behind the last one. Logits of -inf are masked tokens; at a row that has no distribution
     (all -inf, any NaN or +inf) nothing is accepted, ``next`` is -1 and its log-prob
     NaN. A draft outside the vocabulary is rejected. A sequence without rows gives
     0 and -1."""

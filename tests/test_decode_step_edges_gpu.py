@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 from paged_oracle import build_cache, check_attention
+from test_paged_cpu import check_verify, verify_case
 
 from kore_b200.ops import check_device_error, paged
 
@@ -31,3 +32,14 @@ def test_rows_before_the_first_sequence(groups, hq, hkv, max_q, lead):
     got, lse = paged.prefix_attention(**{**a, "q": q, "q_start": a["q_start"] + lead}, max_q=max_q, want_lse=True, out=out)
     assert check_device_error() == 0
     assert (got[:lead] == 7).all() and torch.equal(got[lead:], want) and torch.equal(lse[lead:], wl)
+
+
+@pytest.mark.parametrize("tau", [0.8, 0.0])
+@pytest.mark.parametrize("lens", [[3, 4, 2], [700, 2], [5, 0, 0]])
+def test_verify_rows_before_the_first_sequence(tau, lens):
+    z, tokens, qs, u, _ = verify_case(7, 100, lens, device="cuda")
+    for _ in range(4):
+        junk = torch.full((len(z),), 5.0, device="cuda")          # the log-probs may get this memory
+        del junk
+        v = check_verify((z, tokens, qs[1:].contiguous(), u, None), tau)
+        assert (v.logp[:lens[0]] == 0).all()
