@@ -1203,7 +1203,7 @@ paged_plan(const at::Tensor& ctx, const at::Tensor& new_toks, at::Tensor& table,
   const bool map_rows = B <= kPlanThreads && rows <= kPlanRows;
   plan_kernel<<<1, kPlanThreads, 0, st>>>(p, map_rows);
   check_cuda(cudaGetLastError(), "paged_plan");
-  if (!map_rows) launch_after("paged_plan rows", plan_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), 0, st, p);
+  if (!map_rows && rows > 0) launch_after("paged_plan rows", plan_rows_kernel, dim3((unsigned)((rows + 1023) / 1024)), dim3(256), 0, st, p);
   return {q_start, lens, pos, slots, ok, held_out, count_out};
 }
 

@@ -3,7 +3,7 @@ import math
 
 import pytest
 import torch
-from paged_oracle import build_cache, check_attention
+from paged_oracle import build_cache, check_attention, plan_oracle
 from test_paged_cpu import check_verify, verify_case
 
 from kore_b200.ops import check_device_error, paged
@@ -43,3 +43,18 @@ def test_verify_rows_before_the_first_sequence(tau, lens):
         del junk
         v = check_verify((z, tokens, qs[1:].contiguous(), u, None), tau)
         assert (v.logp[:lens[0]] == 0).all()
+
+
+@pytest.mark.parametrize("B", [1024, 1025, 5000])
+@pytest.mark.parametrize("pool", [False, True])
+def test_plan_without_rows(B, pool):
+    """Many sequences and no row to plan, whatever they ask for."""
+    ctx, new, table = [b % 40 for b in range(B)], [b % 3 for b in range(B)], [[b, b + 1, b + 2] for b in range(B)]
+    free = list(range(7)) if pool else None
+    held = [0] * B if pool else None
+    want = plan_oracle(ctx, new, table, 16, 0, held, free, 7)
+    t = _i(table)
+    p = paged.plan(_i(ctx), _i(new), t, 16, 0, held=_i(held) if pool else None, free=_i(free) if pool else None, free_count=_i([7]) if pool else None)
+    for k in ("q_start", "lens", "pos", "slots", "held", "ok"):
+        assert getattr(p, k).tolist() == want[k], k
+    assert t.tolist() == want["table"] and (not pool or p.free_count.tolist() == [want["free_count"]])
