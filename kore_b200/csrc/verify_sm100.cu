@@ -295,7 +295,10 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   const RowView<T> v(logits + row * p.ld, p.V);
   const long per = (v.nvec + nblk - 1) / nblk, lo = min(rank * per, v.nvec), hi = min(lo + per, v.nvec);
   const float* qrow = p.probs && over ? p.probs + row * p.ld_probs : nullptr;
-  const double m = rs.m, shift = -m * p.inv_tau;
+  // Exponents are (z - m) / tau with the difference taken first: 0 at the maximum for every
+  // tau. (z / tau - m / tau in one fma saves an operation, but has the rounding of m / tau,
+  // which passes 1 from tau = 1e-15 on and leaves no weight at all from 1e-18.)
+  const double m = rs.m;
   const Exp ex = {tab};
   const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
   // Weights of a vector's tokens: p s (mode 0), without the draft (1), max(0, p - q) (2).
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
         if (v.elem(j) + e == x) f[e] = -INFINITY;
     }
 #pragma unroll
-    for (int e = 0; e < VE; ++e) w[e] = ex(fma((double)f[e], p.inv_tau, shift));   // 0 at -inf
+    for (int e = 0; e < VE; ++e) w[e] = ex(((double)f[e] - m) * p.inv_tau);   // 0 at -inf
     if (mode == 2) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) w[e] = fmax(__dmul_rn(w[e], inv_s) - (double)q[e], 0.0);
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   };
   int mode = over && !qrow ? 1 : 0, slot = 0;
   double before, total = sums(mode, 1.0, slot, before), s64 = total;
-  if (mode == 1 && x >= 0 && x < p.V) s64 += ex(fma((double)to_float(logits[row * p.ld + x]), p.inv_tau, shift));
+  if (mode == 1 && x >= 0 && x < p.V) s64 += ex(((double)to_float(logits[row * p.ld + x]) - m) * p.inv_tau);
   const double inv_s = 1.0 / s64;
   if (qrow) {
     mode = 2;

@@ -6,7 +6,7 @@ import torch
 from paged_oracle import build_cache, check_attention, plan_oracle
 from test_paged_cpu import check_verify, verify_case
 
-from kore_b200.ops import check_device_error, paged
+from kore_b200.ops import check_device_error, paged, spec
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,23 @@ def test_plan_without_rows(B, pool):
     for k in ("q_start", "lens", "pos", "slots", "held", "ok"):
         assert getattr(p, k).tolist() == want[k], k
     assert t.tolist() == want["table"] and (not pool or p.free_count.tolist() == [want["free_count"]])
+
+
+@pytest.mark.parametrize("tau", [1e-10, 1e-13, 1e-18, 1e-30])
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_at_small_temperatures(tau, probs):
+    """All weight is on the largest logit. Those of the definition's quotients that are not the
+    maximum lie at least 2^-23 / tau below it: their weights are 0 whatever these are rounded to."""
+    check_verify(verify_case(7, 5000, [3, 4, 2], probs=probs, device="cuda"), tau)
+
+
+def test_draw_among_equal_logits_at_small_temperatures():
+    V = 3001
+    z = torch.randn(8, V, device="cuda")
+    z[:, [0, 1500, 1501, 3000]] = 17.3
+    u = torch.tensor([0.0, 0.25, 0.2499, 0.5, 0.7499, 0.75, 0.9999999, 0.5001], device="cuda")
+    u = torch.stack([u.flip(0), u], 1)
+    for tau in (1e-4, 1e-9, 1e-14, 1e-17, 1e-25):
+        v = spec.verify(z, torch.zeros(8, dtype=torch.long, device="cuda"), _i(list(range(9))), u, tau)
+        assert v.next.tolist() == [0, 1500, 0, 1501, 1501, 3000, 3000, 1501]
+        assert (v.logp + math.log(4.0)).abs().max() <= 2.0 ** -22          # an fp32 result of 1.39
