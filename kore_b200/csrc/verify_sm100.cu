@@ -132,11 +132,6 @@ KORE_DEV void join(Stat& a, const Stat& b, float c) {
 }
 
 // Another block's shared memory (the variable at the same place there).
-KORE_DEV uint32_t peer_u32(const void* p, uint32_t rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-  return v;
-}
 KORE_DEV double peer_f64(const double* p, uint32_t rank) {
   double v;
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
