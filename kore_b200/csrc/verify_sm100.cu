@@ -21,6 +21,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
+#include <cmath>
+#include <limits>
 #include <tuple>
 
 #include "common.cuh"
@@ -48,6 +50,7 @@ struct Params {
   long B, T;
   int blocks, parts;              // blocks of a sequence in the draw, of a row in the statistics
   double inv_tau;                 // 1 when greedy
+  float c;                        // inv_tau log2 e, kept a normal number: 0 x inf is NaN at the maximum and at masked tokens
   bool greedy;
   int* accepted;
   long* next;
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(kStatThreads) stats_kernel(Params p) {
   pdl_trigger();
   const long row = blockIdx.x / p.parts;
   const int own = blockIdx.x - (int)(row * p.parts), warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const float c = (float)(p.inv_tau * 1.4426950408889634);
+  const float c = p.c;
   const RowView<T> v(static_cast<const T*>(p.logits) + row * p.ld, p.V);
   const long step = (long)p.parts * kStatThreads;
   const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;      // -inf
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(Params p) {
   pdl_wait();
   const long t0 = min(max((long)p.q_start[b], 0L), p.T), t1 = min(max((long)p.q_start[b + 1], t0), p.T);
   const T* logits = static_cast<const T*>(p.logits);
-  const float c = (float)(p.inv_tau * 1.4426950408889634);
+  const float c = p.c;
   const bool first = rank == 0;   // the block that writes what all know
   if (b == 0 && first)            // rows before the first sequence
     for (long t = threadIdx.x; t < t0; t += kThreads) p.logp[t] = 0.f;
@@ -483,7 +486,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
                   q_start.is_contiguous() && B >= 0, "verify: q_start must be contiguous int32 [sequences + 1]");
   TORCH_CHECK(u.device() == logits.device() && u.scalar_type() == at::kFloat && u.dim() == 2 && u.is_contiguous() &&
                   u.size(0) == T && u.size(1) == 2, "verify: u must be contiguous fp32 [T, 2]");
-  TORCH_CHECK(temperature >= 0, "verify: temperature must not be negative");
+  TORCH_CHECK(temperature >= 0 && std::isfinite(temperature), "verify: temperature must be finite and not negative");
   if (probs)
     TORCH_CHECK(probs->device() == logits.device() && probs->scalar_type() == at::kFloat && probs->dim() == 2 &&
                     probs->size(0) == T && probs->size(1) == V && (V <= 1 || probs->stride(1) == 1),
@@ -506,7 +509,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
   p.B = B;
   p.T = T;
   p.greedy = temperature == 0;
-  p.inv_tau = p.greedy ? 1.0 : 1.0 / temperature;
+  p.inv_tau = p.greedy ? 1.0 : std::min(1.0 / temperature, std::numeric_limits<double>::max());
+  p.c = (float)std::clamp(p.inv_tau * 1.4426950408889634, (double)std::numeric_limits<float>::min(), (double)std::numeric_limits<float>::max());
   p.accepted = accepted.data_ptr<int>();
   p.next = next.data_ptr<int64_t>();
   p.logp = logp.data_ptr<float>();

@@ -68,8 +68,8 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, u:
     (all -inf, any NaN or +inf) nothing is accepted, ``next`` is -1 and its log-prob
     NaN. A draft outside the vocabulary is rejected. A sequence without rows gives
     0 and -1."""
-    if not temperature >= 0:
-        raise ValueError("verify: temperature must not be negative")
+    if not 0 <= temperature < math.inf:
+        raise ValueError("verify: temperature must be finite and not negative")
     if logits.is_cuda:
         return Verdict(*native().spec_verify(logits, tokens, q_start, u, float(temperature), draft_probs))
     T, V = logits.shape
@@ -79,8 +79,8 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, u:
     for a, b in zip(starts[:-1], starts[1:]):
         t, y = a, -1
         while t < b:
-            z = logits[t].double() / (temperature if temperature > 0 else 1.0)
-            lp = torch.log_softmax(z, -1)
+            z = logits[t].double()
+            lp = torch.log_softmax((z - z.max()) / (temperature if temperature > 0 else 1.0), -1)
             p = lp.exp()
             x = int(tokens[t + 1]) if t + 1 < b else -1
             if torch.isnan(p).any():

@@ -7,7 +7,7 @@ from paged_oracle import attention_oracle, build_cache
 
 from test_paged_cpu import check_verify, verify_case
 
-from kore_b200.ops import paged
+from kore_b200.ops import paged, spec
 
 
 def _i(x):
@@ -29,3 +29,22 @@ def test_verify_rows_before_the_first_sequence(tau):
     z, tokens, qs, u, _ = verify_case(7, 100, [3, 4, 2])
     v = check_verify((z, tokens, qs[1:].contiguous(), u, None), tau)
     assert (v.logp[:3] == 0).all()
+
+
+def check_extreme_temperatures(device):
+    """From the smallest to the largest double: all weight on the largest logits, or the same on every token that is not masked."""
+    z = torch.tensor([[0.0, 9.0, -math.inf, 9.0, 8.0, -math.inf, 3.0, 2.0]] * 2, device=device)
+    u = torch.tensor([[0.5, 0.2], [0.5, 0.8]], device=device)
+    tokens, qs = torch.zeros(2, dtype=torch.long, device=device), _i([0, 1, 2]).to(device)
+    for tau, want, n in ((5e-324, [1, 3], 2), (1e-310, [1, 3], 2), (1e-200, [1, 3], 2), (1e-39, [1, 3], 2), (1e-30, [1, 3], 2),
+                         (1e36, [1, 6], 6), (1e40, [1, 6], 6), (1e46, [1, 6], 6), (1e300, [1, 6], 6)):
+        v = spec.verify(z, tokens, qs, u, tau)
+        assert v.accepted.tolist() == [0, 0] and v.next.tolist() == want, tau
+        assert (v.logp.cpu() + math.log(n)).abs().max() <= 2.0 ** -21, tau       # an fp32 result of up to 1.8 and sums of terms near 1
+    for tau in (math.inf, math.nan, -1e-300):
+        with pytest.raises(ValueError):
+            spec.verify(z, tokens, qs, u, tau)
+
+
+def test_verify_at_extreme_temperatures():
+    check_extreme_temperatures("cpu")

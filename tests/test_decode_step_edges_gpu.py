@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 from paged_oracle import build_cache, check_attention, plan_oracle
+from test_decode_step_edges_cpu import check_extreme_temperatures
 from test_paged_cpu import check_verify, verify_case
 
 from kore_b200.ops import check_device_error, paged, spec
@@ -78,3 +79,7 @@ def test_draw_among_equal_logits_at_small_temperatures():
         v = spec.verify(z, torch.zeros(8, dtype=torch.long, device="cuda"), _i(list(range(9))), u, tau)
         assert v.next.tolist() == [0, 1500, 0, 1501, 1501, 3000, 3000, 1501]
         assert (v.logp + math.log(4.0)).abs().max() <= 2.0 ** -22          # an fp32 result of 1.39
+
+
+def test_verify_at_extreme_temperatures():
+    check_extreme_temperatures("cuda")
