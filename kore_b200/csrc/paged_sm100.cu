@@ -31,7 +31,7 @@ struct PlanParams {
   long ld_table;
   int M, page_size;
   long B, rows;
-  const int *free_stack, *free_count;   // null: no pool
+  const int *free_stack, *free_count;   // free_count null: no pool (an empty stack has no address either)
   long nfree;
   int *q_start, *lens, *pos, *slots, *held_out, *count_out;
   bool* ok;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p, bool m
   __shared__ long part[32];
   __shared__ int starts[kPlanThreads + 1], granted, asks[kPlanThreads], holds[kPlanThreads];
   pdl_trigger();
-  const int count = p.free_stack ? (int)min((long)max(*p.free_count, 0), p.nfree) : 0;
+  const int count = p.free_count ? (int)min((long)max(*p.free_count, 0), p.nfree) : 0;
   long rows = 0, asked = 0, total;
   if (threadIdx.x == 0) {
     p.q_start[0] = starts[0] = 0;
@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p, bool m
     const long n = min(to, p.rows) - min(to - want, p.rows);   // a batch has p.rows rows: what is behind them is cut
     const long ps = p.page_size, need = (ctx + n + ps - 1) / ps, held = p.held ? have : (ctx + ps - 1) / ps;
     const bool fits = need <= p.M;
-    const long take = p.free_stack && fits ? max(need - held, 0L) : 0;
+    const long take = p.free_count && fits ? max(need - held, 0L) : 0;
     long upto = 0;
-    if (p.free_stack) {
+    if (p.free_count) {
       upto = block_scan(take, part, total) + asked;
       asked += total;
     }
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanParams p, bool m
       p.ok[b] = ok;
       p.held_out[b] = (int)held + got;
     }
-    if (p.free_stack) {
+    if (p.free_count) {
       // pages to threads, not sequences to threads: a long prompt alone may ask for hundreds
       const long before = asked - total;
       asks[threadIdx.x] = (int)min(upto - before, (long)count + 1);

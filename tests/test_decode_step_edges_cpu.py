@@ -48,3 +48,21 @@ def check_extreme_temperatures(device):
 
 def test_verify_at_extreme_temperatures():
     check_extreme_temperatures("cpu")
+
+
+def check_plan_with_an_empty_pool(device):
+    """A stack without an entry is a pool: who lacks a page gets none, nor does who comes behind
+    (the pages asked for up to there, 2, are more than the pool has)."""
+    i = lambda x: _i(x).to(device)
+    for free in (i([]), i([3, 4])[:0]):
+        table = i([[5, 5], [6, 6], [7, 7]])
+        p = paged.plan(i([0, 16, 15]), i([1, 1, 1]), table, 16, 3, free=free, free_count=i([0]))
+        assert p.ok.tolist() == [False, False, False] and p.slots.tolist() == [-1, -1, -1]
+        assert p.lens.tolist() == [0, 16, 15] and p.held.tolist() == [0, 1, 1] and p.free_count.tolist() == [0]
+        assert table.tolist() == [[5, 5], [6, 6], [7, 7]]
+        p = paged.plan(i([15, 16]), i([1, 1]), table[:2], 16, 2, free=free, free_count=i([0]))
+        assert p.ok.tolist() == [True, False] and p.slots.tolist() == [5 * 16 + 15, -1] and p.lens.tolist() == [16, 16]
+
+
+def test_plan_with_an_empty_pool():
+    check_plan_with_an_empty_pool("cpu")
