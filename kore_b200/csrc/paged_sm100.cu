@@ -1172,6 +1172,7 @@ paged_plan(const at::Tensor& ctx, const at::Tensor& new_toks, at::Tensor& table,
   if (free_stack) {
     check_ints(*free_stack, ctx, -1, "free");
     check_ints(*free_count, ctx, 1, "free_count");
+    TORCH_CHECK(B <= 1 || table.stride(0) >= table.size(1), "paged: rows of a table that pages are written to must not overlap");
   }
   c10::cuda::CUDAGuard g(ctx.device());
   const auto i32 = ctx.options();

@@ -40,7 +40,7 @@ def plan(ctx: torch.Tensor, new: torch.Tensor, table: torch.Tensor, page_size: i
     that ``ctx`` fills). With a pool (``free``: a stack of page ids of which the
     first ``free_count`` are free), the pages that a sequence lacks are taken from
     the top of the stack, in the order of the sequences, and written into the
-    table in place; the stack itself is only read, and ``Plan.free_count`` says how
+    table in place (its rows must not overlap); the stack itself is only read, and ``Plan.free_count`` says how
     many are left. A sequence whose tokens do not fit its table row, or whose
     pages together with those that the sequences before it asked for are more than
     the pool has, is not ``ok``: it gets no page, its rows have slot -1 and its
@@ -58,6 +58,8 @@ def plan(ctx: torch.Tensor, new: torch.Tensor, table: torch.Tensor, page_size: i
     B, M = table.shape
     if ctx.numel() != B or new.numel() != B or (held is not None and held.numel() != B):
         raise ValueError("paged: ctx, new and held need one entry for each row of the table")
+    if free is not None and B > 1 and table.stride(0) < M:
+        raise ValueError("paged: rows of a table that pages are written to must not overlap")
     count = min(max(int(free_count), 0), free.numel()) if free is not None else 0
     asked = granted = at = 0
     q_start, lens, ok, held_out = [0], [], [], []

@@ -66,3 +66,19 @@ def check_plan_with_an_empty_pool(device):
 
 def test_plan_with_an_empty_pool():
     check_plan_with_an_empty_pool("cpu")
+
+
+def check_plan_refuses_overlapping_rows(device):
+    i = lambda x: _i(x).to(device)
+    one, rows = i([1] * 5), i(list(range(20)))
+    for table in (i([[0, 1, 2, 3]]).expand(5, 4), rows.as_strided((5, 4), (3, 1))):
+        with pytest.raises((ValueError, RuntimeError)):
+            paged.plan(i([0] * 5), one, table, 16, 5, free=i(list(range(9))), free_count=i([9]))
+        p = paged.plan(i([0] * 5), one, table, 16, 5)              # without a pool a table is only read
+        assert p.slots.tolist() == [16 * t for t in table[:, 0].tolist()]
+    p = paged.plan(i([0]), i([40]), i([[7, 7, 7, 7]]).expand(1, 4).contiguous(), 16, 40, free=i([0, 1, 2]), free_count=i([3]))
+    assert p.ok.tolist() == [True]
+
+
+def test_plan_refuses_overlapping_rows():
+    check_plan_refuses_overlapping_rows("cpu")

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 from paged_oracle import build_cache, check_attention, plan_oracle
-from test_decode_step_edges_cpu import check_extreme_temperatures, check_plan_with_an_empty_pool
+from test_decode_step_edges_cpu import check_extreme_temperatures, check_plan_refuses_overlapping_rows, check_plan_with_an_empty_pool
 from test_paged_cpu import check_verify, verify_case
 
 from kore_b200.ops import check_device_error, paged, spec
@@ -87,3 +87,7 @@ def test_verify_at_extreme_temperatures():
 
 def test_plan_with_an_empty_pool():
     check_plan_with_an_empty_pool("cuda")
+
+
+def test_plan_refuses_overlapping_rows():
+    check_plan_refuses_overlapping_rows("cuda")
