@@ -1244,7 +1244,7 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
                     lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq,
                 "prefix_attention: lse must be contiguous fp32 [T, Hq]");
   TORCH_CHECK(scale > 0, "prefix_attention: scale must be positive");
-  if (T == 0 || B == 0) return;
+  if (T == 0 || B == 0 || Hq == 0) return;
   c10::cuda::CUDAGuard g(q.device());
   const int G = (int)(Hq / Hkv), ngroups = prefix_len ? (int)prefix_len->numel() : 0;
   AttnParams p;

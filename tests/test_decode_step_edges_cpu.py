@@ -82,3 +82,9 @@ def check_plan_refuses_overlapping_rows(device):
 
 def test_plan_refuses_overlapping_rows():
     check_plan_refuses_overlapping_rows("cpu")
+
+
+def test_attention_without_query_heads():
+    a = build_cache([(20, [(25, 2), (21, 1)])], 16, 8, 2)
+    out, lse = paged.prefix_attention(**{**a, "q": a["q"][:, :0]}, max_q=2, want_lse=True)
+    assert out.shape == (3, 0, 128) and lse.shape == (3, 0)

@@ -91,3 +91,10 @@ def test_plan_with_an_empty_pool():
 
 def test_plan_refuses_overlapping_rows():
     check_plan_refuses_overlapping_rows("cuda")
+
+
+def test_attention_without_query_heads():
+    a = build_cache([(20, [(25, 2), (21, 1)])], 16, 8, 2, device="cuda")
+    for q in (a["q"][:, :0], torch.empty(3, 0, 128, dtype=torch.bfloat16, device="cuda")):
+        out, lse = paged.prefix_attention(**{**a, "q": q}, max_q=2, want_lse=True)
+        assert out.shape == (3, 0, 128) and lse.shape == (3, 0)
