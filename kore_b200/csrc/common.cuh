@@ -18,7 +18,8 @@ namespace kore {
 
 // Error word of this translation unit (no relocatable device code, so each
 // .cu file owns one), read by the host after a launch when checking is enabled.
-// Codes: 1 = mbarrier wait timed out, 2 = peer flag wait timed out.
+// Codes: 1 = mbarrier wait timed out, 2 = peer flag wait timed out, 3 = an argument's
+// values that only the device sees were out of order.
 static __device__ int g_error = 0;
 
 // Every translation unit registers a reader for its own error word; the host

@@ -958,14 +958,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     }
     w.grp[b] = (short)(lo > 0 && b < w.gs[lo] ? lo - 1 : -1);
   }
-  __syncthreads();
+  // Starts that decrease would give rows or sequences to several units, whose tiles are more
+  // than the host allowed for: such a call has no tiles (its rows get zeros) and sets the error word.
+  bool falls = false;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < p.B; i += kAttnThreads) falls = falls || w.qs[i] > w.qs[i + 1] || (i < p.ngroups && w.gs[i] > w.gs[i + 1]);
+  const bool refused = __syncthreads_or(falls);
+  if (refused && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(&g_error, 3);
   {
     const int u0 = min((int)threadIdx.x * per, nu), u1 = min(u0 + per, nu);
     int mine = 0;
 #pragma unroll 1
     for (int u = u0; u < u1; ++u) {
       cum[u] = mine;
-      mine += w.tiles(u);
+      mine += refused ? 0 : w.tiles(u);
     }
     int upto = mine;
 #pragma unroll

@@ -54,7 +54,7 @@ void launch_after(const char* what, void (*kernel)(P...), dim3 grid, dim3 block,
 }
 
 // Reads and clears the device-side error word (1 = barrier wait timeout,
-// 2 = peer flag timeout). Synchronizes the current device.
+// 2 = peer flag timeout, 3 = values out of order). Synchronizes the current device.
 int read_and_clear_device_error();
 
 }  // namespace kore

@@ -75,5 +75,6 @@ def available() -> bool:
 def check_device_error() -> int:
     """Synchronize and return (and clear) the kernels' device error word.
 
-    1 = an mbarrier wait timed out, 2 = a peer-flag wait timed out."""
+    1 = an mbarrier wait timed out, 2 = a peer-flag wait timed out, 3 = values that only
+    the device sees (row or group starts) were out of order."""
     return int(native().read_and_clear_device_error())

@@ -110,7 +110,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     are not read there. Without groups each sequence reads its own history.
 
     ``max_q`` is the largest number of rows of a sequence as far as the host knows
-    (it chooses the split, not the result). CUDA: bf16, D = 128, page_size a
+    (it chooses the split, not the result). Neither q_start nor group_start may
+    decrease: on CUDA the rows of such a call get zeros and ``check_device_error``
+    reports 3, on the CPU it raises. CUDA: bf16, D = 128, page_size a
     multiple of 8, at most 512 sequences. What the cache holds behind a
     sequence's last token does not matter, NaN included; among the tokens of a
     call, a row's value that is not finite reaches the sequence's earlier rows too."""
@@ -127,6 +129,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     hq, hkv = q.shape[1], k_cache.shape[1]
     if hkv == 0 or hq % hkv:
         raise ValueError("prefix_attention: Hq must be a multiple of Hkv")
+    if any((t is not None and (t[1:] < t[:-1]).any()) for t in (q_start, group_start)):
+        raise ValueError("prefix_attention: q_start and group_start must not decrease")
     lead, shared = list(range(lens.numel())), [0] * lens.numel()
     if prefix_len is not None:
         for g, n in enumerate(prefix_len.tolist()):

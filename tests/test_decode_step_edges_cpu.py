@@ -88,3 +88,10 @@ def test_attention_without_query_heads():
     a = build_cache([(20, [(25, 2), (21, 1)])], 16, 8, 2)
     out, lse = paged.prefix_attention(**{**a, "q": a["q"][:, :0]}, max_q=2, want_lse=True)
     assert out.shape == (3, 0, 128) and lse.shape == (3, 0)
+
+
+def test_attention_refuses_starts_that_decrease():
+    a = build_cache([(5, [(9, 2), (6, 1)]), (0, [(30, 3)])], 8, 6, 2, dtype=torch.float32, D=16)
+    for bad in (dict(q_start=_i([0, 3, 2, 6])), dict(q_start=_i([4, 2, 3, 6])), dict(group_start=_i([2, 1, 3])), dict(group_start=_i([0, 3, 2]))):
+        with pytest.raises(ValueError):
+            paged.prefix_attention(**{**a, **bad}, max_q=3)

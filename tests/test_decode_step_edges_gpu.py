@@ -98,3 +98,15 @@ def test_attention_without_query_heads():
     for q in (a["q"][:, :0], torch.empty(3, 0, 128, dtype=torch.bfloat16, device="cuda")):
         out, lse = paged.prefix_attention(**{**a, "q": q}, max_q=2, want_lse=True)
         assert out.shape == (3, 0, 128) and lse.shape == (3, 0)
+
+
+@pytest.mark.parametrize("max_q", [1, 3, 9])
+def test_starts_that_decrease_give_zeros_and_an_error(max_q):
+    a = build_cache([(100, [(300, 2), (160, 1)]), (0, [(90, 3)])], 16, 10, 2, device="cuda")
+    want, _ = paged.prefix_attention(**a, max_q=max_q)
+    assert check_device_error() == 0
+    for bad in (dict(q_start=_i([0, 3, 2, 6])), dict(q_start=_i([0, 6, 3, 6])), dict(group_start=_i([2, 1, 3])), dict(group_start=_i([0, 3, 2]))):
+        out, lse = paged.prefix_attention(**{**a, **bad}, max_q=max_q, want_lse=True)
+        assert check_device_error() == 3 and (out == 0).all() and lse.isneginf().all()
+    got, _ = paged.prefix_attention(**a, max_q=max_q)
+    assert check_device_error() == 0 and torch.equal(got, want)
