@@ -15,6 +15,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
+#include <cmath>
 #include <numeric>
 #include <tuple>
 
@@ -1249,7 +1250,9 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
     TORCH_CHECK(lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() &&
                     lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq,
                 "prefix_attention: lse must be contiguous fp32 [T, Hq]");
-  TORCH_CHECK(scale > 0, "prefix_attention: scale must be positive");
+  // a factor that underflows makes NaN of a masked score
+  const float scale_log2 = (float)(scale * 1.4426950408889634);
+  TORCH_CHECK(scale_log2 > 0 && std::isnormal(scale_log2), "prefix_attention: scale must be a positive normal fp32 number");
   if (T == 0 || B == 0 || Hq == 0) return;
   c10::cuda::CUDAGuard g(q.device());
   const int G = (int)(Hq / Hkv), ngroups = prefix_len ? (int)prefix_len->numel() : 0;
@@ -1274,7 +1277,7 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   p.group_start = group_start ? group_start->data_ptr<int>() : nullptr;
   p.prefix = prefix_len ? prefix_len->data_ptr<int>() : nullptr;
   p.ngroups = ngroups;
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.out = (__nv_bfloat16*)out.data_ptr();
   p.lse = lse ? lse->data_ptr<float>() : nullptr;
   const int64_t tiles = (table.size(1) * page_size + BK - 1) / BK + 1;

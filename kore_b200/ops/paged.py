@@ -113,7 +113,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     (it chooses the split, not the result). Neither q_start nor group_start may
     decrease: on CUDA the rows of such a call get zeros and ``check_device_error``
     reports 3, on the CPU it raises. CUDA: bf16, D = 128, page_size a
-    multiple of 8, at most 512 sequences. What the cache holds behind a
+    multiple of 8, at most 512 sequences, scale a positive normal fp32 number. What the cache holds behind a
     sequence's last token does not matter, NaN included; among the tokens of a
     call, a row's value that is not finite reaches the sequence's earlier rows too."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])

@@ -110,3 +110,14 @@ def test_starts_that_decrease_give_zeros_and_an_error(max_q):
         assert check_device_error() == 3 and (out == 0).all() and lse.isneginf().all()
     got, _ = paged.prefix_attention(**a, max_q=max_q)
     assert check_device_error() == 0 and torch.equal(got, want)
+
+
+def test_scales():
+    """The smallest and large scales that fp32 holds; what it cannot hold is refused."""
+    a = build_cache([(20, [(25, 2), (21, 1)]), (0, [(300, 5)])], 16, 8, 2, device="cuda")
+    for scale in (1e-37, 1e-6, 3.0):
+        out, lse = paged.prefix_attention(**a, max_q=5, scale=scale, want_lse=True)
+        check_attention(out, lse, {**a, "scale": scale})
+    for scale in (1e-39, 1e-50, 1e39, math.inf, math.nan):
+        with pytest.raises(RuntimeError):
+            paged.prefix_attention(**a, max_q=5, scale=scale)
