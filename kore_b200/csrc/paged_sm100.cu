@@ -1254,6 +1254,9 @@ void paged_prefix_attention(const at::Tensor& q, const at::Tensor& kc, const at:
   const float scale_log2 = (float)(scale * 1.4426950408889634);
   TORCH_CHECK(scale_log2 > 0 && std::isnormal(scale_log2), "prefix_attention: scale must be a positive normal fp32 number");
   if (T == 0 || B == 0 || Hq == 0) return;
+  // Blocks read q while others write results.
+  const uintptr_t q0 = (uintptr_t)q.data_ptr(), q1 = q0 + 2 * ((T - 1) * q.stride(0) + Hq * D), o0 = (uintptr_t)out.data_ptr();
+  TORCH_CHECK(o0 + 2 * T * Hq * D <= q0 || o0 >= q1, "prefix_attention: out must not overlap q");
   c10::cuda::CUDAGuard g(q.device());
   const int G = (int)(Hq / Hkv), ngroups = prefix_len ? (int)prefix_len->numel() : 0;
   AttnParams p;

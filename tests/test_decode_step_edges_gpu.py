@@ -121,3 +121,17 @@ def test_scales():
     for scale in (1e-39, 1e-50, 1e39, math.inf, math.nan):
         with pytest.raises(RuntimeError):
             paged.prefix_attention(**a, max_q=5, scale=scale)
+
+
+def test_out_may_not_overlap_q():
+    a = build_cache([(20, [(25, 2), (21, 1)])], 16, 8, 2, device="cuda")
+    both = torch.empty(6, 8, 128, dtype=torch.bfloat16, device="cuda")
+    q = both[:3].copy_(a["q"])
+    for out in (q, both[2:5]):
+        with pytest.raises(RuntimeError):
+            paged.prefix_attention(**{**a, "q": q}, max_q=2, out=out)
+    out, lse = paged.prefix_attention(**{**a, "q": q}, max_q=2, out=both[3:], want_lse=True)
+    check_attention(out, lse, a)
+    wide = torch.empty(4, 8 * 128 + 64, dtype=torch.bfloat16, device="cuda")
+    q = wide[:3, 64:].copy_(a["q"].flatten(1)).unflatten(1, (8, 128))
+    check_attention(*paged.prefix_attention(**{**a, "q": q}, max_q=2, want_lse=True), a)
