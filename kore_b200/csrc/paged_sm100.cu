@@ -385,12 +385,22 @@ struct Bars {
   uint64_t *o_done, *o_final;                        // [2] by the tile's parity; one phase per item
   uint64_t *q_full, *q_empty, *o_free;               // wide: one buffer each
   uint64_t *qn_full, *qn_empty, *on_free;            // narrow: by the Q or O buffer
+  uint64_t* drained;                                 // [2] after an abort: S products, O products
   volatile int* aborted;
 };
+// The producer's loads by full barrier: how many phases it has begun there (parity) and whether any.
+struct Sent {
+  unsigned parity, any;
+  KORE_DEV void add(int bar) {
+    parity ^= 1u << bar;
+    any |= 1u << bar;
+  }
+};
+constexpr int kSentK = 0, kSentV = 2, kSentQ = 4, kSentQn = 5;
 
 // ---- producer warp: Q of each item, K and V of each tile
 template <int N>
-KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, int& cnt,
+KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk r, uint8_t* smem, const Bars& bar, int& cnt, Sent& sent,
                       const CUtensorMap* tmQp, const CUtensorMap* tmQo, const CUtensorMap* tmK, const CUtensorMap* tmV) {
   using S = AttnSmem;
   constexpr int QB = 2;
@@ -418,6 +428,7 @@ KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk
         const CUtensorMap* tm = pre ? tmQp : tmQo;
         uint8_t* q = smem + S::Q_OFF + qi * N * 256;
         mbar_arrive_expect_tx(full, 2 * 128 * p.G * tb);
+        sent.add(wide ? kSentQ : kSentQn + qi);
         tma_load_3d(q, tm, full, 0, it.h * p.G, t0);
         tma_load_3d(q + (wide ? 16384 : N * 128), tm, full, 64, it.h * p.G, t0);
       }
@@ -440,7 +451,10 @@ KORE_DEV bool produce(const bool wide, const AttnParams& p, const Units& w, Walk
         uint8_t* dst = smem + (kv ? S::V_OFF : S::K_OFF) + st * kTileBytes;
         if (lane == 0 && ok) {
           ok = wait_on((kv ? bar.v_empty : bar.k_empty) + st, ph ^ 1);
-          if (ok) mbar_arrive_expect_tx(full, __popc(held) * p.box * 256);
+          if (ok) {
+            mbar_arrive_expect_tx(full, __popc(held) * p.box * 256);
+            sent.add((kv ? kSentV : kSentK) + st);
+          }
         }
         if (nbox == 1) {                        // one box of 64 keys x two 64-column halves
           const int z = __shfl_sync(0xffffffff, slot, first - window);
@@ -910,8 +924,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   int* warp_sum = reinterpret_cast<int*>(tmem_slot + 2);             // [8]
   const Bars bar = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 12, bars + 14, bars + 15,
-                    bars + 16, bars + 17, bars + 18, bars + 20, bars + 22, reinterpret_cast<volatile int*>(tmem_slot + 1)};
-  static_assert(kStages == 2, "barrier layout");
+                    bars + 16, bars + 17, bars + 18, bars + 20, bars + 22, bars + 29, reinterpret_cast<volatile int*>(tmem_slot + 1)};
+  static_assert(kStages == 2 && 31 * 8 <= S::X_OFF - S::BAR_OFF, "barrier layout: 24, the two words and eight sums, 2");
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const Units w(p, smem + S::UNITS_OFF);
   int* const cum = w.cum;
@@ -943,6 +957,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll 1
     for (int i = 0; i < 24; ++i)     // p_full, wide q_empty, o_free, on_free: a lane of each softmax warp
       mbar_init(bars + i, i == 10 || i == 11 || i == 16 || i == 17 || i >= 22 ? 4 : 1);
+    mbar_init(bar.drained, 1);
+    mbar_init(bar.drained + 1, 1);
     *bar.aborted = 0;
     fence_barrier_init();
   }
@@ -997,13 +1013,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const int cw = blockIdx.x, cn = gridDim.x - 1 - blockIdx.x;       // few runs of both forms land on different blocks
   const Walk wide = make_walk(cum, nu, 0, wides, cw), narrow = make_walk(cum, nu, Ww, narrows, cn);
-  // The end of a turn: both forms use the same buffers. True: give up.
-  auto turned = [&](bool ok) {
+  // The end of a turn: both forms use the same buffers. True: give up, once `drain` has seen
+  // to what the warp has in flight.
+  auto turned = [&](bool ok, auto drain) {
     if (!ok) *bar.aborted = 1;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const bool stop = *bar.aborted;
+    if (stop) drain();
     __syncthreads();
     return stop;
   };
@@ -1013,6 +1031,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const bool lead = elect_one();
+    Sent sent = {0, 0};
+    auto drain = [&] {               // waits, up to their limit, for this thread's loads or products
+      if (warp == 0 && lane == 0) {
+        uint64_t* const full[7] = {bar.k_full, bar.k_full + 1, bar.v_full, bar.v_full + 1, bar.q_full, bar.qn_full, bar.qn_full + 1};
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (sent.any >> i & 1) mbar_wait(full[i], (sent.parity >> i & 1) ^ 1);
+      } else if ((warp == 1 || warp == 2) && lead) {
+        umma_commit(bar.drained + (warp - 1));
+        mbar_wait(bar.drained + (warp - 1), 0);
+      }
+    };
     if (warp == 3) {
       // ---- for the join: first tile (of head 0) of the token's prefix and own items, tiles of an item, tiles to the next head, row in the block
       const int id = blockIdx.x * 32 + lane;
@@ -1036,14 +1066,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const bool is_wide = turn == 1;
       bool ok = true;
       if (warp == 0) {
-        ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, &tmQp, &tmQo, &tmK, &tmV);
+        ok = produce<N>(is_wide, p, w, is_wide ? wide : narrow, smem, bar, cnt, sent, &tmQp, &tmQo, &tmK, &tmV);
       } else if (warp == 1) {
         if (lead) ok = is_wide ? multiply_s<true, N>(w, wide, smem, bar, tmem, cnt) : multiply_s<false, N>(w, narrow, smem, bar, tmem, cnt);
       } else if (warp == 2) {
         if (lead) ok = is_wide ? multiply_o<true, N>(w, wide, smem, bar, tmem, cnt) : multiply_o<false, N>(w, narrow, smem, bar, tmem, cnt);
       }
       __syncwarp();
-      if (turned(ok)) break;
+      if (turned(ok, drain)) break;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -1052,7 +1082,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     for (int turn = 0; turn < 2; ++turn) {
       const bool is_wide = turn == 1;
       const bool ok = is_wide ? softmax_wide(p, w, wide, smem, bar, tmem, cnt, items, cw) : softmax_narrow<N, NL>(p, w, narrow, smem, bar, tmem, cnt, items, cn);
-      if (turned(ok)) break;
+      if (turned(ok, [] {})) break;
     }
   }
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
