@@ -325,10 +325,22 @@ class RolloutEngine:
             for s in list(active):
                 if s.done:
                     active.remove(s)
+                    self._hand_on_prefix(s, active)
                     self.cache.release(s.pages)
                     done[s.req.rid] = GenResult(s.req.rid, s.out, s.logps, s.reason)
         self._prefix.clear()
         return [done[r.rid] for r in requests]
+
+    def _hand_on_prefix(self, s: _Seq, active: List[_Seq]) -> None:
+        """Later requests of a group share the pages of its first sequence: when that one
+        ends, those of another sequence that shares them, or none (its own are free again)."""
+        key = s.req.share_key
+        if key is None or key not in self._prefix or self._prefix[key][0] is not s.pages:
+            return
+        plen = self._prefix.pop(key)[1]
+        heir = next((t for t in active if t.req.share_key == key), None)
+        if heir is not None:
+            self._prefix[key] = (heir.pages, min(plen, len(heir.req.prompt)))
 
     def _emit(self, seqs, logits, temperature, top_p, seed, eos):
         tok, lp = self._sample(logits, temperature, top_p, seed)
