@@ -302,33 +302,37 @@ class RolloutEngine:
         active: List[_Seq] = []
         done: Dict[int, GenResult] = {}
         eos = set(int(e) for e in eos_ids)
-        while waiting or active:
-            admitted = self._admit(waiting, active)
-            if admitted:
-                fresh = [s for s in admitted if s.length == 0]
-                extend = [s for s in admitted if s.length > 0]
-                for group, is_fresh in ((fresh, True), (extend, False)):
-                    if not group:
-                        continue
-                    logits = self._forward(group, fresh=is_fresh)
-                    self._emit(group, logits, temperature, top_p, seed, eos)
-            if not active:
-                if waiting:
-                    raise RuntimeError("KV cache too small for the next request")
-                break
-            decoding = [s for s in active if s.pending and s not in admitted]
-            if decoding and draft_tokens:
-                self._drafted_step(decoding, temperature, seed, eos, draft_tokens, draft_ngram)
-            elif decoding:
-                logits = self._forward(decoding, fresh=False)
-                self._emit(decoding, logits, temperature, top_p, seed, eos)
-            for s in list(active):
-                if s.done:
-                    active.remove(s)
-                    self._hand_on_prefix(s, active)
-                    self.cache.release(s.pages)
-                    done[s.req.rid] = GenResult(s.req.rid, s.out, s.logps, s.reason)
-        self._prefix.clear()
+        try:
+            while waiting or active:
+                admitted = self._admit(waiting, active)
+                if admitted:
+                    fresh = [s for s in admitted if s.length == 0]
+                    extend = [s for s in admitted if s.length > 0]
+                    for group, is_fresh in ((fresh, True), (extend, False)):
+                        if not group:
+                            continue
+                        logits = self._forward(group, fresh=is_fresh)
+                        self._emit(group, logits, temperature, top_p, seed, eos)
+                if not active:
+                    if waiting:
+                        raise RuntimeError("KV cache too small for the next request")
+                    break
+                decoding = [s for s in active if s.pending and s not in admitted]
+                if decoding and draft_tokens:
+                    self._drafted_step(decoding, temperature, seed, eos, draft_tokens, draft_ngram)
+                elif decoding:
+                    logits = self._forward(decoding, fresh=False)
+                    self._emit(decoding, logits, temperature, top_p, seed, eos)
+                for s in list(active):
+                    if s.done:
+                        active.remove(s)
+                        self._hand_on_prefix(s, active)
+                        self.cache.release(s.pages)
+                        done[s.req.rid] = GenResult(s.req.rid, s.out, s.logps, s.reason)
+        finally:                        # after an error: the cache is whole for the next call
+            for s in active:
+                self.cache.release(s.pages)
+            self._prefix.clear()
         return [done[r.rid] for r in requests]
 
     def _hand_on_prefix(self, s: _Seq, active: List[_Seq]) -> None:

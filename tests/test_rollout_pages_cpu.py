@@ -33,3 +33,30 @@ def test_a_groups_first_sequence_ends_before_its_last_are_admitted(max_batch, k)
     eng.cache.alloc = checked
     got = eng.generate([GenRequest(p, n, rid=i, share_key="a") for i, n in enumerate(budgets)], temperature=0.0, draft_tokens=k)
     assert [o.tokens for o in got] == [o.tokens for o in want] and _complete(eng)
+
+
+@pytest.mark.parametrize("k", [0, 3])
+@pytest.mark.parametrize("at", [0, 1, 2, 4])
+def test_an_error_loses_no_page(k, at):
+    """A forward that fails, and a row of logits without a distribution; then the same engine again."""
+    reqs = lambda: [GenRequest(_prompt(37), 12, rid=i, share_key="a") for i in range(5)]
+    want = _engine().generate(reqs(), temperature=0.0)
+    eng = _engine()
+    eng.max_batch = 3
+    forward, calls = eng._forward, []
+
+    def failing(*a, **kw):
+        calls.append(1)
+        if len(calls) == at + 1 and k == 0:
+            raise KeyError("forward")
+        out = forward(*a, **kw)
+        if len(calls) >= at + 1 and kw.get("all_rows"):
+            out[0].fill_(float("nan"))
+        return out
+
+    eng._forward = failing
+    with pytest.raises(RuntimeError if k else KeyError):
+        eng.generate(reqs(), temperature=0.0, draft_tokens=k)
+    assert _complete(eng)
+    eng._forward = forward
+    assert [o.tokens for o in eng.generate(reqs(), temperature=0.0, draft_tokens=k)] == [o.tokens for o in want] and _complete(eng)
