@@ -30,7 +30,7 @@ Reference parity: replaces HF ``model.generate`` on a dense cache
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -298,6 +298,7 @@ class RolloutEngine:
             if top_p < 1.0:
                 raise ValueError("generate: drafted tokens are verified against the whole distribution (top_p = 1)")
             self._check_paged("draft_tokens")
+        requests = [replace(r) for r in requests]     # told apart as objects: their rid is the caller's
         waiting = list(requests)
         active: List[_Seq] = []
         done: Dict[int, GenResult] = {}
@@ -328,12 +329,12 @@ class RolloutEngine:
                         active.remove(s)
                         self._hand_on_prefix(s, active)
                         self.cache.release(s.pages)
-                        done[s.req.rid] = GenResult(s.req.rid, s.out, s.logps, s.reason)
+                        done[id(s.req)] = GenResult(s.req.rid, s.out, s.logps, s.reason)
         finally:                        # after an error: the cache is whole for the next call
             for s in active:
                 self.cache.release(s.pages)
             self._prefix.clear()
-        return [done[r.rid] for r in requests]
+        return [done[id(r)] for r in requests]
 
     def _hand_on_prefix(self, s: _Seq, active: List[_Seq]) -> None:
         """Later requests of a group share the pages of its first sequence: when that one

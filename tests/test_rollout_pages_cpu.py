@@ -60,3 +60,13 @@ def test_an_error_loses_no_page(k, at):
     assert _complete(eng)
     eng._forward = forward
     assert [o.tokens for o in eng.generate(reqs(), temperature=0.0, draft_tokens=k)] == [o.tokens for o in want] and _complete(eng)
+
+
+@pytest.mark.parametrize("k", [0, 3])
+def test_results_are_in_the_requests_order_whatever_their_ids(k):
+    """Requests of one rid (as the serving policy makes them), one of them twice."""
+    prompts = [_prompt(n, n) for n in (5, 20, 11)]
+    want = [_engine().generate([GenRequest(p, n)], temperature=0.0)[0].tokens for p, n in zip(prompts, (9, 4, 6))]
+    reqs = [GenRequest(p, n) for p, n in zip(prompts, (9, 4, 6))]
+    got = _engine().generate(reqs + reqs[1:2], temperature=0.0, draft_tokens=k)
+    assert [o.tokens for o in got] == want + want[1:2] and all(o.rid == 0 for o in got)
