@@ -209,15 +209,15 @@ class MultiTurnRollout:
             seqs.append(s)
         outs = [TrajectoryOut() for _ in range(n)]
         transcripts = [list(p) for p in prompts]
-        g = DecodeGraph(eng, n, max_new, nsplit=self.nsplit, temperature=temperature, top_p=top_p,
-                        seed=seed, eos_ids=eos_ids)
-        g.bt.zero_()
-        for i, s in enumerate(seqs):
-            g.bt[i, : len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
-        if g.groups is not None:
-            for t, v in zip(g.groups, eng.prefix_groups(seqs, n)):
-                t.copy_(v)
         try:
+            g = DecodeGraph(eng, n, max_new, nsplit=self.nsplit, temperature=temperature, top_p=top_p,
+                            seed=seed, eos_ids=eos_ids)
+            g.bt.zero_()
+            for i, s in enumerate(seqs):
+                g.bt[i, : len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
+            if g.groups is not None:
+                for t, v in zip(g.groups, eng.prefix_groups(seqs, n)):
+                    t.copy_(v)
             for turn in range(num_turns):
                 for i in range(n):
                     outs[i].contexts.append(list(transcripts[i]))

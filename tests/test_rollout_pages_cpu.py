@@ -3,7 +3,8 @@ import pytest
 import torch
 from test_rollout_paged_cpu import _engine
 
-from kore_b200.engine.rollout import GenRequest
+from kore_b200.engine.multiturn import MultiTurnRollout
+from kore_b200.engine.rollout import GenRequest, RolloutEngine
 
 
 def _complete(eng):
@@ -70,3 +71,11 @@ def test_results_are_in_the_requests_order_whatever_their_ids(k):
     reqs = [GenRequest(p, n) for p, n in zip(prompts, (9, 4, 6))]
     got = _engine().generate(reqs + reqs[1:2], temperature=0.0, draft_tokens=k)
     assert [o.tokens for o in got] == want + want[1:2] and all(o.rid == 0 for o in got)
+
+
+def test_more_trajectories_than_shared_attention_takes_lose_no_page():
+    eng = _engine()
+    eng = RolloutEngine(eng.w, max_batch=8, page_size=8, num_pages=1200, max_seq_len=64, shared_attention=True)
+    with pytest.raises(ValueError):
+        MultiTurnRollout(eng).run([[1, 2, 3]] * 513, num_turns=1, max_new=2, feedback=lambda t, i, gen: [], max_feedback=1)
+    assert _complete(eng)
