@@ -397,10 +397,14 @@ class RolloutEngine:
         u = torch.rand(ids.numel(), 2, generator=g, device=self.dev)
         v = spec.verify(logits, ids, q_start, u, max(float(temperature), 0.0))
         acc, nxt, lp = v.accepted.tolist(), v.next.tolist(), v.logp.tolist()
+        if min(nxt) < 0:
+            raise RuntimeError("generate: a row of logits has no distribution (NaN or infinite)")
+        for s, a, (length, _) in zip(seqs, acc, start):      # pages of rejected drafts, before any sequence asks for more
+            keep = -(-(length + 1 + a) // self.page_size)
+            self.cache.release(s.pages[keep:])
+            del s.pages[keep:]
         row = 0
         for s, a, y, (length, fed) in zip(seqs, acc, nxt, start):
-            if y < 0:
-                raise RuntimeError("generate: a row of logits has no distribution (NaN or infinite)")
             for j, t in enumerate(fed[1: 1 + a] + [y]):
                 s.length, s.pending = length + 1 + j, []
                 self._take(s, int(t), float(lp[row + j]), eos)

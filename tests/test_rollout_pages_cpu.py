@@ -5,6 +5,7 @@ from test_rollout_paged_cpu import _engine
 
 from kore_b200.engine.multiturn import MultiTurnRollout
 from kore_b200.engine.rollout import GenRequest, RolloutEngine
+from kore_b200.ops import spec
 
 
 def _complete(eng):
@@ -79,3 +80,22 @@ def test_more_trajectories_than_shared_attention_takes_lose_no_page():
     with pytest.raises(ValueError):
         MultiTurnRollout(eng).run([[1, 2, 3]] * 513, num_turns=1, max_new=2, feedback=lambda t, i, gen: [], max_feedback=1)
     assert _complete(eng)
+
+
+@pytest.mark.parametrize("pool", [5, 6, 7, 12])
+def test_rejected_drafts_keep_no_page(pool, monkeypatch):
+    """Drafts that are all wrong change nothing: not which sequence the pool's last page goes to, nor who runs out."""
+    reqs = lambda: [GenRequest(_prompt(20), 30, rid=0), GenRequest(_prompt(6), 4, rid=1), GenRequest(_prompt(9), 12, rid=2)][:2 + (pool > 6)]
+
+    def outs(k):
+        eng = _engine()
+        eng._num_pages = pool
+        got = eng.generate(reqs(), temperature=0.0, draft_tokens=k)
+        assert _complete(eng)
+        return [(o.tokens, o.finish_reason) for o in got]
+
+    want = outs(0)
+    used = {t for tokens, _ in want for t in tokens}
+    wrong = next(t for t in range(200) if t not in used)
+    monkeypatch.setattr(spec.Lookup, "draft", lambda self, k: [wrong] * max(k, 0))
+    assert outs(7) == want
