@@ -179,6 +179,8 @@ class RolloutEngine:
         new = [len(s.pending) for s in seqs]
         lens = [s.length + n for s, n in zip(seqs, new)]
         T, max_q = len(toks), max(new)
+        if any(n > len(s.pages) * self.page_size or len(s.pages) > self.max_pages_per_seq for s, n in zip(seqs, lens)):
+            raise RuntimeError("a sequence has no room for its tokens (max_seq_len, or pages that it does not hold)")
         ids = torch.tensor(toks, dtype=torch.long, device=dev)
         bt = torch.zeros(len(seqs), self.max_pages_per_seq, dtype=torch.int32)
         for i, s in enumerate(seqs):

@@ -4,7 +4,7 @@ import torch
 from test_rollout_paged_cpu import _engine
 
 from kore_b200.engine.multiturn import MultiTurnRollout
-from kore_b200.engine.rollout import GenRequest, RolloutEngine
+from kore_b200.engine.rollout import GenRequest, RolloutEngine, _Seq
 from kore_b200.ops import spec
 
 
@@ -99,3 +99,21 @@ def test_rejected_drafts_keep_no_page(pool, monkeypatch):
     wrong = next(t for t in range(200) if t not in used)
     monkeypatch.setattr(spec.Lookup, "draft", lambda self, k: [wrong] * max(k, 0))
     assert outs(7) == want
+
+
+def test_a_sequence_without_room_is_an_error():
+    """Pages that a sequence does not hold are another's: page 0 is not written in their place."""
+    eng = _engine()
+    for c in eng.cache.k + eng.cache.v:
+        c.fill_(7.0)
+    pages = eng.cache.alloc(2)
+    s = _Seq(GenRequest([1] * 20, 1), pages, 0, 0, [1] * 20)
+    with pytest.raises(RuntimeError, match="no room"):
+        eng._forward([s], fresh=True)
+    assert all((c == 7).all() for c in eng.cache.k + eng.cache.v) and s.length == 0 and len(s.pending) == 20
+    eng.cache.release(pages)
+    with pytest.raises(RuntimeError, match="no room"):              # 300 tokens with max_seq_len = 256
+        eng.generate([GenRequest(_prompt(300), 1)], temperature=0.0)
+    with pytest.raises(RuntimeError, match="no room"):
+        eng.generate([GenRequest(_prompt(250), 20)], temperature=0.0, draft_tokens=3)
+    assert _complete(eng)
