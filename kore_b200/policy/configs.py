@@ -229,8 +229,8 @@ class GRPOConfig(DistributedMixin):
     old_logp_source: str = "trainer"    # "trainer" (policy forward of the update) | "sampler"
     offload_state: str = "auto"         # optimizer state / frozen ref to host between phases: auto|always|never
     ref_placement: str = "auto"         # frozen KL reference: resident | host (streamed) | shard (all-gathered) | auto
-    rollout_shared_attention: bool = False  # attention reads the pages that a group's samples share once for all of them
-    rollout_draft_tokens: int = 0       # drafts per decode step of the unbatched rollout (look-up in the transcript; needs top_p 1)
+    rollout_shared_attention: bool = False  # attention reads the pages that a group's samples share once for all of them (not with tp)
+    rollout_draft_tokens: int = 0       # drafts per decode step of the unbatched rollout (look-up in the transcript; needs top_p 1; batched_rollout and tp do not draft)
     rollout_parallel: str = "replica"   # several GPUs: replica (each rank decodes its own rows) | tp (heads split)
 
 

@@ -226,6 +226,10 @@ class GRPOTrainer:
         Same transcripts as :meth:`rollout_group` while they fit ``max_prompt_length``."""
         from ..engine.multiturn import MultiTurnRollout
         cfg = self.cfg
+        unused, self._unused_told = self._unused_options(), getattr(self, "_unused_told", False)
+        if unused and not self._unused_told and self.ctx.is_main:
+            log.warning("options without effect in the batched rollout", options=unused, tensor_parallel=self._use_tp())
+            self._unused_told = True
         max_new = max_new_tokens or cfg.max_response_length
         G = len(traj_ids)
         prompts, keys = [], []
@@ -261,6 +265,11 @@ class GRPOTrainer:
         for o, tr in zip(outs, flat):
             tr.contexts, tr.gens, tr.gen_logps, tr.finish = o.contexts, o.gens, o.logps, o.finish
         return groups
+
+    def _unused_options(self) -> List[str]:
+        """Rollout options that are set and that the batched rollout does not have."""
+        names = ["rollout_draft_tokens"] + (["rollout_shared_attention"] if self._use_tp() else [])
+        return [n for n in names if getattr(self.cfg, n, 0)]
 
     def _use_tp(self) -> bool:
         return getattr(self.cfg, "rollout_parallel", "replica") == "tp" and self.ctx.world > 1

@@ -117,3 +117,28 @@ def test_a_sequence_without_room_is_an_error():
     with pytest.raises(RuntimeError, match="no room"):
         eng.generate([GenRequest(_prompt(250), 20)], temperature=0.0, draft_tokens=3)
     assert _complete(eng)
+
+
+@pytest.mark.parametrize("kw,tp,want", [(dict(rollout_draft_tokens=3), False, ["rollout_draft_tokens"]), (dict(rollout_shared_attention=True), False, []),
+                                        (dict(rollout_draft_tokens=2, rollout_shared_attention=True), True, ["rollout_draft_tokens", "rollout_shared_attention"]),
+                                        ({}, True, []), (dict(rollout_draft_tokens=3, batched_rollout=False), False, [])])
+def test_grpo_names_options_that_its_rollout_does_not_use(kw, tp, want, monkeypatch):
+    from kore_b200.env.base import SyntheticRewardEnv
+    from kore_b200.policy import grpo
+    from kore_b200.policy.configs import GRPOConfig
+    eng = _engine()
+    gc = GRPOConfig(num_trajectories=2, num_turns=1, tasks_per_step=1, max_response_length=4, max_prompt_length=64, temperature=1.0,
+                    dynamic_sampling=False, starpo_s=False, bf16=False, total_steps=2, overlong_mask=False, top_p=1.0, **kw)
+    tr = grpo.GRPOTrainer(gc, weights=eng.w, env=SyntheticRewardEnv(seed=0, prompt_len=16, feedback_len=4, vocab_size=eng.w.cfg.vocab_size),
+                          rollout_kwargs=dict(num_pages=256, page_size=16, max_seq_len=512))
+    said = []
+    monkeypatch.setattr(grpo.log, "warning", lambda *a, **k: said.append(k["options"]))
+    if tp:                              # the engine itself needs several GPUs
+        monkeypatch.setattr(tr, "_use_tp", lambda: True)
+        monkeypatch.setattr(tr, "_rollout_tp", lambda *a: [])
+        tr.rollout_batch(["a"], [0, 1])
+        tr.rollout_batch(["a"], [0, 1])
+    else:
+        tr.train_step(["a"])
+        tr.train_step(["b"])
+    assert said == ([want] if want else [])
