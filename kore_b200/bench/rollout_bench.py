@@ -1,13 +1,16 @@
 """Decode-step benchmark of the rollout engine (CUDA-graph decode loop).
 
-    python -m kore_b200.bench.rollout_bench [--batch 64] [--ctx 4096] [--layers 0] [--shared 0]
+    python -m kore_b200.bench.rollout_bench [--batch 64] [--ctx 4096] [--layers 0]
+        [--shared 0] [--attention auto|paged|prefix]
 
 Times one replay of the captured decode step for ``batch`` sequences whose KV
 history is ``ctx`` tokens, plus its parts in isolation (the decode GEMMs at
 M = batch, the paged attention, the sampler). Prints one JSON line with the
 step time, the bytes a step must read (weights + KV history) and the achieved
 fraction of the measured HBM bandwidth (MEASURED_PEAKS.json). ``--shared N``: all
-rows share their first N tokens' pages and the attention reads those once.
+rows share their first N tokens' pages. ``--attention``: which one reads them, the
+plain paged attention (every row by itself) or the shared-prefix attention (``auto``:
+this one where tokens are shared); two runs with the same ``--shared`` compare them.
 """
 from __future__ import annotations
 
@@ -34,7 +37,9 @@ def main(argv=None):
     ap.add_argument("--nsplit", type=int, default=4)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--shared", type=int, default=0)
+    ap.add_argument("--attention", choices=("auto", "paged", "prefix"), default="auto")
     args = ap.parse_args(argv)
+    prefix = args.shared > 0 if args.attention == "auto" else args.attention == "prefix"
     cfg = PRESETS[args.model]()
     if args.layers:
         cfg.num_hidden_layers = args.layers
@@ -43,7 +48,7 @@ def main(argv=None):
     B, L, ps = args.batch, args.ctx, 64
     pages_per = (L + 1 + ps - 1) // ps + 1
     eng = RolloutEngine(w, max_batch=B, page_size=ps, num_pages=B * pages_per, max_seq_len=L + 2 * ps,
-                        shared_attention=args.shared > 0)
+                        shared_attention=prefix)
     for t in eng.cache.k + eng.cache.v:
         t.normal_(0, 1)
     g = DecodeGraph(eng, B, 1 << 20, nsplit=args.nsplit, temperature=1.0)
@@ -52,15 +57,17 @@ def main(argv=None):
     if args.shared:
         whole = min(args.shared, L) // ps
         g.bt[:, :whole] = g.bt[:1, :whole]
-        g.groups[0].fill_(B)
-        g.groups[0][0] = 0
-        g.groups[1][0] = whole * ps
+        if g.groups is not None:
+            g.groups[0].fill_(B)
+            g.groups[0][0] = 0
+            g.groups[1][0] = whole * ps
     g.pos.fill_(L)
     g.active.fill_(False)   # keep the position fixed: every replay decodes at context L
     g.budget.fill_(1 << 30)
     g.tok.random_(0, cfg.vocab_size)
     g.step()                # capture
-    out = {"batch": B, "ctx": L, "layers": cfg.num_hidden_layers, "nsplit": args.nsplit, "shared": args.shared}
+    out = {"batch": B, "ctx": L, "layers": cfg.num_hidden_layers, "nsplit": args.nsplit, "shared": args.shared,
+           "attention": "prefix" if prefix else "paged"}
     out["step_ms"] = median_ms(time_cuda(g.step, args.iters, flush_l2=False))
     wbytes = sum(b.numel() * b.element_size() for b in w.bufs)
     kvbytes = (B * (L + 1) - (B - 1) * (min(args.shared, L) // ps * ps)) * eng.kv_bytes_per_token()
