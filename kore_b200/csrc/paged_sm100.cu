@@ -6,11 +6,18 @@
 //                       its paged history; the keys that a group of sequences
 //                       shares are read and scored once for all their rows
 //
-// Measured on one B200 (bf16, D = 128, 40 query and 8 kv heads; times of whole calls):
-//   plan, 64 x 1 rows: 5 us on the device, 14 with its host side; 523k rows of 256
-//   prompts: 16 us. prefix_attention, 8 groups x 8 sequences, prefixes of 512 to 1024 and
-//   own keys of 432 to 6912 tokens: 127 us = 4.9 TB/s of the keys read once; one group of
-//   256 on 16,384 shared tokens: 221 us = 400 TFLOP/s; 4 sequences of 260 tokens: 14 us.
+// Measured on one B200 (bf16, D = 128, 40 query and 8 kv heads; device times, from replays
+// of a CUDA graph; a call outside one adds 2 to 9 us of host side):
+//   plan, 64 x 1 rows: 5 us; 510k rows of 256 prompts: 14 us. prefix_attention, 8 groups x
+//   8 sequences, prefixes of 512 to 1024 and own keys of 432 to 6912 tokens: 132 us = 4.7
+//   TB/s of the keys read once; one group of 256 on 16,384 shared tokens: 224 us = 391
+//   TFLOP/s; 4 sequences of 260 tokens: 15 us.
+// Groups cost a second unit and the join. Beside attention that reads every sequence's own
+// history (paged_attention in decode_sm100.cu, whose repeated pages come from L2), one token
+// a sequence: 8 groups x 8 on 1024 / 4096 / 8192 shared tokens and up to 500 own ones take
+// 52 / 65 / 87 us against 28 / 72 / 140, one group of 64 on 4096 50 against 80; on short
+// prefixes they lose. Several tokens a sequence are for this kernel with or without groups:
+// 64 new tokens behind 1,024 shared ones, 64 sequences, 0.6 ms (0.2 without groups) against 11.7.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

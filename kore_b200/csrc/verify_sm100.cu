@@ -14,9 +14,12 @@
 // such an error moves a token in up to 1% of the draws of a flat distribution, so
 // the one row that is drawn from is summed again in fp64.
 //
-// Measured on one B200, V = 151,936: 64 sequences x 5 rows in bf16 51 us (statistics 26:
-// one pass of exponentials over 97 MB; the draw 25, bound by fp64 exponentials), with
-// draft probabilities 48 x 8 rows 87 us; greedy 200 x 2 rows of 50,257 in fp32 18 us.
+// Measured on one B200 (device times, from replays of a CUDA graph), V = 151,936: 64
+// sequences with 0 to 4 drafts (240 rows, 73 MB in bf16) 52 us, half of it the statistics;
+// 48 with 0 to 7 drafts and their probabilities (310 rows) 90 us; greedy, 200 with at most
+// one (294 rows of 50,257 in fp32) 19 us. The statistics issue in 73% of their cycles, with
+// the exponentials' unit busy for 49% and HBM for 34%; the draw issues in 49%, its fp64
+// pipe is busy for 24%, and it waits mostly at barriers and for its own results (ncu).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -144,7 +147,7 @@ KORE_DEV double peer_f64(const double* p, uint32_t rank) {
 // 2^(i / 32), i < 32, and exp(x) for x <= 0 from it: x = (32 k + i) ln2 / 32 + r with
 // |r| <= ln2 / 64, exp(r) by its series up to r^4 / 24 (off by r^5 / 120 < 2e-12: a draw
 // from 152k tokens moves with probability 3e-7). Nine fp64 operations, where the
-// library's exp takes more than twice as many: the pass is bound by them.
+// library's exp takes more than twice as many.
 struct Exp {
   const double* tab;
   KORE_DEV double operator()(double x) const {
@@ -520,7 +523,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> spec_verify(const at::Tensor& log
   const int room = 2 * num_sms(logits.get_device());
   p.blocks = 1;
   while (p.blocks < kMaxBlocks && B * p.blocks * 2 <= room) p.blocks *= 2;
-  // Statistics: eight blocks to an SM, each thread with a vector at least.
+  // Statistics: blocks for eight to an SM, each thread with a vector at least. (Six of the
+  // bf16 form fit by its registers, four of the fp32 form: the rest are a second wave.)
   p.parts = (int)std::min<int64_t>(kMaxParts, std::max<int64_t>(1, std::min<int64_t>(4 * room / T, V / (8 * kStatThreads))));
   at::Tensor stats = at::empty({T * p.parts, 3}, u.options());
   p.stats = reinterpret_cast<Stat*>(stats.data_ptr<float>());

@@ -15,7 +15,8 @@
 * Where a step's rows go (positions, cache slots, row starts) is planned on the
   device from the sequences' lengths (``ops.paged.plan``).
 * ``shared_attention=True``: multi-token and decode attention read the pages that
-  consecutive sequences share once for all of them (``ops.paged.prefix_attention``).
+  consecutive sequences share once for all of them (``ops.paged.prefix_attention``);
+  for decode steps worth it from a few thousand shared tokens on.
 * ``generate(draft_tokens=k)``: up to k tokens a sequence are drafted by look-up in
   its own transcript and verified against the model in one step (``ops.spec``).
 
