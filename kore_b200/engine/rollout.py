@@ -30,8 +30,9 @@ Reference parity: replaces HF ``model.generate`` on a dense cache
 """
 from __future__ import annotations
 
+import copy
 import math
-from dataclasses import dataclass, field, replace
+from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -301,7 +302,7 @@ class RolloutEngine:
             if top_p < 1.0:
                 raise ValueError("generate: drafted tokens are verified against the whole distribution (top_p = 1)")
             self._check_paged("draft_tokens")
-        requests = [replace(r) for r in requests]     # told apart as objects: their rid is the caller's
+        requests = [copy.copy(r) for r in requests]   # told apart as objects: their rid is the caller's
         waiting = list(requests)
         active: List[_Seq] = []
         done: Dict[int, GenResult] = {}
